@@ -472,6 +472,72 @@ int pdw_block_bwd(const void *gy, const void *x, const void *saved, const void *
                   size_t workspace_bytes, int B, int H, int W, int h, int w, int D, int I, int K, int dtype,
                   void *stream);
 
+/* Norms over the channels of rows x[N][C], one row a pixel or token, and the gated residual that closes a block.  They go
+ * before and after a mixing block (the reference's block has neither norm nor residual: conv_block.py:36-49 is what goes between).
+ *
+ *   PDW_NORM_LAYER   norm(v) = (v - mean v) / sqrt(mean (v - mean v)^2 + eps) * weight + bias
+ *   PDW_NORM_RMS     norm(v) = v / sqrt(mean v^2 + eps) * weight + bias
+ *   PDW_NORM_NONE    norm(v) = v * weight + bias
+ *
+ * 1 <= C <= PDW_NORM_MAX_CHANNELS; weight, bias and scale [C] or NULL (1, 0 and 1).  Statistics and sums are fp32, a result is
+ * rounded once.  stats (optional, 2 N floats): each row's mean and reciprocal deviation, which the backward reads.  Tensors may
+ * have any alignment.  All of it is one pass over the tensors, and one launch more for the sums over rows that are weights' gradients;
+ * those are added in a fixed order (no atomics). */
+enum { PDW_NORM_NONE = 0, PDW_NORM_RMS = 1, PDW_NORM_LAYER = 2 };
+enum { PDW_ACT_NONE = 0, PDW_ACT_SIGMOID = 1, PDW_ACT_SILU = 2 };
+#define PDW_NORM_MAX_CHANNELS 8192
+
+/* y = norm(x); kind is not PDW_NORM_NONE. */
+int pdw_norm_fwd(const void *x, const void *weight, const void *bias, void *y, float *stats, long long N, int C, int kind,
+                 float eps, int dtype, void *stream);
+/* gx, gweight, gbias from gy (each may be NULL: not wanted), x and what the forward left in stats.  Workspace: needed where
+ * gweight or gbias is wanted. */
+size_t pdw_norm_bwd_workspace_bytes(long long N, int C, int dtype);
+int pdw_norm_bwd(const void *gy, const void *x, const void *weight, const float *stats, void *gx, void *gweight, void *gbias,
+                 void *workspace, size_t workspace_bytes, long long N, int C, int kind, int dtype, void *stream);
+
+/* out = x + scale * act(gate) * norm(y), and with next_kind other than PDW_NORM_NONE also next = norm'(out), the norm before
+ * the block that follows (of out as it is before rounding).  gate: NULL; one row for P consecutive rows of x (an image's; N must be a
+ * multiple of P); with P = 1 a value for each.  Gate rows are ldgate elements apart (0: C).  stats: y's. */
+int pdw_residual_fwd(const void *x, const void *y, const void *gate, const void *scale, const void *weight, const void *bias,
+                     const void *next_weight, const void *next_bias, void *out, void *next, float *stats, long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
+                     void *stream);
+/* The gradients, from those of out (gout) and next (gnext), either of which may be NULL (0).  `out` is the forward's result (read only
+ * with a next norm, whose statistics are taken again, of out as it was stored).  gx [N][C] is written only with a next norm (without one it is gout itself); ggate like gate, dense.  Each result
+ * may be NULL (not wanted).  Workspace: needed where any of ggate (with P > 1), gscale, gweight, gbias, gnext_weight, gnext_bias is
+ * wanted. */
+size_t pdw_residual_bwd_workspace_bytes(long long N, int C, long long P, int next_kind, int dtype);
+int pdw_residual_bwd(const void *gout, const void *gnext, const void *out, const void *y, const void *gate, const void *scale,
+                     const void *weight, const void *bias, const void *next_weight, const float *stats, float eps, void *gx, void *gy, void *ggate, void *gscale, void *gweight, void *gbias, void *gnext_weight,
+                     void *gnext_bias, void *workspace, size_t workspace_bytes, long long N, int C, long long P,
+                     long long ldgate, int act, int kind, int next_kind, int dtype, void *stream);
+
+/* The gated linear recurrence  h_t = a_t h_(t-1) + (1 - a_t) x_t,  a_t = sigmoid(g_t),  y_t = h_t,  along the second axis of
+ * [O][T][W][I], each of the O * W * I chains by itself: the recursive counterpart of the depthwise convolution, whose reach is its
+ * filter's (dwconv_triton.py:20-104).  An axis h of images [B][h][w][C] is O = B, T = h, W = w, I = C (dense tensors are faster as
+ * W = 1, I = w * C), an axis w is O = B * h, T = w, W = 1.
+ *
+ * xs[3], gs[3] (host): the strides of x and g in elements, element (o, t, w, i) is x[o * xs[0] + t * xs[1] + w * xs[2] + i]; y and
+ * gy are dense.  h0, last [O][W][I]: the state before the first and after the last step, fp32, either may be NULL (h0: 0).
+ * lengths[O] (device, may be NULL): the chains of o have lengths[o] steps, clamped to 0..T; x, g and gy behind them are not read, and
+ * y, gx and gg are 0 there.  reverse: from the last step to the first.  `states` (pdw_scan_states_bytes; NULL where no backward
+ * follows): what the backward needs.  States and sums are fp32; y is rounded once.  A chain is composed in pieces, so a state
+ * that overflows to infinity can come out as NaN further on.  Workspaces: pdw_scan_workspace_bytes (0: none needed). */
+size_t pdw_scan_states_bytes(int O, long long T, int W, int I);
+size_t pdw_scan_workspace_bytes(int O, long long T, int W, int I, int backward);
+int pdw_scan_fwd(const void *x, const void *g, const float *h0, const int *lengths, void *y, float *last, float *states,
+                 void *workspace, size_t workspace_bytes, int O, long long T, int W, int I, const long long *xs,
+                 const long long *gs, int reverse, int dtype, void *stream);
+/* gx, gg (at the strides gxs, ggs) and gh0 from gy and glast, either of which may be NULL (0), as may each result. */
+int pdw_scan_bwd(const void *gy, const float *glast, const void *x, const void *g, const int *lengths, const float *states,
+                 void *gx, void *gg, float *gh0, void *workspace, size_t workspace_bytes, int O, long long T, int W, int I,
+                 const long long *xs, const long long *gs, const long long *gxs, const long long *ggs, int reverse, int dtype,
+                 void *stream);
+/* One step of B x C chains (a token for each of B streams): y = new_state = sigmoid(g) state + sigmoid(-g) x.  Rows of x and g are
+ * ldx and ldg elements apart, the others dense.  new_state may be state itself, but must not overlap it otherwise. */
+int pdw_scan_step(const void *x, const void *g, const float *state, float *new_state, void *y, long long B, int C,
+                  long long ldx, long long ldg, int dtype, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,7 +10,7 @@ import ctypes
 import importlib.util
 import threading
 import os
-from ctypes import c_char_p, c_int, c_longlong, c_size_t, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_void_p
 
 import torch
 
@@ -103,6 +103,21 @@ _SIGS = {
     "pdw_dense_bwd_pair_colsum_supported": (c_int, [c_int] * 3),
     "pdw_dense_bwd_pair": (c_int, [c_void_p] * 7 + [c_size_t, c_void_p, c_int, c_longlong, c_int, c_int, c_int,
                                    c_void_p]),
+    "pdw_norm_fwd": (c_int, [c_void_p] * 5 + [c_longlong, c_int, c_int, c_float, c_int, c_void_p]),
+    "pdw_norm_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int]),
+    "pdw_norm_bwd": (c_int, [c_void_p] * 8 + [c_size_t, c_longlong] + [c_int] * 3 + [c_void_p]),
+    "pdw_residual_fwd": (c_int, [c_void_p] * 11 + [c_longlong, c_int, c_longlong, c_longlong] + [c_int] * 3
+                         + [c_float, c_int, c_void_p]),
+    "pdw_residual_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int, c_longlong, c_int, c_int]),
+    "pdw_residual_bwd": (c_int, [c_void_p] * 10 + [c_float] + [c_void_p] * 9 + [c_size_t, c_longlong, c_int, c_longlong, c_longlong] + [c_int] * 4
+                         + [c_void_p]),
+    "pdw_scan_states_bytes": (c_size_t, [c_int, c_longlong, c_int, c_int]),
+    "pdw_scan_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int, c_int, c_int]),
+    "pdw_scan_fwd": (c_int, [c_void_p] * 8 + [c_size_t, c_int, c_longlong, c_int, c_int] + [c_void_p] * 2 + [c_int] * 2
+                     + [c_void_p]),
+    "pdw_scan_bwd": (c_int, [c_void_p] * 10 + [c_size_t, c_int, c_longlong, c_int, c_int] + [c_void_p] * 4 + [c_int] * 2
+                     + [c_void_p]),
+    "pdw_scan_step": (c_int, [c_void_p] * 5 + [c_longlong, c_int, c_longlong, c_longlong, c_int, c_void_p]),
 }
 EXPORTS = tuple(_SIGS)
 

@@ -3,7 +3,7 @@
     python -m pyramidconvblock_amd.build [--force]
 
 Every csrc/*.hip file is compiled to an object (in parallel) and linked into
-pyramidconvblock_amd/libpdw.so; csrc/torch_ops.cpp (the operators' host path, no device code) is
+pyramidconvblock_amd/libpdw.so; csrc/torch_*.cpp (the operators' host path, no device code) are
 compiled with the host compiler against torch's headers and linked to it as the extension module
 of ext_path().  hipcc cross-compiles, so no GPU is needed.  libpdw.so needs no torch: run as a script
 (python pyramidconvblock_amd/build.py) where there is none, this builds the library alone.
@@ -70,14 +70,14 @@ def build_ext(force: bool = False) -> str:
     """The host extension: libpdw.so is found beside it ($ORIGIN), torch's libraries are loaded by `import torch`."""
     import torch
 
-    src, ext = os.path.join(CSRC, "torch_ops.cpp"), ext_path(torch.__version__)
-    if not (force or _stale(ext, [src] + _headers())):
+    srcs, ext = sorted(glob.glob(os.path.join(CSRC, "torch_*.cpp"))), ext_path(torch.__version__)
+    if not (force or _stale(ext, srcs + _headers())):
         return ext
     troot = os.path.dirname(torch.__file__)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall",
            "-D__HIP_PLATFORM_AMD__=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            "-isystem", os.path.join(troot, "include"), "-isystem", os.path.join(troot, "include/torch/csrc/api/include"),
-           "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], src, "-o", ext,
+           "-isystem", "/opt/rocm/include", "-isystem", sysconfig.get_paths()["include"], *srcs, "-o", ext,
            LIB, "-L" + os.path.join(troot, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_hip",
            "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)

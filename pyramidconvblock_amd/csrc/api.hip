@@ -14,6 +14,7 @@
 #include "kernels.h"
 #include "pool_branch.h"
 #include "reduce_parts.h"
+#include "scan.h"
 
 namespace pdw {
 
@@ -45,6 +46,34 @@ static int check_conv(const char* fn, const void* a, const void* b, const void* 
     if (SH < 1 || SW < 1 || DH < 1 || DW < 1 || PH < 0 || PW < 0)
         return set_error("%s: bad stride/padding/dilation (%d,%d)/(%d,%d)/(%d,%d)", fn, SH, SW, PH, PW, DH, DW), 1;
     if (B > 0 && (!a || !b || !c)) return set_error("%s: null pointer", fn), 1;
+    return 0;
+}
+
+static int check_rows(const char* fn, long long N, int C, int kind, int next_kind, int act, int dtype) {
+    if (!valid_dtype(dtype)) return set_error("%s: unknown dtype %d", fn, dtype), 1;
+    if (N < 0 || C < 1 || C > PDW_NORM_MAX_CHANNELS)
+        return set_error("%s: need N >= 0 and 1 <= C <= %d (N=%lld C=%d)", fn, PDW_NORM_MAX_CHANNELS, N, C), 1;
+    for (int k : {kind, next_kind})
+        if (k < kNormNone || k > kNormLayer) return set_error("%s: unknown norm %d", fn, k), 1;
+    if (act < kActNone || act > kActSilu) return set_error("%s: unknown activation %d", fn, act), 1;
+    return 0;
+}
+
+// The gate of a residual: a row for P rows, or a value for each.
+static int check_gate(const char* fn, const void* gate, long long N, int C, long long P, long long* ldgate) {
+    if (!gate) return 0;
+    if (P < 1 || N % P) return set_error("%s: %lld rows are no multiple of P=%lld", fn, N, P), 1;
+    if (*ldgate == 0) *ldgate = C;
+    if (*ldgate < 0) return set_error("%s: ldgate=%lld", fn, *ldgate), 1;
+    return 0;
+}
+
+static int check_scan(const char* fn, const void* x, const void* g, const long long* xs, const long long* gs, int O, long long T,
+                      int W, int I, int dtype) {
+    if (!valid_dtype(dtype)) return set_error("%s: unknown dtype %d", fn, dtype), 1;
+    if (O < 0 || T < 0 || W < 0 || I < 0 || (long long)O * W > 0x7fffffffLL)
+        return set_error("%s: bad extents O=%d T=%lld W=%d I=%d", fn, O, T, W, I), 1;
+    if (O > 0 && T > 0 && W > 0 && I > 0 && (!x || !g || !xs || !gs)) return set_error("%s: null pointer", fn), 1;
     return 0;
 }
 
@@ -749,6 +778,115 @@ int pdw_dense_bwd_pair(const void* gy, const void* w, const void* x, void* dx, f
         return set_error("pdw_dense_bwd_pair: O=%d I=%d dtype=%d (P=%d) not covered (see pdw_dense_bwd_pair_supported)",
                          O, I, dtype, P), 3;
     return r;
+}
+
+int pdw_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats, long long N, int C, int kind,
+                 float eps, int dtype, void* stream) {
+    if (int e = check_rows("pdw_norm_fwd", N, C, kind, kNormNone, kActNone, dtype)) return e;
+    if (kind == kNormNone) return set_error("pdw_norm_fwd: no norm asked for"), 1;
+    if (N > 0 && (!x || !y)) return set_error("pdw_norm_fwd: null pointer"), 1;
+    RowArgs p{};
+    p.x = x, p.w2 = weight, p.b2 = bias, p.next = y, p.st2 = stats, p.N = N, p.P = N, p.C = C, p.kind2 = kind, p.eps = eps;
+    return rows_forward_launch(p, dtype, (hipStream_t)stream);
+}
+
+size_t pdw_norm_bwd_workspace_bytes(long long N, int C, int dtype) {
+    if (check_rows("pdw_norm_bwd_workspace_bytes", N, C, 0, 0, 0, dtype)) return 0;
+    return rows_backward_workspace(N, 1, C, 2, dtype);
+}
+
+int pdw_norm_bwd(const void* gy, const void* x, const void* weight, const float* stats, void* gx, void* gweight, void* gbias,
+                 void* workspace, size_t workspace_bytes, long long N, int C, int kind, int dtype, void* stream) {
+    if (int e = check_rows("pdw_norm_bwd", N, C, kind, kNormNone, kActNone, dtype)) return e;
+    if (kind == kNormNone) return set_error("pdw_norm_bwd: no norm asked for"), 1;
+    if (N > 0 && (!gy || !x || !stats)) return set_error("pdw_norm_bwd: null pointer"), 1;
+    RowArgs p{};
+    p.x = x, p.gz = gy, p.w2 = weight, p.st2 = const_cast<float*>(stats), p.gx = gx, p.N = N, p.P = N, p.C = C, p.kind2 = kind;
+    return rows_backward_launch(p, nullptr, nullptr, nullptr, gweight, gbias, workspace, workspace_bytes, dtype, (hipStream_t)stream);
+}
+
+int pdw_residual_fwd(const void* x, const void* y, const void* gate, const void* scale, const void* weight, const void* bias,
+                     const void* next_weight, const void* next_bias, void* out, void* next, float* stats, long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
+                     void* stream) {
+    if (int e = check_rows("pdw_residual_fwd", N, C, kind, next_kind, act, dtype)) return e;
+    if (int e = check_gate("pdw_residual_fwd", gate, N, C, P, &ldgate)) return e;
+    if (N > 0 && (!x || !y || !out || (next_kind != kNormNone && !next))) return set_error("pdw_residual_fwd: null pointer"), 1;
+    RowArgs p{};
+    p.x = x, p.y = y, p.gate = gate, p.scale = scale, p.w = weight, p.b = bias, p.w2 = next_weight, p.b2 = next_bias;
+    p.out = out, p.next = next, p.st = stats, p.N = N, p.P = P, p.ldg = ldgate, p.C = C;
+    p.act = act, p.kind = kind, p.kind2 = next_kind, p.gate_rows = !gate ? 0 : P == 1 ? 2 : 1, p.eps = eps;
+    return rows_forward_launch(p, dtype, (hipStream_t)stream);
+}
+
+size_t pdw_residual_bwd_workspace_bytes(long long N, int C, long long P, int next_kind, int dtype) {
+    if (check_rows("pdw_residual_bwd_workspace_bytes", N, C, 0, next_kind, 0, dtype)) return 0;
+    // (P only where a gate row serves several rows; otherwise all rows are one image)
+    return rows_backward_workspace(N, P > 1 && N % P == 0 ? N / P : 1, C, next_kind == kNormNone ? 2 : 4, dtype);
+}
+
+int pdw_residual_bwd(const void* gout, const void* gnext, const void* out, const void* y, const void* gate, const void* scale,
+                     const void* weight, const void* bias, const void* next_weight, const float* stats, float eps, void* gx, void* gy, void* ggate, void* gscale, void* gweight, void* gbias, void* gnext_weight,
+                     void* gnext_bias, void* workspace, size_t workspace_bytes, long long N, int C, long long P,
+                     long long ldgate, int act, int kind, int next_kind, int dtype, void* stream) {
+    if (int e = check_rows("pdw_residual_bwd", N, C, kind, next_kind, act, dtype)) return e;
+    if (int e = check_gate("pdw_residual_bwd", gate, N, C, P, &ldgate)) return e;
+    const bool next = next_kind != kNormNone;
+    if (N > 0 && (!y || (kind != kNormNone && !stats) || (next && !out) || (!gate && ggate)))
+        return set_error("pdw_residual_bwd: null pointer"), 1;
+    RowArgs p{};
+    p.go = gout, p.gz = gnext, p.x = out, p.y = y, p.gate = gate, p.scale = scale, p.w = weight, p.b = bias, p.w2 = next_weight;
+    p.st = const_cast<float*>(stats), p.eps = eps, p.gx = next ? gx : nullptr, p.gy = gy, p.ggate = ggate;
+    p.N = N, p.P = P, p.ldg = ldgate, p.C = C, p.act = act, p.kind = kind, p.kind2 = next_kind;
+    p.gate_rows = !gate ? 0 : P == 1 ? 2 : 1;
+    return rows_backward_launch(p, gscale, gweight, gbias, gnext_weight, gnext_bias, workspace, workspace_bytes, dtype,
+                                (hipStream_t)stream);
+}
+
+size_t pdw_scan_states_bytes(int O, long long T, int W, int I) {
+    return O < 1 || T < 1 || W < 1 || I < 1 ? 0 : scan_states_bytes((long long)O * W, T, I);
+}
+
+size_t pdw_scan_workspace_bytes(int O, long long T, int W, int I, int backward) {
+    return O < 1 || T < 1 || W < 1 || I < 1 ? 0 : scan_workspace((long long)O * W, T, I, backward != 0);
+}
+
+static ScanStrides strides_of(const long long* s) { return s ? ScanStrides{s[0], s[1], s[2]} : ScanStrides{0, 0, 0}; }
+
+int pdw_scan_fwd(const void* x, const void* g, const float* h0, const int* lengths, void* y, float* last, float* states,
+                 void* workspace, size_t workspace_bytes, int O, long long T, int W, int I, const long long* xs,
+                 const long long* gs, int reverse, int dtype, void* stream) {
+    if (int e = check_scan("pdw_scan_fwd", x, g, xs, gs, O, T, W, I, dtype)) return e;
+    if (O == 0 || W == 0 || I == 0) return 0;
+    if (T > 0 && !y) return set_error("pdw_scan_fwd: null pointer"), 1;
+    ScanArgs p{};
+    p.x = x, p.g = g, p.h0 = h0, p.lengths = lengths, p.y = y, p.last = last, p.states = states;
+    p.rows = O * W, p.T = T, p.W = W, p.I = I, p.xs = strides_of(xs), p.gs = strides_of(gs), p.reverse = reverse != 0;
+    p.dense = {T * W * I, (long long)W * I, I};
+    return scan_run(p, false, workspace, workspace_bytes, dtype, (hipStream_t)stream);
+}
+
+int pdw_scan_bwd(const void* gy, const float* glast, const void* x, const void* g, const int* lengths, const float* states,
+                 void* gx, void* gg, float* gh0, void* workspace, size_t workspace_bytes, int O, long long T, int W, int I,
+                 const long long* xs, const long long* gs, const long long* gxs, const long long* ggs, int reverse, int dtype,
+                 void* stream) {
+    if (int e = check_scan("pdw_scan_bwd", x, g, xs, gs, O, T, W, I, dtype)) return e;
+    if (O == 0 || W == 0 || I == 0) return 0;
+    if (T > 0 && (!states || (gx && !gxs) || (gg && !ggs))) return set_error("pdw_scan_bwd: null pointer"), 1;
+    ScanArgs p{};
+    p.x = x, p.g = g, p.gy = gy, p.glast = glast, p.lengths = lengths, p.states = const_cast<float*>(states);
+    p.gx = gx, p.gg = gg, p.gh0 = gh0, p.rows = O * W, p.T = T, p.W = W, p.I = I, p.reverse = reverse != 0;
+    p.xs = strides_of(xs), p.gs = strides_of(gs), p.gxs = strides_of(gxs), p.ggs = strides_of(ggs);
+    p.dense = {T * W * I, (long long)W * I, I};
+    return scan_run(p, true, workspace, workspace_bytes, dtype, (hipStream_t)stream);
+}
+
+int pdw_scan_step(const void* x, const void* g, const float* state, float* new_state, void* y, long long B, int C,
+                  long long ldx, long long ldg, int dtype, void* stream) {
+    if (!valid_dtype(dtype)) return set_error("pdw_scan_step: unknown dtype %d", dtype), 1;
+    if (B < 0 || C < 0) return set_error("pdw_scan_step: bad extents B=%lld C=%d", B, C), 1;
+    if (B == 0 || C == 0) return 0;
+    if (!x || !g || !state || !new_state || !y) return set_error("pdw_scan_step: null pointer"), 1;
+    return scan_step_launch(x, g, state, new_state, y, B, C, ldx, ldg, dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

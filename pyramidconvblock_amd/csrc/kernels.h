@@ -202,4 +202,17 @@ int convblock_fwd_launch(const void* x, const void* w_up, const void* w_dw0, con
                          void* cat, void* m, void* y, float* xparts, float* yp, int B, int H, int W, int D, int I, int K,
                          int dtype, void* stream);
 
+// norm.hip: norms over channels and gated residuals (arguments: row_norm.h); sums: 2 column sums a norm
+int rows_forward_launch(const struct RowArgs& p, int dtype, hipStream_t s);
+size_t rows_backward_workspace(long long N, long long images, int C, int sums, int dtype);
+int rows_backward_launch(const struct RowArgs& p, void* gscale, void* gw, void* gb, void* gw2, void* gb2, void* workspace,
+                         size_t workspace_bytes, int dtype, hipStream_t s);
+
+// scan.hip: the gated linear recurrence (arguments: scan.h) and its form for a single token
+size_t scan_states_bytes(long long rows, long long T, int I);
+size_t scan_workspace(long long rows, long long T, int I, bool backward);
+int scan_run(const struct ScanArgs& p, bool backward, void* workspace, size_t workspace_bytes, int dtype, hipStream_t s);
+int scan_step_launch(const void* x, const void* g, const float* state, float* new_state, void* y, long long B, int C, long long ldx,
+                     long long ldg, int dtype, hipStream_t s);
+
 }  // namespace pdw

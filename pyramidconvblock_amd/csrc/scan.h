@@ -1,0 +1,435 @@
+// The gated linear recurrence  h_t = a_t h_(t-1) + m_t x_t,  a_t = sigmoid(g_t), m_t = 1 - a_t,  along the second axis of
+// x[O][T][W][I], every one of the O x W x I chains by itself, and its gradients.
+//
+// A step maps h to a h + b; such maps compose associatively, (a, b) then (a', b') = (a a', a' b + b'), and a composition
+// of a's in (0, 1) never grows, so a stretch of time can be cut anywhere: each piece is composed by itself, the pieces' maps are
+// scanned, and each piece is run again from its own starting state.  Backwards, with d_t the gradient of h_t, the quantity handed from
+// step t to step t - 1 is e_t = a_t d_t = a_t (gy_t + e_(t+1)): maps of the same kind with the same a, composed from the end.
+//     gx_t = d_t m_t        gg_t = d_t (h_(t-1) - x_t) a_t m_t        (gradient of the initial state) = e_0
+// The states h_(t-1) that gg needs are not kept: the forward leaves the 32-bit state before every tile, and the backward runs the tile
+// from it again, in the same order, from x and g, which it reads anyway.
+//
+// A workgroup has a strip of channels (LC lanes of VEC channels: 128 bytes in 16-bit types, so that a time step is a whole cache
+// line) and walks over tiles of NW wavefronts x 64/LC lanes x K steps: a lane composes its K consecutive steps in registers, lanes
+// and wavefronts exchange their maps (shuffles; LDS), and every lane runs its K steps from its state.  So x and g are read once.  Where
+// there are too few strips to fill the chip, time is cut into segments of whole tiles: a first launch composes each segment's
+// map (x and g are read once more for it), and the second starts each segment from the maps before it.
+//
+// All of it is in fp32.  No atomics: results are the same from call to call.
+#pragma once
+#include "common.h"
+#include "gate_math.h"
+#include "row_norm.h"
+
+namespace pdw {
+
+// Element (o, t, w, i) of a tensor is base[o * o + t * t + w * w + i].
+struct ScanStrides {
+    long long o, t, w;
+};
+
+struct ScanArgs {
+    const void *x, *g, *gy;
+    void *y, *gx, *gg;
+    ScanStrides xs, gs, gxs, ggs, dense;   // dense: of y and gy
+    const float *h0, *glast;            // [O][W][I], or null (0)
+    float *last, *gh0;                  // [O][W][I], or null
+    float* states;                      // [O * W][state_tiles][I]: the state before every tile of the backward, or null
+    float* maps;                        // [segment][O * W][I] x (a, b): the segments' maps
+    const int* lengths;                 // [O], or null (T)
+    long long T;
+    int rows, W, I;                     // rows = O * W
+    int strips, tiles, segments, seg_tiles, state_tiles;
+    int reverse;
+};
+
+// Maps of a lane's VEC channels.
+template <int VEC>
+struct Maps {
+    float a[VEC], b[VEC];
+};
+
+// Composes `first` before `m`.
+template <int VEC>
+__device__ __forceinline__ void after(Maps<VEC>& m, const float (&a)[VEC], const float (&b)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) m.b[v] = __builtin_fmaf(m.a[v], b[v], m.b[v]), m.a[v] *= a[v];
+}
+
+// Where a lane stands: its channels, and its steps within a tile.
+template <int VEC, int LC, int NW, int K>
+struct ScanLane {
+    static constexpr int kSub = 64 / LC, kTile = NW * kSub * K;
+    int lane, wave, c, sub;   // c: first channel
+    bool on;
+    __device__ __forceinline__ ScanLane(int strip, int I) {
+        lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        c = (strip * LC + lane % LC) * VEC;
+        on = c < I;
+        if (c + VEC > I) c = I - VEC;   // the last lane overlaps the one before it: the same chains, the same values (I >= VEC)
+        sub = wave * kSub + lane / LC;
+    }
+};
+
+// The map from the start of the tile to the start of this lane's steps applied to `carry` (the state at the tile's start), and
+// carry taken to the tile's end.  BACK: in the order of falling time.  lds[NW][LC * VEC] x 2 floats, one such buffer a call in turn.
+template <int VEC, int LC, int NW, bool BACK>
+__device__ __forceinline__ void scan_tile(Maps<VEC> m, float (&carry)[VEC], float (&start)[VEC], float2* lds, int lane, int wave) {
+    constexpr int W = LC * VEC;
+    const int cl = lane % LC;
+#pragma unroll
+    for (int d = LC; d < 64; d *= 2) {
+        float a[VEC], b[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            a[v] = BACK ? __shfl_down(m.a[v], d) : __shfl_up(m.a[v], d);
+            b[v] = BACK ? __shfl_down(m.b[v], d) : __shfl_up(m.b[v], d);
+        }
+        if (BACK ? lane + d < 64 : lane >= d) after<VEC>(m, a, b);
+    }
+    float ea[VEC], eb[VEC];   // the lanes before this one
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        const float a = BACK ? __shfl_down(m.a[v], LC) : __shfl_up(m.a[v], LC);
+        const float b = BACK ? __shfl_down(m.b[v], LC) : __shfl_up(m.b[v], LC);
+        const bool edge = LC == 64 || (BACK ? lane + LC >= 64 : lane < LC);
+        ea[v] = edge ? 1.f : a, eb[v] = edge ? 0.f : b;
+    }
+    if (BACK ? lane < LC : lane >= 64 - LC) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) lds[wave * W + cl * VEC + v] = make_float2(m.a[v], m.b[v]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+        const int w = BACK ? NW - 1 - i : i;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            if (w == wave) start[v] = carry[v];
+            const float2 t = lds[w * W + cl * VEC + v];
+            carry[v] = __builtin_fmaf(t.x, carry[v], t.y);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) start[v] = __builtin_fmaf(ea[v], start[v], eb[v]);
+}
+
+// The state that a segment starts from: `first` (the initial state, or the last one's gradient) through the maps of the segments
+// before it (BACK: behind it).  The workgroup's lanes share them out as they share the steps of a tile.
+template <int VEC, int LC, int NW, int K, bool BACK>
+__device__ __forceinline__ void segment_start(const ScanArgs& p, int o, int seg, const ScanLane<VEC, LC, NW, K>& at,
+                                              const float* first, float (&carry)[VEC], float2* lds) {
+    constexpr int TS = NW * ScanLane<VEC, LC, NW, K>::kSub;
+    const long long row = (long long)o * p.I + at.c, ld = (long long)p.rows * p.I;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) carry[v] = first && at.on ? first[row + v] : 0.f;
+    const int n = BACK ? p.segments - 1 - seg : seg;   // maps to go through
+    if (n == 0) return;
+    const int each = (n + TS - 1) / TS;
+    const int turn = BACK ? TS - 1 - at.sub : at.sub;   // this lane's place in the order of composition
+    Maps<VEC> m;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) m.a[v] = 1.f, m.b[v] = 0.f;
+    for (int k = 0; k < each; ++k) {
+        const int i = turn * each + k;
+        if (i >= n || !at.on) break;
+        const float2* t = reinterpret_cast<const float2*>(p.maps) + (BACK ? p.segments - 1 - i : i) * ld + row;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            const float2 u = t[v];
+            m.b[v] = __builtin_fmaf(u.x, m.b[v], u.y), m.a[v] *= u.x;
+        }
+    }
+    float unused[VEC];
+    scan_tile<VEC, LC, NW, BACK>(m, carry, unused, lds, at.lane, at.wave);
+    __syncthreads();
+}
+
+// Position in memory of step s of a chain of `len` steps; steps behind its end stay where they are.
+__device__ __forceinline__ long long scan_pos(long long s, long long len, int reverse) {
+    return reverse && s < len ? len - 1 - s : s;
+}
+
+// What a workgroup's index says: its strip of channels, its row (o, w) and its segment; and its chains' length.
+struct ScanWhere {
+    int strip, row, o, w, seg;
+    long long len;
+    __device__ __forceinline__ ScanWhere(const ScanArgs& p) {
+        strip = blockIdx.x % (unsigned)p.strips;
+        const unsigned rest = blockIdx.x / (unsigned)p.strips;
+        row = rest % (unsigned)p.rows, seg = rest / (unsigned)p.rows;
+        o = row / p.W, w = row - o * p.W;
+        const long long n = p.lengths ? p.lengths[o] : p.T;
+        len = n < 0 ? 0 : n > p.T ? p.T : n;
+    }
+    template <typename T>
+    __device__ __forceinline__ T* base(T* t, const ScanStrides& s, int c) const {
+        return t + o * s.o + w * s.w + c;
+    }
+};
+
+// (a, m) of one piece of g
+template <typename T, int VEC>
+__device__ __forceinline__ void gates(const Piece<T, VEC>& g, float (&a)[VEC], float (&m)[VEC]) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) sigmoid_pair(to_f32(g.v[v]), a[v], m[v]);
+}
+
+// A lane's K pieces of one tensor; `n` of them are there.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void load_steps(const T* base, long long stride, long long s0, long long len, int reverse, bool on,
+                                           Piece<T, VEC> (&r)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (on && s0 + k < len) r[k] = load_any<T, VEC>(base + scan_pos(s0 + k, len, reverse) * stride);
+        else
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) r[k].v[v] = from_f32<T>(0.f);
+    }
+}
+
+// The map of every segment but the one that no other starts from (forward the last, BACK the first).  A lane composes a
+// contiguous run of the segment's steps by itself, so the lanes exchange once, at the end.
+template <typename T, int VEC, int LC, int NW, int K, bool BACK>
+__global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
+    typedef ScanLane<VEC, LC, NW, K> Lane;
+    constexpr int TS = NW * Lane::kSub;
+    __shared__ float2 lds[NW * LC * VEC];
+    const ScanWhere my(p);
+    const int seg = my.seg + (BACK ? 1 : 0);
+    const Lane at(my.strip, p.I);
+    const long long len = my.len;
+    const T* other = my.base((const T*)(BACK ? p.gy : p.x), BACK ? p.dense : p.xs, at.c);
+    const bool given = !BACK || p.gy;
+    const long long ot = BACK ? p.dense.t : p.xs.t;
+    const T* g = my.base((const T*)p.g, p.gs, at.c);
+    const long long first = (long long)seg * p.seg_tiles * Lane::kTile;
+    const int run = p.seg_tiles * (Lane::kTile / TS);   // a lane's steps: a multiple of K
+    const long long s0 = first + (long long)at.sub * run;
+    Maps<VEC> m;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) m.a[v] = 1.f, m.b[v] = 0.f;
+    for (int i = 0; i < run; i += K) {
+        const long long s = BACK ? s0 + run - K - i : s0 + i;
+        Piece<T, VEC> xr[K], gr[K];
+        load_steps<T, VEC, K>(g, p.gs.t, s, len, p.reverse, at.on, gr);
+        load_steps<T, VEC, K>(other, ot, s, len, p.reverse, at.on && given, xr);
+#pragma unroll
+        for (int j = 0; j < K; ++j) {
+            const int k = BACK ? K - 1 - j : j;
+            float a[VEC], q[VEC];
+            gates<T, VEC>(gr[k], a, q);
+            const bool valid = s + k < len;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float u = to_f32(xr[k].v[v]);
+                const float b = BACK ? a[v] * (u + m.b[v]) : __builtin_fmaf(a[v], m.b[v], q[v] * u);
+                m.b[v] = valid ? b : m.b[v], m.a[v] = valid ? m.a[v] * a[v] : m.a[v];
+            }
+        }
+    }
+    float zero[VEC], one[VEC], unused[VEC];
+    Maps<VEC> product = m;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) zero[v] = 0.f, one[v] = 1.f, product.b[v] = 0.f;
+    scan_tile<VEC, LC, NW, BACK>(m, zero, unused, lds, at.lane, at.wave);
+    __syncthreads();
+    scan_tile<VEC, LC, NW, BACK>(product, one, unused, lds, at.lane, at.wave);   // the maps' first halves, as what 1 becomes
+    if (!at.on || at.sub != 0) return;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v)
+        reinterpret_cast<float2*>(p.maps)[((long long)seg * p.rows + my.row) * p.I + at.c + v] = make_float2(one[v], zero[v]);
+}
+
+template <typename T, int VEC, int LC, int NW, int K>
+__global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
+    typedef ScanLane<VEC, LC, NW, K> Lane;
+    constexpr int TS = NW * Lane::kSub;
+    __shared__ float2 lds[2][NW * LC * VEC];
+    const ScanWhere my(p);
+    const int seg = my.seg;
+    const Lane at(my.strip, p.I);
+    const long long len = my.len, row = (long long)my.row * p.I + at.c;
+    const T* x = my.base((const T*)p.x, p.xs, at.c);
+    const T* g = my.base((const T*)p.g, p.gs, at.c);
+    T* y = my.base((T*)p.y, p.dense, at.c);
+    float carry[VEC];
+    segment_start<VEC, LC, NW, K, false>(p, my.row, seg, at, p.h0, carry, lds[1]);
+    const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
+    for (int tile = t0; tile < t1; ++tile) {
+        const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
+        float a[K][VEC], b[K][VEC], start[VEC];
+        {
+            Piece<T, VEC> xr[K], gr[K];
+            load_steps<T, VEC, K>(x, p.xs.t, s0, len, p.reverse, at.on, xr);
+            load_steps<T, VEC, K>(g, p.gs.t, s0, len, p.reverse, at.on, gr);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                gates<T, VEC>(gr[k], a[k], b[k]);
+                const bool valid = s0 + k < len;
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) {
+                    b[k][v] = valid ? b[k][v] * to_f32(xr[k].v[v]) : 0.f;
+                    if (!valid) a[k][v] = 1.f;
+                }
+            }
+        }
+        Maps<VEC> m;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) m.a[v] = a[0][v], m.b[v] = b[0][v];
+#pragma unroll
+        for (int k = 1; k < K; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) m.b[v] = __builtin_fmaf(a[k][v], m.b[v], b[k][v]), m.a[v] *= a[k][v];
+        scan_tile<VEC, LC, NW, false>(m, carry, start, lds[tile & 1], at.lane, at.wave);
+        // (a tile is two of the backward's: the states before its first and its middle step)
+        if (p.states && at.on && (at.sub == 0 || at.sub == TS / 2) && s0 < p.T) {
+            float* st = p.states + ((long long)my.row * p.state_tiles + 2 * tile + (at.sub != 0)) * p.I + at.c;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) st[v] = start[v];
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) start[v] = __builtin_fmaf(a[k][v], start[v], b[k][v]);
+            float out[VEC];
+            const bool valid = s0 + k < len;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) out[v] = valid ? start[v] : 0.f;
+            if (at.on && s0 + k < p.T)
+                store_any<T, VEC>(y + scan_pos(s0 + k, len, p.reverse) * p.dense.t, out);
+        }
+    }
+    if (p.last && seg == p.segments - 1 && at.on && at.sub == 0) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p.last[row + v] = carry[v];
+    }
+}
+
+template <typename T, int VEC, int LC, int NW, int K>
+__global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
+    typedef ScanLane<VEC, LC, NW, K> Lane;
+    __shared__ float2 lds[2][2][NW * LC * VEC];
+    const ScanWhere my(p);
+    const int seg = my.seg;
+    const Lane at(my.strip, p.I);
+    const long long len = my.len, row = (long long)my.row * p.I + at.c;
+    const T* x = my.base((const T*)p.x, p.xs, at.c);
+    const T* g = my.base((const T*)p.g, p.gs, at.c);
+    const T* gy = my.base((const T*)p.gy, p.dense, at.c);
+    T *gx = my.base((T*)p.gx, p.gxs, at.c), *gg = my.base((T*)p.gg, p.ggs, at.c);
+    float carry[VEC];
+    segment_start<VEC, LC, NW, K, true>(p, my.row, seg, at, p.glast, carry, lds[1][0]);
+    const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
+    for (int tile = t1 - 1; tile >= t0; --tile) {
+        const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
+        float a[K][VEC], m[K][VEC], e[VEC], hs[VEC];
+        Piece<T, VEC> xr[K], gyr[K];
+        {
+            Piece<T, VEC> gr[K];
+            load_steps<T, VEC, K>(x, p.xs.t, s0, len, p.reverse, at.on, xr);
+            load_steps<T, VEC, K>(g, p.gs.t, s0, len, p.reverse, at.on, gr);
+            load_steps<T, VEC, K>(gy, p.dense.t, s0, len, p.reverse, at.on && p.gy, gyr);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                gates<T, VEC>(gr[k], a[k], m[k]);
+                if (!(s0 + k < len)) {
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, m[k][v] = 0.f;
+                }
+            }
+        }
+        Maps<VEC> back;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) back.a[v] = 1.f, back.b[v] = 0.f;
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                back.b[v] = a[k][v] * (to_f32(gyr[k].v[v]) + back.b[v]), back.a[v] *= a[k][v];
+        scan_tile<VEC, LC, NW, true>(back, carry, e, lds[tile & 1][0], at.lane, at.wave);
+        Maps<VEC> fore;
+        float h[VEC];
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+            fore.a[v] = back.a[v], fore.b[v] = 0.f;
+            h[v] = at.on ? p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v)
+                fore.b[v] = __builtin_fmaf(a[k][v], fore.b[v], m[k][v] * to_f32(xr[k].v[v]));
+        scan_tile<VEC, LC, NW, false>(fore, h, hs, lds[tile & 1][1], at.lane, at.wave);
+        float hp[K][VEC];
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                hp[k][v] = hs[v];
+                hs[v] = __builtin_fmaf(a[k][v], hs[v], m[k][v] * to_f32(xr[k].v[v]));
+            }
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) {
+            float ox[VEC], og[VEC];
+            const bool valid = s0 + k < len;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const float d = to_f32(gyr[k].v[v]) + e[v];
+                ox[v] = valid ? d * m[k][v] : 0.f;
+                og[v] = valid ? d * (hp[k][v] - to_f32(xr[k].v[v])) * (a[k][v] * m[k][v]) : 0.f;
+                e[v] = a[k][v] * d;
+            }
+            if (at.on && s0 + k < p.T) {
+                const long long t = scan_pos(s0 + k, len, p.reverse);
+                if (p.gx) store_any<T, VEC>(gx + t * p.gxs.t, ox);
+                if (p.gg) store_any<T, VEC>(gg + t * p.ggs.t, og);
+            }
+        }
+    }
+    if (p.gh0 && seg == 0 && at.on && at.sub == 0) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p.gh0[row + v] = carry[v];
+    }
+}
+
+enum ScanPass { kScanForward, kScanBackward };
+
+// Wavefronts of a workgroup: as few as have a short chain in one tile, and up to eight.  Steps of a lane: eight forward; four
+// backward, where three tensors and two scans are held (with eight: 370 bytes a lane spilled).
+constexpr int kForwardSteps = 8, kBackwardSteps = 4;
+inline int scan_waves(long long T, int I) {
+    if (I < 4) return 4;
+    return T <= 32 ? 1 : T <= 64 ? 2 : T <= 128 ? 4 : 8;
+}
+inline int scan_lanes(int I) { return I < 4 ? 4 : 16; }          // LC
+inline int scan_width(int I) { return I < 4 ? 4 : 64; }          // channels of a strip
+inline int scan_tile_steps(long long T, int I, ScanPass pass) {
+    return scan_waves(T, I) * (64 / scan_lanes(I)) * (pass == kScanForward ? kForwardSteps : kBackwardSteps);
+}
+
+template <typename T, int VEC, int LC, int NW>
+void scan_launch(const ScanArgs& p, ScanPass pass, hipStream_t s) {
+    const unsigned columns = (unsigned)p.strips * (unsigned)p.rows;
+    if (p.segments > 1) {
+        const unsigned n = columns * (unsigned)(p.segments - 1);
+        if (pass == kScanForward) scan_maps_k<T, VEC, LC, NW, kForwardSteps, false><<<n, NW * 64, 0, s>>>(p);
+        else scan_maps_k<T, VEC, LC, NW, kBackwardSteps, true><<<n, NW * 64, 0, s>>>(p);
+    }
+    const unsigned n = columns * (unsigned)p.segments;
+    if (pass == kScanForward) scan_fwd_k<T, VEC, LC, NW, kForwardSteps><<<n, NW * 64, 0, s>>>(p);
+    else scan_bwd_k<T, VEC, LC, NW, kBackwardSteps><<<n, NW * 64, 0, s>>>(p);
+}
+
+template <typename T>
+void scan_dispatch(const ScanArgs& p, ScanPass pass, hipStream_t s) {
+    if (p.I < 4) return scan_launch<T, 1, 4, 4>(p, pass, s);
+    switch (scan_waves(p.T, p.I)) {
+        case 1: return scan_launch<T, 4, 16, 1>(p, pass, s);
+        case 2: return scan_launch<T, 4, 16, 2>(p, pass, s);
+        case 4: return scan_launch<T, 4, 16, 4>(p, pass, s);
+        default: return scan_launch<T, 4, 16, 8>(p, pass, s);
+    }
+}
+
+}  // namespace pdw

@@ -1,0 +1,6 @@
+// The gated linear recurrence (scan.h) on f16 tensors.
+#include "scan.h"
+
+namespace pdw {
+void scan_launch_f16(const ScanArgs& p, ScanPass pass, hipStream_t s) { scan_dispatch<f16_t>(p, pass, s); }
+}  // namespace pdw

@@ -3,80 +3,13 @@
 // training step of a block cost 250-900 us of host time (one interpreter-level call per launch, 10-20 us each, where the
 // library's kernels run 3-30 us each); a Node here is entered by the autograd engine without the interpreter lock.
 // Plain C++ (no device code): built with the host compiler against torch's headers and linked to libpdw.so beside it.
-#include <Python.h>
+#include "torch_node.h"
 
-#include <ATen/ATen.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-#include <torch/csrc/autograd/function.h>
-#include <torch/csrc/autograd/functions/utils.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-
-#include "../../include/pdw.h"
+PyMethodDef* pdw_mixer_methods();   // torch_mixer.cpp
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::SavedVariable;
-using torch::autograd::variable_list;
-
-int dtype_code(at::ScalarType t) {
-    switch (t) {
-        case at::kFloat: return PDW_F32;
-        case at::kHalf: return PDW_F16;
-        case at::kBFloat16: return PDW_BF16;
-        default: return -1;
-    }
-}
-
-void check(int status, const char* what) {
-    TORCH_CHECK(status == 0, what, ": ", pdw_last_error(), " (status ", status, ")");
-}
-
-void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
-
-// Contiguous and 16-byte aligned (the kernels move 16-byte pieces; a view at an odd storage offset is copied).
-Tensor dense(const Tensor& t) {
-    Tensor c = t.is_contiguous() ? t : t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone(at::MemoryFormat::Contiguous);
-}
-
-// What a node keeps of an input: the input itself where it went to the kernels as it is, so that a later change of it in
-// place is noticed, else the copy that they read.
-SavedVariable save(const Tensor& in, const Tensor& read) { return SavedVariable(read.is_same(in) ? in : read, false); }
-
-// What a node has saved, as it comes back: a saved-tensor hook may have put another tensor in its place, and the kernels
-// take addresses.  (Of another type: converted.)
-Tensor restored(const SavedVariable& v, const std::shared_ptr<torch::autograd::Node>& node, at::IntArrayRef sizes,
-                at::ScalarType type, c10::Device device) {
-    Tensor t = v.unpack(node);
-    TORCH_CHECK(t.defined() && t.sizes() == sizes && t.device() == device, node->name(),
-                ": a saved tensor came back as another one (", sizes, " on ", device, " was saved)");
-    return t.scalar_type() == type ? t : t.to(type);
-}
-
-// The gradient of a node's only output; zeros where the engine has none (a later node's backward returned none), as
-// torch.autograd.Function gives them, so that inputs and parameters get gradients of zero and not none.
-Tensor output_gradient(const torch::autograd::Node& node, const variable_list& grads) {
-    return grads[0].defined() ? grads[0] : node.input_metadata(0).zeros_like();
-}
-
-void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-
-Tensor bytes(size_t n, const Tensor& like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
-
-// Whether a call belongs to the nodes below.  They have no forward-mode derivative and no batching rule, so such calls go
-// on to the torch.autograd.Function forms, which refuse them; and a trace (torch.jit.trace) would record of them the
-// allocation of the result alone, where a Function becomes a node of the graph that calls it again.
-bool plain_call(const Tensor* in, int n) {
-    if (torch::jit::tracer::isTracing()) return false;
-    if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode)) return false;
-    for (int i = 0; i < n; ++i)
-        if (in[i].defined() && in[i]._fw_grad(0).defined()) return false;
-    return true;
-}
+using namespace pdw_torch;
 
 // ---------------------------------------------------------------------------------------------------------------
 // The block
@@ -285,16 +218,6 @@ Tensor conv_forward(const Tensor& x, const Tensor& w, const ConvGeo& g) {
 // ---------------------------------------------------------------------------------------------------------------
 // Python entry points
 
-bool tensor_arg(PyObject* o, Tensor* t) {
-    if (o == Py_None) return true;
-    if (!THPVariable_Check(o)) {
-        PyErr_Format(PyExc_TypeError, "expected a Tensor or None, got %s", Py_TYPE(o)->tp_name);
-        return false;
-    }
-    *t = THPVariable_Unpack(o);
-    return true;
-}
-
 // block(x, w_up, b_up, w_out, b_out, w_pool, b_pool, w_dw0, w_dw1, s0, s1): the block's output; None where ConvBlockFunction
 // has to answer (a case that the library's block calls do not cover, a transform, a trace); True where no gradient is wanted and its inference call (block_infer) covers it.
 PyObject* py_block(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -388,4 +311,11 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_pdw_torch", nullptr, -1, kMethod
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__pdw_torch(void) { return PyModule_Create(&kModule); }
+PyMODINIT_FUNC PyInit__pdw_torch(void) {
+    PyObject* m = PyModule_Create(&kModule);
+    if (m && PyModule_AddFunctions(m, pdw_mixer_methods()) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

@@ -451,3 +451,131 @@ def pool_branch_backward(gy, m, w_pool, parts=None):
             gbias[1].data_ptr(), gwp.data_ptr(), dmean.data_ptr(), ws.data_ptr(), ws.numel() * 4, B, P, D,
             _lib.dtype_code(gy.dtype))
     return gbias, gwp, dmean
+
+
+# Norms over channels, the gated residual and the gated scan (channel_norm, gated_residual and gated_scan check their
+# arguments; these take dense tensors and make the call).
+
+NORM_KINDS = {"none": 0, "rms": 1, "layer": 2}
+ACTIVATIONS = {"none": 0, "sigmoid": 1, "silu": 2}
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _bytes(n, dev):
+    return torch.empty(max(int(n), 4), device=dev, dtype=torch.uint8)
+
+
+def norm_forward(x, weight, bias, kind, eps, stats=False):
+    """-> (norm of x [..., C], (mean, 1 / deviation) of each row [N, 2] fp32 or None); kind: a value of NORM_KINDS."""
+    dev = _lib.require_device(x)
+    C = x.shape[-1]
+    N = x.numel() // C
+    y = torch.empty_like(x)
+    st = torch.empty((N, 2), device=dev, dtype=torch.float32) if stats else None
+    if N:
+        _launch("pdw_norm_fwd", dev, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(st), N, C, kind, float(eps),
+                _lib.dtype_code(x.dtype))
+    return y, st
+
+
+def norm_backward(gy, x, weight, stats, kind, has_bias):
+    """-> (gx, gweight or None, gbias or None)."""
+    dev = _lib.require_device(gy, x)
+    C = x.shape[-1]
+    N = x.numel() // C
+    code = _lib.dtype_code(x.dtype)
+    gx = torch.empty_like(x)
+    gw = None if weight is None else torch.zeros_like(weight)
+    gb = x.new_zeros(C) if has_bias else None
+    if N:
+        ws = _bytes(_lib.lib().pdw_norm_bwd_workspace_bytes(N, C, code), dev)
+        _launch("pdw_norm_bwd", dev, gy.data_ptr(), x.data_ptr(), _ptr(weight), stats.data_ptr(), gx.data_ptr(), _ptr(gw),
+                _ptr(gb), ws.data_ptr(), ws.numel(), N, C, kind, code)
+    return gx, gw, gb
+
+
+def _gate_rows(x, gate):
+    """Rows of x that a row of the gate serves."""
+    return 1 if gate is None or gate.shape == x.shape else max(x.numel() // max(gate.numel(), 1), 1)
+
+
+def residual_forward(x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps, stats=False):
+    """-> (out, next or None, rows' statistics of y or None)."""
+    dev = _lib.require_device(x, y)
+    C = x.shape[-1]
+    N = x.numel() // C
+    out, nxt = torch.empty_like(x), torch.empty_like(x) if next_kind else None
+    st = torch.empty((N, 2), device=dev, dtype=torch.float32) if stats and kind else None
+    if N:
+        _launch("pdw_residual_fwd", dev, x.data_ptr(), y.data_ptr(), _ptr(gate), _ptr(scale), _ptr(weight), _ptr(bias),
+                _ptr(next_weight), _ptr(next_bias), out.data_ptr(), _ptr(nxt), _ptr(st), N, C, _gate_rows(x, gate), 0,
+                act, kind, next_kind, float(eps), _lib.dtype_code(x.dtype))
+    return out, nxt, st
+
+
+def residual_backward(gout, gnext, out, y, gate, scale, weight, bias, next_weight, has_next_bias, stats, act, kind, next_kind,
+                      eps):
+    """-> gradients of (x, y, gate, scale, weight, bias, next_weight, next_bias), None for what there was none of."""
+    dev = _lib.require_device(y)
+    C = y.shape[-1]
+    N = y.numel() // C
+    code = _lib.dtype_code(y.dtype)
+    zeros = lambda t: None if t is None else torch.zeros(t.shape, device=dev, dtype=t.dtype)
+    gx, gy, gg = torch.empty_like(y) if next_kind else gout, torch.empty_like(y), zeros(gate)
+    gs, gw, gb, gnw = zeros(scale), zeros(weight), zeros(bias), zeros(next_weight)
+    gnb = y.new_zeros(C) if has_next_bias else None
+    if N:
+        P = _gate_rows(y, gate)
+        ws = _bytes(_lib.lib().pdw_residual_bwd_workspace_bytes(N, C, P, next_kind, code), dev)
+        _launch("pdw_residual_bwd", dev, _ptr(gout), _ptr(gnext), _ptr(out), y.data_ptr(), _ptr(gate), _ptr(scale), _ptr(weight),
+                _ptr(bias), _ptr(next_weight), _ptr(stats), float(eps), gx.data_ptr() if next_kind else None, gy.data_ptr(),
+                _ptr(gg), _ptr(gs), _ptr(gw), _ptr(gb), _ptr(gnw), _ptr(gnb), ws.data_ptr(), ws.numel(), N, C, P, 0, act, kind,
+                next_kind, code)
+    return gx, gy, gg, gs, gw, gb, gnw, gnb
+
+
+def _scan_extents(x, dim):
+    O = T = W = 1
+    for d, n in enumerate(x.shape[:-1]):
+        O, T, W = (O * n, T, W) if d < dim else (O, n, W) if d == dim else (O, T, W * n)
+    return O, T, W * x.shape[-1]
+
+
+def _scan_strides(T, I):
+    from ctypes import c_longlong
+
+    return (c_longlong * 3)(T * I, I, I)
+
+
+def scan_forward(x, g, state, lengths, dim, reverse, states=False):
+    """Dense x, g [..., T, ..., C], the recurrence along `dim` -> (y, last state fp32, what the backward needs or None)."""
+    dev = _lib.require_device(x, g)
+    O, T, I = _scan_extents(x, dim)
+    y = torch.empty_like(x)
+    last = torch.empty(x.shape[:dim] + x.shape[dim + 1:], device=dev, dtype=torch.float32)
+    L = _lib.lib()
+    st = _bytes(L.pdw_scan_states_bytes(O, T, 1, I), dev) if states else None
+    if O and I:
+        ws = _bytes(L.pdw_scan_workspace_bytes(O, T, 1, I, 0), dev)
+        s = _scan_strides(T, I)
+        _launch("pdw_scan_fwd", dev, x.data_ptr(), g.data_ptr(), _ptr(state), _ptr(lengths), y.data_ptr(), last.data_ptr(), _ptr(st),
+                ws.data_ptr(), ws.numel(), O, T, 1, I, s, s, int(bool(reverse)), _lib.dtype_code(x.dtype))
+    return y, last, st
+
+
+def scan_backward(gy, glast, x, g, lengths, states, dim, reverse):
+    """-> gradients of (x, g, the initial state)."""
+    dev = _lib.require_device(x, g)
+    O, T, I = _scan_extents(x, dim)
+    gx, gg = torch.empty_like(x), torch.empty_like(g)
+    gstate = torch.empty(x.shape[:dim] + x.shape[dim + 1:], device=dev, dtype=torch.float32)
+    if O and I:
+        ws = _bytes(_lib.lib().pdw_scan_workspace_bytes(O, T, 1, I, 1), dev)
+        s = _scan_strides(T, I)
+        _launch("pdw_scan_bwd", dev, _ptr(gy), _ptr(glast), x.data_ptr(), g.data_ptr(), _ptr(lengths), states.data_ptr(),
+                gx.data_ptr(), gg.data_ptr(), gstate.data_ptr(), ws.data_ptr(), ws.numel(), O, T, 1, I, s, s, s, s,
+                int(bool(reverse)), _lib.dtype_code(x.dtype))
+    return gx, gg, gstate
