@@ -498,17 +498,19 @@ int pdw_norm_bwd(const void *gy, const void *x, const void *weight, const float 
 
 /* out = x + scale * act(gate) * norm(y), and with next_kind other than PDW_NORM_NONE also next = norm'(out), the norm before
  * the block that follows (of out as it is before rounding).  gate: NULL; one row for P consecutive rows of x (an image's; N must be a
- * multiple of P); with P = 1 a value for each.  Gate rows are ldgate elements apart (0: C).  stats: y's. */
+ * multiple of P); with P = 1 a value for each.  Gate rows are ldgate elements apart (0: C).  stats, next_stats: of y and of out. */
 int pdw_residual_fwd(const void *x, const void *y, const void *gate, const void *scale, const void *weight, const void *bias,
-                     const void *next_weight, const void *next_bias, void *out, void *next, float *stats, long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
+                     const void *next_weight, const void *next_bias, void *out, void *next, float *stats, float *next_stats,
+                     long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
                      void *stream);
-/* The gradients, from those of out (gout) and next (gnext), either of which may be NULL (0).  `out` is the forward's result (read only
- * with a next norm, whose statistics are taken again, of out as it was stored).  gx [N][C] is written only with a next norm (without one it is gout itself); ggate like gate, dense.  Each result
+/* The gradients, from those of out (gout) and next (gnext), either of which may be NULL (0).  x is read only
+ * with a next norm.  gx [N][C] is written only with a next norm (without one it is gout itself); ggate like gate, dense.  Each result
  * may be NULL (not wanted).  Workspace: needed where any of ggate (with P > 1), gscale, gweight, gbias, gnext_weight, gnext_bias is
  * wanted. */
 size_t pdw_residual_bwd_workspace_bytes(long long N, int C, long long P, int next_kind, int dtype);
-int pdw_residual_bwd(const void *gout, const void *gnext, const void *out, const void *y, const void *gate, const void *scale,
-                     const void *weight, const void *bias, const void *next_weight, const float *stats, float eps, void *gx, void *gy, void *ggate, void *gscale, void *gweight, void *gbias, void *gnext_weight,
+int pdw_residual_bwd(const void *gout, const void *gnext, const void *x, const void *y, const void *gate, const void *scale,
+                     const void *weight, const void *bias, const void *next_weight, const float *stats, const float *next_stats,
+                     void *gx, void *gy, void *ggate, void *gscale, void *gweight, void *gbias, void *gnext_weight,
                      void *gnext_bias, void *workspace, size_t workspace_bytes, long long N, int C, long long P,
                      long long ldgate, int act, int kind, int next_kind, int dtype, void *stream);
 

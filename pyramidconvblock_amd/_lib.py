@@ -106,10 +106,10 @@ _SIGS = {
     "pdw_norm_fwd": (c_int, [c_void_p] * 5 + [c_longlong, c_int, c_int, c_float, c_int, c_void_p]),
     "pdw_norm_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int, c_int]),
     "pdw_norm_bwd": (c_int, [c_void_p] * 8 + [c_size_t, c_longlong] + [c_int] * 3 + [c_void_p]),
-    "pdw_residual_fwd": (c_int, [c_void_p] * 11 + [c_longlong, c_int, c_longlong, c_longlong] + [c_int] * 3
+    "pdw_residual_fwd": (c_int, [c_void_p] * 12 + [c_longlong, c_int, c_longlong, c_longlong] + [c_int] * 3
                          + [c_float, c_int, c_void_p]),
     "pdw_residual_bwd_workspace_bytes": (c_size_t, [c_longlong, c_int, c_longlong, c_int, c_int]),
-    "pdw_residual_bwd": (c_int, [c_void_p] * 10 + [c_float] + [c_void_p] * 9 + [c_size_t, c_longlong, c_int, c_longlong, c_longlong] + [c_int] * 4
+    "pdw_residual_bwd": (c_int, [c_void_p] * 20 + [c_size_t, c_longlong, c_int, c_longlong, c_longlong] + [c_int] * 4
                          + [c_void_p]),
     "pdw_scan_states_bytes": (c_size_t, [c_int, c_longlong, c_int, c_int]),
     "pdw_scan_workspace_bytes": (c_size_t, [c_int, c_longlong, c_int, c_int, c_int]),

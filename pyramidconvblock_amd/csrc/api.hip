@@ -806,14 +806,15 @@ int pdw_norm_bwd(const void* gy, const void* x, const void* weight, const float*
 }
 
 int pdw_residual_fwd(const void* x, const void* y, const void* gate, const void* scale, const void* weight, const void* bias,
-                     const void* next_weight, const void* next_bias, void* out, void* next, float* stats, long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
+                     const void* next_weight, const void* next_bias, void* out, void* next, float* stats, float* next_stats,
+                     long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
                      void* stream) {
     if (int e = check_rows("pdw_residual_fwd", N, C, kind, next_kind, act, dtype)) return e;
     if (int e = check_gate("pdw_residual_fwd", gate, N, C, P, &ldgate)) return e;
     if (N > 0 && (!x || !y || !out || (next_kind != kNormNone && !next))) return set_error("pdw_residual_fwd: null pointer"), 1;
     RowArgs p{};
     p.x = x, p.y = y, p.gate = gate, p.scale = scale, p.w = weight, p.b = bias, p.w2 = next_weight, p.b2 = next_bias;
-    p.out = out, p.next = next, p.st = stats, p.N = N, p.P = P, p.ldg = ldgate, p.C = C;
+    p.out = out, p.next = next, p.st = stats, p.st2 = next_stats, p.N = N, p.P = P, p.ldg = ldgate, p.C = C;
     p.act = act, p.kind = kind, p.kind2 = next_kind, p.gate_rows = !gate ? 0 : P == 1 ? 2 : 1, p.eps = eps;
     return rows_forward_launch(p, dtype, (hipStream_t)stream);
 }
@@ -824,18 +825,19 @@ size_t pdw_residual_bwd_workspace_bytes(long long N, int C, long long P, int nex
     return rows_backward_workspace(N, P > 1 && N % P == 0 ? N / P : 1, C, next_kind == kNormNone ? 2 : 4, dtype);
 }
 
-int pdw_residual_bwd(const void* gout, const void* gnext, const void* out, const void* y, const void* gate, const void* scale,
-                     const void* weight, const void* bias, const void* next_weight, const float* stats, float eps, void* gx, void* gy, void* ggate, void* gscale, void* gweight, void* gbias, void* gnext_weight,
+int pdw_residual_bwd(const void* gout, const void* gnext, const void* x, const void* y, const void* gate, const void* scale,
+                     const void* weight, const void* bias, const void* next_weight, const float* stats, const float* next_stats,
+                     void* gx, void* gy, void* ggate, void* gscale, void* gweight, void* gbias, void* gnext_weight,
                      void* gnext_bias, void* workspace, size_t workspace_bytes, long long N, int C, long long P,
                      long long ldgate, int act, int kind, int next_kind, int dtype, void* stream) {
     if (int e = check_rows("pdw_residual_bwd", N, C, kind, next_kind, act, dtype)) return e;
     if (int e = check_gate("pdw_residual_bwd", gate, N, C, P, &ldgate)) return e;
     const bool next = next_kind != kNormNone;
-    if (N > 0 && (!y || (kind != kNormNone && !stats) || (next && !out) || (!gate && ggate)))
+    if (N > 0 && (!y || (kind != kNormNone && !stats) || (next && (!x || !next_stats)) || (!gate && ggate)))
         return set_error("pdw_residual_bwd: null pointer"), 1;
     RowArgs p{};
-    p.go = gout, p.gz = gnext, p.x = out, p.y = y, p.gate = gate, p.scale = scale, p.w = weight, p.b = bias, p.w2 = next_weight;
-    p.st = const_cast<float*>(stats), p.eps = eps, p.gx = next ? gx : nullptr, p.gy = gy, p.ggate = ggate;
+    p.go = gout, p.gz = gnext, p.x = x, p.y = y, p.gate = gate, p.scale = scale, p.w = weight, p.b = bias, p.w2 = next_weight;
+    p.st = const_cast<float*>(stats), p.st2 = const_cast<float*>(next_stats), p.gx = next ? gx : nullptr, p.gy = gy, p.ggate = ggate;
     p.N = N, p.P = P, p.ldg = ldgate, p.C = C, p.act = act, p.kind = kind, p.kind2 = next_kind;
     p.gate_rows = !gate ? 0 : P == 1 ? 2 : 1;
     return rows_backward_launch(p, gscale, gweight, gbias, gnext_weight, gnext_bias, workspace, workspace_bytes, dtype,

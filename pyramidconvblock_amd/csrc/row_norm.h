@@ -6,6 +6,8 @@
 //             of its weight and bias the sums over rows of t n and t.  Of the residual, with g = out's gradient:
 //             S1 = sum g act n and S0 = sum g act give scale's gradient w S1 + b S0, w's scale S1 and b's scale S0, so two column
 //             sums serve all three; with a gate row for each image the sums are kept by image and give the gate's gradient too.
+//             The backward makes out again from x and y (y it reads anyway): read back as it was stored, its rounding would be in
+//             every gradient (0.0027 off the exact ones in bf16, 0.0017 this way; one rounding of a result is 0.0017).
 //
 // Every kernel is bound by memory: it reads each tensor once and writes each once.  A row belongs to TPR neighbouring lanes (a
 // power of two up to a wavefront, so that several short rows share one, or a workgroup of 256), each holding NCH pieces of VEC
@@ -25,9 +27,9 @@ namespace pdw {
 enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 
 struct RowArgs {
-    const void *x, *y, *gate, *scale, *w, *b, *w2, *b2;  // forward inputs (backward: x is out where there is a next norm)
+    const void *x, *y, *gate, *scale, *w, *b, *w2, *b2;  // forward inputs
     void *out, *next;
-    float *st, *st2;                                     // (mean, rstd) of each row: of y; of x, for the norm by itself
+    float *st, *st2;                                     // (mean, rstd) of each row: of y, and of the next norm's input
     const void *go, *gz;                                 // gradients of out and next (either may be null)
     void *gx, *gy, *ggate;
     float* parts;                                        // column sums of a segment: [segment][sums][C]
@@ -160,6 +162,11 @@ __device__ __forceinline__ void row_stats(const float (&v)[NCH][VEC], const COLS
     rstd = 1.f / sqrtf(q / (float)C + eps);
 }
 
+// x + f * norm(y), y's mean and reciprocal deviation in st.
+__device__ __forceinline__ float residual_sum(float x, float f, float y, float2 st, float w, float b) {
+    return __builtin_fmaf(f, __builtin_fmaf((y - st.x) * st.y, w, b), x);
+}
+
 // BRANCH: the residual (otherwise the norm by itself, of x); NEXT: the norm of the sum.
 template <typename T, int VEC, int TPR, int NCH, bool RAG, bool BRANCH, bool NEXT>
 __global__ __launch_bounds__(256) void rows_fwd_k(RowArgs p) {
@@ -204,10 +211,9 @@ __global__ __launch_bounds__(256) void rows_fwd_k(RowArgs p) {
             for (int n = 0; n < NCH; ++n) {
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
-                    const float t = __builtin_fmaf((v[n][i] - mean) * rstd, to_f32(w[n].v[i]), to_f32(b[n].v[i]));
                     float fi = f[n][i];
                     if (p.gate_rows == 2) fi *= gate_act(to_f32(gr[n].v[i]), p.act);
-                    v[n][i] = __builtin_fmaf(fi, t, to_f32(xr[n].v[i]));
+                    v[n][i] = residual_sum(to_f32(xr[n].v[i]), fi, v[n][i], make_float2(mean, rstd), to_f32(w[n].v[i]), to_f32(b[n].v[i]));
                 }
                 cols.store((T*)p.out + r * p.C, n, v[n]);
             }
@@ -307,30 +313,27 @@ __global__ __launch_bounds__(256) void rows_bwd_k(RowArgs p) {
             cols.load((const T*)p.y + r * p.C, yr);
             if (p.gate_rows == 2) cols.load((const T*)p.gate + r * p.ldg, gr);
         }
+        float2 sty = make_float2(0.f, 1.f);
+        if (BRANCH && p.kind != kNormNone) sty = reinterpret_cast<const float2*>(p.st)[r];
 #pragma unroll
         for (int n = 0; n < NCH; ++n)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) go[n][i] = to_f32(gor[n].v[i]);
         if (NEXT) {
-            // Of a residual the statistics are taken again, of the sum as it was stored: with those from before its rounding a row
-            // whose deviation is as small as that rounding would be centred wrong by a multiple of its deviation.
-            float2 st;
-            if (BRANCH) {
-#pragma unroll
-                for (int n = 0; n < NCH; ++n)
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) nv[n][i] = to_f32(xr[n].v[i]);
-                row_stats<VEC, TPR, NCH>(nv, cols, p.C, p.kind2, p.eps, st.x, st.y, red, flip);
-            } else {
-                st = reinterpret_cast<const float2*>(p.st2)[r];
-            }
+            const float2 st = reinterpret_cast<const float2*>(p.st2)[r];
             float a1 = 0.f, a0 = 0.f;
 #pragma unroll
             for (int n = 0; n < NCH; ++n)
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) {
                     const float gz = to_f32(gzr[n].v[i]);
-                    nv[n][i] = (to_f32(xr[n].v[i]) - st.x) * st.y;
+                    float v = to_f32(xr[n].v[i]);
+                    if (BRANCH) {   // the sum as the forward had it
+                        float fi = f[n][i];
+                        if (p.gate_rows == 2) fi *= gate_act(to_f32(gr[n].v[i]), p.act);
+                        v = residual_sum(v, fi, to_f32(yr[n].v[i]), sty, to_f32(w[n].v[i]), to_f32(b[n].v[i]));
+                    }
+                    nv[n][i] = (v - st.x) * st.y;
                     un[n][i] = gz * to_f32(w2[n].v[i]);
                     const bool mine = cols.mine(n, i);
                     a1 += mine ? un[n][i] * nv[n][i] : 0.f, a0 += mine ? un[n][i] : 0.f;
@@ -347,8 +350,7 @@ __global__ __launch_bounds__(256) void rows_bwd_k(RowArgs p) {
             }
         }
         if (BRANCH) {
-            float2 st = make_float2(0.f, 1.f);
-            if (p.kind != kNormNone) st = reinterpret_cast<const float2*>(p.st)[r];
+            const float2 st = sty;
             float a1 = 0.f, a0 = 0.f;
 #pragma unroll
             for (int n = 0; n < NCH; ++n) {

@@ -70,7 +70,6 @@ struct Kept {
         if (!read.defined()) return;
         v = save(in, read), sizes = read.sizes(), there = true;
     }
-    void keep_output(const Tensor& out) { v = SavedVariable(out, true), sizes = out.sizes(), there = true; }
     Tensor get(const std::shared_ptr<torch::autograd::Node>& node, at::ScalarType type, c10::Device device) const {
         return there ? restored(v, node, sizes, type, device) : Tensor();
     }
@@ -176,15 +175,14 @@ Tensor gate_rows(const Tensor& gate, int C, int64_t* ld) {
 }
 
 struct ResidualNode : public torch::autograd::Node {
-    Kept out, y, gate, scale, weight, next_weight, bias, stats;
+    Kept x, y, gate, scale, weight, next_weight, bias, stats, next_stats;
     ResidualShape s;
-    double eps;
     bool has_next_bias;
 
     std::string name() const override { return "GatedResidualBackward"; }
     void release_variables() override {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (Kept* k : {&out, &y, &gate, &scale, &weight, &next_weight, &bias, &stats}) k->v.reset_data();
+        for (Kept* k : {&x, &y, &gate, &scale, &weight, &next_weight, &bias, &stats, &next_stats}) k->v.reset_data();
     }
 
     variable_list apply(variable_list&& grads) override {
@@ -198,10 +196,10 @@ struct ResidualNode : public torch::autograd::Node {
         const auto type = some.scalar_type();
         const auto dev = some.device();
         auto take = [&](const Kept& k) { return k.get(self, type, dev); };
-        Tensor o = take(out), yv = take(y), q = take(gate), sc = take(scale), w = take(weight), nw = take(next_weight), b = take(bias);
-        Tensor st = stats.get(self, at::kFloat, dev);
+        Tensor xv = take(x), yv = take(y), q = take(gate), sc = take(scale), w = take(weight), nw = take(next_weight), b = take(bias);
+        Tensor st = stats.get(self, at::kFloat, dev), nst = next_stats.get(self, at::kFloat, dev);
         at::AutoDispatchBelowADInplaceOrView below;
-        for (Tensor* t : {&o, &yv, &sc, &w, &nw, &b, &st}) *t = packed(*t);
+        for (Tensor* t : {&xv, &yv, &sc, &w, &nw, &b, &st, &nst}) *t = packed(*t);
         q = gate_rows(q, s.C, &s.ldgate);
         const Tensor go = packed(gout), gn = packed(gnext);
         const c10::DeviceGuard guard(dev);
@@ -220,8 +218,8 @@ struct ResidualNode : public torch::autograd::Node {
         bool sums = s.P > 1 && r[kRGate].defined();
         for (int i : {kRScale, kRWeight, kRBias, kRNextWeight, kRNextBias}) sums = sums || r[i].defined();
         if (sums) ws = bytes(pdw_residual_bwd_workspace_bytes(s.N, s.C, s.P, s.next_kind, s.dtype), yv);
-        check(pdw_residual_bwd(ptr(go), ptr(gn), ptr(o), ptr(yv), ptr(q), ptr(sc), ptr(w), ptr(b), ptr(nw), (const float*)ptr(st),
-                               (float)eps, next ? ptr(r[kRX]) : nullptr, ptr(r[kRY]), ptr(r[kRGate]), ptr(r[kRScale]),
+        check(pdw_residual_bwd(ptr(go), ptr(gn), ptr(xv), ptr(yv), ptr(q), ptr(sc), ptr(w), ptr(b), ptr(nw), (const float*)ptr(st),
+                               (const float*)ptr(nst), next ? ptr(r[kRX]) : nullptr, ptr(r[kRY]), ptr(r[kRGate]), ptr(r[kRScale]),
                                ptr(r[kRWeight]), ptr(r[kRBias]), ptr(r[kRNextWeight]), ptr(r[kRNextBias]), ptr(ws),
                                ws.defined() ? ws.numel() : 0, s.N, s.C, s.P, s.ldgate, s.act, s.kind, s.next_kind, s.dtype, stream_of(yv)),
               "pdw_residual_bwd");
@@ -232,7 +230,7 @@ struct ResidualNode : public torch::autograd::Node {
 void residual_forward(const Tensor* in, ResidualShape s, double eps, bool grad, Tensor* out, Tensor* next) {
     const c10::DeviceGuard guard(in[kRX].device());
     const bool norm = s.kind != PDW_NORM_NONE, nnorm = s.next_kind != PDW_NORM_NONE;
-    Tensor d[kResidualInputs], stats;
+    Tensor d[kResidualInputs], stats, next_stats;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         for (int i = 0; i < kResidualInputs; ++i) d[i] = i == kRGate ? gate_rows(in[i], s.C, &s.ldgate) : packed(in[i]);
@@ -240,9 +238,11 @@ void residual_forward(const Tensor* in, ResidualShape s, double eps, bool grad, 
         *out = at::empty(x.sizes(), x.options());
         if (nnorm) *next = at::empty(x.sizes(), x.options());
         if (grad && norm) stats = floats({s.N, 2}, x);
+        if (grad && nnorm) next_stats = floats({s.N, 2}, x);
         if (s.N)
             check(pdw_residual_fwd(ptr(x), ptr(d[kRY]), ptr(d[kRGate]), ptr(d[kRScale]), ptr(d[kRWeight]), ptr(d[kRBias]),
-                                   ptr(d[kRNextWeight]), ptr(d[kRNextBias]), ptr(*out), ptr(*next), (float*)ptr(stats), s.N, s.C, s.P, s.ldgate, s.act, s.kind, s.next_kind, (float)eps, s.dtype,
+                                   ptr(d[kRNextWeight]), ptr(d[kRNextBias]), ptr(*out), ptr(*next), (float*)ptr(stats),
+                                   (float*)ptr(next_stats), s.N, s.C, s.P, s.ldgate, s.act, s.kind, s.next_kind, (float)eps, s.dtype,
                                    stream_of(x)),
                   "pdw_residual_fwd");
     }
@@ -253,13 +253,11 @@ void residual_forward(const Tensor* in, ResidualShape s, double eps, bool grad, 
         auto keep = [&](Kept& k, int i) { k.keep(in[i], d[i]); };
         keep(node->y, kRY), keep(node->gate, kRGate), keep(node->scale, kRScale), keep(node->weight, kRWeight);
         keep(node->bias, kRBias), keep(node->next_weight, kRNextWeight);
-        node->stats.keep(stats, stats);
-        node->s = s, node->eps = eps, node->has_next_bias = in[kRNextBias].defined();
+        if (nnorm) keep(node->x, kRX);
+        node->stats.keep(stats, stats), node->next_stats.keep(next_stats, next_stats);
+        node->s = s, node->has_next_bias = in[kRNextBias].defined();
         torch::autograd::set_history(*out, node);
-        if (nnorm) {
-            torch::autograd::set_history(*next, node);
-            node->out.keep_output(*out);
-        }
+        if (nnorm) torch::autograd::set_history(*next, node);
     }
 }
 

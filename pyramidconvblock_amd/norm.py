@@ -65,17 +65,17 @@ class GatedResidualFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps):
         x, *rest = (_dense(t) for t in (x, y, gate, scale, weight, bias, next_weight, next_bias))
-        out, nxt, stats = ops.residual_forward(x, *rest, act, kind, next_kind, eps, stats=True)
-        ctx.codes, ctx.has_next_bias = (act, kind, next_kind, eps), next_bias is not None
-        ctx.save_for_backward(out if next_kind else None, *rest[:-1], stats)
+        out, nxt, stats, next_stats = ops.residual_forward(x, *rest, act, kind, next_kind, eps, stats=True)
+        ctx.codes, ctx.has_next_bias = (act, kind, next_kind), next_bias is not None
+        ctx.save_for_backward(x if next_kind else None, *rest[:-1], stats, next_stats)
         return out if nxt is None else (out, nxt)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout, gnext=None):
-        out, *rest, stats = ctx.saved_tensors
+        x, *rest, stats, next_stats = ctx.saved_tensors
         gout, gnext = (None if t is None else t.contiguous() for t in (gout, gnext))
-        grads = ops.residual_backward(gout, gnext, out, *rest, ctx.has_next_bias, stats, *ctx.codes)
+        grads = ops.residual_backward(gout, gnext, x, *rest, ctx.has_next_bias, stats, next_stats, *ctx.codes)
         return (*grads, None, None, None, None)
 
 
@@ -85,8 +85,7 @@ def gated_residual(x, y, weight=None, bias=None, gate=None, scale=None, kind="no
 
     x, y [..., C].  gate: of their shape (it may be a slice of a wider tensor's channels), or [x.shape[0], C], one row for each image.
     weight, bias, scale, next_weight, next_bias [C]; None stands for 1, 0 and 1.  kind and next_kind: rms, layer or none; activation:
-    none, sigmoid or silu.  The next norm is taken of the sum before it is rounded; its
-    gradient is that at the sum as it was stored."""
+    none, sigmoid or silu.  The next norm is taken of the sum before it is rounded."""
     codes = (_code(ops.ACTIVATIONS, activation, "activation"), _code(ops.NORM_KINDS, kind, "kind"),
              _code(ops.NORM_KINDS, next_kind, "next_kind"))
     if codes[0] and gate is None:

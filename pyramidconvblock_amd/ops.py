@@ -503,21 +503,22 @@ def _gate_rows(x, gate):
 
 
 def residual_forward(x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps, stats=False):
-    """-> (out, next or None, rows' statistics of y or None)."""
+    """-> (out, next or None, rows' statistics of y or None, of out or None)."""
     dev = _lib.require_device(x, y)
     C = x.shape[-1]
     N = x.numel() // C
+    new_stats = lambda k: torch.empty((N, 2), device=dev, dtype=torch.float32) if stats and k else None
     out, nxt = torch.empty_like(x), torch.empty_like(x) if next_kind else None
-    st = torch.empty((N, 2), device=dev, dtype=torch.float32) if stats and kind else None
+    st, nst = new_stats(kind), new_stats(next_kind)
     if N:
         _launch("pdw_residual_fwd", dev, x.data_ptr(), y.data_ptr(), _ptr(gate), _ptr(scale), _ptr(weight), _ptr(bias),
-                _ptr(next_weight), _ptr(next_bias), out.data_ptr(), _ptr(nxt), _ptr(st), N, C, _gate_rows(x, gate), 0,
+                _ptr(next_weight), _ptr(next_bias), out.data_ptr(), _ptr(nxt), _ptr(st), _ptr(nst), N, C, _gate_rows(x, gate), 0,
                 act, kind, next_kind, float(eps), _lib.dtype_code(x.dtype))
-    return out, nxt, st
+    return out, nxt, st, nst
 
 
-def residual_backward(gout, gnext, out, y, gate, scale, weight, bias, next_weight, has_next_bias, stats, act, kind, next_kind,
-                      eps):
+def residual_backward(gout, gnext, x, y, gate, scale, weight, bias, next_weight, has_next_bias, stats, next_stats, act, kind,
+                      next_kind):
     """-> gradients of (x, y, gate, scale, weight, bias, next_weight, next_bias), None for what there was none of."""
     dev = _lib.require_device(y)
     C = y.shape[-1]
@@ -530,8 +531,8 @@ def residual_backward(gout, gnext, out, y, gate, scale, weight, bias, next_weigh
     if N:
         P = _gate_rows(y, gate)
         ws = _bytes(_lib.lib().pdw_residual_bwd_workspace_bytes(N, C, P, next_kind, code), dev)
-        _launch("pdw_residual_bwd", dev, _ptr(gout), _ptr(gnext), _ptr(out), y.data_ptr(), _ptr(gate), _ptr(scale), _ptr(weight),
-                _ptr(bias), _ptr(next_weight), _ptr(stats), float(eps), gx.data_ptr() if next_kind else None, gy.data_ptr(),
+        _launch("pdw_residual_bwd", dev, _ptr(gout), _ptr(gnext), _ptr(x), y.data_ptr(), _ptr(gate), _ptr(scale), _ptr(weight),
+                _ptr(bias), _ptr(next_weight), _ptr(stats), _ptr(next_stats), gx.data_ptr() if next_kind else None, gy.data_ptr(),
                 _ptr(gg), _ptr(gs), _ptr(gw), _ptr(gb), _ptr(gnw), _ptr(gnb), ws.data_ptr(), ws.numel(), N, C, P, 0, act, kind,
                 next_kind, code)
     return gx, gy, gg, gs, gw, gb, gnw, gnb

@@ -111,11 +111,11 @@ def test_library_refuses_before_any_launch():
     need = L.pdw_norm_bwd_workspace_bytes(1000, 128, 2)
     assert need >= 2 * 128 * 4 and L.pdw_norm_bwd_workspace_bytes(0, 128, 2) == 0 and L.pdw_norm_bwd_workspace_bytes(8, 9999, 2) == 0
     res = lambda N=8, P=4, act=0, kind=1, nxt=0, out2=None, gate=1: L.pdw_residual_fwd(
-        1, 1, gate, 1, 1, 1, 1, 1, 1, out2, None, N, 8, P, 0, act, kind, nxt, 1e-6, 0, None)
+        1, 1, gate, 1, 1, 1, 1, 1, 1, out2, None, None, N, 8, P, 0, act, kind, nxt, 1e-6, 0, None)
     for bad in (dict(P=3), dict(P=0), dict(act=3), dict(act=-1), dict(kind=-1), dict(nxt=5), dict(nxt=1)):
         assert res(**bad) == 1, bad
     assert res(N=0) == 0
-    bwd = lambda ws, nbytes, P=4, stats=1, out=1: L.pdw_residual_bwd(1, 1, out, 1, 1, 1, 1, 1, 1, stats, 1e-6, 1, 1, 1, 1, 1, 1, 1, 1,
+    bwd = lambda ws, nbytes, P=4, stats=1, out=1: L.pdw_residual_bwd(1, 1, out, 1, 1, 1, 1, 1, 1, stats, 1, 1, 1, 1, 1, 1, 1, 1, 1,
                                                                            ws, nbytes, 8, 8, P, 0, 0, 1, 1, 0, None)
     assert bwd(None, 0) == 1 and b"workspace" in L.pdw_last_error()
     need = L.pdw_residual_bwd_workspace_bytes(8, 8, 4, 1, 0)
