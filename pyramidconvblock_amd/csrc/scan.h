@@ -40,7 +40,7 @@ struct ScanArgs {
     long long T;
     int rows, W, I;                     // rows = O * W
     int strips, tiles, segments, seg_tiles, state_tiles;
-    int reverse;
+    int reverse, near;                  // near: TilePtr's offsets fit
 };
 
 // Maps of a lane's VEC channels.
@@ -63,7 +63,7 @@ struct ScanLane {
     int lane, wave, c, sub;   // c: first channel
     bool on;
     __device__ __forceinline__ ScanLane(int strip, int I) {
-        lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         c = (strip * LC + lane % LC) * VEC;
         on = c < I;
         if (c + VEC > I) c = I - VEC;   // the last lane overlaps the one before it: the same chains, the same values (I >= VEC)
@@ -100,7 +100,7 @@ __device__ __forceinline__ void scan_tile(Maps<VEC> m, float (&carry)[VEC], floa
         for (int v = 0; v < VEC; ++v) lds[wave * W + cl * VEC + v] = make_float2(m.a[v], m.b[v]);
     }
     __syncthreads();
-#pragma unroll
+#pragma unroll 2   // (unrolled whole, the wavefronts' maps alone take 64 registers)
     for (int i = 0; i < NW; ++i) {
         const int w = BACK ? NW - 1 - i : i;
 #pragma unroll
@@ -150,21 +150,28 @@ __device__ __forceinline__ long long scan_pos(long long s, long long len, int re
     return reverse && s < len ? len - 1 - s : s;
 }
 
-// What a workgroup's index says: its strip of channels, its row (o, w) and its segment; and its chains' length.
+// What a workgroup's index says: its strip of channels, its row (o, w) and its segment; and its chains' length.  Neighbouring strips
+// share cache lines, so those of a row go to one of the eight dies (workgroups go to them in turn), one after the other.
 struct ScanWhere {
     int strip, row, o, w, seg;
     long long len;
     __device__ __forceinline__ ScanWhere(const ScanArgs& p) {
-        strip = blockIdx.x % (unsigned)p.strips;
-        const unsigned rest = blockIdx.x / (unsigned)p.strips;
+        const unsigned strips = p.strips, rows8 = gridDim.x / strips & ~7u;
+        unsigned rest;
+        if (blockIdx.x < rows8 * strips) {
+            const unsigned turn = blockIdx.x >> 3;
+            strip = turn % strips, rest = turn / strips * 8 + (blockIdx.x & 7);
+        } else {
+            strip = blockIdx.x % strips, rest = blockIdx.x / strips;
+        }
         row = rest % (unsigned)p.rows, seg = rest / (unsigned)p.rows;
         o = row / p.W, w = row - o * p.W;
         const long long n = p.lengths ? p.lengths[o] : p.T;
         len = n < 0 ? 0 : n > p.T ? p.T : n;
     }
     template <typename T>
-    __device__ __forceinline__ T* base(T* t, const ScanStrides& s, int c) const {
-        return t + o * s.o + w * s.w + c;
+    __device__ __forceinline__ T* base(T* t, const ScanStrides& s) const {
+        return t + o * s.o + w * s.w;
     }
 };
 
@@ -175,13 +182,60 @@ __device__ __forceinline__ void gates(const Piece<T, VEC>& g, float (&a)[VEC], f
     for (int v = 0; v < VEC; ++v) sigmoid_pair(to_f32(g.v[v]), a[v], m[v]);
 }
 
-// A lane's K pieces of one tensor; `n` of them are there.
-template <typename T, int VEC, int K>
-__device__ __forceinline__ void load_steps(const T* base, long long stride, long long s0, long long len, int reverse, bool on,
-                                           Piece<T, VEC> (&r)[K]) {
+// Where a lane's K steps of a tile of `tile` steps, from step `base` on, lie in one tensor: a base that all lanes share, a lane's
+// offset in bytes (unsigned, 32 bits: the host has checked that a tile's extent fits), and the distance of a step.  A tile that is
+// inside its chain is addressed this way, so that an address costs a lane nothing; others step by step, with 64 bits.
+struct TilePtr {
+    const char* shared;
+    unsigned lane;
+    long long step;
+    // strip: the base of the chain's row, t: elements between positions, at: this lane's first step in the tile, c: its channel
+    template <typename T>
+    __device__ __forceinline__ TilePtr(const T* strip, long long t, long long base, int tile, long long len, int reverse, int at, int c) {
+        const long long first = reverse ? len - base - tile : base;   // the tile's lowest position
+        shared = (const char*)(strip + first * t);
+        lane = (unsigned)(((reverse ? tile - 1 - at : at) * (unsigned)t + c) * (unsigned)sizeof(T));
+        step = (reverse ? -t : t) * (long long)sizeof(T);
+    }
+    template <typename T>
+    __device__ __forceinline__ T* of(int k) const {
+        return (T*)(const_cast<char*>(shared) + k * step + lane);
+    }
+};
+
+// A lane's K pieces of one tensor: all of them (whole), or those inside the chain, zeros for the others.
+template <typename T, int VEC, int LC, int NW, int K>
+__device__ __forceinline__ void load_steps(const T* strip, long long t, long long base, long long len, int reverse, bool whole,
+                                           const ScanLane<VEC, LC, NW, K>& at, Piece<T, VEC> (&r)[K]) {
+    if (whole) {
+        const TilePtr p(strip, t, base, at.kTile, len, reverse, at.sub * K, at.c);
+#pragma unroll
+        for (int k = 0; k < K; ++k) r[k] = load_any<T, VEC>(p.of<const T>(k));
+        return;
+    }
+    const long long s0 = base + (long long)at.sub * K;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        if (on && s0 + k < len) r[k] = load_any<T, VEC>(base + scan_pos(s0 + k, len, reverse) * stride);
+        if (s0 + k < len) r[k] = load_any<T, VEC>(strip + scan_pos(s0 + k, len, reverse) * t + at.c);
+        else
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) r[k].v[v] = from_f32<T>(0.f);
+    }
+}
+
+// As load_steps step by step, from step s0 of the chain on.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void load_run(const T* base, long long t, long long s0, long long len, int reverse, Piece<T, VEC> (&r)[K]) {
+    if (s0 + K <= len) {
+        const T* p = base + (reverse ? len - 1 - s0 : s0) * t;
+        const long long step = reverse ? -t : t;
+#pragma unroll
+        for (int k = 0; k < K; ++k) r[k] = load_any<T, VEC>(p + k * step);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (s0 + k < len) r[k] = load_any<T, VEC>(base + scan_pos(s0 + k, len, reverse) * t);
         else
 #pragma unroll
             for (int v = 0; v < VEC; ++v) r[k].v[v] = from_f32<T>(0.f);
@@ -199,10 +253,10 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
     const int seg = my.seg + (BACK ? 1 : 0);
     const Lane at(my.strip, p.I);
     const long long len = my.len;
-    const T* other = my.base((const T*)(BACK ? p.gy : p.x), BACK ? p.dense : p.xs, at.c);
+    const T* other = my.base((const T*)(BACK ? p.gy : p.x), BACK ? p.dense : p.xs) + at.c;
     const bool given = !BACK || p.gy;
     const long long ot = BACK ? p.dense.t : p.xs.t;
-    const T* g = my.base((const T*)p.g, p.gs, at.c);
+    const T* g = my.base((const T*)p.g, p.gs) + at.c;
     const long long first = (long long)seg * p.seg_tiles * Lane::kTile;
     const int run = p.seg_tiles * (Lane::kTile / TS);   // a lane's steps: a multiple of K
     const long long s0 = first + (long long)at.sub * run;
@@ -212,8 +266,8 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
     for (int i = 0; i < run; i += K) {
         const long long s = BACK ? s0 + run - K - i : s0 + i;
         Piece<T, VEC> xr[K], gr[K];
-        load_steps<T, VEC, K>(g, p.gs.t, s, len, p.reverse, at.on, gr);
-        load_steps<T, VEC, K>(other, ot, s, len, p.reverse, at.on && given, xr);
+        load_run<T, VEC, K>(g, p.gs.t, s, len, p.reverse, gr);
+        load_run<T, VEC, K>(other, ot, s, given ? len : 0, p.reverse, xr);
 #pragma unroll
         for (int j = 0; j < K; ++j) {
             const int k = BACK ? K - 1 - j : j;
@@ -249,31 +303,38 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
     const ScanWhere my(p);
     const int seg = my.seg;
     const Lane at(my.strip, p.I);
-    const long long len = my.len, row = (long long)my.row * p.I + at.c;
-    const T* x = my.base((const T*)p.x, p.xs, at.c);
-    const T* g = my.base((const T*)p.g, p.gs, at.c);
-    T* y = my.base((T*)p.y, p.dense, at.c);
+    const long long len = my.len;
+    const T *x = my.base((const T*)p.x, p.xs), *g = my.base((const T*)p.g, p.gs);
+    T* y = my.base((T*)p.y, p.dense);
     float carry[VEC];
     segment_start<VEC, LC, NW, K, false>(p, my.row, seg, at, p.h0, carry, lds[1]);
     const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
+    Piece<T, VEC> xr[K], gr[K];
+    auto load = [&](int tile) {
+        const long long base = (long long)tile * Lane::kTile;
+        const bool whole = p.near && base + Lane::kTile <= len;
+        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
+        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
+    };
+    load(t0);
     for (int tile = t0; tile < t1; ++tile) {
         const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
+        const bool whole = p.near && base + Lane::kTile <= len;
         float a[K][VEC], b[K][VEC], start[VEC];
-        {
-            Piece<T, VEC> xr[K], gr[K];
-            load_steps<T, VEC, K>(x, p.xs.t, s0, len, p.reverse, at.on, xr);
-            load_steps<T, VEC, K>(g, p.gs.t, s0, len, p.reverse, at.on, gr);
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                gates<T, VEC>(gr[k], a[k], b[k]);
-                const bool valid = s0 + k < len;
+        for (int k = 0; k < K; ++k) {
+            gates<T, VEC>(gr[k], a[k], b[k]);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    b[k][v] = valid ? b[k][v] * to_f32(xr[k].v[v]) : 0.f;
-                    if (!valid) a[k][v] = 1.f;
-                }
-            }
+            for (int v = 0; v < VEC; ++v) b[k][v] *= to_f32(xr[k].v[v]);
         }
+        if (!whole) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (!(s0 + k < len))
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, b[k][v] = 0.f;
+        }
+        if (tile + 1 < t1) load(tile + 1);   // on its way while this one is computed
         Maps<VEC> m;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) m.a[v] = a[0][v], m.b[v] = b[0][v];
@@ -288,21 +349,24 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) st[v] = start[v];
         }
+        const TilePtr to(y, p.dense.t, base, Lane::kTile, len, p.reverse, at.sub * K, at.c);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) start[v] = __builtin_fmaf(a[k][v], start[v], b[k][v]);
-            float out[VEC];
-            const bool valid = s0 + k < len;
+            if (whole) {
+                if (at.on) store_any<T, VEC>(to.template of<T>(k), start);
+            } else if (at.on && s0 + k < p.T) {
+                float out[VEC];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) out[v] = valid ? start[v] : 0.f;
-            if (at.on && s0 + k < p.T)
-                store_any<T, VEC>(y + scan_pos(s0 + k, len, p.reverse) * p.dense.t, out);
+                for (int v = 0; v < VEC; ++v) out[v] = s0 + k < len ? start[v] : 0.f;
+                store_any<T, VEC>(y + scan_pos(s0 + k, len, p.reverse) * p.dense.t + at.c, out);
+            }
         }
     }
     if (p.last && seg == p.segments - 1 && at.on && at.sub == 0) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) p.last[row + v] = carry[v];
+        for (int v = 0; v < VEC; ++v) p.last[(long long)my.row * p.I + at.c + v] = carry[v];
     }
 }
 
@@ -313,83 +377,95 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
     const ScanWhere my(p);
     const int seg = my.seg;
     const Lane at(my.strip, p.I);
-    const long long len = my.len, row = (long long)my.row * p.I + at.c;
-    const T* x = my.base((const T*)p.x, p.xs, at.c);
-    const T* g = my.base((const T*)p.g, p.gs, at.c);
-    const T* gy = my.base((const T*)p.gy, p.dense, at.c);
-    T *gx = my.base((T*)p.gx, p.gxs, at.c), *gg = my.base((T*)p.gg, p.ggs, at.c);
+    const long long len = my.len;
+    const T *x = my.base((const T*)p.x, p.xs), *g = my.base((const T*)p.g, p.gs), *gy = my.base((const T*)p.gy, p.dense);
+    T *gx = my.base((T*)p.gx, p.gxs), *gg = my.base((T*)p.gg, p.ggs);
     float carry[VEC];
     segment_start<VEC, LC, NW, K, true>(p, my.row, seg, at, p.glast, carry, lds[1][0]);
     const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
+    Piece<T, VEC> xr[K], gr[K], gyr[K];
+    float hr[VEC];
+    auto load = [&](int tile) {
+        const long long base = (long long)tile * Lane::kTile;
+        const bool whole = p.near && base + Lane::kTile <= len;
+        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
+        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
+        load_steps(gy, p.dense.t, base, p.gy ? len : 0, p.reverse, whole && p.gy, at, gyr);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) hr[v] = p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v];
+    };
+    if (t1 > t0) load(t1 - 1);
     for (int tile = t1 - 1; tile >= t0; --tile) {
         const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
-        float a[K][VEC], m[K][VEC], e[VEC], hs[VEC];
-        Piece<T, VEC> xr[K], gyr[K];
-        {
-            Piece<T, VEC> gr[K];
-            load_steps<T, VEC, K>(x, p.xs.t, s0, len, p.reverse, at.on, xr);
-            load_steps<T, VEC, K>(g, p.gs.t, s0, len, p.reverse, at.on, gr);
-            load_steps<T, VEC, K>(gy, p.dense.t, s0, len, p.reverse, at.on && p.gy, gyr);
+        const bool whole = p.near && base + Lane::kTile <= len;
+        float a[K][VEC], m[K][VEC], xv[K][VEC], gv[K][VEC], e[VEC], hs[VEC], h[VEC];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                gates<T, VEC>(gr[k], a[k], m[k]);
-                if (!(s0 + k < len)) {
+        for (int k = 0; k < K; ++k) {
+            gates<T, VEC>(gr[k], a[k], m[k]);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) xv[k][v] = to_f32(xr[k].v[v]), gv[k][v] = to_f32(gyr[k].v[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = hr[v];
+        if (!whole) {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (!(s0 + k < len))
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, m[k][v] = 0.f;
-                }
-            }
         }
-        Maps<VEC> back;
+        if (tile > t0) load(tile - 1);
+        Maps<VEC> back, fore;
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) back.a[v] = 1.f, back.b[v] = 0.f;
+        for (int v = 0; v < VEC; ++v) back.a[v] = 1.f, back.b[v] = fore.b[v] = 0.f;
 #pragma unroll
         for (int k = K - 1; k >= 0; --k)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                back.b[v] = a[k][v] * (to_f32(gyr[k].v[v]) + back.b[v]), back.a[v] *= a[k][v];
-        scan_tile<VEC, LC, NW, true>(back, carry, e, lds[tile & 1][0], at.lane, at.wave);
-        Maps<VEC> fore;
-        float h[VEC];
+            for (int v = 0; v < VEC; ++v) back.b[v] = a[k][v] * (gv[k][v] + back.b[v]), back.a[v] *= a[k][v];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            fore.a[v] = back.a[v], fore.b[v] = 0.f;
-            h[v] = at.on ? p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v] : 0.f;
-        }
+        for (int v = 0; v < VEC; ++v) fore.a[v] = back.a[v];
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                fore.b[v] = __builtin_fmaf(a[k][v], fore.b[v], m[k][v] * to_f32(xr[k].v[v]));
+            for (int v = 0; v < VEC; ++v) fore.b[v] = __builtin_fmaf(a[k][v], fore.b[v], m[k][v] * xv[k][v]);
+        scan_tile<VEC, LC, NW, true>(back, carry, e, lds[tile & 1][0], at.lane, at.wave);
         scan_tile<VEC, LC, NW, false>(fore, h, hs, lds[tile & 1][1], at.lane, at.wave);
-        float hp[K][VEC];
+        float hx[K][VEC];   // h_(t-1) - x_t
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                hp[k][v] = hs[v];
-                hs[v] = __builtin_fmaf(a[k][v], hs[v], m[k][v] * to_f32(xr[k].v[v]));
+                hx[k][v] = hs[v] - xv[k][v];
+                hs[v] = __builtin_fmaf(a[k][v], hs[v], m[k][v] * xv[k][v]);
             }
+        const TilePtr tox(gx, p.gxs.t, base, Lane::kTile, len, p.reverse, at.sub * K, at.c);
+        const TilePtr tog(gg, p.ggs.t, base, Lane::kTile, len, p.reverse, at.sub * K, at.c);
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
             float ox[VEC], og[VEC];
-            const bool valid = s0 + k < len;
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float d = to_f32(gyr[k].v[v]) + e[v];
-                ox[v] = valid ? d * m[k][v] : 0.f;
-                og[v] = valid ? d * (hp[k][v] - to_f32(xr[k].v[v])) * (a[k][v] * m[k][v]) : 0.f;
+                const float d = gv[k][v] + e[v];
+                ox[v] = d * m[k][v];
                 e[v] = a[k][v] * d;
+                og[v] = ox[v] * a[k][v] * hx[k][v];
             }
-            if (at.on && s0 + k < p.T) {
+            if (whole) {
+                if (at.on && p.gx) store_any<T, VEC>(tox.template of<T>(k), ox);
+                if (at.on && p.gg) store_any<T, VEC>(tog.template of<T>(k), og);
+            } else if (at.on && s0 + k < p.T) {
                 const long long t = scan_pos(s0 + k, len, p.reverse);
-                if (p.gx) store_any<T, VEC>(gx + t * p.gxs.t, ox);
-                if (p.gg) store_any<T, VEC>(gg + t * p.ggs.t, og);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v)
+                    if (!(s0 + k < len)) ox[v] = og[v] = 0.f;
+                if (p.gx) store_any<T, VEC>(gx + t * p.gxs.t + at.c, ox);
+                if (p.gg) store_any<T, VEC>(gg + t * p.ggs.t + at.c, og);
             }
         }
     }
     if (p.gh0 && seg == 0 && at.on && at.sub == 0) {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) p.gh0[row + v] = carry[v];
+        for (int v = 0; v < VEC; ++v) p.gh0[(long long)my.row * p.I + at.c + v] = carry[v];
     }
 }
 

@@ -49,6 +49,9 @@ int scan_run(const ScanArgs& in, bool backward, void* workspace, size_t workspac
         return set_error("scan: workspace too small (%zu of %zu bytes)", workspace_bytes, need), 1;
     p.strips = (int)c.strips, p.tiles = (int)c.tiles, p.seg_tiles = (int)c.seg_tiles, p.segments = (int)c.segments;
     p.maps = (float*)workspace;
+    p.near = 1;
+    for (const ScanStrides& t : {p.xs, p.gs, p.gxs, p.ggs, p.dense})   // (no tile is longer than 1024 steps)
+        if (t.t < 0 || 1024 * t.t + p.I > 0x0fffffffLL) p.near = 0;
     p.state_tiles = (int)scan_cut(p.rows, p.T, p.I, kScanBackward).tiles;
     if (dtype == kF32) scan_launch_f32(p, pass, s);
     else if (dtype == kF16) scan_launch_f16(p, pass, s);
