@@ -6,17 +6,15 @@ namespace pdw {
 
 enum : int { kActNone = 0, kActSigmoid = 1, kActSilu = 2 };
 
-// a = sigmoid(g) and m = 1 - a = sigmoid(-g): with e = exp(-|g|) they are 1 / (1 + e) and e / (1 + e), whichever way round, so
-// neither is a difference and nothing overflows (g = +-inf gives 1 and 0, NaN both NaN).  The larger is good to 2 u (u = 2^-24), the
-// smaller to (|g| + 4) u of itself, which is less than u of the larger: |g| log2(e) is rounded, so e is off by |g| u, and what that
-// moves a and m by is a m |g| u < u / 4.  (Taking the product's remainder along and a Newton step behind the reciprocal, both measured,
-// changed no result's distance from the exact one and cost the recurrence a third of its instructions.)
+// a = sigmoid(g) = 1 / (1 + e) and m = 1 - a = sigmoid(-g) = e / (1 + e) with e = exp(-g), so m is no difference.  e is limited to 2^126,
+// from where a is 2^-126 instead of less (g = -inf: m = 1; g = inf: a = 1 and m = 0; NaN passes).  g log2(e) is rounded, so e is off
+// by |g| u (u = 2^-24): that moves the smaller of a and m by that much of itself, and the larger by a m |g| u < u / 4.  (Taking the product's
+// remainder along and a Newton step behind the reciprocal, both measured, changed no result's distance from the exact one and cost the
+// recurrence a third of its instructions.)
 __device__ __forceinline__ void sigmoid_pair(float g, float& a, float& m) {
-    const float e = __builtin_amdgcn_exp2f(-fabsf(g) * 1.44269504f);
-    const float r = __builtin_amdgcn_rcpf(1.f + e);
-    const float s = e * r;
-    const bool pos = g >= 0.f;
-    a = pos ? r : s, m = pos ? s : r;
+    const float e = __builtin_amdgcn_exp2f(__builtin_elementwise_minimum(g * -1.44269504f, 126.f));
+    a = __builtin_amdgcn_rcpf(1.f + e);
+    m = e * a;
 }
 
 // act(v), and act'(v)

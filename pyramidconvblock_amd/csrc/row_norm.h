@@ -54,19 +54,53 @@ struct Piece {
     T v[VEC];
 };
 
+// A piece moves as one access of its size, wherever it lies (as an array of 16-bit values a store of it comes out in halves).
+template <int BYTES>
+struct AccessOf;
+template <>
+struct AccessOf<2> {
+    typedef unsigned short type;
+};
+template <>
+struct AccessOf<4> {
+    typedef unsigned type;
+};
+template <>
+struct AccessOf<8> {
+    typedef unsigned type __attribute__((ext_vector_type(2)));
+};
+template <>
+struct AccessOf<16> {
+    typedef unsigned type __attribute__((ext_vector_type(4)));
+};
+template <typename T, int VEC>
+struct Access {
+    typedef typename AccessOf<sizeof(T) * VEC>::type word;
+    typedef word type __attribute__((aligned(sizeof(T)), may_alias));
+};
+
 template <typename T, int VEC>
 __device__ __forceinline__ Piece<T, VEC> load_any(const T* p) {
+    typename Access<T, VEC>::word w = *reinterpret_cast<const typename Access<T, VEC>::type*>(p);
+    return __builtin_bit_cast(Piece<T, VEC>, w);
+}
+
+template <typename T, int VEC>
+__device__ __forceinline__ Piece<T, VEC> round_piece(const float (&v)[VEC]) {
     Piece<T, VEC> r;
-    __builtin_memcpy(&r, p, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r.v[i] = from_f32<T>(v[i]);
     return r;
 }
 
 template <typename T, int VEC>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T, VEC>& r) {
+    *reinterpret_cast<typename Access<T, VEC>::type*>(p) = __builtin_bit_cast(typename Access<T, VEC>::word, r);
+}
+
+template <typename T, int VEC>
 __device__ __forceinline__ void store_any(T* p, const float (&v)[VEC]) {
-    Piece<T, VEC> r;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) r.v[i] = from_f32<T>(v[i]);
-    __builtin_memcpy(p, &r, sizeof(r));
+    store_piece<T, VEC>(p, round_piece<T, VEC>(v));
 }
 
 // A lane's pieces of a row.

@@ -9,13 +9,17 @@
 // The states h_(t-1) that gg needs are not kept: the forward leaves the 32-bit state before every tile, and the backward runs the tile
 // from it again, in the same order, from x and g, which it reads anyway.
 //
-// A workgroup has a strip of channels (LC lanes of VEC channels: 128 bytes in 16-bit types, so that a time step is a whole cache
-// line) and walks over tiles of NW wavefronts x 64/LC lanes x K steps: a lane composes its K consecutive steps in registers, lanes
+// A workgroup has a strip of channels (LC lanes of two channels) and walks over tiles of NW wavefronts x 64/LC lanes x K steps: a lane composes its K consecutive steps in registers, lanes
 // and wavefronts exchange their maps (shuffles; LDS), and every lane runs its K steps from its state.  So x and g are read once.  Where
 // there are too few strips to fill the chip, time is cut into segments of whole tiles: a first launch composes each segment's
 // map (x and g are read once more for it), and the second starts each segment from the maps before it.
 //
 // All of it is in fp32.  No atomics: results are the same from call to call.
+//
+// What bounds it ([32,3136,128] bf16): instructions first.  Forward a value takes 22 (six of them the sigmoid, two of those at a quarter of
+// the rate), 9 us of the 27 us kernel; backward 41, 16 us of 46; the exchange between lanes and wavefronts, which every wavefront
+// waits for, has most of the rest.  The tensors themselves would take 9 and 15 us.  Two channels a lane rather than four (half the exchanged
+// values for as many steps): forward and backward 107 -> 87 us; stores of whole pieces and one branch a tile: 87 -> 78.
 #pragma once
 #include "common.h"
 #include "gate_math.h"
@@ -40,7 +44,7 @@ struct ScanArgs {
     long long T;
     int rows, W, I;                     // rows = O * W
     int strips, tiles, segments, seg_tiles, state_tiles;
-    int reverse, near;                  // near: TilePtr's offsets fit
+    int reverse, near, near_segments;   // TilePtr's offsets fit, of a tile and of a segment
 };
 
 // Maps of a lane's VEC channels.
@@ -175,6 +179,19 @@ struct ScanWhere {
     }
 };
 
+// Keeps the compiler from carrying what it has made of the pieces so far along with them.
+template <typename T, int VEC, int K>
+__device__ __forceinline__ void keep_packed(Piece<T, VEC> (&r)[K]) {
+    if constexpr (sizeof(T) * VEC == 4) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            unsigned u = __builtin_bit_cast(unsigned, r[k]);
+            asm("" : "+v"(u));
+            r[k] = __builtin_bit_cast(Piece<T, VEC>, u);
+        }
+    }
+}
+
 // (a, m) of one piece of g
 template <typename T, int VEC>
 __device__ __forceinline__ void gates(const Piece<T, VEC>& g, float (&a)[VEC], float (&m)[VEC]) {
@@ -194,7 +211,7 @@ struct TilePtr {
     __device__ __forceinline__ TilePtr(const T* strip, long long t, long long base, int tile, long long len, int reverse, int at, int c) {
         const long long first = reverse ? len - base - tile : base;   // the tile's lowest position
         shared = (const char*)(strip + first * t);
-        lane = (unsigned)(((reverse ? tile - 1 - at : at) * (unsigned)t + c) * (unsigned)sizeof(T));
+        lane = ((unsigned)(reverse ? tile - 1 - at : at) * (unsigned)t + (unsigned)c) * (unsigned)sizeof(T);
         step = (reverse ? -t : t) * (long long)sizeof(T);
     }
     template <typename T>
@@ -223,22 +240,27 @@ __device__ __forceinline__ void load_steps(const T* strip, long long t, long lon
     }
 }
 
-// As load_steps step by step, from step s0 of the chain on.
-template <typename T, int VEC, int K>
-__device__ __forceinline__ void load_run(const T* base, long long t, long long s0, long long len, int reverse, Piece<T, VEC> (&r)[K]) {
-    if (s0 + K <= len) {
-        const T* p = base + (reverse ? len - 1 - s0 : s0) * t;
-        const long long step = reverse ? -t : t;
+// Stores a lane's K pieces; zeros at positions behind the chain's end.
+template <typename T, int VEC, int LC, int NW, int K>
+__device__ __forceinline__ void store_steps(T* strip, long long t, long long base, long long T_, long long len, int reverse, bool whole,
+                                            const ScanLane<VEC, LC, NW, K>& at, const Piece<T, VEC> (&r)[K]) {
+    if (!at.on) return;
+    if (whole) {
+        const TilePtr p(strip, t, base, at.kTile, len, reverse, at.sub * K, at.c);
 #pragma unroll
-        for (int k = 0; k < K; ++k) r[k] = load_any<T, VEC>(p + k * step);
+        for (int k = 0; k < K; ++k) store_piece<T, VEC>(p.of<T>(k), r[k]);
         return;
     }
+    const long long s0 = base + (long long)at.sub * K;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        if (s0 + k < len) r[k] = load_any<T, VEC>(base + scan_pos(s0 + k, len, reverse) * t);
-        else
+        if (s0 + k >= T_) break;
+        Piece<T, VEC> q = r[k];
+        if (!(s0 + k < len)) {
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) r[k].v[v] = from_f32<T>(0.f);
+            for (int v = 0; v < VEC; ++v) q.v[v] = from_f32<T>(0.f);
+        }
+        store_piece<T, VEC>(strip + scan_pos(s0 + k, len, reverse) * t + at.c, q);
     }
 }
 
@@ -253,33 +275,52 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
     const int seg = my.seg + (BACK ? 1 : 0);
     const Lane at(my.strip, p.I);
     const long long len = my.len;
-    const T* other = my.base((const T*)(BACK ? p.gy : p.x), BACK ? p.dense : p.xs) + at.c;
+    const T* other = my.base((const T*)(BACK ? p.gy : p.x), BACK ? p.dense : p.xs);
     const bool given = !BACK || p.gy;
     const long long ot = BACK ? p.dense.t : p.xs.t;
-    const T* g = my.base((const T*)p.g, p.gs) + at.c;
-    const long long first = (long long)seg * p.seg_tiles * Lane::kTile;
-    const int run = p.seg_tiles * (Lane::kTile / TS);   // a lane's steps: a multiple of K
-    const long long s0 = first + (long long)at.sub * run;
+    const T* g = my.base((const T*)p.g, p.gs);
+    const int steps = p.seg_tiles * Lane::kTile, run = steps / TS;   // the segment's steps and a lane's: multiples of K
+    const long long first = (long long)seg * steps;
     Maps<VEC> m;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) m.a[v] = 1.f, m.b[v] = 0.f;
-    for (int i = 0; i < run; i += K) {
-        const long long s = BACK ? s0 + run - K - i : s0 + i;
-        Piece<T, VEC> xr[K], gr[K];
-        load_run<T, VEC, K>(g, p.gs.t, s, len, p.reverse, gr);
-        load_run<T, VEC, K>(other, ot, s, given ? len : 0, p.reverse, xr);
+    auto compose = [&](const Piece<T, VEC>& gp, const Piece<T, VEC>& op) {
+        float a[VEC], q[VEC];
+        gates<T, VEC>(gp, a, q);
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            const int k = BACK ? K - 1 - j : j;
-            float a[VEC], q[VEC];
-            gates<T, VEC>(gr[k], a, q);
-            const bool valid = s + k < len;
+        for (int v = 0; v < VEC; ++v) {
+            const float u = to_f32(op.v[v]);
+            m.b[v] = BACK ? a[v] * (u + m.b[v]) : __builtin_fmaf(a[v], m.b[v], q[v] * u), m.a[v] *= a[v];
+        }
+    };
+    if (p.near_segments && given && first + steps <= len) {
+        const int end = at.sub * run + (BACK ? run - 1 : 0);   // the lane's first step in the order of composition
+        const TilePtr pg(g, p.gs.t, first, steps, len, p.reverse, end, at.c), po(other, ot, first, steps, len, p.reverse, end, at.c);
+        for (int i = 0; i < run; i += K) {
+            Piece<T, VEC> xr[K], gr[K];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float u = to_f32(xr[k].v[v]);
-                const float b = BACK ? a[v] * (u + m.b[v]) : __builtin_fmaf(a[v], m.b[v], q[v] * u);
-                m.b[v] = valid ? b : m.b[v], m.a[v] = valid ? m.a[v] * a[v] : m.a[v];
+            for (int k = 0; k < K; ++k) gr[k] = load_any<T, VEC>(pg.of<const T>(BACK ? -i - k : i + k));
+#pragma unroll
+            for (int k = 0; k < K; ++k) xr[k] = load_any<T, VEC>(po.of<const T>(BACK ? -i - k : i + k));
+#pragma unroll
+            for (int k = 0; k < K; ++k) compose(gr[k], xr[k]);
+        }
+    } else {
+        for (int i = 0; i < run; i += K) {
+            Piece<T, VEC> xr[K], gr[K];
+            const long long from = first + at.sub * run + (BACK ? run - 1 - i : i);
+            if ((BACK ? from - K + 1 : from) >= len) continue;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const long long s = BACK ? from - k : from + k, t = scan_pos(s, len, p.reverse);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) xr[k].v[v] = gr[k].v[v] = from_f32<T>(0.f);
+                if (s < len) gr[k] = load_any<T, VEC>(g + t * p.gs.t + at.c);
+                if (s < len && given) xr[k] = load_any<T, VEC>(other + t * ot + at.c);
             }
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if ((BACK ? from - k : from + k) < len) compose(gr[k], xr[k]);
         }
     }
     float zero[VEC], one[VEC], unused[VEC];
@@ -296,7 +337,7 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
 }
 
 template <typename T, int VEC, int LC, int NW, int K>
-__global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
+__global__ __launch_bounds__(NW * 64, 4) void scan_fwd_k(ScanArgs p) {
     typedef ScanLane<VEC, LC, NW, K> Lane;
     constexpr int TS = NW * Lane::kSub;
     __shared__ float2 lds[2][NW * LC * VEC];
@@ -309,17 +350,12 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
     float carry[VEC];
     segment_start<VEC, LC, NW, K, false>(p, my.row, seg, at, p.h0, carry, lds[1]);
     const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
-    Piece<T, VEC> xr[K], gr[K];
-    auto load = [&](int tile) {
-        const long long base = (long long)tile * Lane::kTile;
-        const bool whole = p.near && base + Lane::kTile <= len;
-        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
-        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
-    };
-    load(t0);
     for (int tile = t0; tile < t1; ++tile) {
         const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
         const bool whole = p.near && base + Lane::kTile <= len;
+        Piece<T, VEC> xr[K], gr[K];
+        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
+        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
         float a[K][VEC], b[K][VEC], start[VEC];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -334,7 +370,6 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, b[k][v] = 0.f;
         }
-        if (tile + 1 < t1) load(tile + 1);   // on its way while this one is computed
         Maps<VEC> m;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) m.a[v] = a[0][v], m.b[v] = b[0][v];
@@ -349,20 +384,14 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) st[v] = start[v];
         }
-        const TilePtr to(y, p.dense.t, base, Lane::kTile, len, p.reverse, at.sub * K, at.c);
+        Piece<T, VEC> out[K];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int v = 0; v < VEC; ++v) start[v] = __builtin_fmaf(a[k][v], start[v], b[k][v]);
-            if (whole) {
-                if (at.on) store_any<T, VEC>(to.template of<T>(k), start);
-            } else if (at.on && s0 + k < p.T) {
-                float out[VEC];
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) out[v] = s0 + k < len ? start[v] : 0.f;
-                store_any<T, VEC>(y + scan_pos(s0 + k, len, p.reverse) * p.dense.t + at.c, out);
-            }
+            out[k] = round_piece<T, VEC>(start);
         }
+        store_steps(y, p.dense.t, base, p.T, len, p.reverse, whole, at, out);
     }
     if (p.last && seg == p.segments - 1 && at.on && at.sub == 0) {
 #pragma unroll
@@ -371,7 +400,7 @@ __global__ __launch_bounds__(NW * 64) void scan_fwd_k(ScanArgs p) {
 }
 
 template <typename T, int VEC, int LC, int NW, int K>
-__global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && NW > 2 ? 4 : 3) void scan_bwd_k(ScanArgs p) {
     typedef ScanLane<VEC, LC, NW, K> Lane;
     __shared__ float2 lds[2][2][NW * LC * VEC];
     const ScanWhere my(p);
@@ -383,30 +412,21 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
     float carry[VEC];
     segment_start<VEC, LC, NW, K, true>(p, my.row, seg, at, p.glast, carry, lds[1][0]);
     const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
-    Piece<T, VEC> xr[K], gr[K], gyr[K];
-    float hr[VEC];
-    auto load = [&](int tile) {
-        const long long base = (long long)tile * Lane::kTile;
-        const bool whole = p.near && base + Lane::kTile <= len;
-        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
-        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
-        load_steps(gy, p.dense.t, base, p.gy ? len : 0, p.reverse, whole && p.gy, at, gyr);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) hr[v] = p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v];
-    };
-    if (t1 > t0) load(t1 - 1);
     for (int tile = t1 - 1; tile >= t0; --tile) {
         const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
         const bool whole = p.near && base + Lane::kTile <= len;
-        float a[K][VEC], m[K][VEC], xv[K][VEC], gv[K][VEC], e[VEC], hs[VEC], h[VEC];
+        float a[K][VEC], m[K][VEC], e[VEC], hs[VEC], h[VEC];
+        Piece<T, VEC> xr[K], gyr[K];
+        {
+            Piece<T, VEC> gr[K];
+            load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
+            load_steps(gy, p.dense.t, base, p.gy ? len : 0, p.reverse, whole && p.gy, at, gyr);
+            load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            gates<T, VEC>(gr[k], a[k], m[k]);
+            for (int v = 0; v < VEC; ++v) h[v] = p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v];
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) xv[k][v] = to_f32(xr[k].v[v]), gv[k][v] = to_f32(gyr[k].v[v]);
+            for (int k = 0; k < K; ++k) gates<T, VEC>(gr[k], a[k], m[k]);
         }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) h[v] = hr[v];
         if (!whole) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -414,20 +434,21 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, m[k][v] = 0.f;
         }
-        if (tile > t0) load(tile - 1);
         Maps<VEC> back, fore;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) back.a[v] = 1.f, back.b[v] = fore.b[v] = 0.f;
 #pragma unroll
         for (int k = K - 1; k >= 0; --k)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) back.b[v] = a[k][v] * (gv[k][v] + back.b[v]), back.a[v] *= a[k][v];
+            for (int v = 0; v < VEC; ++v) back.b[v] = a[k][v] * (to_f32(gyr[k].v[v]) + back.b[v]), back.a[v] *= a[k][v];
 #pragma unroll
         for (int v = 0; v < VEC; ++v) fore.a[v] = back.a[v];
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) fore.b[v] = __builtin_fmaf(a[k][v], fore.b[v], m[k][v] * xv[k][v]);
+            for (int v = 0; v < VEC; ++v) fore.b[v] = __builtin_fmaf(a[k][v], fore.b[v], m[k][v] * to_f32(xr[k].v[v]));
+        // (kept as they were loaded, and converted again where they are used: 16 registers instead of 32)
+        keep_packed(xr), keep_packed(gyr);
         scan_tile<VEC, LC, NW, true>(back, carry, e, lds[tile & 1][0], at.lane, at.wave);
         scan_tile<VEC, LC, NW, false>(fore, h, hs, lds[tile & 1][1], at.lane, at.wave);
         float hx[K][VEC];   // h_(t-1) - x_t
@@ -435,33 +456,24 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                hx[k][v] = hs[v] - xv[k][v];
-                hs[v] = __builtin_fmaf(a[k][v], hs[v], m[k][v] * xv[k][v]);
+                hx[k][v] = hs[v] - to_f32(xr[k].v[v]);
+                hs[v] = __builtin_fmaf(a[k][v], hs[v], m[k][v] * to_f32(xr[k].v[v]));
             }
-        const TilePtr tox(gx, p.gxs.t, base, Lane::kTile, len, p.reverse, at.sub * K, at.c);
-        const TilePtr tog(gg, p.ggs.t, base, Lane::kTile, len, p.reverse, at.sub * K, at.c);
+        Piece<T, VEC> ox[K], og[K];
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
-            float ox[VEC], og[VEC];
+            float fx[VEC], fg[VEC];
 #pragma unroll
             for (int v = 0; v < VEC; ++v) {
-                const float d = gv[k][v] + e[v];
-                ox[v] = d * m[k][v];
+                const float d = to_f32(gyr[k].v[v]) + e[v];
+                fx[v] = d * m[k][v];
                 e[v] = a[k][v] * d;
-                og[v] = ox[v] * a[k][v] * hx[k][v];
+                fg[v] = fx[v] * a[k][v] * hx[k][v];
             }
-            if (whole) {
-                if (at.on && p.gx) store_any<T, VEC>(tox.template of<T>(k), ox);
-                if (at.on && p.gg) store_any<T, VEC>(tog.template of<T>(k), og);
-            } else if (at.on && s0 + k < p.T) {
-                const long long t = scan_pos(s0 + k, len, p.reverse);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v)
-                    if (!(s0 + k < len)) ox[v] = og[v] = 0.f;
-                if (p.gx) store_any<T, VEC>(gx + t * p.gxs.t + at.c, ox);
-                if (p.gg) store_any<T, VEC>(gg + t * p.ggs.t + at.c, og);
-            }
+            ox[k] = round_piece<T, VEC>(fx), og[k] = round_piece<T, VEC>(fg);
         }
+        if (p.gx) store_steps(gx, p.gxs.t, base, p.T, len, p.reverse, whole, at, ox);
+        if (p.gg) store_steps(gg, p.ggs.t, base, p.T, len, p.reverse, whole, at, og);
     }
     if (p.gh0 && seg == 0 && at.on && at.sub == 0) {
 #pragma unroll
@@ -471,17 +483,33 @@ __global__ __launch_bounds__(NW * 64) void scan_bwd_k(ScanArgs p) {
 
 enum ScanPass { kScanForward, kScanBackward };
 
-// Wavefronts of a workgroup: as few as have a short chain in one tile, and up to eight.  Steps of a lane: eight forward; four
-// backward, where three tensors and two scans are held (with eight: 370 bytes a lane spilled).
-constexpr int kForwardSteps = 8, kBackwardSteps = 4;
-inline int scan_waves(long long T, int I) {
-    if (I < 4) return 4;
-    return T <= 32 ? 1 : T <= 64 ? 2 : T <= 128 ? 4 : 8;
-}
-inline int scan_lanes(int I) { return I < 4 ? 4 : 16; }          // LC
-inline int scan_width(int I) { return I < 4 ? 4 : 64; }          // channels of a strip
-inline int scan_tile_steps(long long T, int I, ScanPass pass) {
-    return scan_waves(T, I) * (64 / scan_lanes(I)) * (pass == kScanForward ? kForwardSteps : kBackwardSteps);
+// A lane has two channels and 16 steps of a tile forward, eight backward, where three tensors and two scans are held.
+constexpr int kForwardSteps = 16, kBackwardSteps = 8;
+
+// How a call is cut: channels of a lane, lanes of a strip, wavefronts of a workgroup, and whether time is cut into segments.
+struct ScanShape {
+    int vec, lanes, waves;
+    bool segments;
+    int width() const { return vec * lanes; }
+    int tile(ScanPass pass) const { return waves * (64 / lanes) * (pass == kScanForward ? kForwardSteps : kBackwardSteps); }
+};
+
+// Strips of 32 channels give a chip full of workgroups of four wavefronts where there are 1024 of them; where there are fewer but at least
+// one strip of 32 or 16 channels for every compute unit, workgroups of eight wavefronts, and no segments: x and g are read once, in one
+// launch ([32,3136,128] bf16 forward and backward: 73 us, with segments 78; and twice the traffic where the tensors are in no cache).
+// Fewer than that need segments.  As many wavefronts as a chain's steps need, at most; a chain of up
+// to 32 steps has a strip of 64 channels.
+inline ScanShape scan_shape(long long rows, long long T, int I) {
+    if (I < 2) return {1, 4, 4, true};
+    const long long wide = rows * ((I + 31) / 32), narrow = rows * ((I + 15) / 16);
+    const bool many = wide >= 1024, segments = narrow < 256;
+    int lanes = T <= 32 ? 32 : many || segments || wide >= 256 ? 16 : 8;
+    const int most = many || segments ? 4 : 8;
+    int waves = 1;
+    while (waves < most && waves * (64 / lanes) * kForwardSteps < T) waves *= 2;
+    if (const char* e = tune_env("PDW_SCAN_LANES")) lanes = atoi(e);
+    if (const char* e = tune_env("PDW_SCAN_WAVES")) waves = atoi(e);
+    return {2, lanes, waves, segments};
 }
 
 template <typename T, int VEC, int LC, int NW>
@@ -497,15 +525,20 @@ void scan_launch(const ScanArgs& p, ScanPass pass, hipStream_t s) {
     else scan_bwd_k<T, VEC, LC, NW, kBackwardSteps><<<n, NW * 64, 0, s>>>(p);
 }
 
+template <typename T, int LC>
+void scan_waves(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) {
+    if (shape.waves == 1) scan_launch<T, 2, LC, 1>(p, pass, s);
+    else if (shape.waves == 2) scan_launch<T, 2, LC, 2>(p, pass, s);
+    else if (shape.waves == 4) scan_launch<T, 2, LC, 4>(p, pass, s);
+    else scan_launch<T, 2, LC, 8>(p, pass, s);
+}
+
 template <typename T>
-void scan_dispatch(const ScanArgs& p, ScanPass pass, hipStream_t s) {
-    if (p.I < 4) return scan_launch<T, 1, 4, 4>(p, pass, s);
-    switch (scan_waves(p.T, p.I)) {
-        case 1: return scan_launch<T, 4, 16, 1>(p, pass, s);
-        case 2: return scan_launch<T, 4, 16, 2>(p, pass, s);
-        case 4: return scan_launch<T, 4, 16, 4>(p, pass, s);
-        default: return scan_launch<T, 4, 16, 8>(p, pass, s);
-    }
+void scan_dispatch(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) {
+    if (shape.vec == 1) scan_launch<T, 1, 4, 4>(p, pass, s);
+    else if (shape.lanes == 32) scan_waves<T, 32>(p, shape, pass, s);
+    else if (shape.lanes == 16) scan_waves<T, 16>(p, shape, pass, s);
+    else scan_waves<T, 8>(p, shape, pass, s);
 }
 
 }  // namespace pdw

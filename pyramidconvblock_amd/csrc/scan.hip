@@ -5,23 +5,24 @@
 
 namespace pdw {
 
-void scan_launch_f32(const ScanArgs& p, ScanPass pass, hipStream_t s);
-void scan_launch_f16(const ScanArgs& p, ScanPass pass, hipStream_t s);
-void scan_launch_bf16(const ScanArgs& p, ScanPass pass, hipStream_t s);
+void scan_launch_f32(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s);
+void scan_launch_f16(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s);
+void scan_launch_bf16(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s);
 
-// Tiles of a chain, and segments of whole tiles: one where the strips alone give every compute unit a workgroup, else as many as make
-// two for each.
+// Tiles of a chain, and segments of whole tiles: where there are any, about 1024 workgroups of four wavefronts.
 struct ScanCut {
+    ScanShape shape;
     long long strips, tiles, seg_tiles, segments;
 };
 
 static ScanCut scan_cut(long long rows, long long T, int I, ScanPass pass) {
     ScanCut c;
-    c.strips = cdiv(I, scan_width(I));
-    const int step = scan_tile_steps(T, I, pass);
+    c.shape = scan_shape(rows, T, I);
+    c.strips = cdiv(I, c.shape.width());
+    const int step = c.shape.tile(pass);
     c.tiles = (T + step - 1) / step;
     const long long columns = rows * c.strips;
-    long long want = columns >= 256 || c.tiles < 2 ? 1 : (512 + columns - 1) / columns;
+    long long want = c.shape.segments ? (1024 + columns - 1) / columns : 1;
     if (want > c.tiles) want = c.tiles;
     if (want < 1) want = 1;
     c.seg_tiles = c.tiles ? (c.tiles + want - 1) / want : 1;
@@ -49,13 +50,17 @@ int scan_run(const ScanArgs& in, bool backward, void* workspace, size_t workspac
         return set_error("scan: workspace too small (%zu of %zu bytes)", workspace_bytes, need), 1;
     p.strips = (int)c.strips, p.tiles = (int)c.tiles, p.seg_tiles = (int)c.seg_tiles, p.segments = (int)c.segments;
     p.maps = (float*)workspace;
-    p.near = 1;
-    for (const ScanStrides& t : {p.xs, p.gs, p.gxs, p.ggs, p.dense})   // (no tile is longer than 1024 steps)
-        if (t.t < 0 || 1024 * t.t + p.I > 0x0fffffffLL) p.near = 0;
+    long long far = 0;
+    for (const ScanStrides& t : {p.xs, p.gs, p.gxs, p.ggs, p.dense}) {
+        if (t.t < 0) far = 1LL << 40;
+        if (t.t > far) far = t.t;
+    }
+    const long long step = c.shape.tile(pass), most = 0x3fffffffLL - p.I;   // elements: 32 bits of bytes
+    p.near = far <= most / step, p.near_segments = far <= most / (step * c.seg_tiles);
     p.state_tiles = (int)scan_cut(p.rows, p.T, p.I, kScanBackward).tiles;
-    if (dtype == kF32) scan_launch_f32(p, pass, s);
-    else if (dtype == kF16) scan_launch_f16(p, pass, s);
-    else scan_launch_bf16(p, pass, s);
+    if (dtype == kF32) scan_launch_f32(p, c.shape, pass, s);
+    else if (dtype == kF16) scan_launch_f16(p, c.shape, pass, s);
+    else scan_launch_bf16(p, c.shape, pass, s);
     return check_launch(backward ? "scan_bwd_k" : "scan_fwd_k");
 }
 

@@ -2,5 +2,5 @@
 #include "scan.h"
 
 namespace pdw {
-void scan_launch_bf16(const ScanArgs& p, ScanPass pass, hipStream_t s) { scan_dispatch<bf16_t>(p, pass, s); }
+void scan_launch_bf16(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) { scan_dispatch<bf16_t>(p, shape, pass, s); }
 }  // namespace pdw

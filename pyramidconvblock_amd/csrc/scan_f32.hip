@@ -2,5 +2,5 @@
 #include "scan.h"
 
 namespace pdw {
-void scan_launch_f32(const ScanArgs& p, ScanPass pass, hipStream_t s) { scan_dispatch<float>(p, pass, s); }
+void scan_launch_f32(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) { scan_dispatch<float>(p, shape, pass, s); }
 }  // namespace pdw
