@@ -503,8 +503,7 @@ int pdw_residual_fwd(const void *x, const void *y, const void *gate, const void 
                      const void *next_weight, const void *next_bias, void *out, void *next, float *stats, float *next_stats,
                      long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,
                      void *stream);
-/* The gradients, from those of out (gout) and next (gnext), either of which may be NULL (0).  x is read only
- * with a next norm.  gx [N][C] is written only with a next norm (without one it is gout itself); ggate like gate, dense.  Each result
+/* The gradients, from those of out (gout) and, with a next norm, of next (gnext).  x is read only with a next norm.  gx [N][C] is written only with a next norm (without one it is gout itself); ggate like gate, dense.  Each result
  * may be NULL (not wanted).  Workspace: needed where any of ggate (with P > 1), gscale, gweight, gbias, gnext_weight, gnext_bias is
  * wanted. */
 size_t pdw_residual_bwd_workspace_bytes(long long N, int C, long long P, int next_kind, int dtype);

@@ -833,7 +833,7 @@ int pdw_residual_bwd(const void* gout, const void* gnext, const void* x, const v
     if (int e = check_rows("pdw_residual_bwd", N, C, kind, next_kind, act, dtype)) return e;
     if (int e = check_gate("pdw_residual_bwd", gate, N, C, P, &ldgate)) return e;
     const bool next = next_kind != kNormNone;
-    if (N > 0 && (!y || (kind != kNormNone && !stats) || (next && (!x || !next_stats)) || (!gate && ggate)))
+    if (N > 0 && (!gout || !y || (kind != kNormNone && !stats) || (next && (!gnext || !x || !next_stats)) || (!gate && ggate)))
         return set_error("pdw_residual_bwd: null pointer"), 1;
     RowArgs p{};
     p.go = gout, p.gz = gnext, p.x = x, p.y = y, p.gate = gate, p.scale = scale, p.w = weight, p.b = bias, p.w2 = next_weight;

@@ -34,4 +34,41 @@ __device__ __forceinline__ void gate_act_slope(float v, int act, float& f, float
     else f = v * q, slope = q * __builtin_fmaf(v, m, 1.f);
 }
 
+// The same for a lane's pieces of a row (one branch for all of them).
+template <typename P, int N, int VEC>
+__device__ __forceinline__ void gate_acts(const P (&g)[N], int act, float (&a)[N][VEC]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) a[n][i] = to_f32(g[n].v[i]);
+    if (act == kActNone) return;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float q, m;
+            sigmoid_pair(a[n][i], q, m);
+            a[n][i] = act == kActSilu ? a[n][i] * q : q;
+        }
+}
+
+template <typename P, int N, int VEC>
+__device__ __forceinline__ void gate_acts_slopes(const P (&g)[N], int act, float (&a)[N][VEC], float (&slope)[N][VEC]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) a[n][i] = to_f32(g[n].v[i]), slope[n][i] = 1.f;
+    if (act == kActNone) return;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float v = a[n][i];
+            float q, m;
+            sigmoid_pair(v, q, m);
+            a[n][i] = act == kActSilu ? v * q : q;
+            slope[n][i] = q * (act == kActSilu ? __builtin_fmaf(v, m, 1.f) : m);
+        }
+}
+
 }  // namespace pdw

@@ -12,13 +12,12 @@ void rows_launch_f32(const RowArgs& p, unsigned grid, bool backward, hipStream_t
 void rows_launch_f16(const RowArgs& p, unsigned grid, bool backward, hipStream_t s);
 void rows_launch_bf16(const RowArgs& p, unsigned grid, bool backward, hipStream_t s);
 
-// Workgroups of a forward and of a backward pass where there are rows for them: eight and four on each of 256 compute units.
-constexpr int kForwardGroups = 2048, kBackwardGroups = 1024;
-
-// Segments of an image's P rows, and rows of one, for `images` images: a segment is whole passes of a workgroup.
-static void plan_segments(long long images, long long P, int C, int dtype, int target, int* S, long long* L) {
+// Segments of an image's P rows, and rows of one, for `images` images: whole passes of a workgroup, and as many as give a forward pass
+// 2048 workgroups and a backward pass 512 (of eight wavefronts; 1024 where a row takes the whole workgroup).
+static void plan_segments(long long images, long long P, int C, int dtype, bool backward, int* S, long long* L) {
     const int lanes = dtype == kF32 ? rows_lanes_f32(C) : rows_lanes_f16(C);
-    const long long G = 256 / lanes;
+    const long long G = lanes > 64 ? 1 : (backward ? 512 : 256) / lanes;
+    const long long target = !backward ? 2048 : lanes > 256 ? 512 : lanes > 64 ? 1024 : 512;
     long long want = (target + images - 1) / images;
     const long long passes = (P + G - 1) / G;
     if (want > passes) want = passes;
@@ -107,11 +106,11 @@ static void launch_rows(const RowArgs& p, unsigned grid, bool backward, int dtyp
 static long long images_of(const RowArgs& p) { return p.gate_rows == 1 && p.N > 0 ? p.N / p.P : 1; }
 
 // Where there is no gate row an image, all rows are one image.
-static RowArgs cut(const RowArgs& in, int target, int dtype, long long* grid) {
+static RowArgs cut(const RowArgs& in, bool backward, int dtype, long long* grid) {
     RowArgs p = in;
     const long long images = images_of(p);
     if (p.gate_rows != 1) p.P = p.N;
-    plan_segments(images, p.P, p.C, dtype, target, &p.S, &p.L);
+    plan_segments(images, p.P, p.C, dtype, backward, &p.S, &p.L);
     *grid = images * p.S;
     return p;
 }
@@ -119,7 +118,7 @@ static RowArgs cut(const RowArgs& in, int target, int dtype, long long* grid) {
 int rows_forward_launch(const RowArgs& in, int dtype, hipStream_t s) {
     if (in.N == 0) return 0;
     long long grid;
-    const RowArgs p = cut(in, kForwardGroups, dtype, &grid);
+    const RowArgs p = cut(in, false, dtype, &grid);
     if (grid > 0x7fffffffLL) return set_error("norm: too many images (%lld)", images_of(in)), 1;
     launch_rows(p, (unsigned)grid, false, dtype, s);
     return check_launch("rows_fwd_k");
@@ -129,7 +128,7 @@ size_t rows_backward_workspace(long long N, long long images, int C, int sums, i
     if (N <= 0) return 0;
     int S;
     long long L;
-    plan_segments(images, N / images, C, dtype, kBackwardGroups, &S, &L);
+    plan_segments(images, N / images, C, dtype, true, &S, &L);
     return (size_t)images * S * sums * C * sizeof(float);
 }
 
@@ -142,7 +141,7 @@ int rows_backward_launch(const RowArgs& in, void* gscale, void* gw, void* gb, vo
     long long grid = 0;
     p.parts = nullptr, p.S = 0;
     if (in.N > 0) {
-        p = cut(in, kBackwardGroups, dtype, &grid);
+        p = cut(in, true, dtype, &grid);
         if (grid > 0x7fffffffLL) return set_error("norm: too many images (%lld)", images_of(in)), 1;
         p.parts = sums ? (float*)workspace : nullptr;
         const size_t need = (size_t)grid * (branch && next ? 4 : 2) * p.C * sizeof(float);

@@ -190,11 +190,12 @@ struct ResidualNode : public torch::autograd::Node {
         no_second_derivative(*this);
         const bool next = s.next_kind != PDW_NORM_NONE;
         Tensor gout = grads[0], gnext = next ? grads[1] : Tensor();
-        if (!gout.defined() && !gnext.defined()) gout = input_metadata(0).zeros_like();
-        const Tensor& some = gout.defined() ? gout : gnext;
+        // (an output that nothing was made of has a gradient of zero)
+        if (!gout.defined()) gout = input_metadata(0).zeros_like();
+        if (next && !gnext.defined()) gnext = input_metadata(1).zeros_like();
         const auto self = shared_from_this();
-        const auto type = some.scalar_type();
-        const auto dev = some.device();
+        const auto type = gout.scalar_type();
+        const auto dev = gout.device();
         auto take = [&](const Kept& k) { return k.get(self, type, dev); };
         Tensor xv = take(x), yv = take(y), q = take(gate), sc = take(scale), w = take(weight), nw = take(next_weight), b = take(bias);
         Tensor st = stats.get(self, at::kFloat, dev), nst = next_stats.get(self, at::kFloat, dev);

@@ -74,7 +74,7 @@ class GatedResidualFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, gout, gnext=None):
         x, *rest, stats, next_stats = ctx.saved_tensors
-        gout, gnext = (None if t is None else t.contiguous() for t in (gout, gnext))
+        gout, gnext = gout.contiguous(), None if gnext is None else gnext.contiguous()
         grads = ops.residual_backward(gout, gnext, x, *rest, ctx.has_next_bias, stats, next_stats, *ctx.codes)
         return (*grads, None, None, None, None)
 
