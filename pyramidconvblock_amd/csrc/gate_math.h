@@ -59,15 +59,25 @@ __device__ __forceinline__ void gate_acts_slopes(const P (&g)[N], int act, float
 #pragma unroll
         for (int i = 0; i < VEC; ++i) a[n][i] = to_f32(g[n].v[i]), slope[n][i] = 1.f;
     if (act == kActNone) return;
+    if (act == kActSigmoid) {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float m;
+                sigmoid_pair(a[n][i], a[n][i], m);
+                slope[n][i] = a[n][i] * m;
+            }
+        return;
+    }
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float v = a[n][i];
             float q, m;
-            sigmoid_pair(v, q, m);
-            a[n][i] = act == kActSilu ? v * q : q;
-            slope[n][i] = q * (act == kActSilu ? __builtin_fmaf(v, m, 1.f) : m);
+            sigmoid_pair(a[n][i], q, m);
+            slope[n][i] = q * __builtin_fmaf(a[n][i], m, 1.f);
+            a[n][i] *= q;
         }
 }
 

@@ -13,11 +13,11 @@ void rows_launch_f16(const RowArgs& p, unsigned grid, bool backward, hipStream_t
 void rows_launch_bf16(const RowArgs& p, unsigned grid, bool backward, hipStream_t s);
 
 // Segments of an image's P rows, and rows of one, for `images` images: whole passes of a workgroup, and as many as give a forward pass
-// 2048 workgroups and a backward pass 512 (of eight wavefronts; 1024 where a row takes the whole workgroup).
+// 2048 workgroups and a backward pass 512 (of eight wavefronts, or as many as a row takes).
 static void plan_segments(long long images, long long P, int C, int dtype, bool backward, int* S, long long* L) {
     const int lanes = dtype == kF32 ? rows_lanes_f32(C) : rows_lanes_f16(C);
-    const long long G = lanes > 64 ? 1 : (backward ? 512 : 256) / lanes;
-    const long long target = !backward ? 2048 : lanes > 256 ? 512 : lanes > 64 ? 1024 : 512;
+    const long long G = lanes == 0 ? 1 : (backward ? 512 : 256) / lanes;
+    const long long target = !backward ? 2048 : 512;
     long long want = (target + images - 1) / images;
     const long long passes = (P + G - 1) / G;
     if (want > passes) want = passes;

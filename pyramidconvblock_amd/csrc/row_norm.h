@@ -112,9 +112,10 @@ struct RowCols {
     bool on[NCH];
 
     __device__ __forceinline__ RowCols(int lane, int C) {
+        const int lanes = TPR > 64 ? (int)blockDim.x : TPR;
 #pragma unroll
         for (int n = 0; n < NCH; ++n) {
-            const int c = (n * TPR + lane) * VEC;
+            const int c = (n * lanes + lane) * VEC;
             on[n] = c < C;
             at[n] = on[n] ? c : 0, own[n] = 0;
             if (RAG && on[n] && c + VEC > C) at[n] = C - VEC, own[n] = c - at[n];
@@ -152,6 +153,12 @@ struct RowCols {
     }
 };
 
+template <typename P, int N>
+__device__ __forceinline__ void copy_row(P (&to)[N], const P (&from)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) to[n] = from[n];
+}
+
 // Sum over lanes l, l ^ CTRL pattern within 16 lanes, in the VALU (data-parallel primitives).
 template <int CTRL>
 __device__ __forceinline__ float dpp_add(float v) {
@@ -159,28 +166,68 @@ __device__ __forceinline__ float dpp_add(float v) {
     return v + __builtin_bit_cast(float, o);
 }
 
-// Sums of two values over the TPR lanes of a row, in every one of them.  Rows of several wavefronts go through LDS, two buffers in turn
-// (`flip`), so that one barrier a sum is enough.
+// Sum of lanes l and l ^ 16, and l ^ 32: the exchange of two rows of 16 lanes, and of the halves, leaves one side's values in one register
+// and the other side's in the other.
+__device__ __forceinline__ float swap_add16(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const unsigned a = r[0], b = r[1];   // (a bit cast of an element would take the first one both times)
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+__device__ __forceinline__ float swap_add32(float v) {
+    const unsigned u = __builtin_bit_cast(unsigned, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const unsigned a = r[0], b = r[1];   // (a bit cast of an element would take the first one both times)
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// Sums of N values over the lanes of a row, in every one of them.  Rows of several wavefronts go through LDS, two buffers in turn
+// (`flip`), so that one barrier a sum is enough; slots of wavefronts that there are not hold 0 (row_red_clear), so that all are read
+// at once.
+struct RowRed {
+    float v[2][2][16];
+};
 template <int TPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float2 (*red)[16], int& flip) {
-    auto step = [&](auto f) { a = f(a), b = f(b); };
-    step([](float v) { return dpp_add<0xB1>(v); });    // quad permutation 1 0 3 2
-    step([](float v) { return dpp_add<0x4E>(v); });    // quad permutation 2 3 0 1
-    step([](float v) { return dpp_add<0x141>(v); });   // mirrored within 8
-    if constexpr (TPR >= 16) step([](float v) { return dpp_add<0x140>(v); });   // mirrored within 16
-    if constexpr (TPR >= 32) step([](float v) { return v + __shfl_xor(v, 16); });
-    if constexpr (TPR >= 64) step([](float v) { return v + __shfl_xor(v, 32); });
+__device__ __forceinline__ void row_red_clear(RowRed& red) {
     if constexpr (TPR > 64) {
-        if ((threadIdx.x & 63) == 0) red[flip][threadIdx.x >> 6] = make_float2(a, b);
+        if (threadIdx.x < 64) red.v[threadIdx.x >> 5][threadIdx.x >> 4 & 1][threadIdx.x & 15] = 0.f;
         __syncthreads();
-        a = b = 0.f;
+    }
+}
+template <int TPR, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], RowRed& red, int& flip) {
 #pragma unroll
-        for (int w = 0; w < TPR / 64; ++w) a += red[flip][w].x, b += red[flip][w].y;
+    for (int i = 0; i < N; ++i) {
+        v[i] = dpp_add<0xB1>(v[i]);    // quad permutation 1 0 3 2
+        v[i] = dpp_add<0x4E>(v[i]);    // quad permutation 2 3 0 1
+        v[i] = dpp_add<0x141>(v[i]);   // mirrored within 8
+        if constexpr (TPR >= 16) v[i] = dpp_add<0x140>(v[i]);   // mirrored within 16
+        if constexpr (TPR >= 32) v[i] = swap_add16(v[i]);
+        if constexpr (TPR >= 64) v[i] = swap_add32(v[i]);
+    }
+    if constexpr (TPR > 64) {
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i) red.v[flip][i][threadIdx.x >> 6] = v[i];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float* r = red.v[flip][i];
+            float s[TPR / 64];
+#pragma unroll
+            for (int w = 0; w < TPR / 64; ++w) s[w] = r[w];
+#pragma unroll
+            for (int h = TPR / 128; h > 0; h /= 2)
+#pragma unroll
+                for (int w = 0; w < h; ++w) s[w] += s[w + h];
+            v[i] = s[0];
+        }
         flip ^= 1;
     }
 }
 
-// Threads of a workgroup: rows of up to a wavefront share one, longer ones have it to themselves.
+// Threads of a workgroup, at most: rows of up to a wavefront share one, longer ones have it to themselves and as many wavefronts as
+// they need.
 template <int TPR>
 constexpr int row_threads(bool backward) {
     return TPR > 64 ? TPR : backward ? 512 : 256;
@@ -189,16 +236,16 @@ constexpr int row_threads(bool backward) {
 // Mean and reciprocal deviation of a row held in registers.
 template <int VEC, int TPR, int NCH, typename COLS>
 __device__ __forceinline__ float2 row_stats(const float (&v)[NCH][VEC], const COLS& cols, float inv_c, int kind, float eps,
-                                            float2 (*red)[16], int& flip) {
-    float mean = 0.f, zero = 0.f;
+                                            RowRed& red, int& flip) {
+    float mean = 0.f;
     if (kind == kNormLayer) {
-        mean = cols.sum([&](int n, int i) { return v[n][i]; });
-        row_sum2<TPR>(mean, zero, red, flip);
-        mean *= inv_c;
+        float t[1] = {cols.sum([&](int n, int i) { return v[n][i]; })};
+        row_sums<TPR, 1>(t, red, flip);
+        mean = t[0] * inv_c;
     }
-    float q = cols.sum([&](int n, int i) { return (v[n][i] - mean) * (v[n][i] - mean); });
-    row_sum2<TPR>(q, zero, red, flip);
-    return make_float2(mean, __builtin_amdgcn_rsqf(__builtin_fmaf(q, inv_c, eps)));
+    float q[1] = {cols.sum([&](int n, int i) { return (v[n][i] - mean) * (v[n][i] - mean); })};
+    row_sums<TPR, 1>(q, red, flip);
+    return make_float2(mean, __builtin_amdgcn_rsqf(__builtin_fmaf(q[0], inv_c, eps)));
 }
 
 // x + f * norm(y), y's mean and reciprocal deviation in st.
@@ -209,10 +256,11 @@ __device__ __forceinline__ float residual_sum(float x, float f, float y, float2 
 // BRANCH: the residual (otherwise the norm by itself, of x); NEXT: the norm of the sum; FULL: a gate row for every row.
 template <typename T, int VEC, int TPR, int NCH, bool RAG, bool BRANCH, bool NEXT, bool FULL>
 __global__ __launch_bounds__(row_threads<TPR>(false)) void rows_fwd_k(RowArgs p) {
-    constexpr int G = row_threads<TPR>(false) / TPR;
-    __shared__ float2 red[2][16];
+    constexpr int G = TPR > 64 ? 1 : row_threads<TPR>(false) / TPR;
+    __shared__ RowRed red;
     int flip = 0;
-    const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    row_red_clear<TPR>(red);
+    const int lane = TPR > 64 ? threadIdx.x : threadIdx.x % TPR, group = TPR > 64 ? 0 : threadIdx.x / TPR;
     const RowCols<T, VEC, TPR, NCH, RAG> cols(lane, p.C);
     typedef typename RowCols<T, VEC, TPR, NCH, RAG>::Row Row;
     long long r0, r1, image;
@@ -233,12 +281,20 @@ __global__ __launch_bounds__(row_threads<TPR>(false)) void rows_fwd_k(RowArgs p)
             }
     }
     if (NEXT) cols.load_or((const T*)p.w2, 1.f, w2), cols.load_or((const T*)p.b2, 0.f, b2);
+    Row xn, yn, gn;   // of the next row, on their way while this one is computed (behind the last one: the last again)
+    auto load = [&](long long r) {
+        if (BRANCH) cols.load((const T*)p.y + r * p.C, yn);
+        if (FULL) cols.load((const T*)p.gate + r * p.ldg, gn);
+        cols.load((const T*)p.x + r * p.C, xn);
+    };
+    if (r0 + group < r1) load(r0 + group);
     for (long long r = r0 + group; r < r1; r += G) {
         float v[NCH][VEC];
         Row xr, yr, gr;
-        if (BRANCH) cols.load((const T*)p.y + r * p.C, yr);
-        if (FULL) cols.load((const T*)p.gate + r * p.ldg, gr);
-        cols.load((const T*)p.x + r * p.C, xr);
+        copy_row(xr, xn);
+        if (BRANCH) copy_row(yr, yn);
+        if (FULL) copy_row(gr, gn);
+        load(r + G < r1 ? r + G : r);
         if (BRANCH) {
 #pragma unroll
             for (int n = 0; n < NCH; ++n)
@@ -318,12 +374,13 @@ __device__ __forceinline__ void cols_out(float (&acc)[NCH][VEC], const COLS& col
 
 template <typename T, int VEC, int TPR, int NCH, bool RAG, bool BRANCH, bool NEXT, bool FULL>
 __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) {
-    constexpr int THREADS = row_threads<TPR>(true), G = THREADS / TPR;
+    constexpr int THREADS = row_threads<TPR>(true), G = TPR > 64 ? 1 : THREADS / TPR;
     constexpr int SUMS = 2 * ((BRANCH ? 1 : 0) + (NEXT ? 1 : 0));
-    __shared__ float2 red[2][16];
+    __shared__ RowRed red;
     __shared__ float lds[TPR <= 64 ? THREADS / 64 * TPR * NCH * VEC : 1];
     int flip = 0;
-    const int lane = threadIdx.x % TPR, group = threadIdx.x / TPR;
+    row_red_clear<TPR>(red);
+    const int lane = TPR > 64 ? threadIdx.x : threadIdx.x % TPR, group = TPR > 64 ? 0 : threadIdx.x / TPR;
     const RowCols<T, VEC, TPR, NCH, RAG> cols(lane, p.C);
     typedef typename RowCols<T, VEC, TPR, NCH, RAG>::Row Row;
     long long r0, r1, image;
@@ -349,16 +406,27 @@ __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) 
             }
     }
     if (NEXT) cols.load_or((const T*)p.w2, 1.f, w2);
+    Row gon, xn, gzn, yn, gn;   // of the next row, as in the forward
+    float2 stn = make_float2(0.f, 1.f), st2n = stn;
+    auto load = [&](long long r) {
+        if (NEXT) st2n = reinterpret_cast<const float2*>(p.st2)[r];
+        if (BRANCH && p.kind != kNormNone) stn = reinterpret_cast<const float2*>(p.st)[r];
+        if (FULL) cols.load((const T*)p.gate + r * p.ldg, gn);
+        if (BRANCH) cols.load((const T*)p.y + r * p.C, yn);
+        if (NEXT) cols.load((const T*)p.x + r * p.C, xn), cols.load((const T*)p.gz + r * p.C, gzn);
+        if (BRANCH) cols.load((const T*)p.go + r * p.C, gon);
+    };
+    constexpr bool AHEAD = true;
+    if (AHEAD && r0 + group < r1) load(r0 + group);
     for (long long r = r0 + group; r < r1; r += G) {
         float go[NCH][VEC], nv[NCH][VEC], un[NCH][VEC];
         Row gor, xr, gzr, yr, gr;
-        float2 st = make_float2(0.f, 1.f), st2 = st;
-        if (NEXT) st2 = reinterpret_cast<const float2*>(p.st2)[r];
-        if (BRANCH && p.kind != kNormNone) st = reinterpret_cast<const float2*>(p.st)[r];
-        if (FULL) cols.load((const T*)p.gate + r * p.ldg, gr);
-        if (BRANCH) cols.load((const T*)p.y + r * p.C, yr);
-        if (NEXT) cols.load((const T*)p.x + r * p.C, xr), cols.load((const T*)p.gz + r * p.C, gzr);
-        if (BRANCH) cols.load((const T*)p.go + r * p.C, gor);
+        if (!AHEAD) load(r);
+        const float2 st = stn, st2 = st2n;
+        if (FULL) copy_row(gr, gn);
+        if (BRANCH) copy_row(yr, yn), copy_row(gor, gon);
+        if (NEXT) copy_row(xr, xn), copy_row(gzr, gzn);
+        if (AHEAD) load(r + G < r1 ? r + G : r);
         float a[NCH][VEC], slope[NCH][VEC];
         if (FULL) gate_acts_slopes(gr, p.act, a, slope);
         if (NEXT) {
@@ -375,10 +443,9 @@ __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) 
                     un[n][i] = gz * to_f32(w2[n].v[i]);
                     s1n[n][i] = __builtin_fmaf(gz, nv[n][i], s1n[n][i]), s0n[n][i] += gz;
                 }
-            float a1 = cols.sum([&](int n, int i) { return un[n][i] * nv[n][i]; });
-            float a0 = cols.sum([&](int n, int i) { return un[n][i]; });
-            row_sum2<TPR>(a1, a0, red, flip);
-            a1 *= inv_c, a0 = p.kind2 == kNormLayer ? a0 * inv_c : 0.f;
+            float t[2] = {cols.sum([&](int n, int i) { return un[n][i] * nv[n][i]; }), cols.sum([&](int n, int i) { return un[n][i]; })};
+            row_sums<TPR, 2>(t, red, flip);
+            const float a1 = t[0] * inv_c, a0 = p.kind2 == kNormLayer ? t[1] * inv_c : 0.f;
 #pragma unroll
             for (int n = 0; n < NCH; ++n) {
 #pragma unroll
@@ -411,10 +478,9 @@ __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) 
             }
             float a1 = 0.f, a0 = 0.f;
             if (p.kind != kNormNone) {
-                a1 = cols.sum([&](int n, int i) { return un[n][i] * nv[n][i]; });
-                a0 = cols.sum([&](int n, int i) { return un[n][i]; });
-                row_sum2<TPR>(a1, a0, red, flip);
-                a1 *= inv_c, a0 = p.kind == kNormLayer ? a0 * inv_c : 0.f;
+                float t[2] = {cols.sum([&](int n, int i) { return un[n][i] * nv[n][i]; }), cols.sum([&](int n, int i) { return un[n][i]; })};
+                row_sums<TPR, 2>(t, red, flip);
+                a1 = t[0] * inv_c, a0 = p.kind == kNormLayer ? t[1] * inv_c : 0.f;
             }
             if (p.gy) {
 #pragma unroll
@@ -438,12 +504,14 @@ __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) 
 
 template <typename T, int VEC, int TPR, int NCH, bool RAG, bool BRANCH, bool NEXT, bool FULL>
 void rows_pass(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) {
-    if (backward) rows_bwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<grid, row_threads<TPR>(true), 0, s>>>(p);
-    else rows_fwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<grid, row_threads<TPR>(false), 0, s>>>(p);
+    int threads = row_threads<TPR>(backward);
+    if (TPR > 64) threads = ((p.C + VEC - 1) / VEC + 64 * NCH - 1) / (64 * NCH) * 64;
+    if (backward) rows_bwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<grid, threads, 0, s>>>(p);
+    else rows_fwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<grid, threads, 0, s>>>(p);
 }
 
 template <typename T, int VEC, int TPR, int NCH, bool RAG>
-void rows_launch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) {
+void rows_kind(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) {
     const bool branch = p.y != nullptr, next = p.kind2 != kNormNone, full = p.gate_rows == 2;
     if (!branch) rows_pass<T, VEC, TPR, NCH, RAG, false, true, false>(p, grid, backward, s);
     else if (next && full) rows_pass<T, VEC, TPR, NCH, RAG, true, true, true>(p, grid, backward, s);
@@ -452,37 +520,36 @@ void rows_launch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) 
     else rows_pass<T, VEC, TPR, NCH, RAG, true, false, false>(p, grid, backward, s);
 }
 
-// Lanes of a row: as few as hold it in one piece each, so that a wavefront's loads cover whole rows and a lane's column sums stay
-// few (with three pieces a lane the backward of a gated residual had 430 registers, one wavefront on a SIMD and 227 us at
-// [4,64,64,1152] fp16).
+template <typename T, int VEC, int TPR, int NCH>
+void rows_launch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) {
+    if (VEC > 1 && p.C % VEC) rows_kind<T, VEC, TPR, NCH, (VEC > 1)>(p, grid, backward, s);
+    else rows_kind<T, VEC, TPR, NCH, false>(p, grid, backward, s);
+}
+
+// Lanes of a row: one piece of 16 bytes each, in a part of a wavefront or in as many wavefronts as that takes (0 here; of fp32
+// rows beyond 4096 channels two pieces).  The backward of a gated residual with its next norm, [4,64,64,1152] fp16: 24 channels a lane in one
+// wavefront 227 us (430 registers), eight in three wavefronts 84, four in five 104 (the wavefronts wait for each other twice a row).
 template <typename T>
 int row_lanes(int C) {
     constexpr int V = 16 / sizeof(T);
     if (C < V) return 8;
     const int n = (C + V - 1) / V;
-    return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 192 ? 192 : n <= 256 ? 256 : n <= 512 ? 512 : 1024;
+    return n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : n <= 64 ? 64 : 0;
 }
 
 template <typename T>
 void rows_dispatch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) {
     constexpr int V = 16 / sizeof(T);
-    const int n = (p.C + V - 1) / V;
-#define PDW_ROWS(tpr, nch)                                                                       \
-    (p.C % V ? rows_launch<T, V, tpr, nch, true>(p, grid, backward, s) : rows_launch<T, V, tpr, nch, false>(p, grid, backward, s))
-    if (p.C < V) return rows_launch<T, 1, 8, 1, false>(p, grid, backward, s);
+    if (p.C < V) return rows_launch<T, 1, 8, 1>(p, grid, backward, s);
     switch (row_lanes<T>(p.C)) {
-        case 8: return PDW_ROWS(8, 1);
-        case 16: return PDW_ROWS(16, 1);
-        case 32: return PDW_ROWS(32, 1);
-        case 64: return PDW_ROWS(64, 1);
-        case 128: return PDW_ROWS(128, 1);
-        case 192: return PDW_ROWS(192, 1);
-        case 256: return PDW_ROWS(256, 1);
-        case 512: return PDW_ROWS(512, 1);
+        case 8: return rows_launch<T, V, 8, 1>(p, grid, backward, s);
+        case 16: return rows_launch<T, V, 16, 1>(p, grid, backward, s);
+        case 32: return rows_launch<T, V, 32, 1>(p, grid, backward, s);
+        case 64: return rows_launch<T, V, 64, 1>(p, grid, backward, s);
     }
-    if (n <= 1024) PDW_ROWS(1024, 1);
-    else if constexpr (sizeof(T) == 4) PDW_ROWS(1024, 2);
-#undef PDW_ROWS
+    if (p.C <= 512 * V) rows_launch<T, V, 512, 1>(p, grid, backward, s);
+    else if (p.C <= 1024 * V) rows_launch<T, V, 1024, 1>(p, grid, backward, s);
+    else if constexpr (sizeof(T) == 4) rows_launch<T, V, 1024, 2>(p, grid, backward, s);
 }
 
 }  // namespace pdw
