@@ -55,11 +55,41 @@ Tensor packed(const Tensor& t) { return !t.defined() || t.is_contiguous() ? t : 
 
 Tensor floats(at::IntArrayRef sizes, const Tensor& like) { return at::empty(sizes, like.options().dtype(at::kFloat)); }
 
-// Results of a call without rows: gradients of parameters are zero.
-Tensor new_grad(const Tensor& t, bool want, bool empty) {
-    if (!want || !t.defined()) return {};
-    return empty ? at::zeros(t.sizes(), t.options()) : at::empty(t.sizes(), t.options());
-}
+Tensor new_like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
+
+// The gradients of a call's parameters, as pieces of one allocation of 64-byte multiples: an allocation each is 1.4 us on the backward's
+// thread (a gated residual's backward with seven gradients: 75 us of host time, this way 69).
+class ParamGrads {
+  public:
+    // Wants a gradient like t (of these sizes) in *to, unless there is no t.
+    void add(bool want, at::IntArrayRef sizes, Tensor* to) {
+        if (!want) return;
+        parts_.push_back({sizes.vec(), total_, to});
+        int64_t n = 1;
+        for (int64_t e : sizes) n *= e;
+        total_ += (n + 31) / 32 * 32;
+    }
+    // Makes them (zeros for a call without rows).
+    void make(const at::TensorOptions& options, bool zero) {
+        if (parts_.empty()) return;
+        const Tensor all = zero ? at::zeros({total_}, options) : at::empty({total_}, options);
+        for (const Part& q : parts_) {
+            *q.to = at::detail::make_tensor<c10::TensorImpl>(c10::TensorImpl::VIEW, c10::Storage(all.storage()), all.key_set(), all.dtype());
+            q.to->unsafeGetTensorImpl()->set_storage_offset(q.offset);
+            q.to->unsafeGetTensorImpl()->set_sizes_contiguous(q.sizes);
+        }
+    }
+    bool any() const { return !parts_.empty(); }
+
+  private:
+    struct Part {
+        std::vector<int64_t> sizes;
+        int64_t offset;
+        Tensor* to;
+    };
+    std::vector<Part> parts_;
+    int64_t total_ = 0;
+};
 
 // What a node keeps: the input, and its sizes.
 struct Kept {
@@ -106,13 +136,14 @@ struct NormNode : public torch::autograd::Node {
         const int C = (int)xs.size(-1), dt = dtype_code(type);
         const int64_t N = xs.numel() / C;
         variable_list out(kNormInputs);
-        out[kNX] = new_grad(xs, task_should_compute_output(kNX), false);
-        out[kNWeight] = new_grad(w, task_should_compute_output(kNWeight), N == 0);
-        if (has_bias && task_should_compute_output(kNBias))
-            out[kNBias] = N ? at::empty({C}, xs.options()) : at::zeros({C}, xs.options());
+        if (task_should_compute_output(kNX)) out[kNX] = new_like(xs);
+        ParamGrads params;
+        params.add(w.defined() && task_should_compute_output(kNWeight), {C}, &out[kNWeight]);
+        params.add(has_bias && task_should_compute_output(kNBias), {C}, &out[kNBias]);
+        params.make(xs.options(), N == 0);
         if (N == 0) return out;
         Tensor ws;
-        if (out[kNWeight].defined() || out[kNBias].defined()) ws = bytes(pdw_norm_bwd_workspace_bytes(N, C, dt), xs);
+        if (params.any()) ws = bytes(pdw_norm_bwd_workspace_bytes(N, C, dt), xs);
         check(pdw_norm_bwd(ptr(gy), ptr(xs), ptr(w), (const float*)ptr(st), ptr(out[kNX]), ptr(out[kNWeight]), ptr(out[kNBias]), ptr(ws),
                            ws.defined() ? ws.numel() : 0, N, C, kind, dt, stream_of(xs)),
               "pdw_norm_bwd");
@@ -207,18 +238,24 @@ struct ResidualNode : public torch::autograd::Node {
         const bool empty = s.N == 0;
         variable_list r(kResidualInputs);
         auto want = [&](int i) { return task_should_compute_output(i); };
-        if (want(kRX)) r[kRX] = next ? new_grad(yv, true, false) : gout;   // without a next norm x's gradient is out's
-        r[kRY] = new_grad(yv, want(kRY), false);
-        r[kRGate] = new_grad(q, want(kRGate), empty);
-        r[kRScale] = new_grad(sc, want(kRScale), empty), r[kRWeight] = new_grad(w, want(kRWeight), empty);
-        r[kRBias] = new_grad(b, want(kRBias), empty), r[kRNextWeight] = new_grad(nw, want(kRNextWeight), empty);
-        if (has_next_bias && want(kRNextBias))
-            r[kRNextBias] = empty ? at::zeros({s.C}, yv.options()) : at::empty({s.C}, yv.options());
-        if (empty) return r;
+        if (want(kRX)) r[kRX] = next ? new_like(yv) : gout;   // without a next norm x's gradient is out's
+        if (want(kRY)) r[kRY] = new_like(yv);
+        ParamGrads params;
+        const bool image_gate = q.defined() && s.P > 1 && want(kRGate);
+        if (q.defined() && !image_gate && want(kRGate)) r[kRGate] = at::empty(q.sizes(), yv.options());
+        params.add(image_gate, q.defined() ? q.sizes() : at::IntArrayRef(), &r[kRGate]);
+        params.add(sc.defined() && want(kRScale), {s.C}, &r[kRScale]);
+        params.add(w.defined() && want(kRWeight), {s.C}, &r[kRWeight]);
+        params.add(b.defined() && want(kRBias), {s.C}, &r[kRBias]);
+        params.add(nw.defined() && want(kRNextWeight), {s.C}, &r[kRNextWeight]);
+        params.add(has_next_bias && want(kRNextBias), {s.C}, &r[kRNextBias]);
+        params.make(yv.options(), empty);
+        if (empty) {
+            if (r[kRGate].defined()) r[kRGate].zero_();
+            return r;
+        }
         Tensor ws;
-        bool sums = s.P > 1 && r[kRGate].defined();
-        for (int i : {kRScale, kRWeight, kRBias, kRNextWeight, kRNextBias}) sums = sums || r[i].defined();
-        if (sums) ws = bytes(pdw_residual_bwd_workspace_bytes(s.N, s.C, s.P, s.next_kind, s.dtype), yv);
+        if (params.any()) ws = bytes(pdw_residual_bwd_workspace_bytes(s.N, s.C, s.P, s.next_kind, s.dtype), yv);
         check(pdw_residual_bwd(ptr(go), ptr(gn), ptr(xv), ptr(yv), ptr(q), ptr(sc), ptr(w), ptr(b), ptr(nw), (const float*)ptr(st),
                                (const float*)ptr(nst), next ? ptr(r[kRX]) : nullptr, ptr(r[kRY]), ptr(r[kRGate]), ptr(r[kRScale]),
                                ptr(r[kRWeight]), ptr(r[kRBias]), ptr(r[kRNextWeight]), ptr(r[kRNextBias]), ptr(ws),
