@@ -16,10 +16,11 @@
 //
 // All of it is in fp32.  No atomics: results are the same from call to call.
 //
-// What bounds it ([32,3136,128] bf16): instructions first.  Forward a value takes 22 (six of them the sigmoid, two of those at a quarter of
-// the rate), 9 us of the 27 us kernel; backward 41, 16 us of 46; the exchange between lanes and wavefronts, which every wavefront
-// waits for, has most of the rest.  The tensors themselves would take 9 and 15 us.  Two channels a lane rather than four (half the exchanged
-// values for as many steps): forward and backward 107 -> 87 us; stores of whole pieces and one branch a tile: 87 -> 78.
+// What bounds it ([32,3136,128] bf16): instructions and their latencies, with eight wavefronts on a compute unit.  Forward a value takes 22
+// (six of them the sigmoid, two of those at a quarter of the rate), 9 us of the 26 us kernel; backward 41, 16 us of 41; the rest is
+// waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward: four
+// channels a lane 107 us, two (half the exchanged values for as many steps) 87; stores of whole pieces and one branch a tile 78; strips
+// of 16 channels without segments 73; lanes exchanged in the vector unit and one barrier for both scans of the backward 71.
 #pragma once
 #include "common.h"
 #include "gate_math.h"
@@ -47,19 +48,6 @@ struct ScanArgs {
     int reverse, near, near_segments;   // TilePtr's offsets fit, of a tile and of a segment
 };
 
-// Maps of a lane's VEC channels.
-template <int VEC>
-struct Maps {
-    float a[VEC], b[VEC];
-};
-
-// Composes `first` before `m`.
-template <int VEC>
-__device__ __forceinline__ void after(Maps<VEC>& m, const float (&a)[VEC], const float (&b)[VEC]) {
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) m.b[v] = __builtin_fmaf(m.a[v], b[v], m.b[v]), m.a[v] *= a[v];
-}
-
 // Where a lane stands: its channels, and its steps within a tile.
 template <int VEC, int LC, int NW, int K>
 struct ScanLane {
@@ -75,47 +63,98 @@ struct ScanLane {
     }
 };
 
-// The map from the start of the tile to the start of this lane's steps applied to `carry` (the state at the tile's start), and
-// carry taken to the tile's end.  BACK: in the order of falling time.  lds[NW][LC * VEC] x 2 floats, one such buffer a call in turn.
-template <int VEC, int LC, int NW, bool BACK>
-__device__ __forceinline__ void scan_tile(Maps<VEC> m, float (&carry)[VEC], float (&start)[VEC], float2* lds, int lane, int wave) {
-    constexpr int W = LC * VEC;
-    const int cl = lane % LC;
-#pragma unroll
-    for (int d = LC; d < 64; d *= 2) {
-        float a[VEC], b[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            a[v] = BACK ? __shfl_down(m.a[v], d) : __shfl_up(m.a[v], d);
-            b[v] = BACK ? __shfl_down(m.b[v], d) : __shfl_up(m.b[v], d);
-        }
-        if (BACK ? lane + d < 64 : lane >= d) after<VEC>(m, a, b);
+// The values of lanes l and l ^ D: that of the lower one and that of the upper one, in both.  Across 16 and 32 lanes an exchange in the
+// vector unit, across eight a rotation of the row of 16, across four a permutation through LDS.
+template <int D>
+__device__ __forceinline__ void lane_pair(float x, int lane, float& lower, float& upper) {
+    const unsigned u = __builtin_bit_cast(unsigned, x);
+    unsigned lo, hi;
+    if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        lo = r[0], hi = r[1];
+    } else if constexpr (D == 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        lo = r[0], hi = r[1];
+    } else {
+        const unsigned o = D == 8 ? (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, 0x128, 0xf, 0xf, true) : (unsigned)__shfl_xor((int)u, D);
+        lo = lane & D ? o : u, hi = lane & D ? u : o;
     }
-    float ea[VEC], eb[VEC];   // the lanes before this one
+    lower = __builtin_bit_cast(float, lo), upper = __builtin_bit_cast(float, hi);
+}
+
+// What a lane's map (a, b) becomes of a wavefront's: the composition of all (in every lane) and of those before the lane in the order of
+// rising (BACK: falling) time.  Groups of LC lanes are pairs, pairs of pairs, and so on.
+template <int VEC>
+struct WaveMaps {
+    float a[VEC], b[VEC];     // all
+    float ea[VEC], eb[VEC];   // those before
+};
+
+template <int VEC, int LC, int D, bool BACK>
+__device__ __forceinline__ void wave_level(WaveMaps<VEC>& w, const float (&la)[VEC], const float (&ha)[VEC], int lane) {
+    const bool behind = BACK ? !(lane & D) : lane & D;   // the other half comes before this lane's
 #pragma unroll
     for (int v = 0; v < VEC; ++v) {
-        const float a = BACK ? __shfl_down(m.a[v], LC) : __shfl_up(m.a[v], LC);
-        const float b = BACK ? __shfl_down(m.b[v], LC) : __shfl_up(m.b[v], LC);
-        const bool edge = LC == 64 || (BACK ? lane + LC >= 64 : lane < LC);
-        ea[v] = edge ? 1.f : a, eb[v] = edge ? 0.f : b;
+        float lb, hb;
+        lane_pair<D>(w.b[v], lane, lb, hb);
+        const float fa = BACK ? ha[v] : la[v], fb = BACK ? hb : lb, sa = BACK ? la[v] : ha[v], sb = BACK ? lb : hb;
+        w.b[v] = __builtin_fmaf(sa, fb, sb), w.a[v] = sa * fa;
+        if (D == LC) {
+            w.ea[v] = behind ? fa : 1.f, w.eb[v] = behind ? fb : 0.f;
+        } else {
+            const float eb = __builtin_fmaf(w.ea[v], fb, w.eb[v]), ea = w.ea[v] * fa;
+            w.ea[v] = behind ? ea : w.ea[v], w.eb[v] = behind ? eb : w.eb[v];
+        }
     }
-    if (BACK ? lane < LC : lane >= 64 - LC) {
+}
+
+// For one order of time (the other's b NULL), or for both, whose maps have the same a.
+template <int VEC, int LC, int D, bool FORE, bool BACK>
+__device__ __forceinline__ void wave_levels(WaveMaps<VEC>* fore, WaveMaps<VEC>* back, int lane) {
+    if constexpr (D < 64) {
+        float la[VEC], ha[VEC];
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) lds[wave * W + cl * VEC + v] = make_float2(m.a[v], m.b[v]);
+        for (int v = 0; v < VEC; ++v) lane_pair<D>(FORE ? fore->a[v] : back->a[v], lane, la[v], ha[v]);
+        if constexpr (FORE) wave_level<VEC, LC, D, false>(*fore, la, ha, lane);
+        if constexpr (BACK) wave_level<VEC, LC, D, true>(*back, la, ha, lane);
+        wave_levels<VEC, LC, 2 * D, FORE, BACK>(fore, back, lane);
     }
-    __syncthreads();
-#pragma unroll 2   // (unrolled whole, the wavefronts' maps alone take 64 registers)
+}
+
+// The wavefronts' maps: into LDS [NW][LC * VEC] (a, b), and, behind a barrier, through them: `carry`, the state at the tile's start (BACK: the
+// gradient behind its end), is taken to its other side, and `start` is what this lane's steps start from.
+template <int VEC, int LC>
+__device__ __forceinline__ void wave_out(const WaveMaps<VEC>& w, float2* lds, int lane, int wave) {
+    if (lane < LC) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) lds[(wave * LC + lane) * VEC + v] = make_float2(w.a[v], w.b[v]);
+    }
+}
+
+template <int VEC, int LC, int NW, bool BACK>
+__device__ __forceinline__ void wave_in(const WaveMaps<VEC>& m, float (&carry)[VEC], float (&start)[VEC], const float2* lds, int lane, int wave) {
+    const int cl = lane % LC;
+#pragma unroll 2   // (unrolled whole, the wavefronts' maps alone take 32 registers)
     for (int i = 0; i < NW; ++i) {
         const int w = BACK ? NW - 1 - i : i;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
             if (w == wave) start[v] = carry[v];
-            const float2 t = lds[w * W + cl * VEC + v];
+            const float2 t = lds[(w * LC + cl) * VEC + v];
             carry[v] = __builtin_fmaf(t.x, carry[v], t.y);
         }
     }
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) start[v] = __builtin_fmaf(ea[v], start[v], eb[v]);
+    for (int v = 0; v < VEC; ++v) start[v] = __builtin_fmaf(m.ea[v], start[v], m.eb[v]);
+}
+
+// All of it for one order of time; lds: one buffer a call in turn.
+template <int VEC, int LC, int NW, bool BACK>
+__device__ __forceinline__ void scan_tile(WaveMaps<VEC>& m, float (&carry)[VEC], float (&start)[VEC], float2* lds, int lane, int wave) {
+    wave_levels<VEC, LC, LC, !BACK, BACK>(&m, &m, lane);
+    wave_out<VEC, LC>(m, lds, lane, wave);
+    __syncthreads();
+    wave_in<VEC, LC, NW, BACK>(m, carry, start, lds, lane, wave);
 }
 
 // The state that a segment starts from: `first` (the initial state, or the last one's gradient) through the maps of the segments
@@ -131,7 +170,7 @@ __device__ __forceinline__ void segment_start(const ScanArgs& p, int o, int seg,
     if (n == 0) return;
     const int each = (n + TS - 1) / TS;
     const int turn = BACK ? TS - 1 - at.sub : at.sub;   // this lane's place in the order of composition
-    Maps<VEC> m;
+    WaveMaps<VEC> m;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) m.a[v] = 1.f, m.b[v] = 0.f;
     for (int k = 0; k < each; ++k) {
@@ -191,6 +230,9 @@ __device__ __forceinline__ void keep_packed(Piece<T, VEC> (&r)[K]) {
         }
     }
 }
+
+// Steps of a lane that a segment's map is composed in at a time; segments are whole multiples of them.
+constexpr int kMapSteps = 16;
 
 // (a, m) of one piece of g
 template <typename T, int VEC>
@@ -266,9 +308,10 @@ __device__ __forceinline__ void store_steps(T* strip, long long t, long long bas
 
 // The map of every segment but the one that no other starts from (forward the last, BACK the first).  A lane composes a
 // contiguous run of the segment's steps by itself, so the lanes exchange once, at the end.
-template <typename T, int VEC, int LC, int NW, int K, bool BACK>
+template <typename T, int VEC, int LC, int NW, int TK, bool BACK>
 __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
-    typedef ScanLane<VEC, LC, NW, K> Lane;
+    typedef ScanLane<VEC, LC, NW, TK> Lane;
+    constexpr int K = kMapSteps;   // steps under way at once
     constexpr int TS = NW * Lane::kSub;
     __shared__ float2 lds[NW * LC * VEC];
     const ScanWhere my(p);
@@ -279,9 +322,9 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
     const bool given = !BACK || p.gy;
     const long long ot = BACK ? p.dense.t : p.xs.t;
     const T* g = my.base((const T*)p.g, p.gs);
-    const int steps = p.seg_tiles * Lane::kTile, run = steps / TS;   // the segment's steps and a lane's: multiples of K
+    const int steps = p.seg_tiles * Lane::kTile, run = steps / TS;   // the segment's steps and a lane's (a multiple of K)
     const long long first = (long long)seg * steps;
-    Maps<VEC> m;
+    WaveMaps<VEC> m;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) m.a[v] = 1.f, m.b[v] = 0.f;
     auto compose = [&](const Piece<T, VEC>& gp, const Piece<T, VEC>& op) {
@@ -324,7 +367,7 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
         }
     }
     float zero[VEC], one[VEC], unused[VEC];
-    Maps<VEC> product = m;
+    WaveMaps<VEC> product = m;
 #pragma unroll
     for (int v = 0; v < VEC; ++v) zero[v] = 0.f, one[v] = 1.f, product.b[v] = 0.f;
     scan_tile<VEC, LC, NW, BACK>(m, zero, unused, lds, at.lane, at.wave);
@@ -370,7 +413,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scan_fwd_k(ScanArgs p) {
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, b[k][v] = 0.f;
         }
-        Maps<VEC> m;
+        WaveMaps<VEC> m;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) m.a[v] = a[0][v], m.b[v] = b[0][v];
 #pragma unroll
@@ -434,7 +477,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && NW > 2 ? 4 : 3) void sca
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, m[k][v] = 0.f;
         }
-        Maps<VEC> back, fore;
+        WaveMaps<VEC> back, fore;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) back.a[v] = 1.f, back.b[v] = fore.b[v] = 0.f;
 #pragma unroll
@@ -449,8 +492,11 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && NW > 2 ? 4 : 3) void sca
             for (int v = 0; v < VEC; ++v) fore.b[v] = __builtin_fmaf(a[k][v], fore.b[v], m[k][v] * to_f32(xr[k].v[v]));
         // (kept as they were loaded, and converted again where they are used: 16 registers instead of 32)
         keep_packed(xr), keep_packed(gyr);
-        scan_tile<VEC, LC, NW, true>(back, carry, e, lds[tile & 1][0], at.lane, at.wave);
-        scan_tile<VEC, LC, NW, false>(fore, h, hs, lds[tile & 1][1], at.lane, at.wave);
+        wave_levels<VEC, LC, LC, true, true>(&fore, &back, at.lane);
+        wave_out<VEC, LC>(fore, lds[tile & 1][0], at.lane, at.wave), wave_out<VEC, LC>(back, lds[tile & 1][1], at.lane, at.wave);
+        __syncthreads();
+        wave_in<VEC, LC, NW, false>(fore, h, hs, lds[tile & 1][0], at.lane, at.wave);
+        wave_in<VEC, LC, NW, true>(back, carry, e, lds[tile & 1][1], at.lane, at.wave);
         float hx[K][VEC];   // h_(t-1) - x_t
 #pragma unroll
         for (int k = 0; k < K; ++k)
@@ -491,12 +537,13 @@ struct ScanShape {
     int vec, lanes, waves;
     bool segments;
     int width() const { return vec * lanes; }
-    int tile(ScanPass pass) const { return waves * (64 / lanes) * (pass == kScanForward ? kForwardSteps : kBackwardSteps); }
+    int steps(ScanPass pass) const { return pass == kScanForward ? kForwardSteps : kBackwardSteps; }
+    int tile(ScanPass pass) const { return waves * (64 / lanes) * steps(pass); }
 };
 
 // Strips of 32 channels give a chip full of workgroups of four wavefronts where there are 1024 of them; where there are fewer but at least
 // one strip of 32 or 16 channels for every compute unit, workgroups of eight wavefronts, and no segments: x and g are read once, in one
-// launch ([32,3136,128] bf16 forward and backward: 73 us, with segments 78; and twice the traffic where the tensors are in no cache).
+// launch ([32,3136,128] bf16 forward and backward: 71 us, with segments 77, and those read more where the tensors are in no cache).
 // Fewer than that need segments.  As many wavefronts as a chain's steps need, at most; a chain of up
 // to 32 steps has a strip of 64 channels.
 inline ScanShape scan_shape(long long rows, long long T, int I) {

@@ -26,6 +26,8 @@ static ScanCut scan_cut(long long rows, long long T, int I, ScanPass pass) {
     if (want > c.tiles) want = c.tiles;
     if (want < 1) want = 1;
     c.seg_tiles = c.tiles ? (c.tiles + want - 1) / want : 1;
+    const int whole = kMapSteps / c.shape.steps(pass);   // (a segment is whole batches of the kernel that composes its map)
+    if (want > 1 && whole > 1) c.seg_tiles = (c.seg_tiles + whole - 1) / whole * whole;
     c.segments = c.tiles ? (c.tiles + c.seg_tiles - 1) / c.seg_tiles : 1;
     return c;
 }
