@@ -71,7 +71,7 @@ static int check_gate(const char* fn, const void* gate, long long N, int C, long
 static int check_scan(const char* fn, const void* x, const void* g, const long long* xs, const long long* gs, int O, long long T,
                       int W, int I, int dtype) {
     if (!valid_dtype(dtype)) return set_error("%s: unknown dtype %d", fn, dtype), 1;
-    if (O < 0 || T < 0 || W < 0 || I < 0 || (long long)O * W > 0x7fffffffLL)
+    if (O < 0 || T < 0 || W < 0 || I < 0 || (long long)O * W > 0x7fffffffLL || T > 0x7fffffffLL)
         return set_error("%s: bad extents O=%d T=%lld W=%d I=%d", fn, O, T, W, I), 1;
     if (O > 0 && T > 0 && W > 0 && I > 0 && (!x || !g || !xs || !gs)) return set_error("%s: null pointer", fn), 1;
     return 0;

@@ -45,7 +45,7 @@ int scan_run(const ScanArgs& in, bool backward, void* workspace, size_t workspac
     ScanArgs p = in;
     const ScanPass pass = backward ? kScanBackward : kScanForward;
     const ScanCut c = scan_cut(p.rows, p.T, p.I, pass);
-    if (c.strips * p.rows * c.segments > 0x7fffffffLL || c.tiles > 0x7fffffffLL)
+    if (c.strips * p.rows * c.segments > 0x7fffffffLL || c.seg_tiles * c.shape.tile(pass) > 0x7fffffffLL)
         return set_error("scan: too many chains (%d x %d, %lld steps)", p.rows, p.I, p.T), 1;
     const size_t need = scan_workspace(p.rows, p.T, p.I, backward);
     if (need && (!workspace || workspace_bytes < need))

@@ -318,14 +318,15 @@ struct ScanView {
 
 // Strides of t's axes [first, last) as one axis; false where they are none.
 bool collapse(const Tensor& t, int64_t first, int64_t last, long long* stride) {
-    long long step = 0, next = 0;
+    bool any = false;
+    int64_t next = 0;
+    *stride = 0;
     for (int64_t d = last - 1; d >= first; --d) {
         if (t.size(d) == 1) continue;
-        if (step == 0) step = next = t.stride(d);
+        if (!any) *stride = next = t.stride(d), any = true;
         if (t.stride(d) != next) return false;
         next *= t.size(d);
     }
-    *stride = step;
     return true;
 }
 
@@ -349,19 +350,23 @@ void split(const Tensor& xg, Tensor* x, Tensor* g) {
     *x = xg.narrow(-1, 0, C), *g = xg.narrow(-1, C, C);
 }
 
-// Where every tensor's axes behind the recurrence's are dense they are one axis of chains: [O][T][1][W * I].
-void merge(ScanShape* s, std::initializer_list<const ScanView*> views) {
-    if (s->W == 1) return;
+// Where the axes behind the recurrence's are dense in every tensor they are one axis of chains, [O][T][1][W * I].
+bool mergeable(const ScanShape& s, std::initializer_list<const ScanView*> views) {
+    if (s.W == 1 || (int64_t)s.W * s.I > 0x7fffffff) return false;
     for (const ScanView* v : views)
-        if (v->s[2] != s->I) return;
-    if ((int64_t)s->W * s->I > 0x7fffffff) return;
-    s->I *= s->W, s->W = 1;
+        if (v->s[2] != s.I) return false;
+    return true;
+}
+
+ScanShape merged(ScanShape s) {
+    s.I *= s.W, s.W = 1;
+    return s;
 }
 
 struct ScanNode : public torch::autograd::Node {
     Kept x, g, lengths, states;   // (halves: x is the whole tensor)
     ScanShape s;
-    int states_i;   // I of the forward's call: the states lie by it
+    bool one_axis;   // how the forward was called: the states lie by it
     at::DimVector state_sizes;
 
     std::string name() const override { return "GatedScanBackward"; }
@@ -397,14 +402,12 @@ struct ScanNode : public torch::autograd::Node {
         }
         if (task_should_compute_output(kSState)) r[kSState] = floats(state_sizes, xh);
         if (s.O == 0 || s.W == 0 || s.I == 0) return r;
-        const ScanView vx = scan_view(xh, s.dim), vg = scan_view(gh, s.dim);
-        ScanView vgx{gx, {0, 0, 0}}, vgg{gg, {0, 0, 0}};
+        ScanView vx = scan_view(xh, s.dim), vg = scan_view(gh, s.dim), vgx{gx, {0, 0, 0}}, vgg{gg, {0, 0, 0}};
         if (gx.defined()) vgx = scan_view(gx, s.dim);
         if (gg.defined()) vgg = scan_view(gg, s.dim);
-        ScanShape m = s;
-        // (a gradient that is not wanted does not stand in the way)
-        merge(&m, {&vx, &vg, gx.defined() ? &vgx : &vx, gg.defined() ? &vgg : &vg});
-        TORCH_CHECK(m.I == states_i, name(), ": a saved tensor came back in another layout");
+        // (a saved-tensor hook may have brought x and g back in another layout)
+        if (one_axis && !mergeable(s, {&vx, &vg})) vx = scan_view(xh.contiguous(), s.dim), vg = scan_view(gh.contiguous(), s.dim);
+        const ScanShape m = one_axis ? merged(s) : s;
         const size_t need = pdw_scan_workspace_bytes(m.O, m.T, m.W, m.I, 1);
         Tensor ws;
         if (need) ws = bytes(need, xh);
@@ -421,7 +424,7 @@ void scan_forward(const Tensor* in, const Tensor& lengths, const ScanShape& s, a
     const c10::DeviceGuard guard(in[kSX].device());
     Tensor states, len, h0;
     Tensor keep_x = in[kSX], keep_g = in[kSG];   // what the kernels read
-    ScanShape m = s;
+    bool one_axis = false;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         Tensor xh = in[kSX], gh = in[kSG];
@@ -436,7 +439,8 @@ void scan_forward(const Tensor* in, const Tensor& lengths, const ScanShape& s, a
         } else {
             keep_x = vx.t, keep_g = vg.t;
         }
-        merge(&m, {&vx, &vg});
+        one_axis = mergeable(s, {&vx, &vg});
+        const ScanShape m = one_axis ? merged(s) : s;
         len = packed(lengths), h0 = packed(in[kSState]);
         *y = at::empty(y_sizes, in[kSX].options());
         *last = floats(state_sizes, in[kSX]);
@@ -455,7 +459,7 @@ void scan_forward(const Tensor* in, const Tensor& lengths, const ScanShape& s, a
         node->set_next_edges(torch::autograd::collect_next_edges(in[kSX], in[kSG], in[kSState]));
         node->x.keep(in[kSX], keep_x), node->g.keep(in[kSG], keep_g);
         node->lengths.keep(lengths, len), node->states.keep(states, states);
-        node->s = s, node->states_i = m.I, node->state_sizes = state_sizes;
+        node->s = s, node->one_axis = one_axis, node->state_sizes = state_sizes;
         torch::autograd::set_history(*y, node);
         torch::autograd::set_history(*last, node);
     }
@@ -495,6 +499,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (PyErr_Occurred()) return nullptr;
     check_x(in[kNX]);
     check_channels(in[kNX]);
+    TORCH_CHECK_VALUE(eps >= 0, "eps is ", eps);
     check_param(in[kNX], in[kNWeight], "weight"), check_param(in[kNX], in[kNBias], "bias");
     check_devices(in, kNormInputs);
     if (!plain_call(in, kNormInputs)) Py_RETURN_NONE;
@@ -522,6 +527,7 @@ PyObject* py_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor &x = in[kRX], &gate = in[kRGate];
     check_x(x);
     check_channels(x);
+    TORCH_CHECK_VALUE(eps >= 0, "eps is ", eps);
     TORCH_CHECK_TYPE(in[kRY].defined(), "y has to be a tensor");
     check_like(x, in[kRY], "y"), check_like(x, gate, "gate");
     TORCH_CHECK_VALUE(x.sizes() == in[kRY].sizes(), "x and y have to be of one shape, got ", x.sizes(), " and ", in[kRY].sizes());
@@ -580,7 +586,8 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (d < dim) O *= y_sizes[d];
         else if (d > dim && d < rank - 1) W *= y_sizes[d];
     }
-    TORCH_CHECK_VALUE(O <= 0x7fffffff && W <= 0x7fffffff && y_sizes.back() <= 0x7fffffff && O * W <= 0x7fffffff, "too many chains: ", x.sizes());
+    TORCH_CHECK_VALUE(O <= 0x7fffffff && W <= 0x7fffffff && O * W <= 0x7fffffff && y_sizes.back() <= 0x7fffffff && y_sizes[dim] <= 0x7fffffff,
+                      "more than 2^31 chains, channels or steps: ", x.sizes());
     s.O = (int)O, s.T = y_sizes[dim], s.W = (int)W, s.I = (int)y_sizes.back(), s.dim = dim;
     const Tensor& state = in[kSState];
     if (state.defined()) {
@@ -605,10 +612,14 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// Whether two dense tensors share memory without being the same.
-bool overlap(const Tensor& a, const Tensor& b) {
-    const char *p = (const char*)a.data_ptr(), *q = (const char*)b.data_ptr();
-    return p != q && p < q + b.nbytes() && q < p + a.nbytes();
+// Whether a tensor that is written may change what another call's elements are read from: they share memory, and not element by element.
+bool overlap(const Tensor& read, const Tensor& written) {
+    if (!read.defined() || read.numel() == 0) return false;
+    int64_t last = 0;
+    for (int64_t d = 0; d < read.dim(); ++d) last += (read.size(d) - 1) * read.stride(d);
+    const char *p = (const char*)read.data_ptr(), *q = (const char*)written.data_ptr();
+    const bool same = p == q && read.is_contiguous() && read.scalar_type() == written.scalar_type() && read.sizes() == written.sizes();
+    return !same && p < q + written.nbytes() && q < p + (last + 1) * (int64_t)read.element_size();
 }
 
 // scan_step(x, g, state, new_state): y; new_state (or state in place, None) is written.
@@ -633,7 +644,8 @@ PyObject* py_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           at::IntArrayRef(sizes), ", got ", t->sizes());
     }
     const Tensor into = to.defined() ? to : state;
-    TORCH_CHECK_VALUE(!overlap(state, into), "new_state overlaps state");
+    TORCH_CHECK_VALUE(!overlap(state, into) && !overlap(x, into) && !overlap(g, into),
+                      to.defined() ? "new_state" : "state", " overlaps what is read beside it");
     const Tensor all[] = {x, g, state, into};
     check_devices(all, 4);
     TORCH_CHECK(!wants_grad(all, 4), "gated_scan_step has no gradient: call it under torch.no_grad(), or gated_scan");

@@ -181,6 +181,41 @@ def test_slices_transposes_and_odd_addresses():
     assert x.grad.shape == x.shape and x.grad.isfinite().all()
 
 
+@pytest.mark.parametrize("shape,dim,expand", [((3, 4, 50, 8), 2, (0,)), ((3, 4, 50, 8), 2, (1,)), ((3, 4, 50, 8), 2, (0, 1)), ((3, 50, 4, 5, 8), 1, (3,)),
+                                              ((3, 50, 4, 5, 8), 1, (2,)), ((3, 50, 4, 8), 1, (1,)), ((3, 50, 4, 8), 1, (0, 2))], ids=str)
+def test_expanded_dimensions(shape, dim, expand):
+    """Inputs that repeat along some dimensions (strides of zero): bitwise the results of their dense copies, gradients summed."""
+    d = data(shape, dim, torch.float32)
+    index = tuple(slice(0, 1) if i in expand else slice(None) for i in range(len(shape)))
+    small = d["x"][index].cuda().requires_grad_()
+    g, state, gy, glast = (d[k].cuda() for k in ("g", "state", "gy", "glast"))
+    y, last = pcb().gated_scan(small.expand(shape), g, state, dim=dim)
+    (gs,) = torch.autograd.grad([y, last], [small], [gy, glast])
+    dense = small.detach().expand(shape).contiguous().requires_grad_()
+    y2, last2 = pcb().gated_scan(dense, g, state, dim=dim)
+    (gd,) = torch.autograd.grad([y2, last2], [dense], [gy, glast])
+    assert torch.equal(y, y2) and torch.equal(last, last2)
+    assert torch.equal(gs, gd.sum(expand, keepdim=True))
+
+
+def test_saved_tensors_that_come_back_in_another_layout():
+    """Saved-tensor hooks that move tensors to the host and back lay strided ones out anew: the gradients stay as they are."""
+    d = data((2, 40, 6, 8), 1, torch.float32)
+    wide = torch.cat([d["x"], d["g"]], -1).cuda().requires_grad_()
+    turned = d["x"].transpose(1, 2).contiguous().cuda().transpose(1, 2)   # the other way round: dense in no order of its own
+
+    def grads(hooks):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu().contiguous(), lambda t: t.cuda()) if hooks else torch.enable_grad():
+            y, last = pcb().gated_scan(wide, dim=1)
+            z, _ = pcb().gated_scan(turned.requires_grad_(), wide[..., 8:], dim=1)
+            x = d["x"].cuda().requires_grad_()
+            v, _ = pcb().gated_scan(x, d["g"].cuda(), dim=1)
+        return torch.autograd.grad([y, z, v], [wide, turned, x], [d["gy"].cuda()] * 3)
+
+    for a, b in zip(grads(False), grads(True)):
+        assert torch.equal(a, b)
+
+
 def test_extreme_gates():
     """a = 1 holds the state, a = 0 takes the input, exactly, and their gradients are finite."""
     x = torch.randn(2, 200, 16)

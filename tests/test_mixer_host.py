@@ -37,6 +37,8 @@ def test_norm_refusals():
     refused(ValueError, "C <= 8192", f, torch.zeros(1, 8193))
     refused(ValueError, "C <= 8192", f, torch.zeros(3, 0))
     refused(ValueError, "C <= 8192", f, torch.tensor(1.0))
+    refused(ValueError, "eps", f, x, w, eps=-1e-6)
+    refused(ValueError, "eps", pcb().gated_residual, x, x, eps=-1e-6)
     refused(ValueError, "kind", pcb().ChannelNorm, 8, kind="none")
 
 
@@ -94,6 +96,10 @@ def test_scan_refusals():
     refused(ValueError, "one shape", s, x, x[:2], torch.zeros(4, 8))
     store = torch.zeros(64)
     refused(ValueError, "overlap", s, x, x, store[:32].view(4, 8), store[8:40].view(4, 8))
+    refused(ValueError, "overlap", s, store[8:40].view(4, 8), x, store[:32].view(4, 8))
+    refused(ValueError, "overlap", s, x, store.view(4, 16)[:, 8:], x, store[:32].view(4, 8))
+    refused(RuntimeError, "no CPU path", s, x, x, x)                                  # element by element: no harm in it
+    refused(RuntimeError, "no CPU path", s, store[:32].view(4, 8), x, store[32:].view(4, 8))
 
 
 def test_library_refuses_before_any_launch():
@@ -122,7 +128,7 @@ def test_library_refuses_before_any_launch():
     assert need == 2 * 4 * 8 * 4   # a segment for each image, four sums
     assert bwd(1, need - 1) == 1 and bwd(1, need, stats=None) == 1 and bwd(1, need, out=None) == 1
     fwd = lambda O=2, T=5, W=1, I=8, x=1, dtype=0, s=one: L.pdw_scan_fwd(x, 1, None, None, 1, 1, None, None, 0, O, T, W, I, s, s, 0, dtype, None)
-    for bad in (dict(O=-1), dict(T=-1), dict(W=-1), dict(I=-1), dict(x=None), dict(dtype=9), dict(s=None), dict(O=1 << 20, W=1 << 20)):
+    for bad in (dict(O=-1), dict(T=-1), dict(W=-1), dict(I=-1), dict(x=None), dict(dtype=9), dict(s=None), dict(O=1 << 20, W=1 << 20), dict(T=1 << 31)):
         assert fwd(**bad) == 1, bad
     assert fwd(O=0) == 0 and fwd(I=0) == 0
     need = L.pdw_scan_workspace_bytes(1, 10000, 1, 64, 0)
