@@ -9,18 +9,20 @@
 // The states h_(t-1) that gg needs are not kept: the forward leaves the 32-bit state before every tile, and the backward runs the tile
 // from it again, in the same order, from x and g, which it reads anyway.
 //
-// A workgroup has a strip of channels (LC lanes of two channels) and walks over tiles of NW wavefronts x 64/LC lanes x K steps: a lane composes its K consecutive steps in registers, lanes
-// and wavefronts exchange their maps (shuffles; LDS), and every lane runs its K steps from its state.  So x and g are read once.  Where
-// there are too few strips to fill the chip, time is cut into segments of whole tiles: a first launch composes each segment's
-// map (x and g are read once more for it), and the second starts each segment from the maps before it.
+// A workgroup has a strip of channels (LC lanes of two channels) and walks over tiles of NW wavefronts x 64/LC lanes x K steps: a lane
+// composes its K consecutive steps in registers, lanes and wavefronts exchange their maps (vector unit; LDS), and every lane runs its K
+// steps from its state.  So x and g are read once.  Where there are too few strips to fill the chip, time is cut into segments of whole
+// tiles: a first launch composes each segment's map (x and g are read once more for it), and the second starts each segment from the
+// maps before it.
 //
 // All of it is in fp32.  No atomics: results are the same from call to call.
 //
 // What bounds it ([32,3136,128] bf16): instructions and their latencies, with eight wavefronts on a compute unit.  Forward a value takes 22
-// (six of them the sigmoid, two of those at a quarter of the rate), 9 us of the 26 us kernel; backward 41, 16 us of 41; the rest is
+// (six of them the sigmoid, two of those at a quarter of the rate), 9 us of the 25 us kernel; backward 41, 16 us of 37; the rest is
 // waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward: four
 // channels a lane 107 us, two (half the exchanged values for as many steps) 87; stores of whole pieces and one branch a tile 78; strips
-// of 16 channels without segments 73; lanes exchanged in the vector unit and one barrier for both scans of the backward 71.
+// of 16 channels without segments 73; lanes exchanged in the vector unit and one barrier for both scans of the backward 71; the next
+// tile's loads under way 65.  From batches of 64 on it is memory: 4.0 ns for 1000 values, 16 bytes each.
 #pragma once
 #include "common.h"
 #include "gate_math.h"
@@ -379,8 +381,15 @@ __global__ __launch_bounds__(NW * 64) void scan_maps_k(ScanArgs p) {
         reinterpret_cast<float2*>(p.maps)[((long long)seg * p.rows + my.row) * p.I + at.c + v] = make_float2(one[v], zero[v]);
 }
 
+// Workgroups of eight wavefronts, of which a compute unit has one, have the registers for the next tile's loads to be on their way while a
+// tile is computed.
+template <int NW>
+constexpr bool scan_ahead() {
+    return NW == 8;
+}
+
 template <typename T, int VEC, int LC, int NW, int K>
-__global__ __launch_bounds__(NW * 64, 4) void scan_fwd_k(ScanArgs p) {
+__global__ __launch_bounds__(NW * 64, scan_ahead<NW>() ? 2 : 4) void scan_fwd_k(ScanArgs p) {
     typedef ScanLane<VEC, LC, NW, K> Lane;
     constexpr int TS = NW * Lane::kSub;
     __shared__ float2 lds[2][NW * LC * VEC];
@@ -393,12 +402,18 @@ __global__ __launch_bounds__(NW * 64, 4) void scan_fwd_k(ScanArgs p) {
     float carry[VEC];
     segment_start<VEC, LC, NW, K, false>(p, my.row, seg, at, p.h0, carry, lds[1]);
     const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
+    Piece<T, VEC> xr[K], gr[K];
+    auto load = [&](int tile) {
+        const long long base = (long long)tile * Lane::kTile;
+        const bool whole = p.near && base + Lane::kTile <= len;
+        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
+        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
+    };
+    if (scan_ahead<NW>() && t0 < t1) load(t0);
     for (int tile = t0; tile < t1; ++tile) {
         const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
         const bool whole = p.near && base + Lane::kTile <= len;
-        Piece<T, VEC> xr[K], gr[K];
-        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
-        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
+        if (!scan_ahead<NW>()) load(tile);
         float a[K][VEC], b[K][VEC], start[VEC];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -413,6 +428,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scan_fwd_k(ScanArgs p) {
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) a[k][v] = 1.f, b[k][v] = 0.f;
         }
+        if (scan_ahead<NW>() && tile + 1 < t1) load(tile + 1);
         WaveMaps<VEC> m;
 #pragma unroll
         for (int v = 0; v < VEC; ++v) m.a[v] = a[0][v], m.b[v] = b[0][v];
@@ -443,7 +459,7 @@ __global__ __launch_bounds__(NW * 64, 4) void scan_fwd_k(ScanArgs p) {
 }
 
 template <typename T, int VEC, int LC, int NW, int K>
-__global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && NW > 2 ? 4 : 3) void scan_bwd_k(ScanArgs p) {
+__global__ __launch_bounds__(NW * 64, scan_ahead<NW>() ? 2 : sizeof(T) == 2 && NW > 2 && LC > 8 ? 4 : 3) void scan_bwd_k(ScanArgs p) {
     typedef ScanLane<VEC, LC, NW, K> Lane;
     __shared__ float2 lds[2][2][NW * LC * VEC];
     const ScanWhere my(p);
@@ -455,21 +471,32 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 2 && NW > 2 ? 4 : 3) void sca
     float carry[VEC];
     segment_start<VEC, LC, NW, K, true>(p, my.row, seg, at, p.glast, carry, lds[1][0]);
     const int t0 = seg * p.seg_tiles, t1 = t0 + p.seg_tiles < p.tiles ? t0 + p.seg_tiles : p.tiles;
+    Piece<T, VEC> xn[K], gn[K], gyn[K];
+    float hn[VEC];
+    auto load = [&](int tile) {
+        const long long base = (long long)tile * Lane::kTile;
+        const bool whole = p.near && base + Lane::kTile <= len;
+        load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gn);
+        load_steps(gy, p.dense.t, base, p.gy ? len : 0, p.reverse, whole && p.gy, at, gyn);
+        load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xn);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) hn[v] = p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v];
+    };
+    if (scan_ahead<NW>() && t0 < t1) load(t1 - 1);
     for (int tile = t1 - 1; tile >= t0; --tile) {
         const long long base = (long long)tile * Lane::kTile, s0 = base + (long long)at.sub * K;
         const bool whole = p.near && base + Lane::kTile <= len;
         float a[K][VEC], m[K][VEC], e[VEC], hs[VEC], h[VEC];
         Piece<T, VEC> xr[K], gyr[K];
-        {
-            Piece<T, VEC> gr[K];
-            load_steps(g, p.gs.t, base, len, p.reverse, whole, at, gr);
-            load_steps(gy, p.dense.t, base, p.gy ? len : 0, p.reverse, whole && p.gy, at, gyr);
-            load_steps(x, p.xs.t, base, len, p.reverse, whole, at, xr);
+        if (!scan_ahead<NW>()) load(tile);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = p.states[((long long)my.row * p.state_tiles + tile) * p.I + at.c + v];
-#pragma unroll
-            for (int k = 0; k < K; ++k) gates<T, VEC>(gr[k], a[k], m[k]);
+        for (int k = 0; k < K; ++k) {
+            gates<T, VEC>(gn[k], a[k], m[k]);
+            xr[k] = xn[k], gyr[k] = gyn[k];
         }
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) h[v] = hn[v];
+        if (scan_ahead<NW>() && tile > t0) load(tile - 1);
         if (!whole) {
 #pragma unroll
             for (int k = 0; k < K; ++k)
@@ -541,17 +568,23 @@ struct ScanShape {
     int tile(ScanPass pass) const { return waves * (64 / lanes) * steps(pass); }
 };
 
-// Strips of 32 channels give a chip full of workgroups of four wavefronts where there are 1024 of them; where there are fewer but at least
-// one strip of 32 or 16 channels for every compute unit, workgroups of eight wavefronts, and no segments: x and g are read once, in one
-// launch ([32,3136,128] bf16 forward and backward: 71 us, with segments 77, and those read more where the tensors are in no cache).
-// Fewer than that need segments.  As many wavefronts as a chain's steps need, at most; a chain of up
-// to 32 steps has a strip of 64 channels.
+// Without segments x and g are read once, in one launch, as long as there are workgroups for the chip: of eight wavefronts one on each of
+// the 256 compute units, of four wavefronts four on each.  Strips are of 32 channels, of 16 where only those come near 256.
+// Microseconds, forward and backward, [B,3136,128] bf16 (strips of 32: 4 B, of 16: 8 B):
+//     B     32 channels, 8 wavefronts     4 wavefronts     16 channels, 8 wavefronts     segments
+//     32                81                    118                     65                    78
+//     38                82                    121                    107                    90
+//     64               101                    145                    130                   133
+//     96               182                    195                    207                   208
+//     128              207                    219                    282                   276
+// and [275,784,128]: 155, 126, 186, 154.  As many wavefronts as a chain's steps need, at most; a chain of up to 32 steps has a strip
+// of 64 channels.
 inline ScanShape scan_shape(long long rows, long long T, int I) {
     if (I < 2) return {1, 4, 4, true};
     const long long wide = rows * ((I + 31) / 32), narrow = rows * ((I + 15) / 16);
-    const bool many = wide >= 1024, segments = narrow < 256;
-    int lanes = T <= 32 ? 32 : many || segments || wide >= 256 ? 16 : 8;
-    const int most = many || segments ? 4 : 8;
+    const bool segments = narrow < 208;
+    int lanes = T <= 32 ? 32 : !segments && narrow <= 256 ? 8 : 16;
+    const int most = segments || (wide > 256 && wide < 352) || wide > 512 ? 4 : 8;
     int waves = 1;
     while (waves < most && waves * (64 / lanes) * kForwardSteps < T) waves *= 2;
     if (const char* e = tune_env("PDW_SCAN_LANES")) lanes = atoi(e);
