@@ -12,12 +12,22 @@ void rows_launch_f32(const RowArgs& p, unsigned grid, bool backward, hipStream_t
 void rows_launch_f16(const RowArgs& p, unsigned grid, bool backward, hipStream_t s);
 void rows_launch_bf16(const RowArgs& p, unsigned grid, bool backward, hipStream_t s);
 
-// Segments of an image's P rows, and rows of one, for `images` images: whole passes of a workgroup, and as many as give a forward pass
-// 2048 workgroups and a backward pass 512 (of eight wavefronts, or as many as a row takes).
-static void plan_segments(long long images, long long P, int C, int dtype, bool backward, int* S, long long* L) {
+// Segments of an image's P rows, and rows of one, for `images` images: whole passes of a workgroup, and as many as give the chip the
+// workgroups that measured best, a multiple of its 256 compute units: forward 2048, backward 512 (of eight wavefronts).  Rows of several
+// wavefronts have a workgroup to themselves, and those of two to four wavefronts more of them (16-bit norm of 768 channels,
+// forward: 2048 workgroups 4.4 TB/s, 4096 4.8; backward with the forward before it: 512 3.3, 1536 3.9; residual with its next norm, whose
+// four column sums and what goes with them leave room for fewer: 512 3.1, 1024 3.9, 1536 3.5; of 1152 channels 512 3.6, 768 3.4).
+static void plan_segments(long long images, long long P, int C, int dtype, bool backward, int sums, int* S, long long* L) {
     const int lanes = dtype == kF32 ? rows_lanes_f32(C) : rows_lanes_f16(C);
-    const long long G = lanes == 0 ? 1 : (backward ? 512 : 256) / lanes;
-    const long long target = !backward ? 2048 : 512;
+    long long G = 1, target = !backward ? 2048 : 512;
+    if (lanes > 0) {
+        G = (backward ? 512 : 256) / lanes;
+    } else {
+        const int pieces = cdiv(C, dtype == kF32 ? 4 : 8), waves = pieces > 512 ? 8 : cdiv(pieces, 64);
+        if (!backward) target = waves <= 3 ? 4096 : 2048;
+        else if (sums == 4) target = waves == 2 ? 1024 : 512;
+        else target = waves == 2 ? 1536 : waves == 3 ? 1024 : waves == 4 ? 768 : 512;
+    }
     long long want = (target + images - 1) / images;
     const long long passes = (P + G - 1) / G;
     if (want > passes) want = passes;
@@ -110,7 +120,7 @@ static RowArgs cut(const RowArgs& in, bool backward, int dtype, long long* grid)
     RowArgs p = in;
     const long long images = images_of(p);
     if (p.gate_rows != 1) p.P = p.N;
-    plan_segments(images, p.P, p.C, dtype, backward, &p.S, &p.L);
+    plan_segments(images, p.P, p.C, dtype, backward, p.y && p.kind2 != kNormNone ? 4 : 2, &p.S, &p.L);
     *grid = images * p.S;
     return p;
 }
@@ -128,7 +138,7 @@ size_t rows_backward_workspace(long long N, long long images, int C, int sums, i
     if (N <= 0) return 0;
     int S;
     long long L;
-    plan_segments(images, N / images, C, dtype, true, &S, &L);
+    plan_segments(images, N / images, C, dtype, true, sums, &S, &L);
     return (size_t)images * S * sums * C * sizeof(float);
 }
 

@@ -526,8 +526,8 @@ void rows_launch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) 
     else rows_kind<T, VEC, TPR, NCH, false>(p, grid, backward, s);
 }
 
-// Lanes of a row: one piece of 16 bytes each, in a part of a wavefront or in as many wavefronts as that takes (0 here; of fp32
-// rows beyond 4096 channels two pieces).  The backward of a gated residual with its next norm, [4,64,64,1152] fp16: 24 channels a lane in one
+// Lanes of a row: one piece of 16 bytes each, in a part of a wavefront or in as many wavefronts as that takes, up to eight (0 here;
+// behind 4096 channels, in fp32 2048, several pieces).  The backward of a gated residual with its next norm, [4,64,64,1152] fp16: 24 channels a lane in one
 // wavefront 227 us (430 registers), eight in three wavefronts 84, four in five 104 (the wavefronts wait for each other twice a row).
 template <typename T>
 int row_lanes(int C) {
@@ -548,8 +548,8 @@ void rows_dispatch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s
         case 64: return rows_launch<T, V, 64, 1>(p, grid, backward, s);
     }
     if (p.C <= 512 * V) rows_launch<T, V, 512, 1>(p, grid, backward, s);
-    else if (p.C <= 1024 * V) rows_launch<T, V, 1024, 1>(p, grid, backward, s);
-    else if constexpr (sizeof(T) == 4) rows_launch<T, V, 1024, 2>(p, grid, backward, s);
+    else if (p.C <= 1024 * V) rows_launch<T, V, 512, 2>(p, grid, backward, s);
+    else if constexpr (sizeof(T) == 4) rows_launch<T, V, 512, 4>(p, grid, backward, s);
 }
 
 }  // namespace pdw
