@@ -527,8 +527,9 @@ void rows_launch(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) 
 }
 
 // Lanes of a row: one piece of 16 bytes each, in a part of a wavefront or in as many wavefronts as that takes, up to eight (0 here;
-// behind 4096 channels, in fp32 2048, several pieces).  The backward of a gated residual with its next norm, [4,64,64,1152] fp16: 24 channels a lane in one
-// wavefront 227 us (430 registers), eight in three wavefronts 84, four in five 104 (the wavefronts wait for each other twice a row).
+// behind 4096 channels, in fp32 2048, several pieces).  The backward of a gated residual with its next norm, [4,64,64,1152] fp16: 24
+// channels a lane in one wavefront 227 us (430 registers), eight in three wavefronts 84, four in five 104 (the wavefronts wait for each
+// other twice a row).
 template <typename T>
 int row_lanes(int C) {
     constexpr int V = 16 / sizeof(T);
