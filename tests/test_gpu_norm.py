@@ -221,7 +221,7 @@ FORMS = [("none", "none", "none", "", "none", "", False), ("none", "none", "rms"
          ("image", "sigmoid", "rms", "wb", "none", "", False), ("full", "silu", "layer", "wb", "rms", "w", True),
          ("full", "none", "rms", "w", "layer", "wb", False), ("full", "sigmoid", "none", "wb", "layer", "", True)]
 RESIDUAL_SHAPES = [(1, 1, 1), (1, 5, 8), (2, 3, 7), (3, 5, 9), (2, 4, 4, 64), (5, 1, 72), (3, 7, 9, 200), (2, 19, 201), (2, 3, 520),
-                   (2, 3, 1152), (2, 2, 1601), (1, 3, 4096), (2, 1, 8192), (2, 1031, 48)]
+                   (2, 3, 1152), (2, 2, 1601), (1, 3, 4096), (2, 1, 8192), (2, 1031, 48), (3000, 2, 24)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -280,6 +280,32 @@ def test_gradients_against_differences():
         quotient = (loss({**dd, k: dd[k] + h * direction}) - loss({**dd, k: dd[k] - h * direction})) / (2 * h)
         prods = got[g].double().cpu() * direction
         assert abs(quotient - float(prods.sum())) <= 1e-5 * float(prods.abs().sum()) + 1e-5, k
+
+
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^31 values: the last rows are bitwise those of a call on them alone; the weights' gradients are theirs, since
+    every other row's is zero."""
+    N, C, last = (1 << 31) // 4096 + 1000, 4096, 64
+    x = torch.zeros(N, C, device="cuda", dtype=torch.bfloat16)
+    gy = torch.zeros_like(x)
+    gen = torch.Generator().manual_seed(2)
+    xl, gl = rnd(gen, last, C, dtype=torch.bfloat16).cuda(), rnd(gen, last, C, dtype=torch.bfloat16).cuda()
+    x[-last:], gy[-last:] = xl, gl
+    w, b = rnd(gen, C, dtype=torch.bfloat16, mean=1.0, std=0.2).cuda().requires_grad_(), rnd(gen, C, dtype=torch.bfloat16).cuda().requires_grad_()
+    assert x.numel() > 1 << 31
+    x.requires_grad_(), xl.requires_grad_()
+    y, yl = pcb().channel_norm(x, w, b, kind="layer"), pcb().channel_norm(xl, w, b, kind="layer")
+    assert torch.equal(y[-last:], yl) and torch.equal(y[0], b)
+    gx, gw, gb = torch.autograd.grad(y, [x, w, b], gy)
+    gxl, gwl, gbl = torch.autograd.grad(yl, [xl, w, b], gl)
+    assert torch.equal(gx[-last:], gxl) and not gx[:-last].any()
+    n = norm64(xl.detach().double().cpu(), None, None, "layer")
+    check(gw, (gl.double().cpu() * n[1]).sum(0), rows_slack(gl.double().cpu() * n[1], gl.double().cpu().abs() * n[3]), "gw")
+    check(gb, gl.double().cpu().sum(0), rows_slack(gl.double().cpu(), 0 * gl.double().cpu()), "gb")
+    del y, gx
+    out = pcb().gated_residual(x, x, w, b, scale=w, kind="layer")
+    outl = pcb().gated_residual(xl, xl, w, b, scale=w, kind="layer")
+    assert torch.equal(out[-last:], outl)
 
 
 def test_constant_rows_and_large_offsets():
@@ -395,6 +421,30 @@ def test_no_second_derivative_and_function_form():
     gn = torch.randn_like(y)
     for a, b in zip(torch.autograd.grad(pair, [x, w, gate], [g, gn]), torch.autograd.grad(pair_f, [x, w, gate], [g, gn])):
         assert torch.equal(a, b)
+
+
+def test_checkpointed_and_transformed_calls():
+    """Under activation checkpointing the same bits; forward-mode derivatives and batching are refused, not left out."""
+    from torch.utils.checkpoint import checkpoint
+
+    x, gate = torch.randn(3, 5, 24, device="cuda", requires_grad=True), torch.randn(3, 24, device="cuda", requires_grad=True)
+    w = torch.rand(24, device="cuda", requires_grad=True)
+
+    def f(x, gate, w):
+        z = pcb().channel_norm(x, w, kind="layer")
+        y, last = pcb().gated_scan(z, z * 2)
+        out, nxt = pcb().gated_residual(x, y, w, gate=gate, kind="rms", activation="silu", next_weight=w, next_kind="layer")
+        return out.sum() + nxt.square().sum() + last.sum()
+
+    plain = torch.autograd.grad(f(x, gate, w), [x, gate, w])
+    kept = torch.autograd.grad(checkpoint(f, x, gate, w, use_reentrant=False), [x, gate, w])
+    for a, b in zip(plain, kept):
+        assert torch.equal(a, b)
+    for call in (lambda t: pcb().channel_norm(t), lambda t: pcb().gated_residual(t, t, kind="rms"), lambda t: pcb().gated_scan(t, t)[0]):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(call, (x.detach(),), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError):
+            torch.func.vmap(call)(x.detach()[None])
 
 
 def test_saved_tensor_changed_in_place_is_noticed():

@@ -111,7 +111,8 @@ def compare(d, got, dim, reverse):
 # chains of one step to several tiles and segments; channels that fill strips and that do not; axes before, between and behind others
 SHAPES = [((1, 1, 1), 1), ((2, 1, 8), 1), ((3, 2, 3), 1), ((2, 5, 64), 1), ((1, 33, 5), 1), ((4, 16, 66), 1), ((2, 65, 130), 1),
           ((2, 129, 20), 1), ((1, 257, 67), 1), ((3, 600, 24), 1), ((1, 3001, 65), 1), ((2, 1500, 2), 1), ((1, 5000, 1), 1), ((17, 9), 0), ((300, 7), 0),
-          ((2, 9, 11, 24), 1), ((2, 9, 11, 24), 2), ((2, 3, 40, 5, 6), 2), ((300, 40, 16), 1), ((130, 300, 130), 1)]
+          ((2, 9, 11, 24), 1), ((2, 9, 11, 24), 2), ((2, 3, 40, 5, 6), 2), ((300, 40, 16), 1), ((130, 300, 130), 1),
+          ((32, 2100, 100), 1), ((20, 1500, 200), 1)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -124,7 +125,7 @@ def test_scan(shape, dim, reverse, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reverse", [False, True])
-@pytest.mark.parametrize("shape,dim", [((6, 40, 24), 1), ((5, 300, 10), 1), ((4, 2000, 70), 1), ((3, 4, 50, 8), 2), ((3, 50, 4, 8), 1), ((6, 3, 2), 1)],
+@pytest.mark.parametrize("shape,dim", [((6, 40, 24), 1), ((5, 300, 10), 1), ((4, 2000, 70), 1), ((3, 4, 50, 8), 2), ((3, 50, 4, 8), 1), ((6, 3, 2), 1), ((33, 1300, 98), 1)],
                          ids=str)
 def test_lengths_leave_the_rest_alone(shape, dim, reverse, dtype):
     """Lengths of 0, 1, T - 1, T and between, what lies behind them NaN and infinities in x, g and gy: not read, and 0 in results."""
@@ -214,6 +215,42 @@ def test_saved_tensors_that_come_back_in_another_layout():
 
     for a, b in zip(grads(False), grads(True)):
         assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 values, and a step of more than 2^21 values between positions: the results of dense small tensors (the second bitwise;
+    the first is cut otherwise, so its states differ by up to 64 u of the largest, as many roundings as a state has on its way; two
+    results of bfloat16 that are each half a step, 2^-8 of the value, off the state they round differ by up to 2^-7 of it more)."""
+    O, T, C = 3, 360000, 2000
+    x = torch.zeros(O, T, C, device="cuda", dtype=torch.bfloat16)
+    g = torch.full_like(x, 2.0)
+    gen = torch.Generator().manual_seed(4)
+    xl = torch.randn(1, T, 8, generator=gen).bfloat16().cuda()
+    x[2:, :, -8:] = xl
+    assert x.numel() > 1 << 31
+    x.requires_grad_()
+    y, last = pcb().gated_scan(x, g)
+    a = xl.clone().requires_grad_()
+    yl, lastl = pcb().gated_scan(a, g[2:, :, -8:])
+    assert ((y[2:, :, -8:].float() - yl.float()).abs() <= 2.0 ** -7 * yl.float().abs() + 64 * U * 5).all()
+    assert ((last[2:, -8:] - lastl).abs() <= 64 * U * 5).all() and not y[:2].any()
+    gy = torch.zeros_like(x)
+    gy[2:, :, -8:] = xl
+    (gx,), (gl,) = torch.autograd.grad(y, [x], gy), torch.autograd.grad(yl, [a], xl)
+    assert ((gx[2:, :, -8:].float() - gl.float()).abs() <= 2.0 ** -7 * gl.float().abs() + 64 * U * 5).all() and not gx[:2].any()
+    del x, g, y, gy, gx, last
+
+    wide = torch.empty(1, 700, 3 << 20, device="cuda", dtype=torch.bfloat16)
+    d = data((1, 700, 8), 1, torch.bfloat16)
+    base = run(d, 1, True)
+    x, g = wide[..., 5:13], wide[..., -9:-1]
+    x.copy_(d["x"]), g.copy_(d["g"])
+    x, g, state = x.detach().requires_grad_(), g.detach().requires_grad_(), d["state"].cuda().requires_grad_()
+    assert x.stride(1) > 1 << 21
+    y, last = pcb().gated_scan(x, g, state, reverse=True)
+    grads = torch.autograd.grad([y, last], [x, g, state], [d["gy"].cuda(), d["glast"].cuda()])
+    for t, k in zip((y, last, *grads), ("y", "last", "gx", "gg", "gstate")):
+        assert torch.equal(t, base[k]), k
 
 
 def test_extreme_gates():
