@@ -498,7 +498,7 @@ int pdw_norm_bwd(const void *gy, const void *x, const void *weight, const float 
 
 /* out = x + scale * act(gate) * norm(y), and with next_kind other than PDW_NORM_NONE also next = norm'(out), the norm before
  * the block that follows (of out as it is before rounding).  gate: NULL; one row for P consecutive rows of x (an image's; N must be a
- * multiple of P); with P = 1 a value for each.  Gate rows are ldgate elements apart (0: C).  stats, next_stats: of y and of out. */
+ * multiple of P); with P = 1, as without a gate, a value for each.  Gate rows are ldgate elements apart (0: C).  stats, next_stats: of y and of out. */
 int pdw_residual_fwd(const void *x, const void *y, const void *gate, const void *scale, const void *weight, const void *bias,
                      const void *next_weight, const void *next_bias, void *out, void *next, float *stats, float *next_stats,
                      long long N, int C, long long P, long long ldgate, int act, int kind, int next_kind, float eps, int dtype,

@@ -428,6 +428,33 @@ def test_other_stream_and_repeatability():
         assert torch.equal(base[k], again[k]), k
 
 
+def test_two_streams_at_once():
+    """Passes on two streams, under way together, forward and backward of all three operators: bitwise what each is by itself."""
+    dt = torch.bfloat16
+    sets = [[torch.randn(2, 2500, 96, device="cuda").to(dt).requires_grad_() for _ in range(3)] for _ in range(2)]
+    w = torch.rand(96, device="cuda").to(dt)
+
+    def f(x, g, gate):
+        z = pcb().channel_norm(x, w, kind="layer")
+        y, last = pcb().gated_scan(z, g)
+        out, nxt = pcb().gated_residual(x, y, w, gate=gate, kind="rms", activation="sigmoid", next_weight=w, next_kind="rms")
+        return [out.detach(), nxt.detach(), last.detach(), *torch.autograd.grad([out, nxt], [x, g, gate], [z.detach(), y.detach()])]
+
+    alone = [f(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    results = [[], []]
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results[i].append(f(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in results[i]:
+            for a, b in zip(r, alone[i]):
+                assert torch.equal(a, b)
+
+
 def test_captured_passes_replay():
     """Two graphs, one of a long chain cut into segments and one of steps, replayed with eager work between: every replay is the
     eager result on the same inputs."""
