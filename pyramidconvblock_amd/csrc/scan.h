@@ -18,11 +18,12 @@
 // All of it is in fp32.  No atomics: results are the same from call to call.
 //
 // What bounds it ([32,3136,128] bf16): instructions and their latencies, with eight wavefronts on a compute unit.  Forward a value takes 22
-// (six of them the sigmoid, two of those at a quarter of the rate), 9 us of the 25 us kernel; backward 41, 16 us of 37; the rest is
+// (six of them the sigmoid, two of those at a quarter of the rate), 9 us of the 23 us kernel; backward 41, 16 us of 33; the rest is
 // waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward: four
 // channels a lane 107 us, two (half the exchanged values for as many steps) 87; stores of whole pieces and one branch a tile 78; strips
 // of 16 channels without segments 73; lanes exchanged in the vector unit and one barrier for both scans of the backward 71; the next
-// tile's loads under way 65.  From batches of 64 on it is memory: 4.0 ns for 1000 values, 16 bytes each.
+// tile's loads under way 65; steps a lane that leave the last tile least empty 60.  From batches of 64 on it is memory: 3.8 ns for 1000
+// values, 16 bytes each.
 #pragma once
 #include "common.h"
 #include "gate_math.h"
@@ -556,15 +557,14 @@ __global__ __launch_bounds__(NW * 64, scan_ahead<NW>() ? 2 : sizeof(T) == 2 && N
 
 enum ScanPass { kScanForward, kScanBackward };
 
-// A lane has two channels and 16 steps of a tile forward, eight backward, where three tensors and two scans are held.
-constexpr int kForwardSteps = 16, kBackwardSteps = 8;
-
-// How a call is cut: channels of a lane, lanes of a strip, wavefronts of a workgroup, and whether time is cut into segments.
+// How a call is cut: channels of a lane, lanes of a strip, wavefronts of a workgroup, whether time is cut into segments, and a lane's steps
+// of a tile backward, up to eight (three tensors and two scans are held); forward it has twice as many.
 struct ScanShape {
     int vec, lanes, waves;
     bool segments;
+    int back;
     int width() const { return vec * lanes; }
-    int steps(ScanPass pass) const { return pass == kScanForward ? kForwardSteps : kBackwardSteps; }
+    int steps(ScanPass pass) const { return pass == kScanForward ? 2 * back : back; }
     int tile(ScanPass pass) const { return waves * (64 / lanes) * steps(pass); }
 };
 
@@ -578,47 +578,65 @@ struct ScanShape {
 //     96               182                    195                    207                   208
 //     128              207                    219                    282                   276
 // and [275,784,128]: 155, 126, 186, 154.  As many wavefronts as a chain's steps need, at most; a chain of up to 32 steps has a strip
-// of 64 channels.
+// of 64 channels.  A chain without segments ends with a tile that costs as much as a whole one: of eight, seven and six steps a lane the
+// number is taken that has the fewest steps in all, with three for a tile's exchange.  A pass of both directions with eight alone and with
+// this rule: [32,3136,128] 65, 60 us (tiles of 896 steps forward instead of 1024), [64,3136,128] 99, 95, [275,784,128] 127, 120,
+// [275,196,128] 46, 43, [64,1800,128] 61, 61 (six steps there would take 62).
 inline ScanShape scan_shape(long long rows, long long T, int I) {
-    if (I < 2) return {1, 4, 4, true};
+    if (I < 2) return {1, 4, 4, true, 8};
     const long long wide = rows * ((I + 31) / 32), narrow = rows * ((I + 15) / 16);
     const bool segments = narrow < 208;
-    int lanes = T <= 32 ? 32 : !segments && narrow <= 256 ? 8 : 16;
+    const int lanes = T <= 32 ? 32 : !segments && narrow <= 256 ? 8 : 16;
     const int most = segments || (wide > 256 && wide < 352) || wide > 512 ? 4 : 8;
     int waves = 1;
-    while (waves < most && waves * (64 / lanes) * kForwardSteps < T) waves *= 2;
-    if (const char* e = tune_env("PDW_SCAN_LANES")) lanes = atoi(e);
-    if (const char* e = tune_env("PDW_SCAN_WAVES")) waves = atoi(e);
-    return {2, lanes, waves, segments};
+    while (waves < most && waves * (64 / lanes) * 16 < T) waves *= 2;
+    ScanShape shape{2, lanes, waves, segments, 8};
+    auto cost = [&](int back) {
+        const long long tile = (long long)waves * (64 / lanes) * back;
+        return (T + tile - 1) / tile * (back + 3) + (T + 2 * tile - 1) / (2 * tile) * (2 * back + 3);
+    };
+    if (!segments)
+        for (int back : {7, 6})
+            if (cost(back) < cost(shape.back)) shape.back = back;
+    return shape;
 }
 
-template <typename T, int VEC, int LC, int NW>
+template <typename T, int VEC, int LC, int NW, int BACK>
 void scan_launch(const ScanArgs& p, ScanPass pass, hipStream_t s) {
     const unsigned columns = (unsigned)p.strips * (unsigned)p.rows;
-    if (p.segments > 1) {
-        const unsigned n = columns * (unsigned)(p.segments - 1);
-        if (pass == kScanForward) scan_maps_k<T, VEC, LC, NW, kForwardSteps, false><<<n, NW * 64, 0, s>>>(p);
-        else scan_maps_k<T, VEC, LC, NW, kBackwardSteps, true><<<n, NW * 64, 0, s>>>(p);
+    if constexpr (BACK == 8 && NW <= 4 && (LC == 16 || VEC == 1)) {   // (the shapes that are cut into segments)
+        if (p.segments > 1) {
+            const unsigned n = columns * (unsigned)(p.segments - 1);
+            if (pass == kScanForward) scan_maps_k<T, VEC, LC, NW, 2 * BACK, false><<<n, NW * 64, 0, s>>>(p);
+            else scan_maps_k<T, VEC, LC, NW, BACK, true><<<n, NW * 64, 0, s>>>(p);
+        }
     }
     const unsigned n = columns * (unsigned)p.segments;
-    if (pass == kScanForward) scan_fwd_k<T, VEC, LC, NW, kForwardSteps><<<n, NW * 64, 0, s>>>(p);
-    else scan_bwd_k<T, VEC, LC, NW, kBackwardSteps><<<n, NW * 64, 0, s>>>(p);
+    if (pass == kScanForward) scan_fwd_k<T, VEC, LC, NW, 2 * BACK><<<n, NW * 64, 0, s>>>(p);
+    else scan_bwd_k<T, VEC, LC, NW, BACK><<<n, NW * 64, 0, s>>>(p);
 }
 
-template <typename T, int LC>
+template <typename T, int LC, int BACK>
 void scan_waves(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) {
-    if (shape.waves == 1) scan_launch<T, 2, LC, 1>(p, pass, s);
-    else if (shape.waves == 2) scan_launch<T, 2, LC, 2>(p, pass, s);
-    else if (shape.waves == 4) scan_launch<T, 2, LC, 4>(p, pass, s);
-    else scan_launch<T, 2, LC, 8>(p, pass, s);
+    if (shape.waves == 1) scan_launch<T, 2, LC, 1, BACK>(p, pass, s);
+    else if (shape.waves == 2) scan_launch<T, 2, LC, 2, BACK>(p, pass, s);
+    else if (shape.waves == 4) scan_launch<T, 2, LC, 4, BACK>(p, pass, s);
+    else scan_launch<T, 2, LC, 8, BACK>(p, pass, s);
+}
+
+template <typename T, int BACK>
+void scan_lanes(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) {
+    if (shape.lanes == 32) scan_launch<T, 2, 32, 1, BACK>(p, pass, s);   // (one wavefront holds 32 steps)
+    else if (shape.lanes == 16) scan_waves<T, 16, BACK>(p, shape, pass, s);
+    else scan_waves<T, 8, BACK>(p, shape, pass, s);
 }
 
 template <typename T>
 void scan_dispatch(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s) {
-    if (shape.vec == 1) scan_launch<T, 1, 4, 4>(p, pass, s);
-    else if (shape.lanes == 32) scan_waves<T, 32>(p, shape, pass, s);
-    else if (shape.lanes == 16) scan_waves<T, 16>(p, shape, pass, s);
-    else scan_waves<T, 8>(p, shape, pass, s);
+    if (shape.vec == 1) scan_launch<T, 1, 4, 4, 8>(p, pass, s);
+    else if (shape.back == 8) scan_lanes<T, 8>(p, shape, pass, s);
+    else if (shape.back == 7) scan_lanes<T, 7>(p, shape, pass, s);
+    else scan_lanes<T, 6>(p, shape, pass, s);
 }
 
 }  // namespace pdw

@@ -23,7 +23,6 @@ static ScanCut scan_cut(long long rows, long long T, int I, ScanPass pass) {
     c.tiles = (T + step - 1) / step;
     const long long columns = rows * c.strips;
     long long want = c.shape.segments ? (1024 + columns - 1) / columns : 1;
-    if (const char* e = tune_env("PDW_SCAN_SEGMENTS")) want = atoi(e);
     if (want > c.tiles) want = c.tiles;
     if (want < 1) want = 1;
     c.seg_tiles = c.tiles ? (c.tiles + want - 1) / want : 1;

@@ -123,6 +123,16 @@ def test_scan(shape, dim, reverse, dtype):
     compare(d, run(d, dim, reverse), dim, reverse)
 
 
+# many chains: a lane has six, seven or eight steps of a tile, so that the last tile is nearly full; at the ends of such tiles, before and behind
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("batch,channels,steps", [(210, 5, t) for t in (12, 13, 15, 28, 33, 49, 57, 96, 129, 193, 225, 257, 385, 449, 513, 769, 897, 1793)]
+                         + [(130, 20, t) for t in (33, 49, 57, 65, 97, 113, 129, 192, 224, 257, 384, 449, 785)])
+def test_many_chains(batch, channels, steps, reverse, dtype):
+    d = data((batch, steps, channels), 1, dtype, lengths=True, seed=steps)
+    compare(d, run(d, 1, reverse), 1, reverse)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("reverse", [False, True])
 @pytest.mark.parametrize("shape,dim", [((6, 40, 24), 1), ((5, 300, 10), 1), ((4, 2000, 70), 1), ((3, 4, 50, 8), 2), ((3, 50, 4, 8), 1), ((6, 3, 2), 1), ((33, 1300, 98), 1)],
