@@ -2,9 +2,28 @@
 // libpdw.so (torch_ops.cpp has the block and the convolution, and says why they are native).
 #include "torch_node.h"
 
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+
 namespace {
 
 using namespace pdw_torch;
+
+// A gradient accumulator works on the stream that its leaf first met a graph on, and lives as long as any graph of that leaf.  If that is the
+// default stream, which no capture may make wait, a captured backward would end the process when the engine hands the gradient over: so it
+// is refused here, before anything is handed over.
+void no_eager_accumulators(const torch::autograd::Node& node, c10::Device device) {
+    const auto current = c10::hip::getCurrentHIPStream(device.index());
+    const auto eager = c10::hip::getDefaultHIPStream(device.index());
+    if (current == eager) return;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+    for (const auto& edge : node.next_edges()) {
+        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+        const auto stream = edge.function->stream();
+        TORCH_CHECK(!stream || stream->id() != eager.id(), node.name(), ": this backward pass cannot be captured while an output of an eager pass "
+                    "over the same tensors lives, whose gradients go to the default stream: drop that output first");
+    }
+}
 
 // Neither node has a second derivative: its gradients are results of kernels, which a graph of the backward would take for
 // constants.
@@ -125,6 +144,7 @@ struct NormNode : public torch::autograd::Node {
         std::lock_guard<std::mutex> lock(mutex_);
         no_second_derivative(*this);
         const Tensor grad = output_gradient(*this, grads);
+        no_eager_accumulators(*this, grad.device());
         const auto self = shared_from_this();
         const auto type = grad.scalar_type();
         Tensor xs = x.get(self, type, grad.device()), w = weight.get(self, type, grad.device()),
@@ -227,6 +247,7 @@ struct ResidualNode : public torch::autograd::Node {
         const auto self = shared_from_this();
         const auto type = gout.scalar_type();
         const auto dev = gout.device();
+        no_eager_accumulators(*this, dev);
         auto take = [&](const Kept& k) { return k.get(self, type, dev); };
         Tensor xv = take(x), yv = take(y), q = take(gate), sc = take(scale), w = take(weight), nw = take(next_weight), b = take(bias);
         Tensor st = stats.get(self, at::kFloat, dev), nst = next_stats.get(self, at::kFloat, dev);
@@ -383,6 +404,7 @@ struct ScanNode : public torch::autograd::Node {
         const auto self = shared_from_this();
         const auto type = input_metadata(0).options().dtype().toScalarType();
         const auto dev = gy.defined() ? gy.device() : glast.device();
+        no_eager_accumulators(*this, dev);
         Tensor xv = x.get(self, type, dev), gv = g.get(self, type, dev);
         Tensor len = lengths.get(self, at::kInt, dev), st = states.get(self, at::kFloat, dev);
         at::AutoDispatchBelowADInplaceOrView below;

@@ -7,7 +7,8 @@
 Any leading dimensions, 1 to 8192 channels, float32, float16 and bfloat16; every tensor of a call is of one type.  Statistics and
 sums are 32-bit, each result is rounded once, and results are the same from call to call.  The gradients have no derivatives
 of their own (``create_graph=True`` raises).  Everything can be captured in a HIP graph; before a backward pass is captured, drop
-the outputs of eager passes over the same parameters (torch's gradient accumulators remember the stream they were made on).
+the outputs of eager passes over the same tensors: torch's gradient accumulators remember the stream they were made on, and where that is
+the default stream, which a capture cannot make wait, the captured backward raises.
 """
 from __future__ import annotations
 

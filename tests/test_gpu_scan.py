@@ -507,6 +507,49 @@ def test_captured_passes_replay():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("op", ["scan", "norm", "residual"])
+def test_capture_beside_an_eager_graph_is_refused(op):
+    """A backward pass under capture whose gradients would go to accumulators of the default stream raises, and leaves the process as it was;
+    with the eager output gone the same capture works."""
+    x, g = (torch.randn(2, 40, 64, device="cuda").requires_grad_() for _ in range(2))
+    w = torch.ones(64, device="cuda").requires_grad_()
+    gy = torch.randn(2, 40, 64, device="cuda")
+
+    def forward():
+        if op == "scan":
+            return pcb().gated_scan(x, g)[0], [x, g]
+        if op == "norm":
+            return pcb().channel_norm(x, w), [x, w]
+        return pcb().gated_residual(x, g, w, kind="rms"), [x, g, w]
+
+    def step():
+        y, leaves = forward()
+        return torch.autograd.grad(y, leaves, gy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager = forward()
+    with pytest.raises(RuntimeError, match="drop that output first"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    ref = torch.autograd.grad(*eager, gy)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for _ in range(3):
+        for t in res:
+            if t.data_ptr() != gy.data_ptr():   # (the gradient of a residual's x is gy itself)
+                t.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(res, ref):
+            assert torch.equal(a, b)
+
+
 def test_norm_scan_residual_as_a_block():
     """A block around the recurrence as a model has it: norm, one projection for values, decays and gate, the scan down an image's
     columns, gated residual with the next norm; gradients for all of it against the same in plain 64-bit operations.
