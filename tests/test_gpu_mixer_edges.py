@@ -1,0 +1,53 @@
+"""channel_norm, gated_residual and gated_scan where their ranges end.  References and bounds are those of test_gpu_norm.py and
+test_gpu_scan.py: 64 bits, element by element."""
+import pytest
+import torch
+from test_gpu_norm import check, doubles, residual64, residual_data, run_residual
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+# Gates far from zero.  Below -87 the kernels take silu and its slope for 0: there both are under 88 e^-87 < 2^-118, times factors
+# under 2^10 and sums of fewer than 2^8 terms: under 2^-100 in every result.
+LOW = [-1.0, -20.0, -86.0, -87.5, -88.0, -90.0, -110.0, -200.0, -1e4, -1e30, -1e36, "min"]
+
+
+def extreme_gates(shape, dtype, high, seed):
+    info = torch.finfo(dtype)
+    values = torch.tensor([max(info.min if v == "min" else v, info.min) for v in LOW] + high, dtype=torch.float64)
+    gen = torch.Generator().manual_seed(seed)
+    return values[torch.randint(0, len(values), shape, generator=gen)].to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+@pytest.mark.parametrize("gate", ["image", "full"])
+@pytest.mark.parametrize("next_kind", ["none", "rms"])
+@pytest.mark.parametrize("shape", [(3, 5, 40), (2, 7, 9), (2, 3, 1152)], ids=str)
+def test_extreme_gates(shape, next_kind, gate, act, dtype):
+    """Gates down to the type's lowest value, as masks leave them, and large ones: a silu of 0 and not of -4, and no gradient."""
+    d = residual_data(shape, dtype, gate, True, "w", "w" if next_kind != "none" else "")
+    # (a next norm squares the sum; in float16 it has to stay in range itself)
+    high = [30.0, 100.0] + ([1e30] if next_kind == "none" and dtype != torch.float16 else [])
+    d["gate"] = extreme_gates(d["gate"].shape, dtype, high, 7)
+    got = run_residual(d, act, "rms", next_kind, dtype)
+    ref = residual64(doubles(d), act, "rms", next_kind, gate == "image")
+    assert set(got) == set(ref)
+    for k, (value, bound) in ref.items():
+        check(got[k], value, bound + 2.0 ** -100, k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", ["min", "-inf"])
+@pytest.mark.parametrize("gate", ["image", "full"])
+def test_a_masked_branch_adds_nothing(gate, value, dtype):
+    d = residual_data((2, 9, 72), dtype, gate, True, "wb", "")
+    d["gate"] = torch.full_like(d["gate"], torch.finfo(dtype).min if value == "min" else float("-inf"))
+    got = run_residual(d, "silu", "layer", "none", dtype)
+    if dtype == torch.float16 and value == "min":   # (of a float16 gate too: its lowest value is below -87)
+        assert float(d["gate"].max()) < -87
+    assert torch.equal(got["out"].detach().cpu(), d["x"])
+    for k in ("gy", "ggate", "gscale", "gw", "gb"):
+        assert not got[k].any(), k
