@@ -371,9 +371,10 @@ void split(const Tensor& xg, Tensor* x, Tensor* g) {
     *x = xg.narrow(-1, 0, C), *g = xg.narrow(-1, C, C);
 }
 
-// Where the axes behind the recurrence's are dense in every tensor they are one axis of chains, [O][T][1][W * I].
+// Where the axes behind the recurrence's are dense in every tensor they are one axis of chains, [O][T][1][W * I].  Never with halves: rows
+// of x and g may lie side by side (windows that overlap), but those of their gradients, halves of one dense tensor, do not.
 bool mergeable(const ScanShape& s, std::initializer_list<const ScanView*> views) {
-    if (s.W == 1 || (int64_t)s.W * s.I > 0x7fffffff) return false;
+    if (s.halves || s.W == 1 || (int64_t)s.W * s.I > 0x7fffffff) return false;
     for (const ScanView* v : views)
         if (v->s[2] != s.I) return false;
     return true;

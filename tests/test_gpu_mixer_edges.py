@@ -2,7 +2,7 @@
 test_gpu_scan.py: 64 bits, element by element."""
 import pytest
 import torch
-from test_gpu_norm import check, doubles, residual64, residual_data, run_residual
+from test_gpu_norm import check, doubles, pcb, residual64, residual_data, rnd, run_residual
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,30 @@ def test_a_masked_branch_adds_nothing(gate, value, dtype):
     assert torch.equal(got["out"].detach().cpu(), d["x"])
     for k in ("gy", "ggate", "gscale", "gw", "gb"):
         assert not got[k].any(), k
+
+
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,T,W,C", [(2, 9, 5, 8), (1, 40, 3, 33), (2, 300, 4, 16), (70, 20, 6, 64)])
+def test_halves_in_rows_that_overlap(B, T, W, C, dtype, reverse):
+    """Sliding windows over the channels as x and g in one tensor: each half's rows lie side by side, the gradient's do not.  Bitwise
+    the results of a copy without overlap, and the gradients summed where windows share an element."""
+    gen = torch.Generator().manual_seed(W)
+    base = rnd(gen, B, T, (W + 1) * C, dtype=dtype).cuda().requires_grad_()
+    gy, glast = rnd(gen, B, T, W, C, dtype=dtype).cuda(), rnd(gen, B, W, C).cuda()
+    windows = base.unfold(-1, 2 * C, C)
+    assert windows.shape == (B, T, W, 2 * C) and windows.stride()[-2:] == (C, 1)
+    dense = windows.detach().contiguous().requires_grad_()
+    got, ref = (pcb().gated_scan(t, dim=1, reverse=reverse) for t in (windows, dense))
+    for a, b in zip(got, ref):
+        assert torch.equal(a, b)
+    leaf = windows.detach().as_strided(windows.shape, windows.stride()).requires_grad_()
+    (gl,) = torch.autograd.grad(pcb().gated_scan(leaf, dim=1, reverse=reverse), [leaf], [gy, glast])
+    (gd,) = torch.autograd.grad(ref, [dense], [gy, glast])
+    assert torch.equal(gl, gd)
+    (gb,) = torch.autograd.grad(got, [base], [gy, glast])
+    summed = torch.zeros_like(base)
+    for w in range(W):
+        summed[..., w * C:(w + 2) * C] += gd[:, :, w]
+    # two addends at most, in whichever order: one rounding
+    assert torch.equal(gb, summed)
