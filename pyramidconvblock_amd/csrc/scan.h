@@ -61,7 +61,7 @@ struct ScanLane {
         lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
         c = (strip * LC + lane % LC) * VEC;
         on = c < I;
-        if (c + VEC > I) c = I - VEC;   // the last lane overlaps the one before it: the same chains, the same values (I >= VEC)
+        if (c > I - VEC) c = I - VEC;   // the last lane overlaps the one before it: the same chains, the same values (I >= VEC)
         sub = wave * kSub + lane / LC;
     }
 };
@@ -584,7 +584,7 @@ struct ScanShape {
 // [275,196,128] 46, 43, [64,1800,128] 61, 61 (six steps there would take 62).
 inline ScanShape scan_shape(long long rows, long long T, int I) {
     if (I < 2) return {1, 4, 4, true, 8};
-    const long long wide = rows * ((I + 31) / 32), narrow = rows * ((I + 15) / 16);
+    const long long wide = rows * cdiv(I, 32), narrow = rows * cdiv(I, 16);
     const bool segments = narrow < 208;
     const int lanes = T <= 32 ? 32 : !segments && narrow <= 256 ? 8 : 16;
     const int most = segments || (wide > 256 && wide < 352) || wide > 512 ? 4 : 8;

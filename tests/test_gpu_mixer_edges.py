@@ -78,3 +78,22 @@ def test_halves_in_rows_that_overlap(B, T, W, C, dtype, reverse):
         summed[..., w * C:(w + 2) * C] += gd[:, :, w]
     # two addends at most, in whichever order: one rounding
     assert torch.equal(gb, summed)
+
+
+def test_channels_up_to_the_last_32_bit_number():
+    """2^31 - 1 channels, the last of which a lane of the last strip shares with the lane before it: the last ones are bitwise what they are in a
+    call by themselves, the others what zeros give."""
+    C, T, last = (1 << 31) - 1, 2, 45
+    gen = torch.Generator().manual_seed(14)
+    data = [rnd(gen, T, last, dtype=torch.bfloat16).cuda() for _ in range(3)] + [rnd(gen, last).cuda()]
+    wide = [torch.zeros(T, C, device="cuda", dtype=torch.bfloat16) for _ in range(3)] + [torch.zeros(C, device="cuda")]
+    for a, b in zip(wide, data):
+        a[..., -last:] = b
+
+    def call(x, g, gy, state):
+        x, g, state = (t.requires_grad_() for t in (x, g, state))
+        y, end = pcb().gated_scan(x, g, state, dim=0)
+        return [y.detach(), end.detach(), *torch.autograd.grad(y, [x, g, state], gy)]
+
+    for a, b in zip(call(*wide), call(*data)):
+        assert torch.equal(a[..., -last:], b) and int(torch.count_nonzero(a)) == int(torch.count_nonzero(b))
