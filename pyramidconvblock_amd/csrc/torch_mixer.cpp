@@ -610,7 +610,7 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
         else if (d > dim && d < rank - 1) W *= y_sizes[d];
     }
     TORCH_CHECK_VALUE(O <= 0x7fffffff && W <= 0x7fffffff && O * W <= 0x7fffffff && y_sizes.back() <= 0x7fffffff && y_sizes[dim] <= 0x7fffffff,
-                      "more than 2^31 chains, channels or steps: ", x.sizes());
+                      "more than 2^31 - 1 chains, channels or steps: ", x.sizes());
     s.O = (int)O, s.T = y_sizes[dim], s.W = (int)W, s.I = (int)y_sizes.back(), s.dim = dim;
     const Tensor& state = in[kSState];
     if (state.defined()) {
@@ -660,6 +660,7 @@ PyObject* py_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
     TORCH_CHECK_VALUE(halves || g.sizes() == x.sizes(), "x and g have to be of one shape, got ", x.sizes(), " and ", g.sizes());
     at::DimVector sizes(x.sizes());
     if (halves) sizes.back() /= 2;
+    TORCH_CHECK_VALUE(sizes.back() <= 0x7fffffff, "more than 2^31 - 1 channels: ", x.sizes());
     for (const Tensor* t : {&state, &to}) {
         if (!t->defined()) continue;
         TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, "the state is float32, got ", t->scalar_type());

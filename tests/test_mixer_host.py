@@ -151,3 +151,12 @@ def test_modules_have_the_parameters_they_name():
     assert list(pcb().GatedScan(dim=1, reverse=True).parameters()) == []
     assert "dim=1" in repr(pcb().GatedScan(dim=1)) and "rms" in repr(pcb().ChannelNorm(8)) and "silu" in repr(
         pcb().GatedResidual(8, activation="silu"))
+
+
+def test_more_channels_than_32_bits_count_are_refused():
+    """2^31 channels (views of one element: nothing is allocated): refused by name, not cut to 32 bits."""
+    one = torch.zeros(1)
+    x = one.expand(2, 1 << 31)
+    refused(ValueError, "2\\^31 - 1", pcb().gated_scan, x, x, dim=0)
+    refused(ValueError, "2\\^31 - 1", pcb().gated_scan_step, one.expand(1, 1 << 32), one.expand(1, 1 << 32), one.expand(1, 1 << 32))
+    refused(ValueError, "2\\^31 - 1", pcb().gated_scan_step, one.expand(1, (1 << 32) + 8), one.expand(1, (1 << 32) + 8), torch.zeros(1, 8))
