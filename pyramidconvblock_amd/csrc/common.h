@@ -67,6 +67,14 @@ inline int pick_vec(int C, size_t elem, const void* const* ptrs, int nptrs) {
 
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+// A launch has fewer than 2^32 threads (of a larger one HIP cuts the grid without an error): `grid` workgroups in as many launches as that takes,
+// f(first workgroup, workgroups).  Multiples of the eight dies, which workgroups go to in turn.
+template <typename F>
+inline void launch_parts(long long grid, int threads, F f) {
+    const long long most = (0xffffffffLL / threads) & ~7LL;
+    for (long long first = 0; first < grid; first += most) f(first, (unsigned)(grid - first < most ? grid - first : most));
+}
+
 // Entries a per-shape launch-plan cache may hold before it is emptied (a plan costs microseconds to redo).
 constexpr size_t kPlanCacheMax = 256;
 

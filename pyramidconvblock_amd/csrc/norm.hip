@@ -46,6 +46,7 @@ struct ColsArgs {
     void *gscale, *gw, *gb, *gw2, *gb2, *ggate;
     long long ldg;
     int C, S, sums, act, gate_rows;
+    unsigned first;               // the launch's first workgroup (launch_parts)
     int branch_jobs, next_jobs;   // 1 or 0
 };
 
@@ -54,9 +55,10 @@ __global__ __launch_bounds__(1024) void rows_cols_k(ColsArgs p) {
     constexpr int CW = 16, Q = 64;
     __shared__ float2 red[Q][CW];
     const int blocks = (p.C + CW - 1) / CW;
-    const long long job = blockIdx.x / (unsigned)blocks;
+    const unsigned block = p.first + blockIdx.x;
+    const long long job = block / (unsigned)blocks;
     const int cl = threadIdx.x % CW, q = threadIdx.x / CW;
-    const int c = (int)(blockIdx.x - job * blocks) * CW + cl;
+    const int c = (int)(block - job * blocks) * CW + cl;
     const bool image_job = job >= p.branch_jobs + p.next_jobs, next_job = !image_job && job >= p.branch_jobs;
     const long long image = job - p.branch_jobs - p.next_jobs;
     const long long s0 = image_job ? image * p.S : 0, s1 = image_job ? s0 + p.S : p.segments;
@@ -147,6 +149,8 @@ int rows_backward_launch(const RowArgs& in, void* gscale, void* gw, void* gb, vo
     const bool branch = in.y != nullptr, next = in.kind2 != kNormNone, image_gate = in.gate_rows == 1 && in.ggate && in.N > 0;
     const bool branch_sums = branch && (gscale || gw || gb), next_sums = next && (gw2 || gb2);
     const bool sums = branch_sums || next_sums || image_gate;
+    const long long jobs = (long long)branch_sums + next_sums + (image_gate ? images_of(in) : 0), blocks = jobs * cdiv(in.C, 16);
+    if (blocks > 0x7fffffffLL) return set_error("norm backward: too many images (%lld)", images_of(in)), 1;
     RowArgs p = in;
     long long grid = 0;
     p.parts = nullptr, p.S = 0;
@@ -167,13 +171,12 @@ int rows_backward_launch(const RowArgs& in, void* gscale, void* gw, void* gb, vo
     c.gscale = gscale, c.gw = gw, c.gb = gb, c.gw2 = gw2, c.gb2 = gb2, c.ggate = in.ggate;
     c.C = in.C, c.S = p.S, c.sums = branch && next ? 4 : 2, c.act = in.act, c.gate_rows = in.gate_rows;
     c.branch_jobs = branch_sums, c.next_jobs = next_sums;
-    const long long jobs = (long long)branch_sums + next_sums + (image_gate ? images_of(in) : 0);
-    const long long blocks = jobs * cdiv(in.C, 16);
-    if (blocks == 0) return 0;
-    if (blocks > 0x7fffffffLL) return set_error("norm backward: too many images"), 1;
-    if (dtype == kF32) rows_cols_k<float><<<(unsigned)blocks, 1024, 0, s>>>(c);
-    else if (dtype == kF16) rows_cols_k<f16_t><<<(unsigned)blocks, 1024, 0, s>>>(c);
-    else rows_cols_k<bf16_t><<<(unsigned)blocks, 1024, 0, s>>>(c);
+    launch_parts(blocks, 1024, [&](long long first, unsigned n) {
+        c.first = (unsigned)first;
+        if (dtype == kF32) rows_cols_k<float><<<n, 1024, 0, s>>>(c);
+        else if (dtype == kF16) rows_cols_k<f16_t><<<n, 1024, 0, s>>>(c);
+        else rows_cols_k<bf16_t><<<n, 1024, 0, s>>>(c);
+    });
     return check_launch("rows_cols_k");
 }
 

@@ -36,15 +36,17 @@ struct RowArgs {
     long long N, P, L;                                   // rows; rows of an image; rows of a segment
     long long ldg;                                       // elements between gate rows
     int C, S;                                            // channels; segments of an image
+    unsigned first;                                      // the launch's first workgroup (launch_parts)
     int act, kind, kind2;
     int gate_rows;                                       // 0: no gate; 1: a row an image; 2: a row a row
     float eps;
 };
 
-// A row segment: workgroup blockIdx.x has rows [r0, r1) of image `image`.
+// A row segment: a workgroup has rows [r0, r1) of image `image`.
 __device__ __forceinline__ void row_segment(const RowArgs& p, long long& r0, long long& r1, long long& image) {
-    image = blockIdx.x / (unsigned)p.S;
-    const long long s = blockIdx.x - image * p.S, first = image * p.P;
+    const unsigned block = p.first + blockIdx.x;
+    image = block / (unsigned)p.S;
+    const long long s = block - image * p.S, first = image * p.P;
     r0 = first + s * p.L;
     r1 = r0 + p.L < first + p.P ? r0 + p.L : first + p.P;
 }
@@ -494,7 +496,7 @@ __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) 
         }
     }
     if (!p.parts) return;
-    float* out = p.parts + (long long)blockIdx.x * SUMS * p.C;
+    float* out = p.parts + (long long)(p.first + blockIdx.x) * SUMS * p.C;
     if (BRANCH) cols_out<VEC, TPR, NCH>(s1, cols, p.C, out, lds), cols_out<VEC, TPR, NCH>(s0, cols, p.C, out + p.C, lds);
     if (NEXT) {
         out += BRANCH ? 2 * p.C : 0;
@@ -506,8 +508,12 @@ template <typename T, int VEC, int TPR, int NCH, bool RAG, bool BRANCH, bool NEX
 void rows_pass(const RowArgs& p, unsigned grid, bool backward, hipStream_t s) {
     int threads = row_threads<TPR>(backward);
     if (TPR > 64) threads = ((p.C + VEC - 1) / VEC + 64 * NCH - 1) / (64 * NCH) * 64;
-    if (backward) rows_bwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<grid, threads, 0, s>>>(p);
-    else rows_fwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<grid, threads, 0, s>>>(p);
+    RowArgs q = p;
+    launch_parts(grid, threads, [&](long long first, unsigned n) {
+        q.first = (unsigned)first;
+        if (backward) rows_bwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<n, threads, 0, s>>>(q);
+        else rows_fwd_k<T, VEC, TPR, NCH, RAG, BRANCH, NEXT, FULL><<<n, threads, 0, s>>>(q);
+    });
 }
 
 template <typename T, int VEC, int TPR, int NCH, bool RAG>

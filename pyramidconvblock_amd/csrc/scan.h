@@ -48,6 +48,7 @@ struct ScanArgs {
     long long T;
     int rows, W, I;                     // rows = O * W
     int strips, tiles, segments, seg_tiles, state_tiles;
+    unsigned blocks, first;             // workgroups in all, and the launch's first one (launch_parts)
     int reverse, near, near_segments;   // TilePtr's offsets fit, of a tile and of a segment
 };
 
@@ -202,13 +203,13 @@ struct ScanWhere {
     int strip, row, o, w, seg;
     long long len;
     __device__ __forceinline__ ScanWhere(const ScanArgs& p) {
-        const unsigned strips = p.strips, rows8 = gridDim.x / strips & ~7u;
+        const unsigned strips = p.strips, rows8 = p.blocks / strips & ~7u, block = p.first + blockIdx.x;
         unsigned rest;
-        if (blockIdx.x < rows8 * strips) {
-            const unsigned turn = blockIdx.x >> 3;
-            strip = turn % strips, rest = turn / strips * 8 + (blockIdx.x & 7);
+        if (block < rows8 * strips) {
+            const unsigned turn = block >> 3;
+            strip = turn % strips, rest = turn / strips * 8 + (block & 7);
         } else {
-            strip = blockIdx.x % strips, rest = blockIdx.x / strips;
+            strip = block % strips, rest = block / strips;
         }
         row = rest % (unsigned)p.rows, seg = rest / (unsigned)p.rows;
         o = row / p.W, w = row - o * p.W;
@@ -604,16 +605,23 @@ inline ScanShape scan_shape(long long rows, long long T, int I) {
 template <typename T, int VEC, int LC, int NW, int BACK>
 void scan_launch(const ScanArgs& p, ScanPass pass, hipStream_t s) {
     const unsigned columns = (unsigned)p.strips * (unsigned)p.rows;
+    ScanArgs q = p;
     if constexpr (BACK == 8 && NW <= 4 && (LC == 16 || VEC == 1)) {   // (the shapes that are cut into segments)
         if (p.segments > 1) {
-            const unsigned n = columns * (unsigned)(p.segments - 1);
-            if (pass == kScanForward) scan_maps_k<T, VEC, LC, NW, 2 * BACK, false><<<n, NW * 64, 0, s>>>(p);
-            else scan_maps_k<T, VEC, LC, NW, BACK, true><<<n, NW * 64, 0, s>>>(p);
+            q.blocks = columns * (unsigned)(p.segments - 1);
+            launch_parts(q.blocks, NW * 64, [&](long long first, unsigned n) {
+                q.first = (unsigned)first;
+                if (pass == kScanForward) scan_maps_k<T, VEC, LC, NW, 2 * BACK, false><<<n, NW * 64, 0, s>>>(q);
+                else scan_maps_k<T, VEC, LC, NW, BACK, true><<<n, NW * 64, 0, s>>>(q);
+            });
         }
     }
-    const unsigned n = columns * (unsigned)p.segments;
-    if (pass == kScanForward) scan_fwd_k<T, VEC, LC, NW, 2 * BACK><<<n, NW * 64, 0, s>>>(p);
-    else scan_bwd_k<T, VEC, LC, NW, BACK><<<n, NW * 64, 0, s>>>(p);
+    q.blocks = columns * (unsigned)p.segments;
+    launch_parts(q.blocks, NW * 64, [&](long long first, unsigned n) {
+        q.first = (unsigned)first;
+        if (pass == kScanForward) scan_fwd_k<T, VEC, LC, NW, 2 * BACK><<<n, NW * 64, 0, s>>>(q);
+        else scan_bwd_k<T, VEC, LC, NW, BACK><<<n, NW * 64, 0, s>>>(q);
+    });
 }
 
 template <typename T, int LC, int BACK>

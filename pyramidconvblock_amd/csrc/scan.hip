@@ -70,8 +70,8 @@ int scan_run(const ScanArgs& in, bool backward, void* workspace, size_t workspac
 // so the new state may take the old one's place.  A few hundred kilobytes: launch latency is all there is to it.
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void scan_step_k(const T* __restrict__ x, const T* __restrict__ g, const float* state, float* new_state,
-                                                   T* __restrict__ y, long long n, int C, long long ldx, long long ldg) {
-    const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+                                                   T* __restrict__ y, long long n, int C, long long ldx, long long ldg, long long first) {
+    const long long e = (first + blockIdx.x) * 256 + threadIdx.x;
     if (e >= n) return;
     const int per = C / VEC;
     const long long b = e / per;
@@ -91,10 +91,10 @@ static int step_launch(const void* x, const void* g, const float* state, float* 
                        long long ldx, long long ldg, hipStream_t s) {
     const bool wide = C % 4 == 0;
     const long long n = B * (C / (wide ? 4 : 1)), blocks = (n + 255) / 256;
-    if (blocks > 0x7fffffffLL) return set_error("scan step: too many tokens (%lld x %d)", B, C), 1;
-    if (blocks == 0) return 0;
-    if (wide) scan_step_k<T, 4><<<(unsigned)blocks, 256, 0, s>>>((const T*)x, (const T*)g, state, new_state, (T*)y, n, C, ldx, ldg);
-    else scan_step_k<T, 1><<<(unsigned)blocks, 256, 0, s>>>((const T*)x, (const T*)g, state, new_state, (T*)y, n, C, ldx, ldg);
+    launch_parts(blocks, 256, [&](long long first, unsigned m) {
+        if (wide) scan_step_k<T, 4><<<m, 256, 0, s>>>((const T*)x, (const T*)g, state, new_state, (T*)y, n, C, ldx, ldg, first);
+        else scan_step_k<T, 1><<<m, 256, 0, s>>>((const T*)x, (const T*)g, state, new_state, (T*)y, n, C, ldx, ldg, first);
+    });
     return check_launch("scan_step_k");
 }
 

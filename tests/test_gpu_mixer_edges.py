@@ -2,10 +2,11 @@
 test_gpu_scan.py: 64 bits, element by element."""
 import pytest
 import torch
-from test_gpu_norm import check, doubles, pcb, residual64, residual_data, rnd, run_residual
+from test_gpu_norm import check, doubles, norm64, pcb, residual64, residual_data, rnd, run_residual
 
 pytestmark = pytest.mark.gpu
 
+U = 2.0 ** -24
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
@@ -97,3 +98,65 @@ def test_channels_up_to_the_last_32_bit_number():
 
     for a, b in zip(call(*wide), call(*data)):
         assert torch.equal(a[..., -last:], b) and int(torch.count_nonzero(a)) == int(torch.count_nonzero(b))
+
+
+def test_more_images_than_one_launch_holds():
+    """A gate row for each of so many images that the workgroups times their threads pass 2^32, in the forward (256 threads), the backward (512) and
+    the sums over rows (1024): HIP would cut the grid without an error.
+    The last images are bitwise what they are in a call by themselves, the column sums within their bound."""
+    B, P, C, last = (1 << 24) + 3, 2, 8, 37
+    gen = torch.Generator().manual_seed(11)
+    x = torch.zeros(B, P, C, device="cuda", dtype=torch.bfloat16)
+    y, go, gate = torch.zeros_like(x), torch.zeros_like(x), torch.zeros(B, C, device="cuda", dtype=torch.bfloat16)
+    d = {k: rnd(gen, last, P, C, dtype=torch.bfloat16).cuda() for k in ("x", "y", "go")}
+    d["gate"] = rnd(gen, last, C, dtype=torch.bfloat16).cuda()
+    w = rnd(gen, C, dtype=torch.bfloat16, mean=1.0, std=0.2).cuda().requires_grad_()
+    for big, k in ((x, "x"), (y, "y"), (go, "go"), (gate, "gate")):
+        big[-last:] = d[k]
+
+    def call(x, y, gate, go):
+        x, y, gate = (t.requires_grad_() for t in (x, y, gate))
+        out, nxt = pcb().gated_residual(x, y, w, gate=gate, kind="rms", activation="silu", next_kind="layer")
+        return [out, nxt, *torch.autograd.grad([out, nxt], [x, y, gate, w], [go, go])]
+
+    many, few = call(x, y, gate, go), call(d["x"], d["y"], d["gate"], d["go"])
+    for a, b in zip(many[:-1], few[:-1]):
+        assert torch.equal(a[-last:], b) and not a[:-last].any()
+    # the weight's gradient: zeros and the same terms in another order, each sum within 64 u of the terms' magnitudes and rounded once
+    f = lambda t: t.detach().double().cpu()
+    out, _, gx, *_ = few
+    n = norm64(f(d["y"]), None, None, "rms")[1]
+    q = f(d["gate"])[:, None]
+    terms = (f(gx) * n * q * torch.sigmoid(q)).abs().sum((0, 1))
+    # (gx itself is rounded to bfloat16 in `terms` alone: they only scale the bound, by 1 + 2^-8)
+    assert ((f(many[-1]) - f(few[-1])).abs() <= 2.0 ** -7 * f(few[-1]).abs() + 2 * 64 * U * 1.01 * terms).all()
+
+
+def test_more_chains_than_one_launch_holds():
+    """So many chains and tokens that the workgroups times their threads pass 2^32: the last ones are bitwise what they are in a call by themselves."""
+    B, T, last = (1 << 24) + 5, 3, 33   # of one channel: a workgroup of 256 threads each
+    gen = torch.Generator().manual_seed(12)
+    x, g = torch.zeros(B, T, 1, device="cuda", dtype=torch.bfloat16), torch.zeros(B, T, 1, device="cuda", dtype=torch.bfloat16)
+    gy = torch.zeros_like(x)
+    xl, gl, gyl = (rnd(gen, last, T, 1, dtype=torch.bfloat16).cuda() for _ in range(3))
+    x[-last:], g[-last:], gy[-last:] = xl, gl, gyl
+
+    def call(x, g, gy):
+        x, g = x.requires_grad_(), g.requires_grad_()
+        y, state = pcb().gated_scan(x, g)
+        return [y, state, *torch.autograd.grad(y, [x, g], gy)]
+
+    for a, b in zip(call(x, g, gy), call(xl, gl, gyl)):
+        assert torch.equal(a[-last:], b) and not a[:-last].any()
+
+
+def test_more_tokens_than_one_launch_holds():
+    B, C, last = (1 << 30) + 7, 5, 100   # of an odd number of channels: a thread a value
+    gen = torch.Generator().manual_seed(13)
+    x, state = torch.zeros(B, C, device="cuda", dtype=torch.bfloat16), torch.zeros(B, C, device="cuda")
+    xl, hl = rnd(gen, last, C, dtype=torch.bfloat16).cuda(), rnd(gen, last, C).cuda()
+    x[-last:], state[-last:] = xl, hl
+    y, h = pcb().gated_scan_step(x, x, state)
+    yl, hl = pcb().gated_scan_step(xl, xl, hl)
+    assert torch.equal(y[-last:], yl) and torch.equal(h[-last:], hl)
+    assert not y[:-last].any() and not h[:-last].any()
