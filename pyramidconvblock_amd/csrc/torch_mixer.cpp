@@ -10,15 +10,16 @@ using namespace pdw_torch;
 
 // A gradient accumulator works on the stream that its leaf first met a graph on, and lives as long as any graph of that leaf.  If that is the
 // default stream, which no capture may make wait, a captured backward would end the process when the engine hands the gradient over: so it
-// is refused here, before anything is handed over.
+// is refused here, before anything is handed over.  (A leaf whose gradient this pass does not ask for is handed nothing.)
 void no_eager_accumulators(const torch::autograd::Node& node, c10::Device device) {
     const auto current = c10::hip::getCurrentHIPStream(device.index());
     const auto eager = c10::hip::getDefaultHIPStream(device.index());
     if (current == eager) return;
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(current.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
-    for (const auto& edge : node.next_edges()) {
-        if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+    for (size_t i = 0; i < node.num_outputs(); ++i) {
+        const auto& edge = node.next_edge(i);
+        if (!node.task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
         const auto stream = edge.function->stream();
         TORCH_CHECK(!stream || stream->id() != eager.id(), node.name(), ": this backward pass cannot be captured while an output of an eager pass "
                     "over the same tensors lives, whose gradients go to the default stream: drop that output first");

@@ -160,3 +160,40 @@ def test_more_tokens_than_one_launch_holds():
     yl, hl = pcb().gated_scan_step(xl, xl, hl)
     assert torch.equal(y[-last:], yl) and torch.equal(h[-last:], hl)
     assert not y[:-last].any() and not h[:-last].any()
+
+
+@pytest.mark.parametrize("op", ["scan", "norm", "residual"])
+def test_capture_asks_only_for_the_gradients_that_are_wanted(op):
+    """A captured backward pass that wants x's gradient alone, beside an eager graph of the other leaf, whose accumulator works on the default
+    stream: nothing is handed to that one, so the capture goes through, and its replays are the eager result."""
+    x, other, w = torch.randn(2, 40, 64, device="cuda"), torch.randn(2, 40, 64, device="cuda"), torch.ones(64, device="cuda")
+    gy = torch.randn(2, 40, 64, device="cuda")
+    x.requires_grad_(), other.requires_grad_(), w.requires_grad_()
+    unrelated = torch.randn(2, 40, 64, device="cuda")
+
+    def forward(x):
+        if op == "scan":
+            return pcb().gated_scan(x, other)[0]
+        if op == "norm":
+            return pcb().channel_norm(x, w)
+        return pcb().gated_residual(x, other, w, kind="rms", next_weight=w, next_kind="layer")[1]
+
+    def step():
+        return torch.autograd.grad(forward(x), [x], gy)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager = forward(unrelated)   # keeps the accumulators of `other` and `w`, not of x
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = step()
+    for _ in range(3):
+        res.detach().zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = res.clone()
+        assert torch.equal(got, step())
+    assert eager.requires_grad
