@@ -2,7 +2,8 @@
 test_gpu_scan.py: 64 bits, element by element."""
 import pytest
 import torch
-from test_gpu_norm import check, doubles, norm64, pcb, residual64, residual_data, rnd, run_residual
+from test_gpu_norm import (EPS, check, doubles, norm64, norm_bwd64, pcb, residual64, residual_data, rnd, rows_slack,
+                           run_residual)
 
 pytestmark = pytest.mark.gpu
 
@@ -52,6 +53,61 @@ def test_a_masked_branch_adds_nothing(gate, value, dtype):
     assert torch.equal(got["out"].detach().cpu(), d["x"])
     for k in ("gy", "ggate", "gscale", "gw", "gb"):
         assert not got[k].any(), k
+
+
+# Calls in which a row group goes through several rows (its next row's loads under way, its column sums carried along), with a last one that is
+# not full.  A lane's sum is as many additions as its group has rows, at most N / 512 + 1 (the backward aims at 512 workgroups or more), one or a few
+# for segments and 24 for lanes, wavefronts and the sum over segments; rows_slack's 48 + N / 1024 holds that up to N = 24 * 1024 rows
+# of a whole workgroup, and any N of groups of which a workgroup has two or more.
+def backward_rows(N, C, dtype):
+    """Rows of a group in the backward, at most, from the segments that the workspace is made for."""
+    from pyramidconvblock_amd import _lib
+
+    segments = _lib.lib().pdw_norm_bwd_workspace_bytes(N, C, _lib.dtype_code(dtype)) // (2 * C * 4)
+    pieces = -(-C // (4 if dtype == torch.float32 else 8))
+    groups = 1 if pieces > 64 else 512 // max(8, 1 << (pieces - 1).bit_length())
+    return -(-N // segments) / groups
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kind,affine", [("rms", "w"), ("layer", "wb")])
+@pytest.mark.parametrize("shape", [(65573 * 2, 24), (20011, 200), (20011, 201), (9001, 520), (4207, 1152), (2101, 5000)], ids=str)
+def test_norm_of_several_rows_a_group(shape, kind, affine, dtype):
+    N, C = shape
+    assert backward_rows(N, C, dtype) > 1
+    gen = torch.Generator().manual_seed(N)
+    x, gy = rnd(gen, N, C, dtype=dtype, mean=0.5), rnd(gen, N, C, dtype=dtype)
+    w = rnd(gen, C, dtype=dtype, mean=1.0, std=0.3)
+    b = rnd(gen, C, dtype=dtype) if "b" in affine else None
+    leaves = [t.cuda().requires_grad_() for t in (x, w, b) if t is not None]
+    y = pcb().channel_norm(*leaves, kind=kind, eps=EPS)
+    grads = torch.autograd.grad(y, leaves, gy.cuda())
+    f = lambda t: None if t is None else t.double()
+    ry, n, r, dn = norm64(f(x), f(w), f(b), kind)
+    check(y, ry, dn * f(w).abs() + 8 * U * ry.abs(), "y")
+    check(grads[0], *norm_bwd64(f(gy), n, r, dn, f(w), kind), "gx")
+    check(grads[1], (f(gy) * n).sum(0), rows_slack(f(gy) * n, f(gy).abs() * dn), "gw")
+    if b is not None:
+        check(grads[2], f(gy).sum(0), rows_slack(f(gy), 0 * f(gy)), "gb")
+
+
+ROWS_FORMS = [("none", "none", "rms", "w", "none", "", True), ("image", "silu", "layer", "wb", "rms", "w", True),
+              ("image", "sigmoid", "none", "", "none", "", True), ("full", "silu", "layer", "wb", "rms", "w", True),
+              ("full", "none", "rms", "w", "none", "", False), ("none", "none", "none", "", "layer", "wb", True)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("form", ROWS_FORMS, ids=lambda f: "-".join(str(v) for v in f))
+@pytest.mark.parametrize("shape", [(2, 40011, 24), (3, 7001, 201), (3, 3001, 520), (40, 99, 1152), (2, 1051, 5000)], ids=str)
+def test_residual_of_several_rows_a_group(shape, form, dtype):
+    gate, act, kind, affine, next_kind, next_affine, scale = form
+    assert backward_rows(shape[0] * shape[1], shape[2], dtype) > 1
+    d = residual_data(shape, dtype, gate, scale, affine, next_affine, seed=3)
+    got = run_residual(d, act, kind, next_kind, dtype)
+    ref = residual64(doubles(d), act, kind, next_kind, gate == "image")
+    assert set(got) == set(ref)
+    for k, (value, bound) in ref.items():
+        check(got[k], value, bound, k)
 
 
 @pytest.mark.parametrize("reverse", [False, True])
