@@ -418,17 +418,15 @@ __global__ __launch_bounds__(row_threads<TPR>(true)) void rows_bwd_k(RowArgs p) 
         if (NEXT) cols.load((const T*)p.x + r * p.C, xn), cols.load((const T*)p.gz + r * p.C, gzn);
         if (BRANCH) cols.load((const T*)p.go + r * p.C, gon);
     };
-    constexpr bool AHEAD = true;
-    if (AHEAD && r0 + group < r1) load(r0 + group);
+    if (r0 + group < r1) load(r0 + group);
     for (long long r = r0 + group; r < r1; r += G) {
         float go[NCH][VEC], nv[NCH][VEC], un[NCH][VEC];
         Row gor, xr, gzr, yr, gr;
-        if (!AHEAD) load(r);
         const float2 st = stn, st2 = st2n;
         if (FULL) copy_row(gr, gn);
         if (BRANCH) copy_row(yr, yn), copy_row(gor, gon);
         if (NEXT) copy_row(xr, xn), copy_row(gzr, gzn);
-        if (AHEAD) load(r + G < r1 ? r + G : r);
+        load(r + G < r1 ? r + G : r);
         float a[NCH][VEC], slope[NCH][VEC];
         if (FULL) gate_acts_slopes(gr, p.act, a, slope);
         if (NEXT) {
