@@ -17,13 +17,13 @@ __device__ __forceinline__ void sigmoid_pair(float g, float& a, float& m) {
     m = e * a;
 }
 
-// The same for silu(v) = v a and its slope a (1 + v m), which a of 2^-126 would make large again far below zero (-4 at the lowest bfloat16, a
-// mask's usual value).  So v is limited instead, to where e is infinite, a 0 and both results 0, at v = -inf too; the product for m
+// The same for a gate: silu(v) = v a and its slope a (1 + v m) would be made large again far below zero by a of 2^-126 (-4 at the lowest
+// bfloat16, a mask's usual value).  So v is limited instead, to where e is infinite, a 0 and all results 0, at v = -inf too; the product for m
 // is clamped to [0, 1], which takes infinity times 0 to 0 and is part of the multiplication.  (NaN passes: through v and a.)  Between -87.3 and the
-// limit a may be flushed: both results are under 88 e^-87 < 2^-118 there.  As many instructions as sigmoid_pair: the residual of [4,64,64,1152]
-// fp16 with a gate a value, forward and backward, 127.3 us (125.9 with sigmoid_pair and its wrong ends); with comparisons and selections of 0
-// behind sigmoid_pair 128.6, with a minimum for m 127.7.
-__device__ __forceinline__ void silu_parts(float v, float& limited, float& a, float& m) {
+// limit a may be flushed: silu and its slope are under 88 e^-87 < 2^-118 there.  As many instructions as sigmoid_pair.  The residual of
+// [4,64,64,1152] fp16 with a silu gate a value, forward and backward: 126.2 us; with comparisons and selections of 0 behind
+// sigmoid_pair 128.6, with a minimum for m 127.7, with a branch for each activation in the forward 127.8.
+__device__ __forceinline__ void gate_parts(float v, float& limited, float& a, float& m) {
     limited = __builtin_elementwise_maximum(v, -126.f);
     const float e = __builtin_amdgcn_exp2f(limited * -1.44269504f);
     a = __builtin_amdgcn_rcpf(1.f + e);
@@ -33,26 +33,18 @@ __device__ __forceinline__ void silu_parts(float v, float& limited, float& a, fl
 // act(v), and act'(v)
 __device__ __forceinline__ float gate_act(float v, int act) {
     if (act == kActNone) return v;
-    float q, m, s;
-    if (act == kActSigmoid) {
-        sigmoid_pair(v, q, m);
-        return q;
-    }
-    silu_parts(v, s, q, m);
-    return s * q;
+    float s, q, m;
+    gate_parts(v, s, q, m);
+    return act == kActSigmoid ? q : s * q;
 }
 
 __device__ __forceinline__ void gate_act_slope(float v, int act, float& f, float& slope) {
     f = v, slope = 1.f;
     if (act == kActNone) return;
-    float q, m, s;
-    if (act == kActSigmoid) {
-        sigmoid_pair(v, q, m);
-        f = q, slope = q * m;
-    } else {
-        silu_parts(v, s, q, m);
-        f = s * q, slope = q * __builtin_fmaf(s, m, 1.f);
-    }
+    float s, q, m;
+    gate_parts(v, s, q, m);
+    if (act == kActSigmoid) f = q, slope = q * m;
+    else f = s * q, slope = q * __builtin_fmaf(s, m, 1.f);
 }
 
 // The same for a lane's pieces of a row (one branch for all of them).
@@ -63,23 +55,13 @@ __device__ __forceinline__ void gate_acts(const P (&g)[N], int act, float (&a)[N
 #pragma unroll
         for (int i = 0; i < VEC; ++i) a[n][i] = to_f32(g[n].v[i]);
     if (act == kActNone) return;
-    if (act == kActSigmoid) {
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                float m;
-                sigmoid_pair(a[n][i], a[n][i], m);
-            }
-        return;
-    }
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             float s, q, m;
-            silu_parts(a[n][i], s, q, m);
-            a[n][i] = s * q;
+            gate_parts(a[n][i], s, q, m);
+            a[n][i] = act == kActSilu ? s * q : q;
         }
 }
 
@@ -95,8 +77,8 @@ __device__ __forceinline__ void gate_acts_slopes(const P (&g)[N], int act, float
         for (int n = 0; n < N; ++n)
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                float m;
-                sigmoid_pair(a[n][i], a[n][i], m);
+                float s, m;
+                gate_parts(a[n][i], s, a[n][i], m);
                 slope[n][i] = a[n][i] * m;
             }
         return;
@@ -106,7 +88,7 @@ __device__ __forceinline__ void gate_acts_slopes(const P (&g)[N], int act, float
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             float s, q, m;
-            silu_parts(a[n][i], s, q, m);
+            gate_parts(a[n][i], s, q, m);
             slope[n][i] = q * __builtin_fmaf(s, m, 1.f);
             a[n][i] = s * q;
         }
