@@ -235,6 +235,13 @@ constexpr int row_threads(bool backward) {
     return TPR > 64 ? TPR : backward ? 512 : 256;
 }
 
+// 1 / sqrt(v).  The instruction takes subnormals for 0, whose result is infinity: with an eps of 0 rows below 1e-19 have such variances, which
+// are taken 2^96 times as large.
+__device__ __forceinline__ float reciprocal_root(float v) {
+    const bool low = v < 0x1p-126f;
+    return __builtin_amdgcn_rsqf(low ? v * 0x1p96f : v) * (low ? 0x1p48f : 1.f);
+}
+
 // Mean and reciprocal deviation of a row held in registers.
 template <int VEC, int TPR, int NCH, typename COLS>
 __device__ __forceinline__ float2 row_stats(const float (&v)[NCH][VEC], const COLS& cols, float inv_c, int kind, float eps,
@@ -247,7 +254,7 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NCH][VEC], const CO
     }
     float q[1] = {cols.sum([&](int n, int i) { return (v[n][i] - mean) * (v[n][i] - mean); })};
     row_sums<TPR, 1>(q, red, flip);
-    return make_float2(mean, __builtin_amdgcn_rsqf(__builtin_fmaf(q[0], inv_c, eps)));
+    return make_float2(mean, reciprocal_root(__builtin_fmaf(q[0], inv_c, eps)));
 }
 
 // x + f * norm(y), y's mean and reciprocal deviation in st.

@@ -55,6 +55,24 @@ def test_a_masked_branch_adds_nothing(gate, value, dtype):
         assert not got[k].any(), k
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-44])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("value", [1e-18, 1.1e-19, 1e-19, 1e-20, 1e-21])
+def test_tiny_rows_without_an_eps(value, kind, eps):
+    """Rows of +-v whose variance is subnormal: +-1, as far as the square is one of the type's numbers (2^-149 apart: v^2, the sum of 64 of them, exact
+    from there, and its 64th part are each off by half of that at most, and so the result by half of 1.5 * 2^-149 / v^2 and
+    some roundings; eps adds 1e-44 / v^2 / 2), and finite gradients of rows that are not tiny beside them."""
+    x = torch.full((3, 64), value)
+    x[:, ::2] *= -1
+    x[2] = torch.randn(64)
+    xd = x.cuda().requires_grad_()
+    y = pcb().channel_norm(xd, kind=kind, eps=eps)
+    off = 0.75 * 2.0 ** -149 / value ** 2 + eps / value ** 2 / 2 + 16 * U
+    assert float((y[:2].detach().cpu() - x[:2].sign()).abs().max()) <= off
+    (g,) = torch.autograd.grad(y, [xd], torch.randn(3, 64, device="cuda"))
+    assert g[2].isfinite().all()
+
+
 # Calls in which a row group goes through several rows (its next row's loads under way, its column sums carried along), with a last one that is
 # not full.  A lane's sum is as many additions as its group has rows, at most N / 512 + 1 (the backward aims at 512 workgroups or more), one or a few
 # for segments and 24 for lanes, wavefronts and the sum over segments; rows_slack's 48 + N / 1024 holds that up to N = 24 * 1024 rows
