@@ -492,9 +492,18 @@ void scan_forward(const Tensor* in, const Tensor& lengths, const ScanShape& s, a
 // ---------------------------------------------------------------------------------------------------------------
 // Python entry points
 
-bool int_arg(PyObject* o, int* v) {
-    *v = (int)PyLong_AsLong(o);
+bool int_arg(PyObject* o, int64_t* v) {
+    *v = PyLong_AsLong(o);
     return !PyErr_Occurred();
+}
+
+// (a code of ops.py's tables)
+bool code_arg(PyObject* o, int* v) {
+    int64_t n;
+    if (!int_arg(o, &n)) return false;
+    TORCH_CHECK_VALUE(n >= 0 && n < 3, "unknown code ", n);
+    *v = (int)n;
+    return true;
 }
 
 PyObject* pair(Tensor&& a, Tensor&& b) {
@@ -518,7 +527,7 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     int kind;
     for (int i = 0; i < kNormInputs; ++i)
         if (!tensor_arg(args[i], &in[i])) return nullptr;
-    if (!int_arg(args[3], &kind)) return nullptr;
+    if (!code_arg(args[3], &kind)) return nullptr;
     const double eps = PyFloat_AsDouble(args[4]);
     if (PyErr_Occurred()) return nullptr;
     check_x(in[kNX]);
@@ -545,7 +554,7 @@ PyObject* py_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
     ResidualShape s;
     for (int i = 0; i < kResidualInputs; ++i)
         if (!tensor_arg(args[i], &in[i])) return nullptr;
-    if (!int_arg(args[8], &s.act) || !int_arg(args[9], &s.kind) || !int_arg(args[10], &s.next_kind)) return nullptr;
+    if (!code_arg(args[8], &s.act) || !code_arg(args[9], &s.kind) || !code_arg(args[10], &s.next_kind)) return nullptr;
     const double eps = PyFloat_AsDouble(args[11]);
     if (PyErr_Occurred()) return nullptr;
     const Tensor &x = in[kRX], &gate = in[kRGate];
@@ -584,7 +593,7 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!tensor_arg(args[i], &in[i])) return nullptr;
     if (!tensor_arg(args[3], &lengths)) return nullptr;
     ScanShape s;
-    int dim;
+    int64_t dim;
     if (!int_arg(args[4], &dim)) return nullptr;
     s.reverse = PyObject_IsTrue(args[5]);
     if (s.reverse < 0) return nullptr;
@@ -594,7 +603,7 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t rank = x.dim();
     TORCH_CHECK_VALUE(rank >= 2, "expected [..., T, ..., C], got ", x.sizes());
     TORCH_CHECK_INDEX(dim >= -rank && dim < rank, "dim ", dim, " of a tensor of ", rank, " dimensions");
-    if (dim < 0) dim += (int)rank;
+    if (dim < 0) dim += rank;
     TORCH_CHECK_VALUE(dim != rank - 1, "the recurrence runs along any dimension but the channels' (", x.sizes(), ", dim ", dim, ")");
     if (s.halves) {
         TORCH_CHECK_VALUE(x.size(-1) % 2 == 0, "without g, x holds both in halves of its channels: an even number, got ", x.size(-1));
@@ -612,7 +621,7 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     TORCH_CHECK_VALUE(O <= 0x7fffffff && W <= 0x7fffffff && O * W <= 0x7fffffff && y_sizes.back() <= 0x7fffffff && y_sizes[dim] <= 0x7fffffff,
                       "more than 2^31 - 1 chains, channels or steps: ", x.sizes());
-    s.O = (int)O, s.T = y_sizes[dim], s.W = (int)W, s.I = (int)y_sizes.back(), s.dim = dim;
+    s.O = (int)O, s.T = y_sizes[dim], s.W = (int)W, s.I = (int)y_sizes.back(), s.dim = (int)dim;
     const Tensor& state = in[kSState];
     if (state.defined()) {
         TORCH_CHECK_TYPE(state.scalar_type() == at::kFloat, "state is float32, got ", state.scalar_type());

@@ -160,3 +160,10 @@ def test_more_channels_than_32_bits_count_are_refused():
     refused(ValueError, "2\\^31 - 1", pcb().gated_scan, x, x, dim=0)
     refused(ValueError, "2\\^31 - 1", pcb().gated_scan_step, one.expand(1, 1 << 32), one.expand(1, 1 << 32), one.expand(1, 1 << 32))
     refused(ValueError, "2\\^31 - 1", pcb().gated_scan_step, one.expand(1, (1 << 32) + 8), one.expand(1, (1 << 32) + 8), torch.zeros(1, 8))
+
+
+def test_dimensions_past_32_bits_are_refused():
+    x = torch.zeros(2, 5, 8)
+    for dim in (1 << 32, (1 << 32) + 1, -(1 << 32)):
+        refused(IndexError, f"dim {dim}", pcb().gated_scan, x, x, dim=dim)
+    refused(OverflowError, "too large", pcb().gated_scan, x, x, dim=1 << 70)
