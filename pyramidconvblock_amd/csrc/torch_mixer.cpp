@@ -519,22 +519,40 @@ PyObject* pair(Tensor&& a, Tensor&& b) {
     return t;
 }
 
+// A call's arguments, checked; false with a Python error.  (The Function forms, which a trace's replays call with other tensors, have theirs checked
+// by check_norm, check_residual and check_scan.)
+bool norm_args(PyObject* const* args, Py_ssize_t n, Tensor* in, int* kind, double* eps) {
+    TORCH_CHECK(n == 5, "norm: 5 arguments expected");
+    for (int i = 0; i < kNormInputs; ++i)
+        if (!tensor_arg(args[i], &in[i])) return false;
+    if (!code_arg(args[3], kind)) return false;
+    *eps = PyFloat_AsDouble(args[4]);
+    if (PyErr_Occurred()) return false;
+    check_x(in[kNX]);
+    check_channels(in[kNX]);
+    TORCH_CHECK_VALUE(*eps >= 0, "eps is ", *eps);
+    check_param(in[kNX], in[kNWeight], "weight"), check_param(in[kNX], in[kNBias], "bias");
+    check_devices(in, kNormInputs);
+    return true;
+}
+
+PyObject* py_check_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tensor in[kNormInputs];
+    int kind;
+    double eps;
+    if (!norm_args(args, n, in, &kind, &eps)) return nullptr;
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
 // norm(x, weight, bias, kind, eps): the norm; None where ChannelNormFunction has to answer (a transform, a trace).
 PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 5, "norm: 5 arguments expected");
     Tensor in[kNormInputs];
     int kind;
-    for (int i = 0; i < kNormInputs; ++i)
-        if (!tensor_arg(args[i], &in[i])) return nullptr;
-    if (!code_arg(args[3], &kind)) return nullptr;
-    const double eps = PyFloat_AsDouble(args[4]);
-    if (PyErr_Occurred()) return nullptr;
-    check_x(in[kNX]);
-    check_channels(in[kNX]);
-    TORCH_CHECK_VALUE(eps >= 0, "eps is ", eps);
-    check_param(in[kNX], in[kNWeight], "weight"), check_param(in[kNX], in[kNBias], "bias");
-    check_devices(in, kNormInputs);
+    double eps;
+    if (!norm_args(args, n, in, &kind, &eps)) return nullptr;
     if (!plain_call(in, kNormInputs)) Py_RETURN_NONE;
     Tensor y;
     {
@@ -545,18 +563,14 @@ PyObject* py_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// residual(x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps): out, or (out, next); None where
-// GatedResidualFunction has to answer.
-PyObject* py_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
+bool residual_args(PyObject* const* args, Py_ssize_t n, Tensor* in, ResidualShape* shape, double* eps_out) {
+    ResidualShape& s = *shape;
     TORCH_CHECK(n == 12, "residual: 12 arguments expected");
-    Tensor in[kResidualInputs];
-    ResidualShape s;
     for (int i = 0; i < kResidualInputs; ++i)
-        if (!tensor_arg(args[i], &in[i])) return nullptr;
-    if (!code_arg(args[8], &s.act) || !code_arg(args[9], &s.kind) || !code_arg(args[10], &s.next_kind)) return nullptr;
-    const double eps = PyFloat_AsDouble(args[11]);
-    if (PyErr_Occurred()) return nullptr;
+        if (!tensor_arg(args[i], &in[i])) return false;
+    if (!code_arg(args[8], &s.act) || !code_arg(args[9], &s.kind) || !code_arg(args[10], &s.next_kind)) return false;
+    const double eps = *eps_out = PyFloat_AsDouble(args[11]);
+    if (PyErr_Occurred()) return false;
     const Tensor &x = in[kRX], &gate = in[kRGate];
     check_x(x);
     check_channels(x);
@@ -573,6 +587,27 @@ PyObject* py_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
         s.P = s.N ? s.N / x.size(0) : 1;   // (1: every row has a gate row of its own after all)
     }
     check_devices(in, kResidualInputs);
+    return true;
+}
+
+PyObject* py_check_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tensor in[kResidualInputs];
+    ResidualShape s;
+    double eps;
+    if (!residual_args(args, n, in, &s, &eps)) return nullptr;
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// residual(x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps): out, or (out, next); None where
+// GatedResidualFunction has to answer.
+PyObject* py_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Tensor in[kResidualInputs];
+    ResidualShape s;
+    double eps;
+    if (!residual_args(args, n, in, &s, &eps)) return nullptr;
     if (!plain_call(in, kResidualInputs)) Py_RETURN_NONE;
     Tensor out, next;
     {
@@ -584,19 +619,26 @@ PyObject* py_residual(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// scan(x, g, state, lengths, dim, reverse): (y, last); None where GatedScanFunction has to answer.  g None: x holds both, in halves.
-PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    TORCH_CHECK(n == 6, "scan: 6 arguments expected");
+// (x, g, the state; lengths; the result's sizes and the state's)
+struct ScanArguments {
     Tensor in[kScanInputs], lengths;
-    for (int i = 0; i < kScanInputs; ++i)
-        if (!tensor_arg(args[i], &in[i])) return nullptr;
-    if (!tensor_arg(args[3], &lengths)) return nullptr;
     ScanShape s;
+    at::DimVector y_sizes, state_sizes;
+};
+
+bool scan_args(PyObject* const* args, Py_ssize_t n, ScanArguments* a) {
+    Tensor(&in)[kScanInputs] = a->in;
+    Tensor& lengths = a->lengths;
+    ScanShape& s = a->s;
+    at::DimVector &y_sizes = a->y_sizes, &state_sizes = a->state_sizes;
+    TORCH_CHECK(n == 6, "scan: 6 arguments expected");
+    for (int i = 0; i < kScanInputs; ++i)
+        if (!tensor_arg(args[i], &in[i])) return false;
+    if (!tensor_arg(args[3], &lengths)) return false;
     int64_t dim;
-    if (!int_arg(args[4], &dim)) return nullptr;
+    if (!int_arg(args[4], &dim)) return false;
     s.reverse = PyObject_IsTrue(args[5]);
-    if (s.reverse < 0) return nullptr;
+    if (s.reverse < 0) return false;
     const Tensor& x = in[kSX];
     check_x(x);
     s.halves = !in[kSG].defined(), s.dtype = dtype_code(x.scalar_type());
@@ -611,7 +653,7 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
         check_like(x, in[kSG], "g");
         TORCH_CHECK_VALUE(in[kSG].sizes() == x.sizes(), "x and g have to be of one shape, got ", x.sizes(), " and ", in[kSG].sizes());
     }
-    at::DimVector y_sizes(x.sizes()), state_sizes;
+    y_sizes = at::DimVector(x.sizes());
     if (s.halves) y_sizes.back() /= 2;
     int64_t O = 1, W = 1;
     for (int64_t d = 0; d < rank; ++d) {
@@ -635,11 +677,27 @@ PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
     }
     const Tensor all[] = {x, in[kSG], state, lengths};
     check_devices(all, 4);
-    if (!plain_call(in, kScanInputs)) Py_RETURN_NONE;
+    return true;
+}
+
+PyObject* py_check_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    ScanArguments a;
+    if (!scan_args(args, n, &a)) return nullptr;
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+// scan(x, g, state, lengths, dim, reverse): (y, last); None where GatedScanFunction has to answer.  g None: x holds both, in halves.
+PyObject* py_scan(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    ScanArguments a;
+    if (!scan_args(args, n, &a)) return nullptr;
+    if (!plain_call(a.in, kScanInputs)) Py_RETURN_NONE;
     Tensor y, last;
     {
         pybind11::gil_scoped_release no_gil;
-        scan_forward(in, lengths, s, y_sizes, state_sizes, wants_grad(in, kScanInputs), &y, &last);
+        scan_forward(a.in, a.lengths, a.s, a.y_sizes, a.state_sizes, wants_grad(a.in, kScanInputs), &y, &last);
     }
     return pair(std::move(y), std::move(last));
     END_HANDLE_TH_ERRORS
@@ -706,6 +764,9 @@ PyObject* py_scan_step(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 PyMethodDef kMixerMethods[] = {
+    {"check_norm", (PyCFunction)(void (*)(void))py_check_norm, METH_FASTCALL, nullptr},
+    {"check_residual", (PyCFunction)(void (*)(void))py_check_residual, METH_FASTCALL, nullptr},
+    {"check_scan", (PyCFunction)(void (*)(void))py_check_scan, METH_FASTCALL, nullptr},
     {"norm", (PyCFunction)(void (*)(void))py_norm, METH_FASTCALL, nullptr},
     {"residual", (PyCFunction)(void (*)(void))py_residual, METH_FASTCALL, nullptr},
     {"scan", (PyCFunction)(void (*)(void))py_scan, METH_FASTCALL, nullptr},

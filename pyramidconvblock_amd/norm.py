@@ -35,6 +35,7 @@ class ChannelNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, kind, eps):
+        _lib.ext().check_norm(x, weight, bias, kind, eps)
         x, weight, bias = _dense(x), _dense(weight), _dense(bias)
         y, stats = ops.norm_forward(x, weight, bias, kind, eps, stats=True)
         ctx.kind, ctx.has_bias = kind, bias is not None
@@ -65,6 +66,7 @@ class GatedResidualFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps):
+        _lib.ext().check_residual(x, y, gate, scale, weight, bias, next_weight, next_bias, act, kind, next_kind, eps)
         x, *rest = (_dense(t) for t in (x, y, gate, scale, weight, bias, next_weight, next_bias))
         out, nxt, stats, next_stats = ops.residual_forward(x, *rest, act, kind, next_kind, eps, stats=True)
         ctx.codes, ctx.has_next_bias = (act, kind, next_kind), next_bias is not None

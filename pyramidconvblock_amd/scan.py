@@ -20,6 +20,10 @@ class GatedScanFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, g, state, lengths, dim, reverse):
+        if g is None:
+            raise TypeError("g has to be a tensor")
+        _lib.ext().check_scan(x, g, state, lengths, dim, reverse)
+        dim %= x.dim()
         x, g = x.detach().contiguous(), g.detach().contiguous()
         state, lengths = (None if t is None else t.detach().contiguous() for t in (state, lengths))
         y, last, states = ops.scan_forward(x, g, state, lengths, dim, reverse, states=True)
@@ -47,7 +51,7 @@ def gated_scan(x, g=None, state=None, lengths=None, dim=-2, reverse=False):
     if y is None:   # under forward-mode differentiation, a functorch transform or a trace
         if g is None:
             x, g = x.chunk(2, -1)
-        y = GatedScanFunction.apply(x, g, state, lengths, dim % x.dim(), reverse)
+        y = GatedScanFunction.apply(x, g, state, lengths, dim, reverse)
     return y
 
 

@@ -271,3 +271,21 @@ def test_capture_asks_only_for_the_gradients_that_are_wanted(op):
         got = res.clone()
         assert torch.equal(got, step())
     assert eager.requires_grad
+
+
+def test_a_replayed_trace_checks_its_tensors():
+    """A trace calls the function forms again with the tensors that it is given: with ones that fit the results of the plain calls, with others a
+    refusal."""
+    x, w = torch.randn(3, 7, 24, device="cuda"), torch.rand(24, device="cuda")
+    calls = {"norm": lambda t: pcb().channel_norm(t, w, kind="layer"),
+             "residual": lambda t: pcb().gated_residual(t, t * 2, w, scale=w, kind="rms", next_kind="layer")[1],
+             "scan": lambda t: pcb().gated_scan(t, t * 2, dim=-2)[0], "halves": lambda t: pcb().gated_scan(t, dim=-2)[0]}
+    for name, f in calls.items():
+        traced = torch.jit.trace(f, (x,), check_trace=False)
+        other = torch.randn(5, 9, 24, device="cuda")
+        assert torch.equal(traced(other), f(other)), name
+        with pytest.raises((RuntimeError, TypeError, ValueError)):
+            traced(other.double())
+        if name in ("norm", "residual"):
+            with pytest.raises((RuntimeError, TypeError, ValueError)):
+                traced(torch.randn(5, 9, 40, device="cuda"))

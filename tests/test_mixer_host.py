@@ -167,3 +167,28 @@ def test_dimensions_past_32_bits_are_refused():
     for dim in (1 << 32, (1 << 32) + 1, -(1 << 32)):
         refused(IndexError, f"dim {dim}", pcb().gated_scan, x, x, dim=dim)
     refused(OverflowError, "too large", pcb().gated_scan, x, x, dim=1 << 70)
+
+
+def test_function_forms_refuse_the_same():
+    """The Function forms are public, and a trace's replays call them with whatever tensors they are given: as many checks, before any launch."""
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    norm, residual, scan = (getattr(pcb(), n + "Function").apply for n in ("ChannelNorm", "GatedResidual", "GatedScan"))
+    refused(RuntimeError, "no CPU path", norm, x, w, None, 1, 1e-6)
+    refused(ValueError, "weight has to be", norm, x, torch.ones(7), None, 1, 1e-6)
+    refused(TypeError, "bias is", norm, x, w, w.half(), 1, 1e-6)
+    refused(ValueError, "C <= 8192", norm, torch.zeros(1, 8193), None, None, 1, 1e-6)
+    refused(ValueError, "code", norm, x, w, None, 3, 1e-6)
+    args = lambda y=x, gate=None, scale=w, act=0, kind=1, next_kind=0, eps=1e-6: (x, y, gate, scale, w, w, None, None, act, kind, next_kind, eps)
+    refused(RuntimeError, "no CPU path", residual, *args())
+    refused(ValueError, "one shape", residual, *args(y=x[:2]))
+    refused(TypeError, "y is", residual, *args(y=x.half()))
+    refused(ValueError, "gate has to be", residual, *args(gate=torch.zeros(2, 8)))
+    refused(ValueError, "scale has to be", residual, *args(scale=torch.ones(4)))
+    refused(ValueError, "eps", residual, *args(eps=-1.0))
+    x = torch.zeros(2, 5, 8)
+    refused(RuntimeError, "no CPU path", scan, x, x, None, None, 1, False)
+    refused(ValueError, "one shape", scan, x, x[:, :4], None, None, 1, False)
+    refused(TypeError, "g has to be", scan, x, None, None, None, 1, False)
+    refused(ValueError, "state has to be", scan, x, x, torch.zeros(2, 7), None, 1, False)
+    refused(TypeError, "lengths is int32", scan, x, x, None, torch.zeros(2, dtype=torch.int64), 1, False)
+    refused(ValueError, "any dimension but the channels", scan, x, x, None, None, 2, False)
