@@ -539,44 +539,45 @@ def residual_backward(gout, gnext, x, y, gate, scale, weight, bias, next_weight,
 
 
 def _scan_extents(x, dim):
+    """x [lead..., T, behind..., channels] as [O][T][W][I]; the axes behind as one with the channels, as far as an int holds it."""
     O = T = W = 1
     for d, n in enumerate(x.shape[:-1]):
         O, T, W = (O * n, T, W) if d < dim else (O, n, W) if d == dim else (O, T, W * n)
-    return O, T, W * x.shape[-1]
+    return (O, T, 1, W * x.shape[-1]) if W * x.shape[-1] <= 0x7fffffff else (O, T, W, x.shape[-1])
 
 
-def _scan_strides(T, I):
+def _scan_strides(T, W, I):
     from ctypes import c_longlong
 
-    return (c_longlong * 3)(T * I, I, I)
+    return (c_longlong * 3)(T * W * I, W * I, I)
 
 
 def scan_forward(x, g, state, lengths, dim, reverse, states=False):
     """Dense x, g [..., T, ..., C], the recurrence along `dim` -> (y, last state fp32, what the backward needs or None)."""
     dev = _lib.require_device(x, g)
-    O, T, I = _scan_extents(x, dim)
+    O, T, W, I = _scan_extents(x, dim)
     y = torch.empty_like(x)
     last = torch.empty(x.shape[:dim] + x.shape[dim + 1:], device=dev, dtype=torch.float32)
     L = _lib.lib()
-    st = _bytes(L.pdw_scan_states_bytes(O, T, 1, I), dev) if states else None
-    if O and I:
-        ws = _bytes(L.pdw_scan_workspace_bytes(O, T, 1, I, 0), dev)
-        s = _scan_strides(T, I)
+    st = _bytes(L.pdw_scan_states_bytes(O, T, W, I), dev) if states else None
+    if O and W and I:
+        ws = _bytes(L.pdw_scan_workspace_bytes(O, T, W, I, 0), dev)
+        s = _scan_strides(T, W, I)
         _launch("pdw_scan_fwd", dev, x.data_ptr(), g.data_ptr(), _ptr(state), _ptr(lengths), y.data_ptr(), last.data_ptr(), _ptr(st),
-                ws.data_ptr(), ws.numel(), O, T, 1, I, s, s, int(bool(reverse)), _lib.dtype_code(x.dtype))
+                ws.data_ptr(), ws.numel(), O, T, W, I, s, s, int(bool(reverse)), _lib.dtype_code(x.dtype))
     return y, last, st
 
 
 def scan_backward(gy, glast, x, g, lengths, states, dim, reverse):
     """-> gradients of (x, g, the initial state)."""
     dev = _lib.require_device(x, g)
-    O, T, I = _scan_extents(x, dim)
+    O, T, W, I = _scan_extents(x, dim)
     gx, gg = torch.empty_like(x), torch.empty_like(g)
     gstate = torch.empty(x.shape[:dim] + x.shape[dim + 1:], device=dev, dtype=torch.float32)
-    if O and I:
-        ws = _bytes(_lib.lib().pdw_scan_workspace_bytes(O, T, 1, I, 1), dev)
-        s = _scan_strides(T, I)
+    if O and W and I:
+        ws = _bytes(_lib.lib().pdw_scan_workspace_bytes(O, T, W, I, 1), dev)
+        s = _scan_strides(T, W, I)
         _launch("pdw_scan_bwd", dev, _ptr(gy), _ptr(glast), x.data_ptr(), g.data_ptr(), _ptr(lengths), states.data_ptr(),
-                gx.data_ptr(), gg.data_ptr(), gstate.data_ptr(), ws.data_ptr(), ws.numel(), O, T, 1, I, s, s, s, s,
+                gx.data_ptr(), gg.data_ptr(), gstate.data_ptr(), ws.data_ptr(), ws.numel(), O, T, W, I, s, s, s, s,
                 int(bool(reverse)), _lib.dtype_code(x.dtype))
     return gx, gg, gstate

@@ -192,3 +192,14 @@ def test_function_forms_refuse_the_same():
     refused(ValueError, "state has to be", scan, x, x, torch.zeros(2, 7), None, 1, False)
     refused(TypeError, "lengths is int32", scan, x, x, None, torch.zeros(2, dtype=torch.int64), 1, False)
     refused(ValueError, "any dimension but the channels", scan, x, x, None, None, 2, False)
+
+
+def test_axes_behind_a_traced_scan_stay_apart_where_their_product_is_too_large():
+    """The function form's extents: one axis of chains up to 2^31 - 1 of them, two beyond (an int would be cut)."""
+    from pyramidconvblock_amd import ops
+
+    meta = lambda *shape: torch.empty(shape, device="meta")
+    assert ops._scan_extents(meta(2, 3, 4, 5, 8), 1) == (2, 3, 1, 160)
+    assert ops._scan_extents(meta(1, 2, 1 << 20, 1 << 12), 1) == (1, 2, 1 << 20, 1 << 12)
+    assert ops._scan_extents(meta(3, 1, (1 << 31) - 1), 1) == (3, 1, 1, (1 << 31) - 1)
+    assert list(ops._scan_strides(2, 1 << 20, 1 << 12)) == [1 << 33, 1 << 32, 1 << 12]
