@@ -17,9 +17,11 @@
 //
 // All of it is in fp32.  No atomics: results are the same from call to call.
 //
-// What bounds it ([32,3136,128] bf16): instructions and their latencies, with eight wavefronts on a compute unit.  Forward a value takes 22
-// (six of them the sigmoid, two of those at a quarter of the rate), 9 us of the 23 us kernel; backward 41, 16 us of 33; the rest is
-// waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward: four
+// What bounds it ([32,3136,128] bf16): instructions and their latencies, with eight wavefronts on a compute unit.  Forward a value takes 26
+// (six of them the sigmoid, two of those at a quarter of the rate; an eighth of a chain's last tile included that is behind its end), 11 us of the
+// 23 us kernel; backward 44, 18 us of 33; the rest is
+// waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward, replays of
+// a captured pass of separate x and g (calls with x and g in halves of one tensor and other inputs each time: 65 us for the last of these): four
 // channels a lane 107 us, two (half the exchanged values for as many steps) 87; stores of whole pieces and one branch a tile 78; strips
 // of 16 channels without segments 73; lanes exchanged in the vector unit and one barrier for both scans of the backward 71; the next
 // tile's loads under way 65; steps a lane that leave the last tile least empty 60.  From batches of 64 on it is memory: 3.8 ns for 1000
@@ -571,7 +573,7 @@ struct ScanShape {
 
 // Without segments x and g are read once, in one launch, as long as there are workgroups for the chip: of eight wavefronts one on each of
 // the 256 compute units, of four wavefronts four on each.  Strips are of 32 channels, of 16 where only those come near 256.
-// Microseconds, forward and backward, [B,3136,128] bf16 (strips of 32: 4 B, of 16: 8 B):
+// Microseconds, forward and backward, replays of a captured pass with eight steps a lane throughout, [B,3136,128] bf16 (strips of 32: 4 B, of 16: 8 B):
 //     B     32 channels, 8 wavefronts     4 wavefronts     16 channels, 8 wavefronts     segments
 //     32                81                    118                     65                    78
 //     38                82                    121                    107                    90

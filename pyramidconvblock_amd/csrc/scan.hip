@@ -9,7 +9,8 @@ void scan_launch_f32(const ScanArgs& p, const ScanShape& shape, ScanPass pass, h
 void scan_launch_f16(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s);
 void scan_launch_bf16(const ScanArgs& p, const ScanShape& shape, ScanPass pass, hipStream_t s);
 
-// Tiles of a chain, and segments of whole tiles: where there are any, about 1024 workgroups of four wavefronts.
+// Tiles of a chain, and segments of whole tiles, backward of pairs of tiles: where there are any, as many as 1024 workgroups of four wavefronts
+// ask for, rounded up to whole tiles, so fewer workgroups ([2,50176,96]: 588 each way, two tiles and four).
 struct ScanCut {
     ScanShape shape;
     long long strips, tiles, seg_tiles, segments;

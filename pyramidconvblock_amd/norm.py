@@ -6,7 +6,8 @@
 
 Any leading dimensions, 1 to 8192 channels, float32, float16 and bfloat16; every tensor of a call is of one type.  Statistics and
 sums are 32-bit, each result is rounded once, and results are the same from call to call.  The gradients have no derivatives
-of their own (``create_graph=True`` raises).  Everything can be captured in a HIP graph; before a backward pass is captured, drop
+of their own (``create_graph=True`` raises).  A gate of its type's lowest value or -inf closes the branch under sigmoid and silu: 0, with
+gradients of 0.  Everything can be captured in a HIP graph; before a backward pass is captured, drop
 the outputs of eager passes over the same tensors: torch's gradient accumulators remember the stream they were made on, and where that is
 the default stream, which a capture cannot make wait, the captured backward raises.
 """

@@ -44,10 +44,11 @@ def test_extreme_gates(shape, next_kind, gate, act, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("value", ["min", "-inf"])
 @pytest.mark.parametrize("gate", ["image", "full"])
-def test_a_masked_branch_adds_nothing(gate, value, dtype):
+@pytest.mark.parametrize("act", ["silu", "sigmoid"])
+def test_a_masked_branch_adds_nothing(act, gate, value, dtype):
     d = residual_data((2, 9, 72), dtype, gate, True, "wb", "")
     d["gate"] = torch.full_like(d["gate"], torch.finfo(dtype).min if value == "min" else float("-inf"))
-    got = run_residual(d, "silu", "layer", "none", dtype)
+    got = run_residual(d, act, "layer", "none", dtype)
     if dtype == torch.float16 and value == "min":   # (of a float16 gate too: its lowest value is below -87)
         assert float(d["gate"].max()) < -87
     assert torch.equal(got["out"].detach().cpu(), d["x"])
