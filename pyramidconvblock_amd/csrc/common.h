@@ -69,6 +69,7 @@ inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // A launch has fewer than 2^32 threads (of a larger one HIP cuts the grid without an error): `grid` workgroups in as many launches as that takes,
 // f(first workgroup, workgroups).  Multiples of the eight dies, which workgroups go to in turn.
+constexpr long long kMostBlocks256 = 0xffffffffLL / 256;   // workgroups of 256 threads that one launch holds
 template <typename F>
 inline void launch_parts(long long grid, int threads, F f) {
     const long long most = (0xffffffffLL / threads) & ~7LL;

@@ -229,6 +229,7 @@ static int fwd_direct_t(const void* x, const void* w, void* y, const ConvGeom& g
     const long long npix = dgrad ? (long long)g.B * g.H * g.W : (long long)g.B * g.OH * g.OW;
     const long long total = npix * (g.C / vec);
     if (total == 0) return 0;
+    if ((total + 255) / 256 > kMostBlocks256) return set_error("convolution: problem too large for one launch (%lld threads)", total), 1;
     const unsigned blocks = (unsigned)((total + 255) / 256);
 #define PDW_LAUNCH(V)                                                                                              \
     if (dgrad)                                                                                                     \

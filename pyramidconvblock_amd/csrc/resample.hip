@@ -1418,7 +1418,7 @@ static inline int gcd_int(int a, int b) {
 
 static bool grid_for(long long total, unsigned* blocks) {
     const long long nb = (total + 255) / 256;
-    if (nb > 0x7fffffffLL) {
+    if (nb > kMostBlocks256) {
         set_error("problem too large for one launch (%lld threads)", total);
         return false;
     }
@@ -1458,7 +1458,7 @@ int avgpool_with_launch(const void* a, void* xp, int B, int H, int W, int C, int
     const long long total = (long long)B * h * w * (C / vec);
     const int nsums = sums ? colsum_workgroups(*sums) : 0, npack = pack ? pack_workgroups(*pack) : 0;
     unsigned blocks;
-    if (!grid_for(total, &blocks) || (unsigned long long)blocks + nsums + npack > 0x7fffffffULL) return 1;
+    if (!grid_for(total, &blocks) || (unsigned long long)blocks + nsums + npack > (unsigned long long)kMostBlocks256) return 1;
     const size_t lds = sums ? 256 * 16 / esize(dtype) * sizeof(float) : 0;
     const bool flight = pool_in_flight(blocks, H, W, h, w);
 #define CALL(T, V) if (flight) GO(T, V, true); else GO(T, V, false);
@@ -1590,7 +1590,7 @@ int gate_pair_fwd_launch(const void* xf, const void* xh, void* y, int B, int H, 
     unsigned bf, bh;
     if (tf == 0) return 0;
     if (!grid_for((tf + kGateItems - 1) / kGateItems, &bf) || !grid_for(th, &bh) ||
-        (unsigned long long)bf + bh > 0x7fffffffULL)
+        (unsigned long long)bf + bh > (unsigned long long)kMostBlocks256)
         return 1;
     const float sy = (float)h / (float)H, sx = (float)w / (float)W, sc = sqrtf((float)(gw > 0 ? gw : I / 2));
 #define CALL(T, V) hipLaunchKernelGGL((gate_pair_fwd_k<T, V>), dim3(bf + bh), dim3(256), 0, s, (const T*)xf, (const T*)xh, (T*)y, h, w, I, H, W, ldy, sy, sx, sc, bf, tf, th);
@@ -1613,7 +1613,7 @@ int gate_pair_mean_fwd_launch(const void* xf, const void* xh, void* y, int B, in
     const unsigned ndeep = (unsigned)B * (unsigned)cdiv(mean.D, kMeanFew);
     const bool deep = mean.D >= 256 && (unsigned long long)bf + bh + ndeep <= 1024;   // (four to a compute unit)
     const unsigned nmean = deep ? ndeep : (unsigned)(B * mean_slices(mean.D));
-    if ((unsigned long long)bf + bh + nmean > 0x7fffffffULL) return 1;
+    if ((unsigned long long)bf + bh + nmean > (unsigned long long)kMostBlocks256) return 1;
     const float sy = (float)h / (float)H, sx = (float)w / (float)W, sc = sqrtf((float)(gw > 0 ? gw : I / 2));
 #define GO(T, V, DEEP) hipLaunchKernelGGL((gate_pair_mean_fwd_k<T, V, DEEP>), dim3(bf + bh + nmean), dim3(256), mean_lds(mean.D), s, (const T*)xf, (const T*)xh, (T*)y, h, w, I, H, W, ldy, sy, sx, sc, bf, tf, th, mean, nmean)
 #define CALL(T, V) if (deep) GO(T, V, true); else GO(T, V, false);
@@ -1631,7 +1631,7 @@ int gate_pair_colsum_bwd_launch(const void* gy, const void* xf, const void* xh, 
     const unsigned nsums = (unsigned)colsum_workgroups(sums);
     unsigned bf, bh;
     if (!grid_for((tf + kGateItems - 1) / kGateItems, &bf) || !grid_for(th, &bh) ||
-        (unsigned long long)bf + bh + nsums > 0x7fffffffULL)
+        (unsigned long long)bf + bh + nsums > (unsigned long long)kMostBlocks256)
         return 1;
     const float sc = sqrtf((float)(gw > 0 ? gw : I / 2)), sy = (float)h / (float)H, sx = (float)w / (float)W;
     const size_t lds = 256 * 16 / esize(dtype) * sizeof(float);
@@ -1679,7 +1679,7 @@ int gate_pair_bwd_launch(const void* gy, const void* xf, const void* xh, void* g
     unsigned bf, bh;
     if (tf == 0 || th == 0) return tf == 0 && th == 0 ? 0 : -1;
     if (!grid_for((tf + kGateItems - 1) / kGateItems, &bf) || !grid_for(th, &bh) ||
-        (unsigned long long)bf + bh > 0x7fffffffULL)
+        (unsigned long long)bf + bh > (unsigned long long)kMostBlocks256)
         return 1;
     const float sc = sqrtf((float)(gw > 0 ? gw : I / 2));
     if (H != 2 * h || W != 2 * w || h < 2 || w < 2) {   // any ratio of extents
@@ -1709,7 +1709,7 @@ int block_mid_fwd_launch(const void* xf, const void* xh, void* y, int B, int H, 
     unsigned bf, bh;
     if (tf == 0) return -1;
     if (!grid_for((tf + kGateItems - 1) / kGateItems, &bf) || !grid_for(th, &bh) ||
-        (unsigned long long)bf + bh + B > 0x7fffffffULL)
+        (unsigned long long)bf + bh + B > (unsigned long long)kMostBlocks256)
         return 1;
     const float sy = (float)h / (float)H, sx = (float)w / (float)W, sc = sqrtf((float)(gw > 0 ? gw : I / 2));
     const PoolFwdJob job{parts, nparts, B, D, 1.f / (float)P, wp, bp, bo, m, rowbias};
@@ -1733,7 +1733,7 @@ int bilinear_pool_fwd_launch(const void* x, void* y, int B, int h, int w, int C,
     const long long total = (long long)B * H * W * (C / 8);
     unsigned blocks;
     if (total == 0) return -1;
-    if (!grid_for(total, &blocks) || (unsigned long long)blocks + B > 0x7fffffffULL) return 1;
+    if (!grid_for(total, &blocks) || (unsigned long long)blocks + B > (unsigned long long)kMostBlocks256) return 1;
     const float sy = (float)h / (float)H, sx = (float)w / (float)W;
     const PoolFwdJob job{parts, nparts, B, D, 1.f / (float)P, wp, bp, bo, m, rowbias};
     const size_t lds = (size_t)9 * D * sizeof(float);
@@ -1757,7 +1757,7 @@ int block_mid_bwd_launch(const void* gy, const void* xf, const void* xh, void* g
     unsigned bf, bh;
     if (tf == 0) return -1;
     if (!grid_for((tf + kGateItems - 1) / kGateItems, &bf) || !grid_for(th, &bh) ||
-        (unsigned long long)bf + bh + B + D > 0x7fffffffULL)
+        (unsigned long long)bf + bh + B + D > (unsigned long long)kMostBlocks256)
         return 1;
     const float sc = sqrtf((float)(gw > 0 ? gw : I / 2));
     float* gs = ws + spatial_sum_workspace(B, P, D) / sizeof(float);

@@ -203,3 +203,16 @@ def test_axes_behind_a_traced_scan_stay_apart_where_their_product_is_too_large()
     assert ops._scan_extents(meta(1, 2, 1 << 20, 1 << 12), 1) == (1, 2, 1 << 20, 1 << 12)
     assert ops._scan_extents(meta(3, 1, (1 << 31) - 1), 1) == (3, 1, 1, (1 << 31) - 1)
     assert list(ops._scan_strides(2, 1 << 20, 1 << 12)) == [1 << 33, 1 << 32, 1 << 12]
+
+
+def test_calls_of_more_threads_than_a_launch_holds_are_refused():
+    """HIP cuts the grid of 2^32 threads and more without an error, so single launches of that many are refused, before any of them: pools,
+    bilinear maps, gates and direct convolutions of 2^32 results, a thread each."""
+    L = lib()
+    side = 1 << 11   # 2^11 x 2^11 pixels, 2^10 images, one channel: 2^32
+    for call in (lambda b: L.pdw_avgpool_fwd(16, 16, b, side, side, 1, side, side, 0, None),
+                 lambda b: L.pdw_bilinear_fwd(16, 16, b, side, side, 1, side, side, 0, 0, None),
+                 lambda b: L.pdw_gate_fwd(16, 16, b * side * side, 2, 0, 0, None),
+                 lambda b: L.pdw_dwconv_fwd(16, 16, 16, b, side + 1, side + 1, 1, 2, 2, 1, 1, 0, 0, 1, 1, 0, None),
+                 lambda b: L.pdw_dwconv_dgrad(16, 16, 16, b, side, side, 1, 2, 2, 1, 1, 0, 0, 1, 1, 0, None)):
+        assert call(1 << 10) == 1 and b"too large for one launch" in L.pdw_last_error(), L.pdw_last_error()
