@@ -67,9 +67,10 @@ inline int pick_vec(int C, size_t elem, const void* const* ptrs, int nptrs) {
 
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// A launch has fewer than 2^32 threads (of a larger one HIP cuts the grid without an error): `grid` workgroups in as many launches as that takes,
-// f(first workgroup, workgroups).  Multiples of the eight dies, which workgroups go to in turn.
-constexpr long long kMostBlocks256 = 0xffffffffLL / 256;   // workgroups of 256 threads that one launch holds
+// A launch has fewer than 2^32 threads (of a larger one HIP cuts the grid without an error): as many workgroups of 256.
+constexpr long long kMostBlocks256 = 0xffffffffLL / 256;
+
+// `grid` workgroups in as many launches as that takes, f(first workgroup, workgroups).  Multiples of the eight dies, which workgroups go to in turn.
 template <typename F>
 inline void launch_parts(long long grid, int threads, F f) {
     const long long most = (0xffffffffLL / threads) & ~7LL;

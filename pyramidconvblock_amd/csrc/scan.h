@@ -18,9 +18,8 @@
 // All of it is in fp32.  No atomics: results are the same from call to call.
 //
 // What bounds it ([32,3136,128] bf16): instructions and their latencies, with eight wavefronts on a compute unit.  Forward a value takes 26
-// (six of them the sigmoid, two of those at a quarter of the rate; an eighth of a chain's last tile included that is behind its end), 11 us of the
-// 23 us kernel; backward 44, 18 us of 33; the rest is
-// waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward, replays of
+// (six of them the sigmoid, two of those at a quarter of the rate; an eighth of the tiles' steps lie behind a chain's end), 11 us of the
+// 23 us kernel; backward 44, 18 us of 33; the rest is waiting, for loads and for the other wavefronts.  The tensors themselves would take 15 and 25 us from memory.  Forward and backward, replays of
 // a captured pass of separate x and g (calls with x and g in halves of one tensor and other inputs each time: 65 us for the last of these): four
 // channels a lane 107 us, two (half the exchanged values for as many steps) 87; stores of whole pieces and one branch a tile 78; strips
 // of 16 channels without segments 73; lanes exchanged in the vector unit and one barrier for both scans of the backward 71; the next
