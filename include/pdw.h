@@ -539,6 +539,63 @@ int pdw_scan_bwd(const void *gy, const float *glast, const void *x, const void *
 int pdw_scan_step(const void *x, const void *g, const float *state, float *new_state, void *y, long long B, int C,
                   long long ldx, long long ldg, int dtype, void *stream);
 
+/* Norms of the rows of heads (queries, and keys where there are any) with the rotation by positions in the same pass.
+ *   n = x (PDW_HEAD_NONE), x / sqrt(mean x^2 + eps) * weight (PDW_HEAD_RMS) or x / sqrt(sum x^2 + eps) * weight (PDW_HEAD_L2)
+ * for each row of d channels (1 to PDW_HEAD_MAX_CHANNELS); the first 2 P channels of n, P the sum of the sections, are pairs, halves (i, P + i)
+ * or (neighbours != 0) (2 i, 2 i + 1), and pair i is turned by position * frequency_i, the position along the axis in whose section i lies.
+ * Tensor 0 has heads[0] heads, tensor 1 (may be NULL) heads[1]; element (token, head, i) of it is x[token * xt + head * xh + i].
+ * Positions: NULL, tokens are a grid whose last axes have the extents grid[0..axes); or rows of `axes` numbers of position_type, one for each
+ * of the last `positions_rows` tokens' places, repeated (token modulo rows).  Frequencies (device, fp32, radians, P of them): NULL, then
+ * base^(-j / section) for pair j of each section.  Weights have the tensors' type; NULL: 1. */
+enum { PDW_HEAD_NONE = 0, PDW_HEAD_RMS = 1, PDW_HEAD_L2 = 2 };
+enum { PDW_POSITIONS_GRID = 0, PDW_POSITIONS_I32 = 1, PDW_POSITIONS_I64 = 2, PDW_POSITIONS_F32 = 3 };
+#define PDW_HEAD_MAX_CHANNELS 256
+typedef struct {
+    const void *x[2], *weight[2];
+    long long xt[2], xh[2];
+    const void *positions;
+    const float *frequencies;
+    long long tokens, positions_rows;
+    int heads[2], grid[3], sections[3], d, axes, kind, neighbours, position_type, dtype;
+    float eps;
+    double base;
+} pdw_rotary;
+/* y[0], y[1] dense [token][head][d]. */
+int pdw_rotary_fwd(const pdw_rotary *call, void *const y[2], void *stream);
+/* gx[2] (dense) and gweight[2] from gy[2] (dense); each result may be NULL.  Workspace: needed where a gweight is wanted. */
+size_t pdw_rotary_bwd_workspace_bytes(int d);
+int pdw_rotary_bwd(const pdw_rotary *call, const void *const gy[2], void *const gx[2], void *const gweight[2], void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* The gated delta rule along the second axis of [O][T][W][heads][..]: for each of the O * W * Hv chains a state S [dk][dv],
+ *   u_t = beta_t (v_t - a_t S_(t-1)^T k_t),   S_t = a_t S_(t-1) + k_t u_t^T,   y_t = scale S_t^T q_t,
+ * a = sigmoid(g), beta = sigmoid(b) (logits != 0) or a = exp(g), beta = b (g at most 0 by right).  q, k have Hk heads of dk channels, v and y Hv of dv,
+ * g and b a number for each of Hv; value heads share key heads in groups of Hv / Hk.  dk, dv: 1 to PDW_DELTA_MAX_CHANNELS.
+ * Element (o, t, w, head, i) is x[o * s[0] + t * s[1] + w * s[2] + head * s[3] + i].  y and the gradients are dense.
+ * h0, last [O][W][Hv][dk][dv], fp32, either may be NULL.  lengths[O] (device, may be NULL): valid steps, limited to 0..T; what lies behind is not
+ * read, y and the gradients are 0 there.  reverse: from the last valid step to the first.  gates_f32: g and b are fp32 whatever dtype is.
+ * `states` (pdw_delta_states_bytes; NULL where no backward follows): what the backward needs.  States and sums are fp32; y is rounded once.  Products
+ * are made of bf16 planes: infinities in k, q, v or a state come out as NaN. */
+#define PDW_DELTA_MAX_CHANNELS 128
+typedef struct {
+    const void *q, *k, *v, *g, *b;
+    long long qs[4], ks[4], vs[4], gs[4], bs[4];
+    const float *h0;
+    const int *lengths;
+    long long T;
+    int O, W, Hk, Hv, dk, dv, reverse, logits, gates_f32, dtype;
+    float scale;
+} pdw_delta;
+size_t pdw_delta_states_bytes(const pdw_delta *call);
+size_t pdw_delta_workspace_bytes(const pdw_delta *call, int backward, int with_states);
+int pdw_delta_fwd(const pdw_delta *call, void *y, float *last, void *states, void *workspace, size_t workspace_bytes, void *stream);
+/* Gradients from gy (dense) and glast (may be NULL: 0); gh0 may be NULL, as may each of the others. */
+int pdw_delta_bwd(const pdw_delta *call, const void *gy, const float *glast, const void *states, void *gq, void *gk, void *gv, void *gg,
+                  void *gb, float *gh0, void *workspace, size_t workspace_bytes, void *stream);
+/* The same step by step, for single tokens and a few: h0 is the state (NULL: 0), last the new one, which may be h0 itself, but must not overlap
+ * it otherwise. */
+int pdw_delta_step(const pdw_delta *call, void *y, float *last, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -118,8 +118,33 @@ _SIGS = {
     "pdw_scan_bwd": (c_int, [c_void_p] * 10 + [c_size_t, c_int, c_longlong, c_int, c_int] + [c_void_p] * 4 + [c_int] * 2
                      + [c_void_p]),
     "pdw_scan_step": (c_int, [c_void_p] * 5 + [c_longlong, c_int, c_longlong, c_longlong, c_int, c_void_p]),
+    "pdw_rotary_fwd": (c_int, [c_void_p] * 3),
+    "pdw_rotary_bwd_workspace_bytes": (c_size_t, [c_int]),
+    "pdw_rotary_bwd": (c_int, [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "pdw_delta_states_bytes": (c_size_t, [c_void_p]),
+    "pdw_delta_workspace_bytes": (c_size_t, [c_void_p, c_int, c_int]),
+    "pdw_delta_fwd": (c_int, [c_void_p] * 5 + [c_size_t, c_void_p]),
+    "pdw_delta_bwd": (c_int, [c_void_p] * 11 + [c_size_t, c_void_p]),
+    "pdw_delta_step": (c_int, [c_void_p] * 4),
 }
 EXPORTS = tuple(_SIGS)
+
+
+class Rotary(ctypes.Structure):
+    """pdw_rotary"""
+
+    _fields_ = [("x", c_void_p * 2), ("weight", c_void_p * 2), ("xt", c_longlong * 2), ("xh", c_longlong * 2), ("positions", c_void_p),
+                ("frequencies", c_void_p), ("tokens", c_longlong), ("positions_rows", c_longlong), ("heads", c_int * 2), ("grid", c_int * 3),
+                ("sections", c_int * 3), ("d", c_int), ("axes", c_int), ("kind", c_int), ("neighbours", c_int), ("position_type", c_int),
+                ("dtype", c_int), ("eps", c_float), ("base", ctypes.c_double)]
+
+
+class Delta(ctypes.Structure):
+    """pdw_delta"""
+
+    _fields_ = [(n, c_void_p) for n in "qkvgb"] + [(n + "s", c_longlong * 4) for n in "qkvgb"] + [
+        ("h0", c_void_p), ("lengths", c_void_p), ("T", c_longlong)] + [
+        (n, c_int) for n in ("O", "W", "Hk", "Hv", "dk", "dv", "reverse", "logits", "gates_f32", "dtype")] + [("scale", c_float)]
 
 
 def lib():

@@ -14,6 +14,8 @@
 #include "kernels.h"
 #include "pool_branch.h"
 #include "reduce_parts.h"
+#include "delta_common.h"
+#include "rotary.h"
 #include "scan.h"
 
 namespace pdw {
@@ -122,7 +124,7 @@ using namespace pdw;
 
 extern "C" {
 
-int pdw_version(void) { return 6; }
+int pdw_version(void) { return 7; }
 
 const char* pdw_last_error(void) { return g_err; }
 
@@ -889,6 +891,124 @@ int pdw_scan_step(const void* x, const void* g, const float* state, float* new_s
     if (B == 0 || C == 0) return 0;
     if (!x || !g || !state || !new_state || !y) return set_error("pdw_scan_step: null pointer"), 1;
     return scan_step_launch(x, g, state, new_state, y, B, C, ldx, ldg, dtype, (hipStream_t)stream);
+}
+
+static int rotary_args(const char* fn, const pdw_rotary* c, RotaryArgs& p) {
+    if (!c) return set_error("%s: null pointer", fn), 1;
+    if (!valid_dtype(c->dtype)) return set_error("%s: unknown dtype %d", fn, c->dtype), 1;
+    if (c->kind < kRotaryNone || c->kind > kRotaryL2 || c->position_type < kPositionGrid || c->position_type > kPositionF32)
+        return set_error("%s: unknown kind %d or type of positions %d", fn, c->kind, c->position_type), 1;
+    if (c->d < 1 || c->d > kRotaryMaxDim || c->axes < 1 || c->axes > 3 || c->tokens < 0 || c->heads[0] < 0 || c->heads[1] < 0)
+        return set_error("%s: bad extents d=%d axes=%d tokens=%lld heads=%d,%d", fn, c->d, c->axes, c->tokens, c->heads[0], c->heads[1]), 1;
+    // (a workgroup counts the rows of its tokens in 32 bits)
+    if (c->heads[0] > 1 << 16 || c->heads[1] > 1 << 16) return set_error("%s: more than 65536 heads", fn), 1;
+    int P = 0;
+    for (int a = 0; a < c->axes; ++a) {
+        if (c->sections[a] < 0 || c->sections[a] > kRotaryMaxDim) return set_error("%s: section %d of %d pairs", fn, a, c->sections[a]), 1;
+        P += c->sections[a], p.ends[a] = P;
+    }
+    for (int a = c->axes; a < 3; ++a) p.ends[a] = P;
+    if (2 * P > c->d) return set_error("%s: %d pairs of %d channels", fn, P, c->d), 1;
+    if (c->tokens > 0 && ((c->heads[0] && !c->x[0]) || (c->heads[1] && !c->x[1]))) return set_error("%s: null pointer", fn), 1;
+    p.grid[0] = p.grid[1] = p.grid[2] = 1;
+    if (c->position_type == kPositionGrid) {
+        for (int a = 0; a < c->axes; ++a) {
+            if (c->tokens > 0 && c->grid[a] < 1) return set_error("%s: grid extent %d", fn, c->grid[a]), 1;
+            p.grid[3 - c->axes + a] = c->grid[a] < 1 ? 1 : c->grid[a];
+        }
+    } else if (c->tokens > 0 && (!c->positions || c->positions_rows < 1)) {
+        return set_error("%s: no positions", fn), 1;
+    }
+    for (int s = 0; s < 2; ++s)
+        p.x[s] = c->x[s], p.xt[s] = c->xt[s], p.xh[s] = c->xh[s], p.heads[s] = c->heads[s], p.w[s] = c->weight[s];
+    p.positions = c->positions, p.frequencies = c->frequencies, p.N = c->tokens, p.np = c->positions_rows, p.d = c->d, p.P = P;
+    p.axes = c->axes, p.kind = c->kind, p.neighbours = c->neighbours != 0, p.pkind = c->position_type, p.eps = c->eps;
+    if (!c->frequencies) {
+        int i = 0;
+        for (int a = 0; a < c->axes; ++a)
+            for (int j = 0; j < c->sections[a]; ++j) p.turns[i++] = std::pow(c->base, -(double)j / c->sections[a]) * 0.15915494309189535;
+    }
+    return 0;
+}
+
+int pdw_rotary_fwd(const pdw_rotary* c, void* const y[2], void* stream) {
+    RotaryArgs p{};
+    if (int e = rotary_args("pdw_rotary_fwd", c, p)) return e;
+    if (p.N == 0 || (!p.heads[0] && !p.heads[1])) return 0;
+    if (!y || (p.heads[0] && !y[0]) || (p.heads[1] && !y[1])) return set_error("pdw_rotary_fwd: null pointer"), 1;
+    p.y[0] = y[0], p.y[1] = y[1];
+    return rotary_run(p, false, nullptr, nullptr, nullptr, 0, c->dtype, (hipStream_t)stream);
+}
+
+size_t pdw_rotary_bwd_workspace_bytes(int d) { return d < 1 || d > kRotaryMaxDim ? 0 : rotary_workspace(d); }
+
+int pdw_rotary_bwd(const pdw_rotary* c, const void* const gy[2], void* const gx[2], void* const gweight[2], void* workspace,
+                   size_t workspace_bytes, void* stream) {
+    RotaryArgs p{};
+    if (int e = rotary_args("pdw_rotary_bwd", c, p)) return e;
+    if (p.N == 0 || (!p.heads[0] && !p.heads[1])) return 0;
+    if (!gy || !gx || !gweight || (p.heads[0] && !gy[0]) || (p.heads[1] && !gy[1])) return set_error("pdw_rotary_bwd: null pointer"), 1;
+    for (int s = 0; s < 2; ++s) p.gy[s] = gy[s], p.y[s] = gx[s];
+    return rotary_run(p, true, gweight[0], gweight[1], workspace, workspace_bytes, c->dtype, (hipStream_t)stream);
+}
+
+static int delta_args(const char* fn, const pdw_delta* c, DeltaArgs& p) {
+    if (!c) return set_error("%s: null pointer", fn), 1;
+    if (!valid_dtype(c->dtype)) return set_error("%s: unknown dtype %d", fn, c->dtype), 1;
+    if (c->O < 0 || c->W < 0 || c->T < 0 || c->T > 0x7fffffffLL || c->Hk < 0 || c->Hv < 0)
+        return set_error("%s: bad extents O=%d T=%lld W=%d heads=%d,%d", fn, c->O, c->T, c->W, c->Hk, c->Hv), 1;
+    if (c->dk < 1 || c->dk > PDW_DELTA_MAX_CHANNELS || c->dv < 1 || c->dv > PDW_DELTA_MAX_CHANNELS)
+        return set_error("%s: %d and %d channels of a head, 1 to %d are possible", fn, c->dk, c->dv, PDW_DELTA_MAX_CHANNELS), 1;
+    if (c->Hv && (c->Hk < 1 || c->Hv % c->Hk)) return set_error("%s: %d value heads for %d key heads", fn, c->Hv, c->Hk), 1;
+    const long long rows = (long long)c->O * c->W;
+    if (rows > 0x7fffffffLL || rows * c->Hv > 0x7fffffffLL) return set_error("%s: more than 2^31 - 1 chains", fn), 1;
+    if (rows * c->Hv && c->T && (!c->q || !c->k || !c->v || !c->g || !c->b)) return set_error("%s: null pointer", fn), 1;
+    auto strides = [](const long long* s) { return DeltaStrides{s[0], s[1], s[2], s[3]}; };
+    p.q = c->q, p.k = c->k, p.v = c->v, p.g = c->g, p.b = c->b;
+    p.qs = strides(c->qs), p.ks = strides(c->ks), p.vs = strides(c->vs), p.gs = strides(c->gs), p.bs = strides(c->bs);
+    auto dense = [&](long long H, long long d) { return DeltaStrides{c->T * c->W * H * d, c->W * H * d, H * d, d}; };
+    p.ys = dense(c->Hv, c->dv), p.gqs = dense(c->Hk, c->dk), p.gvs = p.ys, p.ggs = dense(c->Hv, 1);
+    p.h0 = c->h0, p.lengths = c->lengths, p.T = c->T, p.O = c->O, p.W = c->W, p.Hk = c->Hk, p.Hv = c->Hv, p.dk = c->dk, p.dv = c->dv;
+    p.chains = (int)(rows * c->Hv), p.reverse = c->reverse != 0, p.logits = c->logits != 0, p.gates_f32 = c->gates_f32 != 0, p.scale = c->scale;
+    return 0;
+}
+
+size_t pdw_delta_states_bytes(const pdw_delta* c) {
+    DeltaArgs p{};
+    return delta_args("pdw_delta_states_bytes", c, p) ? 0 : delta_states_bytes(p.chains, p.T, p.dk, p.dv, c->dtype);
+}
+
+size_t pdw_delta_workspace_bytes(const pdw_delta* c, int backward, int with_states) {
+    DeltaArgs p{};
+    return delta_args("pdw_delta_workspace_bytes", c, p) ? 0 : delta_workspace(p.chains, p.T, p.dk, p.dv, backward != 0, with_states != 0, c->dtype);
+}
+
+int pdw_delta_fwd(const pdw_delta* c, void* y, float* last, void* states, void* workspace, size_t workspace_bytes, void* stream) {
+    DeltaArgs p{};
+    if (int e = delta_args("pdw_delta_fwd", c, p)) return e;
+    if (!p.chains) return 0;
+    if (p.T && !y) return set_error("pdw_delta_fwd: null pointer"), 1;
+    p.y = y, p.last = last;
+    return delta_run(p, states, false, workspace, workspace_bytes, c->dtype, (hipStream_t)stream);
+}
+
+int pdw_delta_bwd(const pdw_delta* c, const void* gy, const float* glast, const void* states, void* gq, void* gk, void* gv, void* gg,
+                  void* gb, float* gh0, void* workspace, size_t workspace_bytes, void* stream) {
+    DeltaArgs p{};
+    if (int e = delta_args("pdw_delta_bwd", c, p)) return e;
+    if (!p.chains) return 0;
+    if (p.T && (!gy || !states)) return set_error("pdw_delta_bwd: null pointer"), 1;
+    p.gy = gy, p.glast = glast, p.gq = gq, p.gk = gk, p.gv = gv, p.gg = gg, p.gb = gb, p.gh0 = gh0;
+    return delta_run(p, const_cast<void*>(states), true, workspace, workspace_bytes, c->dtype, (hipStream_t)stream);
+}
+
+int pdw_delta_step(const pdw_delta* c, void* y, float* last, void* stream) {
+    DeltaArgs p{};
+    if (int e = delta_args("pdw_delta_step", c, p)) return e;
+    if (!p.chains) return 0;
+    if (!last || (p.T && !y)) return set_error("pdw_delta_step: null pointer"), 1;
+    p.y = y, p.last = last;
+    return delta_steps_run(p, c->dtype, (hipStream_t)stream);
 }
 
 }  // extern "C"

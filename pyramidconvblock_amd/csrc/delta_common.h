@@ -1,0 +1,471 @@
+// The gated delta rule: what its kernels share.  (The mathematics: delta_fwd.h and delta_bwd.h.)
+//
+// Products run on the bf16 matrix cores whatever the tensors' type: a value is a sum of bf16 planes (the value rounded, what that left
+// rounded, and so on), and a product of two such sums leaves out the products of planes that are below the result's precision.  What comes from
+// the tensors takes as many planes as hold it exactly, except the last bits of fp32 and of fp16 (1 for bf16, 2 for fp16, 3 for fp32); what
+// was computed in fp32 (the chunk's triangular system, its solutions, states) takes 2 planes for 16-bit tensors, 16 bits and so 2^-17 of a
+// value, and 3 for fp32.  Sums are the matrix cores' fp32.  So results are off by their own rounding and by little else, where single
+// bf16 operands had put 2^-9 of every intermediate into them; and fp32 takes 6 products of 16 cycles where the fp32 matrix instruction takes
+// eight of 32.
+//
+// Fragments of the 16x16x32 instruction: lane l has row (column) l % 16 and 8 values along the inner axis.  A result has column l % 16 and
+// rows 4 (l / 16) + r, so results turn into operands of a next product whose inner axis is their rows without an exchange of lanes: an inner
+// axis of 32 is two tiles of 16 rows, value j of lane group g stands for row 16 (j / 4) + 4 g + j % 4 ("tile order"), and the other operand is
+// read in that order too.
+#pragma once
+#include "common.h"
+#include "row_norm.h"
+
+namespace pdw {
+
+constexpr int kDeltaChunk = 64;   // steps of a chunk
+constexpr int kDeltaPad = 8;      // values behind an LDS row: rows of 16 values in a row stay on different banks
+
+// Element (o, t, w, head, i) of a tensor is base[o * o + t * t + w * w + head * h + i].
+struct DeltaStrides {
+    long long o, t, w, h;
+};
+
+struct DeltaArgs {
+    const void *q, *k, *v, *g, *b, *gy;
+    DeltaStrides qs, ks, vs, gs, bs;
+    DeltaStrides ys;                       // of y and gy
+    void *y, *gq, *gk, *gv, *gg, *gb;      // gradients dense: [O][T][W][heads][..]
+    DeltaStrides gqs, gvs, ggs;            // gqs of gq and gk, ggs of gg and gb
+    const float *h0, *glast;               // [chain][dk][dv], or null (0)
+    float *last, *gh0;                     // [chain][dk][dv], or null
+    const int* lengths;                    // [O], or null (T)
+    // between the kernels, by chain and chunk
+    bf16_t *wp, *kt, *s0, *u, *ka, *ds1;
+    float *ub, *du, *c0, *dec;
+    long long T, NC;                       // steps; chunks of a chain
+    int O, W, Hk, Hv, dk, dv, dvp;         // dvp: dv up to whole 32s
+    int chains;                            // O * W * Hv, one state each
+    long long first;                       // the launch's first workgroup (launch_parts)
+    int reverse, logits, gates_f32;
+    int vec;                               // bits: q, k, v, gy, y, gq and gk, gv lie in aligned rows of whole pieces of 8
+    float scale;
+};
+
+enum : int { kVecQ = 1, kVecK = 2, kVecV = 4, kVecGy = 8, kVecY = 16, kVecGqk = 32, kVecGv = 64 };
+
+template <typename T>
+struct DeltaPlanes;
+template <>
+struct DeltaPlanes<bf16_t> {
+    static constexpr int kRaw = 1, kMade = 2;
+};
+template <>
+struct DeltaPlanes<f16_t> {
+    static constexpr int kRaw = 2, kMade = 2;
+};
+template <>
+struct DeltaPlanes<float> {
+    static constexpr int kRaw = 3, kMade = 3;
+};
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int NP>
+struct Frag {   // inner axis of 32
+    bf16x8 p[NP];
+};
+template <int NP>
+struct Half {   // inner axis of 16: value j of lane group g is 4 g + j
+    bf16x4 p[NP];
+};
+
+// c + a b: the products of planes i and j with i + j below the larger number of planes, the small ones first.
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
+    constexpr int N = NA > NB ? NA : NB;
+#pragma unroll
+    for (int s = N - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i <= s; ++i)
+            if (i < NA && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.p[i], b.p[s - i], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ f32x4 mma16(bf16x4 a, bf16x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma(const Half<NA>& a, const Half<NB>& b, f32x4 c) {
+    constexpr int N = NA > NB ? NA : NB;
+#pragma unroll
+    for (int s = N - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i <= s; ++i)
+            if (i < NA && s - i < NB) c = mma16(a.p[i], b.p[s - i], c);
+    return c;
+}
+
+template <int NP>
+__device__ __forceinline__ Half<NP> split(f32x4 v) {
+    Half<NP> h;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h.p[p][i] = (__bf16)v[i];
+        if (p + 1 < NP) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] -= (float)h.p[p][i];
+        }
+    }
+    return h;
+}
+template <int NP>
+__device__ __forceinline__ Frag<NP> join(const Half<NP>& a, const Half<NP>& b) {
+    Frag<NP> f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) f.p[p] = __builtin_shufflevector(a.p[p], b.p[p], 0, 1, 2, 3, 4, 5, 6, 7);
+    return f;
+}
+template <int NP>
+__device__ __forceinline__ f32x4 sum_of(const Half<NP>& h) {
+    f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = (float)h.p[NP - 1][i];
+#pragma unroll
+        for (int p = NP - 2; p >= 0; --p) v[i] += (float)h.p[p][i];
+    }
+    return v;
+}
+
+// The planes of 8 values of a tensor.
+template <typename T, int NP>
+__device__ __forceinline__ Frag<NP> planes_of(const T (&v)[8]) {
+    Frag<NP> f;
+    if constexpr (sizeof(T) == 2 && NP == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f.p[0][i] = v[i];
+    } else {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = to_f32(v[i]);
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                f.p[p][i] = (__bf16)r[i];
+                r[i] -= (float)f.p[p][i];
+            }
+        }
+    }
+    return f;
+}
+
+// The operand that turns a tile round: 1 where lane and value meet.  (Products by 1 and sums with 0: exact.)
+__device__ __forceinline__ bf16x4 unit_half(int lane) {
+    bf16x4 u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = (__bf16)(4 * (lane >> 4) + j == (lane & 15) ? 1.f : 0.f);
+    return u;
+}
+// A tile's plane, lane = column and values = rows, with lane = row and values = columns.
+__device__ __forceinline__ bf16x4 turned(bf16x4 t, bf16x4 unit) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    const f32x4 r = mma16(t, unit, zero);
+    bf16x4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = (__bf16)r[j];
+    return o;
+}
+
+// LDS rows of R values of planes: value i of row r of plane p at [p][r][i].
+template <int NP, int ROWS, int R>
+struct Rows {
+    static constexpr int kStride = R + kDeltaPad, kPlane = ROWS * kStride, kValues = NP * kPlane;
+    // 8 consecutive values of a lane's row: the inner axis in its own order (32 n + 8 g ..)
+    static __device__ __forceinline__ Frag<NP> natural(const bf16_t* base, int row, int at, int lane) {
+        Frag<NP> f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+            f.p[p] = *reinterpret_cast<const bf16x8*>(base + p * kPlane + (row + (lane & 15)) * kStride + at + 8 * (lane >> 4));
+        return f;
+    }
+    // in tile order
+    static __device__ __forceinline__ Half<NP> half(const bf16_t* base, int row, int at, int lane) {
+        Half<NP> f;
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+            f.p[p] = *reinterpret_cast<const bf16x4*>(base + p * kPlane + (row + (lane & 15)) * kStride + at + 4 * (lane >> 4));
+        return f;
+    }
+    static __device__ __forceinline__ Frag<NP> tiles(const bf16_t* base, int row, int at, int lane) {
+        return join(half(base, row, at, lane), half(base, row, at + 16, lane));
+    }
+    // lane = column `at` + l % 16, values = rows row + 4 g ..: every group of 16 lanes reads four rows of 16 values, transposed on the way
+    static __device__ __forceinline__ Half<NP> down(const bf16_t* base, int row, int at, int lane) {
+        typedef __attribute__((address_space(3))) s16x4 lds_t;
+        Half<NP> f;
+        const int i = lane & 15;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            const bf16_t* q = base + p * kPlane + (row + 4 * (lane >> 4) + (i >> 2)) * kStride + at + 4 * (i & 3);
+            f.p[p] = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(__attribute__((address_space(3))) void*)q));
+        }
+        return f;
+    }
+};
+
+// Where a chain stands in its tensors.
+struct DeltaChain {
+    int o, w, hv, hk;
+    long long len;   // valid steps
+    __device__ __forceinline__ DeltaChain(const DeltaArgs& p, int chain) {
+        hv = chain % p.Hv;
+        const int ow = chain / p.Hv;
+        w = ow % p.W, o = ow / p.W;
+        hk = hv / (p.Hv / p.Hk);
+        len = p.T;
+        if (p.lengths) {
+            const int n = p.lengths[o];
+            len = n < 0 ? 0 : n < p.T ? n : p.T;
+        }
+    }
+    // The step at place i of the chain: from the end of what is valid with `reverse`, and places behind it for themselves.
+    __device__ __forceinline__ long long step(const DeltaArgs& p, long long i) const { return p.reverse && i < len ? len - 1 - i : i; }
+    __device__ __forceinline__ long long at(const DeltaStrides& s, int head) const { return o * s.o + w * s.w + head * s.h; }
+};
+
+// A chunk of a tensor's rows as planes in LDS: 0 behind the chain's end, behind the row's end d, and up to R values.
+template <typename T, int NP, int R>
+__device__ __forceinline__ void stage_rows(bf16_t* to, const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first,
+                                           int col, int d, bool vec) {
+    typedef Rows<NP, kDeltaChunk, R> L;
+    for (int e = threadIdx.x; e < kDeltaChunk * (R / 8); e += blockDim.x) {
+        const int row = e / (R / 8), at = e % (R / 8) * 8;
+        const long long i = first + row;
+        T v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(0.f);
+        if (i < c.len && col + at < d) {
+            const T* q = base + c.step(p, i) * st + col + at;
+            if (vec) {
+                constexpr int VEC = 16 / sizeof(T);
+#pragma unroll
+                for (int m = 0; m < 8 / VEC; ++m) {
+                    const ChanVec<T, VEC> r = *reinterpret_cast<const ChanVec<T, VEC>*>(q + m * VEC);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[m * VEC + j] = r.v[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (col + at + j < d) v[j] = q[j];
+            }
+        }
+        const Frag<NP> f = planes_of<T, NP>(v);
+#pragma unroll
+        for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(to + n * L::kPlane + row * L::kStride + at) = f.p[n];
+    }
+}
+
+// Planes [plane][row][ld] in memory (states, U) to LDS: columns [col, col + R), those of them that there are.
+template <int NP, int ROWS, int R>
+__device__ __forceinline__ void stage_planes(bf16_t* to, const bf16_t* from, int ld, int col) {
+    typedef Rows<NP, ROWS, R> L;
+    for (int e = threadIdx.x; e < NP * ROWS * (R / 8); e += blockDim.x) {
+        const int at = e % (R / 8) * 8, row = e / (R / 8) % ROWS, n = e / (R / 8) / ROWS;
+        if (col + at < ld)
+            *reinterpret_cast<bf16x8*>(to + n * L::kPlane + row * L::kStride + at) =
+                *reinterpret_cast<const bf16x8*>(from + (long long)(n * ROWS + row) * ld + col + at);
+    }
+}
+
+// The gates of a chunk.  c_i, the sum of the log decays up to step i, is summed in 64 bits and kept as two floats, so that differences of
+// far sums lose nothing; log decays below -10000 count as that: e^-10000 is 0 in 32 bits, and differences behind it stay exact where a
+// mask's lowest value, summed, had swallowed them.
+struct DeltaGates {
+    float hi[kDeltaChunk], lo[kDeltaChunk], beta[kDeltaChunk], D[kDeltaChunk], E[kDeltaChunk];   // D = e^c, E = e^(c_end - c)
+    float slope[kDeltaChunk], bslope[kDeltaChunk];   // of the log decay by g, of beta by b
+};
+
+__device__ __forceinline__ float gate_value(const void* base, long long at, int f32, int type) {
+    if (f32 || type == kF32) return ((const float*)base)[at];
+    return type == kF16 ? to_f32(((const f16_t*)base)[at]) : to_f32(((const bf16_t*)base)[at]);
+}
+
+// -> log decay and its slope
+__device__ __forceinline__ void log_decay(float g, int logits, float& la, float& slope) {
+    la = g, slope = 1.f;
+    if (logits) {
+        const float e = expf(-fabsf(g));
+        la = (g < 0.f ? g : 0.f) - log1pf(e);
+        slope = (g < 0.f ? 1.f : e) / (1.f + e);   // sigmoid(-g)
+        if (g != g) la = slope = g;
+    }
+    if (la < -1e4f) la = -1e4f;
+}
+__device__ __forceinline__ void write_strength(float b, int logits, float& beta, float& slope) {
+    beta = b, slope = 1.f;
+    if (logits) {
+        const float e = expf(-fabsf(b)), r = 1.f / (1.f + e);
+        beta = (b < 0.f ? e : 1.f) * r;
+        slope = e * r * r;
+        if (b != b) beta = slope = b;
+    }
+}
+
+// By the first wavefront; the caller's barrier follows.
+__device__ __forceinline__ void chunk_gates(DeltaGates& s, const DeltaArgs& p, const DeltaChain& c, long long first, int type) {
+    if (threadIdx.x >= 64) return;
+    const int lane = threadIdx.x;
+    const long long i = first + lane;
+    float la = 0.f, slope = 0.f, beta = 0.f, bslope = 0.f;
+    if (i < c.len) {
+        const long long t = c.step(p, i);
+        log_decay(gate_value(p.g, c.at(p.gs, c.hv) + t * p.gs.t, p.gates_f32, type), p.logits, la, slope);
+        write_strength(gate_value(p.b, c.at(p.bs, c.hv) + t * p.bs.t, p.gates_f32, type), p.logits, beta, bslope);
+    }
+    double sum = la;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const double other = __shfl_up(sum, d);
+        if (lane >= d) sum += other;
+    }
+    const double end = __shfl(sum, 63);
+    s.hi[lane] = (float)sum;
+    s.lo[lane] = (float)(sum - (double)s.hi[lane]);
+    s.beta[lane] = beta, s.slope[lane] = slope, s.bslope[lane] = bslope;
+    s.D[lane] = expf((float)sum), s.E[lane] = expf((float)(end - sum));
+}
+
+__device__ __forceinline__ float decay_between(const DeltaGates& s, int i, int j) {   // e^(c_i - c_j), i >= j
+    return expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
+}
+
+// (I + A)^-1 of a chunk, A strictly lower, as blocks of 16 x 16 for a substitution by blocks: -A_ba below the diagonal, the inverses of the
+// diagonal's blocks on it.  Block (b, a) is number b (b + 1) / 2 + a.  FORE: lane = row, values = columns, an operand for products with
+// solutions by their rows; else lane = column, values = rows: the same for the transposed system.
+template <int NP>
+struct Blocks {
+    static constexpr int kValues = 10 * NP * 64 * 4;
+    static __device__ __forceinline__ int at(int b, int a) { return b * (b + 1) / 2 + a; }
+    static __device__ __forceinline__ void put(bf16_t* base, int block, const Half<NP>& h, int lane) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x4*>(base + ((block * NP + p) * 64 + lane) * 4) = h.p[p];
+    }
+    static __device__ __forceinline__ Half<NP> get(const bf16_t* base, int block, int lane) {
+        Half<NP> h;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) h.p[p] = *reinterpret_cast<const bf16x4*>(base + ((block * NP + p) * 64 + lane) * 4);
+        return h;
+    }
+};
+
+// The inverse of a block I + A, its A in `tile` [16][20] of LDS: FORE [column][row], else [row][column].  Lane l % 16 has a row (FORE) or a
+// column of it; -> values 4 g .. 4 g + 3 of that.  Row i of T = (I + A)^-1 from T (I + A) = I: t_j = [i = j] - sum over m > j of t_m A_mj.
+template <bool FORE>
+__device__ __forceinline__ f32x4 invert_block(const float* tile, int lane) {
+    const int me = lane & 15;
+    float t[16];
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        const int j = FORE ? 15 - n : n;
+        float s = j == me ? 1.f : 0.f;
+        float a[16];
+#pragma unroll
+        for (int m = 0; m < 16; m += 4) {
+            const f32x4 r = *reinterpret_cast<const f32x4*>(tile + j * 20 + m);
+            a[m] = r[0], a[m + 1] = r[1], a[m + 2] = r[2], a[m + 3] = r[3];
+        }
+#pragma unroll
+        for (int m = 0; m < 16; ++m)
+            if (FORE ? m > j : m < j) s = __builtin_fmaf(-t[m], a[m], s);
+        t[j] = s;
+    }
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int g = lane >> 4;
+        v[r] = g == 0 ? t[r] : g == 1 ? t[4 + r] : g == 2 ? t[8 + r] : t[12 + r];
+    }
+    return v;
+}
+
+// Solutions X of (I + A) X = R by blocks of rows, in place: lane = column, values = rows.
+template <int NP>
+__device__ __forceinline__ void solve_fore(const bf16_t* blocks, f32x4 (&x)[4], int lane) {
+    Half<NP> s[4];
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        f32x4 r = x[b];
+#pragma unroll
+        for (int a = 0; a < b; ++a) r = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s[a], r);
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        x[b] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, b), lane), split<NP>(r), zero);
+        s[b] = split<NP>(x[b]);
+    }
+}
+// of (I + A)^T X = R, from the last block.
+template <int NP>
+__device__ __forceinline__ void solve_back(const bf16_t* blocks, f32x4 (&x)[4], int lane) {
+    Half<NP> s[4];
+#pragma unroll
+    for (int a = 3; a >= 0; --a) {
+        f32x4 r = x[a];
+#pragma unroll
+        for (int b = 3; b > a; --b) r = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s[b], r);
+        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+        x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(a, a), lane), split<NP>(r), zero);
+        s[a] = split<NP>(x[a]);
+    }
+}
+
+// Fragments in memory: [fragment][plane][lane][8].
+template <int NP>
+__device__ __forceinline__ void store_frag(bf16_t* base, int fragment, const Frag<NP>& f, int lane) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(base + ((long long)(fragment * NP + p) * 64 + lane) * 8) = f.p[p];
+}
+template <int NP>
+__device__ __forceinline__ Frag<NP> load_frag(const bf16_t* base, int fragment, int lane) {
+    Frag<NP> f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(base + ((long long)(fragment * NP + p) * 64 + lane) * 8);
+    return f;
+}
+// one of the two tiles of a fragment
+template <int NP>
+__device__ __forceinline__ void store_half(bf16_t* base, int fragment, int half, const Half<NP>& h, int lane) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+        *reinterpret_cast<bf16x4*>(base + ((long long)(fragment * NP + p) * 64 + lane) * 8 + 4 * half) = h.p[p];
+}
+
+// Four neighbouring values of a row of d to memory.
+template <typename T>
+__device__ __forceinline__ void store_four(T* row, int at, int d, f32x4 v, bool vec) {
+    if (vec) {
+        if (at < d) {
+            const float f[4] = {v[0], v[1], v[2], v[3]};
+            store_f32<T, 4>(row + at, f);
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (at + r < d) row[at + r] = from_f32<T>(v[r]);
+    }
+}
+
+// The sum over the four lane groups, in all of them.
+__device__ __forceinline__ float group_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// Sizes of what lies between the kernels, in elements of a chunk.
+struct DeltaSizes {
+    long long rows, frag_made, frag_raw, state, u, cols;
+    __host__ __device__ DeltaSizes(int DK, int dvp, int raw, int made)
+        : rows(kDeltaChunk * (long long)DK), frag_made(rows * made), frag_raw(rows * raw), state((long long)DK * dvp * made),
+          u((long long)kDeltaChunk * dvp * made), cols((long long)kDeltaChunk * dvp) {}
+};
+
+}  // namespace pdw

@@ -1,0 +1,307 @@
+// The gated delta rule, forward.  For every chain (a batch element's value head) with a state S of dk x dv:
+//
+//   u_t = beta_t (v_t - a_t S_(t-1)^T k_t),   S_t = a_t S_(t-1) + k_t u_t^T,   y_t = scale S_t^T q_t
+//
+// in chunks of 64 steps.  With c the sums of log a from the chunk's start, D = e^c, E = e^(c_end - c), G_ij = e^(c_i - c_j) and S0 the state
+// before the chunk, its rows u solve a triangular system:
+//
+//   (I + A) U = beta (V - D K S0),   A_ij = beta_i G_ij k_i.k_j for j < i          U = Ub - W S0,  (I + A) [W Ub] = [beta D K   beta V]
+//   S1 = e^c_end S0 + K^T E U                                                      Y = scale (D Q S0 + (G o Q K^T) U),  j <= i
+//
+// Three launches.  delta_prepare_k, a workgroup a chunk: A, then W and Ub by substitution (16 x 16 blocks: the diagonal's are inverted row by row
+// in fp32, the rest is products; powers of A, the other way to its inverse, cancel where keys repeat).  delta_chain_k, the only part with an
+// order: a wavefront carries 16 columns of a chain's state in registers through its chunks, two products a chunk, whose operands come ready made
+// from memory; results of the first are operands of the second without an exchange.  It leaves the states before the chunks and U.
+// delta_out_k, a workgroup a chunk again: Y.
+#pragma once
+#include "delta_common.h"
+
+namespace pdw {
+
+// A's blocks of the wavefront's row of blocks (FORE) or column of blocks, into LDS; the caller's barrier follows, then invert_blocks.
+// tile: this wavefront's [16][20].
+template <int RAW, int MADE, int DK, bool FORE>
+__device__ __forceinline__ void make_blocks(bf16_t* blocks, float* tile, const bf16_t* k, const DeltaGates& s, int wave, int lane) {
+    typedef Rows<RAW, kDeltaChunk, DK> L;
+    const int col = lane & 15, g4 = 4 * (lane >> 4);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (FORE ? t > wave : t < wave) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < DK; n += 32) acc = mma(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
+        // FORE: lane = row i of the wavefront's block row, values = columns j of block t; else lane = column j, values = rows i
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int mine = 16 * wave + col, other = 16 * t + g4 + r;
+            const int i = FORE ? mine : other, j = FORE ? other : mine;
+            acc[r] = j < i ? s.beta[i] * decay_between(s, i, j) * acc[r] : 0.f;
+        }
+        if (t == wave) {
+            // [column][row] (FORE), [row][column]: the lane's index is the inner one
+#pragma unroll
+            for (int r = 0; r < 4; ++r) tile[(g4 + r) * 20 + col] = acc[r];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = -acc[r];
+            Blocks<MADE>::put(blocks, FORE ? Blocks<MADE>::at(wave, t) : Blocks<MADE>::at(t, wave), split<MADE>(acc), lane);
+        }
+    }
+}
+
+template <int RAW, int DK>
+constexpr int delta_rows_bytes() {
+    return Rows<RAW, kDeltaChunk, DK>::kValues * 2;
+}
+template <typename T, int DK>
+constexpr int delta_prepare_lds() {
+    typedef DeltaPlanes<T> P;
+    return delta_rows_bytes<P::kRaw, DK>() + Blocks<P::kMade>::kValues * 2 + 4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
+    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
+    constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
+    typedef Rows<RAW, kDeltaChunk, DK> L;
+    extern __shared__ __align__(16) unsigned char lds[];
+    bf16_t* k = (bf16_t*)lds;
+    bf16_t* blocks = k + L::kValues;
+    float* tiles = (float*)(blocks + Blocks<MADE>::kValues);
+    DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g4 = 4 * (lane >> 4);
+    const long long id = p.first + blockIdx.x;
+    const int chain = (int)(id / p.NC);
+    const long long first = (id - chain * p.NC) * kDeltaChunk;
+    const DeltaChain c(p, chain);
+
+    chunk_gates(s, p, c, first, type);
+    stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+    __syncthreads();
+    float* tile = tiles + wave * 16 * 20;
+    make_blocks<RAW, MADE, DK, true>(blocks, tile, k, s, wave, lane);
+    // (the tile is this wavefront's own: its LDS operations are in order)
+    Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, wave), split<MADE>(invert_block<true>(tile, lane)), lane);
+    __syncthreads();
+
+    if (threadIdx.x < 64) {
+        float* dec = p.dec + id * 2 * kDeltaChunk;
+        dec[lane] = s.D[lane], dec[64 + lane] = s.E[lane];
+    }
+    const DeltaSizes z(DK, p.dvp, RAW, MADE);
+    const bf16x4 unit = unit_half(lane);
+    const int colv = p.dvp / 16;
+    for (int ct = wave; ct < DK / 16 + colv; ct += 4) {
+        f32x4 x[4];
+        if (ct < DK / 16) {
+            Half<RAW> kr[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                kr[b] = L::down(k, 16 * b, 16 * ct, lane);
+                x[b] = sum_of(kr[b]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) x[b][r] *= s.beta[16 * b + g4 + r] * s.D[16 * b + g4 + r];
+            }
+            store_frag(p.kt + id * z.frag_raw, 2 * ct, join(kr[0], kr[1]), lane);
+            store_frag(p.kt + id * z.frag_raw, 2 * ct + 1, join(kr[2], kr[3]), lane);
+            solve_fore<MADE>(blocks, x, lane);
+            // -W, lane = step: the first operand of the chain's first product
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                Half<MADE> h = split<MADE>(-x[b]);
+#pragma unroll
+                for (int n = 0; n < MADE; ++n) h.p[n] = turned(h.p[n], unit);
+                store_half(p.wp + id * z.frag_made, b * (DK / 32) + ct / 2, ct & 1, h, lane);
+            }
+        } else {
+            const int cv = ct - DK / 16, at = 16 * cv + col;
+            const T* v = (const T*)p.v + c.at(p.vs, c.hv) + at;
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int row = 16 * b + g4 + r;
+                    const long long i = first + row;
+                    x[b][r] = i < c.len && at < p.dv ? s.beta[row] * to_f32(v[c.step(p, i) * p.vs.t]) : 0.f;
+                }
+            solve_fore<MADE>(blocks, x, lane);
+            float* ub = p.ub + id * z.cols + cv * 1024;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) *reinterpret_cast<f32x4*>(ub + (b * 64 + lane) * 4) = x[b];
+        }
+    }
+}
+
+// A state's 16 columns: X[d] has rows 16 d + 4 g + r, lane = column.  From and to the user's [dk][dv].
+template <int DK>
+__device__ __forceinline__ void load_state(f32x4 (&x)[DK / 16], const float* s, int dk, int dv, int at, int lane) {
+#pragma unroll
+    for (int d = 0; d < DK / 16; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * d + 4 * (lane >> 4) + r;
+            x[d][r] = s && row < dk && at < dv ? s[row * (long long)dv + at] : 0.f;
+        }
+}
+template <int DK>
+__device__ __forceinline__ void store_state(float* s, const f32x4 (&x)[DK / 16], int dk, int dv, int at, int lane) {
+    if (!s) return;
+#pragma unroll
+    for (int d = 0; d < DK / 16; ++d)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * d + 4 * (lane >> 4) + r;
+            if (row < dk && at < dv) s[row * (long long)dv + at] = x[d][r];
+        }
+}
+// Planes of a tile (lane = column, values = rows) to [plane][row][ld]: turned, so that a lane has four neighbours of a row.
+template <int NP>
+__device__ __forceinline__ void store_turned(bf16_t* to, long long plane, int ld, int row, int at, const Half<NP>& h, bf16x4 unit, int lane) {
+#pragma unroll
+    for (int n = 0; n < NP; ++n)
+        *reinterpret_cast<bf16x4*>(to + n * plane + (long long)(row + (lane & 15)) * ld + at + 4 * (lane >> 4)) = turned(h.p[n], unit);
+}
+
+// Workgroup -> chain and columns: the parts of a chain, which read the same operands, on one die (workgroups go to the dies in turn).
+__device__ __forceinline__ bool chain_part(const DeltaArgs& p, int parts, int& chain, int& part) {
+    const long long id = p.first + blockIdx.x, turn = id >> 3;
+    part = (int)(turn % parts);
+    const long long n = (turn / parts) * 8 + (id & 7);
+    chain = (int)n;
+    return n < p.chains;
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_chain_k(DeltaArgs p) {
+    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
+    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g4 = 4 * (lane >> 4), colv = p.dvp / 16;
+    int chain, part;
+    if (!chain_part(p, (colv + waves - 1) / waves, chain, part)) return;
+    const int cv = part * waves + wave;
+    if (cv >= colv) return;
+    const DeltaSizes z(DK, p.dvp, RAW, MADE);
+    const bf16x4 unit = unit_half(lane);
+    const int at = 16 * cv + (lane & 15);
+    const long long state = (long long)chain * p.dk * p.dv;
+    f32x4 x[DK / 16];
+    load_state<DK>(x, p.h0 ? p.h0 + state : nullptr, p.dk, p.dv, at, lane);
+    for (long long m = 0; m < p.NC; ++m) {
+        const long long id = chain * p.NC + m;
+        const bf16_t *wp = p.wp + id * z.frag_made, *kt = p.kt + id * z.frag_raw;
+        const float *ub = p.ub + id * z.cols + cv * 1024, *dec = p.dec + id * 2 * kDeltaChunk;
+        bf16_t *s0 = p.s0 + id * z.state, *u = p.u + id * z.u;
+        Frag<MADE> xs[DK / 32];
+#pragma unroll
+        for (int d = 0; d < DK / 32; ++d) {
+            const Half<MADE> a = split<MADE>(x[2 * d]), b = split<MADE>(x[2 * d + 1]);
+            store_turned(s0, (long long)DK * p.dvp, p.dvp, 32 * d, 16 * cv, a, unit, lane);
+            store_turned(s0, (long long)DK * p.dvp, p.dvp, 32 * d + 16, 16 * cv, b, unit, lane);
+            xs[d] = join(a, b);
+        }
+        f32x4 y[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            y[b] = *reinterpret_cast<const f32x4*>(ub + (b * 64 + lane) * 4);
+#pragma unroll
+            for (int d = 0; d < DK / 32; ++d) y[b] = mma(load_frag<MADE>(wp, b * (DK / 32) + d, lane), xs[d], y[b]);
+        }
+        Half<MADE> e[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            store_turned(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * b, 16 * cv, split<MADE>(y[b]), unit, lane);
+            const f32x4 E = *reinterpret_cast<const f32x4*>(dec + 64 + 16 * b + g4);
+            e[b] = split<MADE>(y[b] * E);
+        }
+        const Frag<MADE> e0 = join(e[0], e[1]), e1 = join(e[2], e[3]);
+        const float end = dec[63];
+#pragma unroll
+        for (int d = 0; d < DK / 16; ++d) {
+            f32x4 n = x[d] * end;
+            n = mma(load_frag<RAW>(kt, 2 * d, lane), e0, n);
+            x[d] = mma(load_frag<RAW>(kt, 2 * d + 1, lane), e1, n);
+        }
+    }
+    store_state<DK>(p.last ? p.last + state : nullptr, x, p.dk, p.dv, at, lane);
+}
+
+constexpr int kDeltaCols = 64;   // columns of v that a workgroup of delta_out_k and delta_grads_k has in LDS
+
+template <typename T, int DK>
+constexpr int delta_out_lds() {
+    typedef DeltaPlanes<T> P;
+    const int in = 2 * delta_rows_bytes<P::kRaw, DK>();
+    const int made = (Rows<P::kMade, DK, kDeltaCols>::kValues + Rows<P::kMade, kDeltaChunk, kDeltaCols>::kValues) * 2;
+    return (in > made ? in : made) + (int)sizeof(DeltaGates);
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
+    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
+    constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
+    typedef Rows<RAW, kDeltaChunk, DK> L;
+    typedef Rows<MADE, DK, kDeltaCols> LS;
+    typedef Rows<MADE, kDeltaChunk, kDeltaCols> LU;
+    extern __shared__ __align__(16) unsigned char lds[];
+    DeltaGates& s = *(DeltaGates*)lds;
+    bf16_t *k = (bf16_t*)(lds + sizeof(DeltaGates)), *q = k + L::kValues;
+    bf16_t *s0 = k, *u = s0 + LS::kValues;   // (behind the products with K and Q)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g4 = 4 * (lane >> 4);
+    const long long id = p.first + blockIdx.x;
+    const int chain = (int)(id / p.NC);
+    const long long first = (id - chain * p.NC) * kDeltaChunk;
+    const DeltaChain c(p, chain);
+
+    chunk_gates(s, p, c, first, type);
+    stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+    stage_rows<T, RAW, DK>(q, (const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+    __syncthreads();
+    // the wavefront's 16 steps i: scale G_ij q_i.k_j, lane = i, values = j; and its rows of Q
+    const int i = 16 * wave + col;
+    Half<MADE> pr[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (t > wave) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < DK; n += 32) acc = mma(L::natural(k, 16 * t, n, lane), L::natural(q, 16 * wave, n, lane), acc);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int j = 16 * t + g4 + r;
+            acc[r] = j <= i ? p.scale * decay_between(s, i, j) * acc[r] : 0.f;
+        }
+        pr[t] = split<MADE>(acc);
+    }
+    Frag<RAW> qf[DK / 32];
+#pragma unroll
+    for (int n = 0; n < DK / 32; ++n) qf[n] = L::tiles(q, 16 * wave, 32 * n, lane);
+    const float D = p.scale * s.D[i];
+    const long long step = first + i;
+    const bool there = step < c.len;
+    T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
+    const DeltaSizes z(DK, p.dvp, RAW, MADE);
+    for (int at = 0; at < p.dv; at += kDeltaCols) {
+        __syncthreads();
+        stage_planes<MADE, DK, kDeltaCols>(s0, p.s0 + id * z.state, p.dvp, at);
+        stage_planes<MADE, kDeltaChunk, kDeltaCols>(u, p.u + id * z.u, p.dvp, at);
+        __syncthreads();
+#pragma unroll
+        for (int cv = 0; cv < kDeltaCols; cv += 16) {
+            if (at + cv >= p.dvp) break;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int n = 0; n < DK / 32; ++n)
+                acc = mma(join(LS::down(s0, 32 * n, cv, lane), LS::down(s0, 32 * n + 16, cv, lane)), qf[n], acc);
+            acc *= D;
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+                if (t <= wave) acc = mma(LU::down(u, 16 * t, cv, lane), pr[t], acc);
+            if (!there) acc = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (step < p.T) store_four(row, at + cv + g4, p.dv, acc, p.vec & kVecY);
+        }
+    }
+}
+
+}  // namespace pdw

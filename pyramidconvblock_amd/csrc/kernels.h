@@ -215,4 +215,14 @@ int scan_run(const struct ScanArgs& p, bool backward, void* workspace, size_t wo
 int scan_step_launch(const void* x, const void* g, const float* state, float* new_state, void* y, long long B, int C, long long ldx,
                      long long ldg, int dtype, hipStream_t s);
 
+// rotary.hip: norms of heads with rotated positions (arguments: rotary.h)
+size_t rotary_workspace(int d);
+int rotary_run(const struct RotaryArgs& p, bool backward, void* gw, void* gkw, void* workspace, size_t workspace_bytes, int dtype, hipStream_t s);
+
+// delta.hip: the gated delta rule (arguments: delta_common.h); delta_step.hip: its form for single tokens
+size_t delta_states_bytes(long long chains, long long T, int dk, int dv, int dtype);
+size_t delta_workspace(long long chains, long long T, int dk, int dv, bool backward, bool states, int dtype);
+int delta_run(const struct DeltaArgs& p, void* states, bool backward, void* workspace, size_t workspace_bytes, int dtype, hipStream_t s);
+int delta_steps_run(const struct DeltaArgs& p, int dtype, hipStream_t s);
+
 }  // namespace pdw

@@ -6,6 +6,7 @@
 #include "torch_node.h"
 
 PyMethodDef* pdw_mixer_methods();   // torch_mixer.cpp
+PyMethodDef* pdw_delta_methods();   // torch_delta.cpp
 
 namespace {
 
@@ -313,7 +314,7 @@ PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_pdw_torch", nullptr, -1, kMethod
 
 PyMODINIT_FUNC PyInit__pdw_torch(void) {
     PyObject* m = PyModule_Create(&kModule);
-    if (m && PyModule_AddFunctions(m, pdw_mixer_methods()) < 0) {
+    if (m && (PyModule_AddFunctions(m, pdw_mixer_methods()) < 0 || PyModule_AddFunctions(m, pdw_delta_methods()) < 0)) {
         Py_DECREF(m);
         return nullptr;
     }

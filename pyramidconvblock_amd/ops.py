@@ -581,3 +581,107 @@ def scan_backward(gy, glast, x, g, lengths, states, dim, reverse):
                 gx.data_ptr(), gg.data_ptr(), gstate.data_ptr(), ws.data_ptr(), ws.numel(), O, T, W, I, s, s, s, s,
                 int(bool(reverse)), _lib.dtype_code(x.dtype))
     return gx, gg, gstate
+
+
+# Head norms with rotated positions, and the gated delta rule (head_rotary and gated_delta check their arguments; these take dense tensors and
+# make the call).
+
+HEAD_KINDS = {"none": 0, "rms": 1, "l2": 2}
+POSITION_TYPES = {torch.int32: 1, torch.int64: 2, torch.float32: 3}
+
+
+def _rotary_call(x, weights, positions, frequencies, axes, sections, base, kind, neighbours, eps, sizes):
+    """x: (q, k or None), sizes: theirs (in a backward without a norm there is no x)."""
+    import ctypes
+
+    c = _lib.Rotary()
+    lead, d = sizes[0][:-2], sizes[0][-1]
+    c.tokens = 1
+    for n in lead:
+        c.tokens *= n
+    for s in range(2):
+        if sizes[s] is None:
+            continue
+        c.x[s], c.weight[s], c.heads[s] = _ptr(x[s]), _ptr(weights[s]), sizes[s][-2]
+        c.xt[s], c.xh[s] = sizes[s][-2] * d, d
+    if positions is not None:
+        c.position_type, c.positions, c.positions_rows = POSITION_TYPES[positions.dtype], positions.data_ptr(), positions.numel() // axes
+    else:
+        c.grid[:axes] = lead[len(lead) - axes:]
+    c.frequencies = _ptr(frequencies)
+    c.sections[:axes] = sections
+    c.d, c.axes, c.kind, c.neighbours, c.eps, c.base = d, axes, kind, int(bool(neighbours)), float(eps), float(base)
+    return c, ctypes.addressof(c), ctypes.c_void_p * 2
+
+
+def rotary_forward(q, k, weights, *more):
+    """more: positions, frequencies, axes, sections, base, kind, neighbours, eps -> (y of q, of k or None)"""
+    from ctypes import addressof
+
+    dev = _lib.require_device(q)
+    x = (q, k)
+    c, call, two = _rotary_call(x, weights, *more, [None if t is None else tuple(t.shape) for t in x])
+    c.dtype = _lib.dtype_code(q.dtype)
+    y = [None if t is None else torch.empty_like(t) for t in x]
+    to = two(*(_ptr(t) for t in y))
+    _launch("pdw_rotary_fwd", dev, call, addressof(to))
+    return y
+
+
+def rotary_backward(grads, x, weights, sizes, *more):
+    """-> gradients of q, k and their weights, None for what there was none of."""
+    from ctypes import addressof
+
+    dev = _lib.require_device(grads[0])
+    # (without a norm the input itself is not read)
+    c, call, two = _rotary_call([g if t is None else t for g, t in zip(grads, x)], weights, *more, sizes)
+    c.dtype = _lib.dtype_code(grads[0].dtype)
+    gx = [None if g is None else torch.empty_like(g) for g in grads]
+    gw = [None if w is None else torch.zeros_like(w) for w in weights]
+    ws = _bytes(_lib.lib().pdw_rotary_bwd_workspace_bytes(c.d), dev)
+    arrays = [two(*(_ptr(t) for t in ts)) for ts in (grads, gx, gw)]
+    _launch("pdw_rotary_bwd", dev, call, *(addressof(a) for a in arrays), ws.data_ptr(), ws.numel())
+    return (*gx, *gw)
+
+
+def _delta_call(q, k, v, g, b, state, lengths, dim, reverse, scale, logits):
+    import ctypes
+
+    c = _lib.Delta()
+    O = T = W = 1
+    for d, n in enumerate(q.shape[:-2]):
+        O, T, W = (O * n, T, W) if d < dim else (O, n, W) if d == dim else (O, T, W * n)
+    for name, t, tail in (("q", q, 2), ("k", k, 2), ("v", v, 2), ("g", g, 1), ("b", b, 1)):
+        H, d = t.shape[-tail], t.shape[-1] if tail == 2 else 1
+        setattr(c, name, t.data_ptr())
+        getattr(c, name + "s")[:] = (T * W * H * d, W * H * d, H * d, d)
+    c.h0, c.lengths, c.T, c.O, c.W = _ptr(state), _ptr(lengths), T, O, W
+    c.Hk, c.Hv, c.dk, c.dv = q.shape[-2], v.shape[-2], q.shape[-1], v.shape[-1]
+    c.reverse, c.logits, c.gates_f32 = int(bool(reverse)), int(bool(logits)), int(g.dtype == torch.float32)
+    c.dtype, c.scale = _lib.dtype_code(q.dtype), float(scale)
+    return c, ctypes.addressof(c)
+
+
+def delta_forward(q, k, v, g, b, state, lengths, dim, reverse, scale, logits, states=False):
+    """-> (y, last state fp32, what the backward needs or None)."""
+    dev = _lib.require_device(q)
+    c, call = _delta_call(q, k, v, g, b, state, lengths, dim, reverse, scale, logits)
+    y = torch.empty_like(v)
+    last = torch.empty(q.shape[:dim] + q.shape[dim + 1:-2] + (c.Hv, c.dk, c.dv), device=dev, dtype=torch.float32)
+    L = _lib.lib()
+    st = _bytes(L.pdw_delta_states_bytes(call), dev) if states else None
+    ws = _bytes(L.pdw_delta_workspace_bytes(call, 0, int(states)), dev)
+    _launch("pdw_delta_fwd", dev, call, y.data_ptr(), last.data_ptr(), _ptr(st), ws.data_ptr(), ws.numel())
+    return y, last, st
+
+
+def delta_backward(gy, glast, q, k, v, g, b, lengths, states, dim, reverse, scale, logits):
+    """-> gradients of (q, k, v, g, b, the initial state)."""
+    dev = _lib.require_device(gy)
+    c, call = _delta_call(q, k, v, g, b, None, lengths, dim, reverse, scale, logits)
+    grads = [torch.empty_like(t) for t in (q, k, v, g, b)]
+    gstate = torch.empty(q.shape[:dim] + q.shape[dim + 1:-2] + (c.Hv, c.dk, c.dv), device=dev, dtype=torch.float32)
+    ws = _bytes(_lib.lib().pdw_delta_workspace_bytes(call, 1, 1), dev)
+    _launch("pdw_delta_bwd", dev, call, gy.data_ptr(), _ptr(glast), states.data_ptr(), *(t.data_ptr() for t in grads), gstate.data_ptr(),
+            ws.data_ptr(), ws.numel())
+    return (*grads, gstate)
