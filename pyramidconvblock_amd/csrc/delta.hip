@@ -12,10 +12,29 @@ static int padded_dk(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
 static int padded_dv(int dv) { return (dv + 31) / 32 * 32; }
 static long long delta_chunks(long long T) { return (T + kDeltaChunk - 1) / kDeltaChunk; }
 
-static DeltaSizes sizes_of(int dk, int dv, int dtype) {
-    const int raw = dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1;
-    return DeltaSizes(padded_dk(dk), padded_dv(dv), raw, raw < 2 ? 2 : raw);
+// Chunks of a segment.  A chain's way through n chunks in s segments takes about 2 n / s steps (once for the maps, once with the states) and s - 1 folds,
+// n steps with one; more segments than fill the chip's 512 places for workgroups gain nothing.
+static long long segment_chunks(long long chains, long long NC, int DK, int dvp) {
+    const long long parts = (dvp / 16 + 3) / 4, columns = chains * parts;
+    long long best = NC, cost = NC;
+    for (long long s = 2; s <= NC && s <= 64 && columns * (s - 1) < 512; ++s) {
+        const long long seg = (NC + s - 1) / s, c = 2 * seg + s + 4;
+        if (c < cost) cost = c, best = seg;
+    }
+    return best < 1 ? 1 : best;
 }
+
+// What a call's buffers and launches go by.
+struct DeltaPlan {
+    DeltaSizes z;
+    long long NC, seg;
+    int segments, dvp;
+    DeltaPlan(long long chains, long long T, int dk, int dv, bool backward, bool state_gradient, int dtype)
+        : z(padded_dk(dk), padded_dv(dv), dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1, dtype == kF32 ? 3 : 2,
+            dtype == kF32 || !backward || state_gradient ? kChainPlanes : 2),
+          NC(delta_chunks(T)), seg(segment_chunks(chains, NC, padded_dk(dk), padded_dv(dv))),
+          segments(NC ? (int)((NC + seg - 1) / seg) : 1), dvp(padded_dv(dv)) {}
+};
 
 // Steps up to which a call without gradients goes step by step.
 constexpr long long kDeltaFewSteps = 16;
@@ -23,37 +42,55 @@ bool delta_few_steps(long long T) { return T <= kDeltaFewSteps; }
 
 static size_t whole(size_t n) { return (n + 255) / 256 * 256; }
 
-size_t delta_states_bytes(long long chains, long long T, int dk, int dv, int dtype) {
-    const DeltaSizes z = sizes_of(dk, dv, dtype);
-    const size_t n = (size_t)(chains * delta_chunks(T));
-    return whole(n * z.state * 2) + whole(n * z.u * 2);
+static size_t states_bytes(long long chains, const DeltaPlan& d) {
+    const size_t n = (size_t)(chains * d.NC);
+    return whole(n * d.z.state * 2) + whole(n * d.z.u * 2) + n * sizeof(DeltaGates);
 }
 
-// The buffers of one call one after another: f(pointer, bytes) of each.
+size_t delta_states_bytes(long long chains, long long T, int dk, int dv, int dtype) {
+    return states_bytes(chains, DeltaPlan(chains, T, dk, dv, false, false, dtype));
+}
+
+// The buffers of one call one after another: f(bytes) -> the address of each.
 template <typename F>
-static void delta_buffers(DeltaArgs& p, const DeltaSizes& z, bool backward, F f) {
-    const size_t n = (size_t)(p.chains * p.NC);
+static void delta_buffers(DeltaArgs& p, const DeltaPlan& d, bool backward, F f) {
+    const size_t n = (size_t)(p.chains * d.NC), maps = (size_t)p.chains * (d.segments - 1);
     auto take = [&](auto*& ptr, size_t bytes) { ptr = (std::remove_reference_t<decltype(ptr)>)f(whole(bytes)); };
-    take(p.wp, n * z.frag_made * 2);
-    take(p.dec, n * 2 * kDeltaChunk * 4);
+    take(p.wp, n * d.z.frag_chain * 2);
+    take(p.maps, maps * d.z.map * 2);
+    take(p.shifts, maps * d.z.shift * 4);
     if (!backward) {
-        take(p.kt, n * z.frag_raw * 2);
-        take(p.ub, n * z.cols * 4);
+        take(p.kt, n * d.z.frag_raw * 2);
+        take(p.ub, n * d.z.cols * 4);
     } else {
-        take(p.ka, n * z.frag_raw * 2);
-        take(p.ds1, n * z.state * 2);
-        take(p.du, n * z.cols * 4);
-        take(p.c0, n * (size_t)padded_dk(p.dk) * p.dvp * 4);
+        take(p.ka, n * d.z.frag_raw * 2);
+        take(p.ds1, n * d.z.state * 2);
+        take(p.du, n * d.z.cols * 4);
+        take(p.c0, n * d.z.c0 * 4);
     }
 }
 
+static size_t workspace_bytes_of(long long chains, const DeltaPlan& d, bool backward, bool states) {
+    DeltaArgs p{};
+    p.chains = (int)chains;
+    size_t total = 0;
+    delta_buffers(p, d, backward, [&](size_t bytes) { return total += bytes, (char*)nullptr; });
+    return total + (backward || states ? 0 : states_bytes(chains, d));
+}
+
+// (the most that a backward takes: with the gradient of a state)
 size_t delta_workspace(long long chains, long long T, int dk, int dv, bool backward, bool states, int dtype) {
     if (!backward && !states && delta_few_steps(T)) return 0;
-    DeltaArgs p{};
-    p.chains = (int)chains, p.NC = delta_chunks(T), p.dk = dk, p.dvp = padded_dv(dv);
-    size_t total = 0;
-    delta_buffers(p, sizes_of(dk, dv, dtype), backward, [&](size_t bytes) { return total += bytes, (char*)nullptr; });
-    return total + (backward || states ? 0 : delta_states_bytes(chains, T, dk, dv, dtype));
+    return workspace_bytes_of(chains, DeltaPlan(chains, T, dk, dv, backward, true, dtype), backward, states);
+}
+
+__global__ __launch_bounds__(256) void delta_through_k(const float* from, float* to, long long n, long long first) {
+    const long long i = (first + blockIdx.x) * 256 + threadIdx.x;
+    if (i < n) to[i] = from ? from[i] : 0.f;
+}
+static int delta_states_through(const float* from, float* to, long long n, hipStream_t s) {
+    launch_parts((n + 255) / 256, 256, [&](long long first, unsigned m) { delta_through_k<<<m, 256, 0, s>>>(from, to, n, first); });
+    return check_launch("delta_through_k");
 }
 
 static bool pieces(const void* base, const DeltaStrides& s, int d, int es) {
@@ -63,17 +100,23 @@ static bool pieces(const void* base, const DeltaStrides& s, int d, int es) {
 
 int delta_run(const DeltaArgs& in, void* states, bool backward, void* workspace, size_t workspace_bytes, int dtype, hipStream_t s) {
     DeltaArgs p = in;
-    p.NC = delta_chunks(p.T), p.dvp = padded_dv(p.dv);
     if (!backward && !states && delta_few_steps(p.T)) return delta_steps_run(p, dtype, s);
-    const size_t need = delta_workspace(p.chains, p.T, p.dk, p.dv, backward, states != nullptr, dtype);
+    const DeltaPlan d(p.chains, p.T, p.dk, p.dv, backward, p.gh0 != nullptr, dtype);
+    p.NC = d.NC, p.dvp = d.dvp, p.seg = d.seg, p.segments = d.segments;
+    const size_t need = workspace_bytes_of(p.chains, d, backward, states != nullptr);
     if (need && (!workspace || workspace_bytes < need))
         return set_error("delta: workspace too small (%zu of %zu bytes)", workspace_bytes, need), 1;
-    const DeltaSizes z = sizes_of(p.dk, p.dv, dtype);
+    if (!p.NC) {   // no steps: the states go through as they are
+        const float* from = backward ? p.glast : p.h0;
+        float* to = backward ? p.gh0 : p.last;
+        return to ? delta_states_through(from, to, (long long)p.chains * p.dk * p.dv, s) : 0;
+    }
     char* at = (char*)workspace;
-    delta_buffers(p, z, backward, [&](size_t bytes) { return at += bytes, at - bytes; });
+    delta_buffers(p, d, backward, [&](size_t bytes) { return at += bytes, at - bytes; });
     if (!states) states = at;
     p.s0 = (bf16_t*)states;
-    p.u = (bf16_t*)((char*)states + whole((size_t)(p.chains * p.NC) * z.state * 2));
+    p.u = (bf16_t*)((char*)states + whole((size_t)(p.chains * p.NC) * d.z.state * 2));
+    p.gates = (DeltaGates*)((char*)p.u + whole((size_t)(p.chains * p.NC) * d.z.u * 2));
     const int es = dtype == kF32 ? 4 : 2;
     p.vec = (pieces(p.q, p.qs, p.dk, es) ? kVecQ : 0) | (pieces(p.k, p.ks, p.dk, es) ? kVecK : 0) | (pieces(p.v, p.vs, p.dv, es) ? kVecV : 0) |
             (pieces(p.gy, p.ys, p.dv, es) ? kVecGy : 0) | (pieces(p.y, p.ys, p.dv, es) ? kVecY : 0) |

@@ -35,27 +35,26 @@ template <int MADE, int DK>
 constexpr int delta_wt_values() {
     return DK / 16 * 2 * MADE * 64 * 8;
 }
-template <typename T, int DK>
+template <typename T, int DK, int MADE>
 constexpr int delta_back_prepare_k_values() {   // K, and later W^T in its place
-    typedef DeltaPlanes<T> P;
-    return Rows<P::kRaw, kDeltaChunk, DK>::kValues > delta_wt_values<P::kMade, DK>() ? Rows<P::kRaw, kDeltaChunk, DK>::kValues
-                                                                                    : delta_wt_values<P::kMade, DK>();
+    constexpr int RAW = DeltaPlanes<T>::kRaw;
+    return Rows<RAW, kDeltaChunk, DK>::kValues > delta_wt_values<MADE, DK>() ? Rows<RAW, kDeltaChunk, DK>::kValues : delta_wt_values<MADE, DK>();
 }
-template <typename T, int DK>
+template <typename T, int DK, int MADE>
 constexpr int delta_back_prepare_lds() {
-    typedef DeltaPlanes<T> P;
-    return delta_rows_bytes<P::kRaw, DK>() + delta_back_prepare_k_values<T, DK>() * 2 + 2 * Blocks<P::kMade>::kValues * 2 + 4 * 16 * 20 * 4 +
-           (int)sizeof(DeltaGates);
+    return delta_rows_bytes<DeltaPlanes<T>::kRaw, DK>() + delta_back_prepare_k_values<T, DK, MADE>() * 2 + 2 * Blocks<MADE>::kValues * 2 +
+           4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
 }
 
-template <typename T, int DK>
+// MADE: planes of what the chain's operands are made of: kChainPlanes where the gradient of a state is wanted.
+template <typename T, int DK, int MADE>
 __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
-    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
+    constexpr int RAW = DeltaPlanes<T>::kRaw;
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *wl = k;
-    bf16_t *blocks = k + delta_back_prepare_k_values<T, DK>(), *pb = blocks + Blocks<MADE>::kValues;
+    bf16_t *blocks = k + delta_back_prepare_k_values<T, DK, MADE>(), *pb = blocks + Blocks<MADE>::kValues;
     float* tiles = (float*)(pb + Blocks<MADE>::kValues);
     DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -64,9 +63,9 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
     const int chain = (int)(id / p.NC);
     const long long first = (id - chain * p.NC) * kDeltaChunk;
     const DeltaChain c(p, chain);
-    const DeltaSizes z(DK, p.dvp, RAW, MADE);
+    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
 
-    chunk_gates(s, p, c, first, type);
+    load_gates(s, p.gates + id);
     stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
     stage_rows<T, RAW, DK>(q, (const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
     __syncthreads();
@@ -91,10 +90,6 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
 #pragma unroll
     for (int n = 0; n < DK / 32; ++n) store_frag(p.ka + id * z.frag_raw, wave * (DK / 32) + n, L::tiles(k, 16 * wave, 32 * n, lane), lane);
     __syncthreads();
-    if (threadIdx.x < 64) {
-        float* dec = p.dec + id * 2 * kDeltaChunk;
-        dec[lane] = s.D[lane], dec[64 + lane] = s.E[lane];
-    }
     // -W^T: lane = channel of k, values = steps
     constexpr int NT = DK / 16 < 4 ? 1 : DK / 64;
     Frag<MADE> wt[NT][2];
@@ -113,7 +108,7 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             wt[n][h] = join(split<MADE>(-x[2 * h]), split<MADE>(-x[2 * h + 1]));
-            store_frag(p.wp + id * z.frag_made, 2 * ct + h, wt[n][h], lane);
+            store_frag(p.wp + id * z.frag_chain, 2 * ct + h, wt[n][h], lane);
         }
     }
     __syncthreads();
@@ -125,8 +120,13 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
         store_frag(wl, 2 * ct + 1, wt[n][1], lane);
     }
     __syncthreads();
+    const int lane0 = lane;
     for (int cv = wave; cv < p.dvp / 16; cv += 4) {
-        const int at = 16 * cv + col;
+        // (another lane with every turn, for all that the compiler knows: else it reads all of Q^T and W^T ahead of the loop, into registers that
+        // there are not)
+        int lane = lane0;
+        asm volatile("" : "+v"(lane));
+        const int col = lane & 15, g4 = 4 * (lane >> 4), at = 16 * cv + col;
         const T* gy = (const T*)p.gy + c.at(p.ys, c.hv) + at;
         Half<RAW> dr[4];
         Half<MADE> ds[4];
@@ -150,11 +150,11 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = b; t < 4; ++t) acc = mma(Blocks<MADE>::get(pb, Blocks<MADE>::at(t, b), lane), dr[t], acc);
-            *reinterpret_cast<f32x4*>(du + (b * 64 + lane) * 4) = acc;
+            store_at(du + b * 256, lane * 16, acc);
             us[b] = split<MADE>(acc);
         }
         const Frag<MADE> d0 = join(ds[0], ds[1]), d1 = join(ds[2], ds[3]), u0 = join(us[0], us[1]), u1 = join(us[2], us[3]);
-        float* c0 = p.c0 + id * (long long)DK * p.dvp + cv * (DK * 16);
+        float* c0 = p.c0 + id * z.c0 + cv * (DK * 16);
 #pragma unroll
         for (int d = 0; d < DK / 16; ++d) {
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -162,61 +162,9 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
             acc = mma(join(L::down(q, 32, 16 * d, lane), L::down(q, 48, 16 * d, lane)), d1, acc);
             acc = mma(load_frag<MADE>(wl, 2 * d, lane), u0, acc);
             acc = mma(load_frag<MADE>(wl, 2 * d + 1, lane), u1, acc);
-            *reinterpret_cast<f32x4*>(c0 + (d * 64 + lane) * 4) = acc;
+            store_at(c0 + d * 256, lane * 16, acc);
         }
     }
-}
-
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_back_chain_k(DeltaArgs p) {
-    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
-    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g4 = 4 * (lane >> 4), colv = p.dvp / 16;
-    int chain, part;
-    if (!chain_part(p, (colv + waves - 1) / waves, chain, part)) return;
-    const int cv = part * waves + wave;
-    if (cv >= colv) return;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE);
-    const bf16x4 unit = unit_half(lane);
-    const int at = 16 * cv + (lane & 15);
-    const long long state = (long long)chain * p.dk * p.dv;
-    f32x4 x[DK / 16];
-    load_state<DK>(x, p.glast ? p.glast + state : nullptr, p.dk, p.dv, at, lane);
-    for (long long m = p.NC - 1; m >= 0; --m) {
-        const long long id = chain * p.NC + m;
-        const bf16_t *wt = p.wp + id * z.frag_made, *ka = p.ka + id * z.frag_raw;
-        const float *c0 = p.c0 + id * (long long)DK * p.dvp + cv * (DK * 16), *dec = p.dec + id * 2 * kDeltaChunk;
-        float* du = p.du + id * z.cols + cv * 1024;
-        bf16_t* ds1 = p.ds1 + id * z.state;
-        Frag<MADE> xs[DK / 32];
-#pragma unroll
-        for (int d = 0; d < DK / 32; ++d) {
-            const Half<MADE> a = split<MADE>(x[2 * d]), b = split<MADE>(x[2 * d + 1]);
-            store_turned(ds1, (long long)DK * p.dvp, p.dvp, 32 * d, 16 * cv, a, unit, lane);
-            store_turned(ds1, (long long)DK * p.dvp, p.dvp, 32 * d + 16, 16 * cv, b, unit, lane);
-            xs[d] = join(a, b);
-        }
-        Half<MADE> e[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            f32x4 y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int d = 0; d < DK / 32; ++d) y = mma(load_frag<RAW>(ka, b * (DK / 32) + d, lane), xs[d], y);
-            y *= *reinterpret_cast<const f32x4*>(dec + 64 + 16 * b + g4);
-            f32x4* to = reinterpret_cast<f32x4*>(du + (b * 64 + lane) * 4);
-            *to = *to + y;
-            e[b] = split<MADE>(y);
-        }
-        const Frag<MADE> e0 = join(e[0], e[1]), e1 = join(e[2], e[3]);
-        const float end = dec[63];
-#pragma unroll
-        for (int d = 0; d < DK / 16; ++d) {
-            f32x4 n = x[d] * end + *reinterpret_cast<const f32x4*>(c0 + (d * 64 + lane) * 4);
-            n = mma(load_frag<MADE>(wt, 2 * d, lane), e0, n);
-            x[d] = mma(load_frag<MADE>(wt, 2 * d + 1, lane), e1, n);
-        }
-    }
-    store_state<DK>(p.gh0 ? p.gh0 + state : nullptr, x, p.dk, p.dv, at, lane);
 }
 
 // 8 neighbouring values of a row of d, 0 where there are none.
@@ -254,46 +202,50 @@ __device__ __forceinline__ Frag<NP> load_planes(const bf16_t* from, long long pl
     Frag<NP> f;
 #pragma unroll
     for (int n = 0; n < NP; ++n)
-        f.p[n] = *reinterpret_cast<const bf16x8*>(from + n * plane + (long long)(row + (lane & 15)) * ld + at + 8 * (lane >> 4));
+        f.p[n] = load_at<bf16x8>(from + n * plane + (long long)row * ld + at, ((lane & 15) * ld + 8 * (lane >> 4)) * 2);
     return f;
 }
 
+// Columns of v that a workgroup has in LDS at a time: as many as leave room for two workgroups on a compute unit, or for one.
+template <typename T, int DK>
+constexpr int delta_grads_cols() {
+    return DK == 32 || (sizeof(T) == 4 && DK == 128) ? 32 : 64;
+}
 template <typename T, int DK>
 constexpr int delta_grads_lds() {
     typedef DeltaPlanes<T> P;
-    return 2 * delta_rows_bytes<P::kRaw, DK>() + Rows<P::kMade, kDeltaChunk, kDeltaCols>::kValues * 2 + Blocks<P::kMade>::kValues * 2 +
-           4 * 16 * 20 * 4 + (int)sizeof(DeltaGates) + (kDeltaChunk + 4) * 4;
+    constexpr int COLS = delta_grads_cols<T, DK>();
+    return 2 * delta_rows_bytes<P::kRaw, DK>() + (Rows<P::kMade, kDeltaChunk, COLS>::kValues + Rows<P::kRaw, kDeltaChunk, COLS>::kValues) * 2 +
+           Blocks<P::kMade>::kValues * 2 + (int)sizeof(DeltaGates) + (2 * kDeltaChunk + 4) * 4;
 }
 
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
+// A wavefront has a block of 16 steps: its rows of dQ, dK, dV.  What of dP and dA concerns them are five tiles ("slots"): those of its row, blocks
+// t <= wave (lane = i, its own step, values = j), and those of its column, t >= wave (lane = j, its own step, values = i).  SHARED: value heads share
+// key heads.
+template <typename T, int DK, bool SHARED>
+__global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void delta_grads_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
-    constexpr int ND = DK / 16;
+    constexpr int ND = DK / 16, COLS = delta_grads_cols<T, DK>();
     typedef Rows<RAW, kDeltaChunk, DK> L;
-    typedef Rows<MADE, kDeltaChunk, kDeltaCols> LZ;
+    typedef Rows<MADE, kDeltaChunk, COLS> LZ;
+    typedef Rows<RAW, kDeltaChunk, COLS> LG;
+    static_assert(LZ::kValues * 2 >= 4 * 16 * 20 * 4, "the diagonal's blocks lie in Z's place");
     extern __shared__ __align__(16) unsigned char lds[];
-    bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *zl = k + L::kValues, *blocks = zl + LZ::kValues;
-    float* tiles = (float*)(blocks + Blocks<MADE>::kValues);
-    DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
-    float* dcs = (float*)(&s + 1);   // [64], and a part of dc_end from each wavefront
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4, g4 = 4 * g;
+    bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *zl = k + L::kValues, *gl = zl + LZ::kValues, *blocks = gl + LG::kValues;
+    DeltaGates& s = *(DeltaGates*)(blocks + Blocks<MADE>::kValues);
+    float* dcs = (float*)(&s + 1);   // [64]; x [64]; a part of <S0, dS1> from each wavefront
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long long block = p.first + blockIdx.x;
-    const int kchain = (int)(block / p.NC), group = p.Hv / p.Hk;
+    const int kchain = (int)(block / p.NC), group = SHARED ? p.Hv / p.Hk : 1;
     const long long m = block - kchain * p.NC, first = m * kDeltaChunk;
-    const int chain0 = kchain / p.Hk * p.Hv + kchain % p.Hk * group;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE);
-    const bf16x4 unit = unit_half(lane);
+    const int chain0 = SHARED ? kchain / p.Hk * p.Hv + kchain % p.Hk * group : kchain;
+    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    const int me = 16 * wave + col;   // this lane's step where lanes are steps of the wavefront's block
 
     const DeltaChain ck(p, chain0);
     stage_rows<T, RAW, DK>(k, (const T*)p.k + ck.at(p.ks, ck.hk), p.ks.t, p, ck, first, 0, p.dk, p.vec & kVecK);
     stage_rows<T, RAW, DK>(q, (const T*)p.q + ck.at(p.qs, ck.hk), p.qs.t, p, ck, first, 0, p.dk, p.vec & kVecQ);
-    const long long place = first + me;
-    const bool there = place < ck.len;
-    const long long step = ck.step(p, place);
     f32x4 gq[ND], gk[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) gq[d] = gk[d] = zero;
@@ -302,67 +254,60 @@ __global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
         const int chain = chain0 + e;
         const DeltaChain c(p, chain);
         const long long id = chain * p.NC + m;
-        if (e) __syncthreads();
-        chunk_gates(s, p, c, first, type);
+        if (SHARED) __syncthreads();
+        // (a lane that the compiler takes for another one with every head: else it keeps all addresses of all heads' passes, in scratch memory)
+        int lane = threadIdx.x & 63;
+        if (SHARED) asm volatile("" : "+v"(lane)::"memory");
+        const int col = lane & 15, g = lane >> 4, g4 = 4 * g;
+        const bf16x4 unit = unit_half(lane);
+        const int me = 16 * wave + col;   // this lane's step
+        const long long place = first + me;
+        const bool there = place < ck.len;
+        const long long step = ck.step(p, place);
+        load_gates(s, p.gates + id);
         __syncthreads();
-        float* tile = tiles + wave * 16 * 20;
+        float* tile = (float*)zl + wave * 16 * 20;
         make_blocks<RAW, MADE, DK, false>(blocks, tile, k, s, wave, lane);
         Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, wave), split<MADE>(invert_block<false>(tile, lane)), lane);
-        __syncthreads();
 
-        f32x4 aq[ND], az[ND], au[ND];            // dY S0^T, Z S0^T, U dS1^T of the wavefront's steps: lane = step, values = channels of k
-        f32x4 dp1[4], dp2[4], da1[4], da2[4];    // dP and -dA: 1: lane = i of this block, values = j; 2: lane = j of this block, values = i
+        f32x4 aq[ND], az[ND], au[ND];   // dY S0^T, Z S0^T, U dS1^T: lane = step, values = channels of k
+        f32x4 dp[5], da[5];             // dP and -dA
 #pragma unroll
         for (int d = 0; d < ND; ++d) aq[d] = az[d] = au[d] = zero;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) dp1[t] = dp2[t] = da1[t] = da2[t] = zero;
-        float zv = 0.f, ss = 0.f;                // Z_i.V_i; <S0, dS1>
+        for (int j = 0; j < 5; ++j) dp[j] = da[j] = zero;
+        float zv = 0.f, ss = 0.f;       // Z_i.V_i; <S0, dS1>
         const bf16_t *s0 = p.s0 + id * z.state, *ds1 = p.ds1 + id * z.state, *u = p.u + id * z.u;
-        const T *gy = (const T*)p.gy + c.at(p.ys, c.hv), *v = (const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t;
+        const T* v = (const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t;
         T* gv = (T*)p.gv + c.at(p.gvs, c.hv) + step * p.gvs.t;
         const float beta = s.beta[me];
-        for (int at = 0; at < p.dvp; at += kDeltaCols) {
-            if (at) __syncthreads();
+        for (int at = 0; at < p.dvp; at += COLS) {
+            __syncthreads();
             const int cv = at / 16 + wave;
-            if (cv < p.dvp / 16) {
+            stage_rows<T, RAW, COLS>(gl, (const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
+            if (16 * wave < COLS && cv < p.dvp / 16) {
                 const float* du = p.du + id * z.cols + cv * 1024;
                 f32x4 x[4];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const f32x4*>(du + (b * 64 + lane) * 4);
+                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(du + b * 256, lane * 16);
                 solve_back<MADE>(blocks, x, lane);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) store_turned(zl, LZ::kPlane, LZ::kStride, 16 * b, 16 * wave, split<MADE>(x[b]), unit, lane);
             }
             __syncthreads();
-#pragma unroll
-            for (int n = 0; n < kDeltaCols; n += 32) {
-                if (at + n >= p.dvp) break;
+#pragma unroll 1
+            for (int n = 0; n < COLS && at + n < p.dvp; n += 32) {
                 const int here = at + n + 8 * g;
-                Frag<RAW> of[4];
-                Frag<MADE> zf[4], uf[4];
-#pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    zf[t] = LZ::natural(zl, 16 * t, n, lane);
-                    uf[t] = load_planes<MADE>(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * t, at + n, lane);
-                    const long long i = first + 16 * t + col;
-                    T o[8];
-                    load_eight(o, gy + c.step(p, i) * p.ys.t, i < c.len, here, p.dv, p.vec & kVecGy);
-                    of[t] = planes_of<T, RAW>(o);
-                }
-                // (this block's fragments by a uniform choice: an index that the compiler knows)
-                Frag<RAW> om = of[0];
-                Frag<MADE> zm = zf[0], um = uf[0];
-#pragma unroll
-                for (int t = 1; t < 4; ++t)
-                    if (t == wave) om = of[t], zm = zf[t], um = uf[t];
+                const Frag<RAW> om = LG::natural(gl, 16 * wave, n, lane);
+                const Frag<MADE> zm = LZ::natural(zl, 16 * wave, n, lane);
+                const Frag<MADE> um = load_planes<MADE>(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * wave, at + n, lane);
                 {
                     T vv[8];
                     load_eight(vv, v, there, here, p.dv, p.vec & kVecV);
-                    float zs[8];
-                    sum_eight(zm, zs);
                     float out[8];
+                    sum_eight(zm, out);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) zv = __builtin_fmaf(zs[j], to_f32(vv[j]), zv), out[j] = there ? beta * zs[j] : 0.f;
+                    for (int j = 0; j < 8; ++j) zv = __builtin_fmaf(out[j], to_f32(vv[j]), zv), out[j] = there ? beta * out[j] : 0.f;
                     if (p.gv && place < p.T) {
                         const f32x4 lo = {out[0], out[1], out[2], out[3]}, hi = {out[4], out[5], out[6], out[7]};
                         store_four(gv, here, p.dv, lo, p.vec & kVecGv);
@@ -370,14 +315,16 @@ __global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
                     }
                 }
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    if (t <= wave) {
-                        dp1[t] = mma(uf[t], om, dp1[t]);
-                        da1[t] = mma(uf[t], zm, da1[t]);
-                    }
-                    if (t >= wave) {
-                        dp2[t] = mma(of[t], um, dp2[t]);
-                        da2[t] = mma(zf[t], um, da2[t]);
+                for (int j = 0; j < 5; ++j) {
+                    const bool row = j <= wave;
+                    const int t = row ? j : j - 1;
+                    if (row) {
+                        const Frag<MADE> uf = load_planes<MADE>(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * t, at + n, lane);
+                        dp[j] = mma(uf, om, dp[j]);
+                        da[j] = mma(uf, zm, da[j]);
+                    } else {
+                        dp[j] = mma(LG::natural(gl, 16 * t, n, lane), um, dp[j]);
+                        da[j] = mma(LZ::natural(zl, 16 * t, n, lane), um, da[j]);
                     }
                 }
 #pragma unroll
@@ -397,50 +344,6 @@ __global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
             }
         }
 
-        float rown = 0.f, coln = 0.f, db = 0.f;
-        Half<MADE> p1[4], p2[4], a1[4], a2[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t <= wave) {
-                f32x4 qk = zero, kk = zero;
-#pragma unroll
-                for (int n = 0; n < DK; n += 32) {
-                    const Frag<RAW> kt = L::natural(k, 16 * t, n, lane);
-                    qk = mma(kt, L::natural(q, 16 * wave, n, lane), qk);
-                    kk = mma(kt, L::natural(k, 16 * wave, n, lane), kk);
-                }
-                f32x4 x, y;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = me, j = 16 * t + g4 + r;
-                    const float G = j <= i ? decay_between(s, i, j) : 0.f, A = j < i ? G : 0.f;
-                    x[r] = p.scale * G * dp1[t][r];
-                    y[r] = -beta * A * da1[t][r];
-                    rown += x[r] * qk[r] + y[r] * kk[r];
-                    db -= A * da1[t][r] * kk[r];
-                }
-                p1[t] = split<MADE>(x), a1[t] = split<MADE>(y);
-            }
-            if (t >= wave) {
-                f32x4 qk = zero, kk = zero;
-#pragma unroll
-                for (int n = 0; n < DK; n += 32) {
-                    const Frag<RAW> kw = L::natural(k, 16 * wave, n, lane);
-                    qk = mma(L::natural(q, 16 * t, n, lane), kw, qk);
-                    kk = mma(L::natural(k, 16 * t, n, lane), kw, kk);
-                }
-                f32x4 x, y;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int i = 16 * t + g4 + r, j = me;
-                    const float G = j <= i ? decay_between(s, i, j) : 0.f, A = j < i ? G : 0.f;
-                    x[r] = p.scale * G * dp2[t][r];
-                    y[r] = -s.beta[i] * A * da2[t][r];
-                    coln += x[r] * qk[r] + y[r] * kk[r];
-                }
-                p2[t] = split<MADE>(x), a2[t] = split<MADE>(y);
-            }
-        }
         const float D = s.D[me], E = s.E[me], sD = p.scale * D, Db = -D * beta;
         float qd = 0.f, kz = 0.f, ku = 0.f;
 #pragma unroll
@@ -452,22 +355,48 @@ __global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
                 kz = __builtin_fmaf(kv[r], az[d][r], kz);
                 ku = __builtin_fmaf(kv[r], au[d][r], ku);
             }
-            f32x4 a = gq[d] + aq[d] * sD, b = gk[d] + az[d] * Db + au[d] * E;
+            gq[d] += aq[d] * sD, gk[d] += az[d] * Db + au[d] * E;
+        }
+        float rown = 0.f, coln = 0.f, db = 0.f;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const Half<RAW> kt = L::down(k, 16 * t, 16 * d, lane);
-                if (t <= wave) a = mma(kt, p1[t], a), b = mma(kt, a1[t], b);
-                if (t >= wave) b = mma(kt, a2[t], b), b = mma(L::down(q, 16 * t, 16 * d, lane), p2[t], b);
+        for (int j = 0; j < 5; ++j) {
+            const bool row = j <= wave;
+            const int t = row ? j : j - 1;
+            const bf16_t* qi = q + (row ? 0 : 16 * t * L::kStride);   // rows i of Q: those of this block, or the tile's
+            f32x4 qk = zero, kk = zero;
+#pragma unroll
+            for (int n = 0; n < DK; n += 32) {
+                const Frag<RAW> kt = L::natural(k, 16 * t, n, lane), kw = L::natural(k, 16 * wave, n, lane);
+                kk = mma(kt, kw, kk);
+                if (row) qk = mma(kt, L::natural(q, 16 * wave, n, lane), qk);
+                else qk = mma(L::natural(qi, 0, n, lane), kw, qk);
             }
-            gq[d] = a, gk[d] = b;
+            f32x4 x, y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int other = 16 * t + g4 + r, i = row ? me : other, c = row ? other : me;
+                const float G = c <= i ? decay_between(s, i, c) : 0.f, A = c < i ? -G * da[j][r] : 0.f;
+                x[r] = p.scale * G * dp[j][r];
+                y[r] = s.beta[i] * A;
+                const float n = c < i ? x[r] * qk[r] + y[r] * kk[r] : 0.f;   // (the diagonal is in both sums: it cancels)
+                if (row) rown += n, db += A * kk[r];
+                else coln += n;
+            }
+            const Half<MADE> xs = split<MADE>(x), ys = split<MADE>(y);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const Half<RAW> kt = L::down(k, 16 * t, 16 * d, lane);
+                if (row) gq[d] = mma(kt, xs, gq[d]);
+                else gk[d] = mma(L::down(q, 16 * t, 16 * d, lane), xs, gk[d]);
+                gk[d] = mma(kt, ys, gk[d]);
+            }
         }
         rown = group_sum(rown), coln = group_sum(coln), db = group_sum(db), zv = group_sum(zv);
         qd = group_sum(qd), kz = group_sum(kz), ku = group_sum(ku) * E;
-        if (g == 0) dcs[me] = rown - coln + sD * qd + Db * kz - ku;
-        float end = (g == 0 ? ku : 0.f) + s.D[kDeltaChunk - 1] * ss;
+        if (g == 0) dcs[me] = rown - coln + sD * qd + Db * kz, dcs[kDeltaChunk + me] = ku;
 #pragma unroll
-        for (int o = 1; o < 64; o *= 2) end += __shfl_xor(end, o);
-        if (lane == 0) dcs[kDeltaChunk + wave] = end;
+        for (int o = 1; o < 64; o *= 2) ss += __shfl_xor(ss, o);
+        if (lane == 0) dcs[2 * kDeltaChunk + wave] = ss;
         const float gbeta = (zv - D * kz + db) * s.bslope[me];
         if (p.gb && g == 0 && place < p.T) {
             const long long to = c.at(p.ggs, c.hv) + step * p.ggs.t;
@@ -477,13 +406,17 @@ __global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
         }
         __syncthreads();
         if (wave == 0) {
-            double sum = dcs[lane];
-            if (lane == 63) sum += (double)dcs[64] + dcs[65] + dcs[66] + dcs[67];
+            // sum of dc over i >= lane; x is subtracted from its own dc and added to the end's, so what is left is the x before this step
+            const float own = dcs[kDeltaChunk + lane];
+            double sum = dcs[lane], xs = own;
 #pragma unroll
             for (int o = 1; o < 64; o *= 2) {
-                const double other = __shfl_down(sum, o);
-                if (lane + o < 64) sum += other;
+                const double behind = __shfl_down(sum, o), before = __shfl_up(xs, o);
+                if (lane + o < 64) sum += behind;
+                if (lane >= o) xs += before;
             }
+            sum += xs - own;
+            sum += (double)s.D[kDeltaChunk - 1] * ((dcs[128] + dcs[129]) + (dcs[130] + dcs[131]));
             const long long i = first + lane;
             if (p.gg && i < p.T) {
                 const long long to = c.at(p.ggs, c.hv) + c.step(p, i) * p.ggs.t;
@@ -493,6 +426,9 @@ __global__ __launch_bounds__(256) void delta_grads_k(DeltaArgs p) {
             }
         }
     }
+    const int lane = threadIdx.x & 63, g4 = 4 * (lane >> 4);
+    const long long place = first + 16 * wave + (lane & 15), step = ck.step(p, place);
+    const bool there = place < ck.len;
     if (place < p.T) {
         T *rq = (T*)p.gq + ck.at(p.gqs, ck.hk) + step * p.gqs.t, *rk = (T*)p.gk + ck.at(p.gqs, ck.hk) + step * p.gqs.t;
 #pragma unroll

@@ -3,8 +3,8 @@
 // Products run on the bf16 matrix cores whatever the tensors' type: a value is a sum of bf16 planes (the value rounded, what that left
 // rounded, and so on), and a product of two such sums leaves out the products of planes that are below the result's precision.  What comes from
 // the tensors takes as many planes as hold it exactly, except the last bits of fp32 and of fp16 (1 for bf16, 2 for fp16, 3 for fp32); what
-// was computed in fp32 (the chunk's triangular system, its solutions, states) takes 2 planes for 16-bit tensors, 16 bits and so 2^-17 of a
-// value, and 3 for fp32.  Sums are the matrix cores' fp32.  So results are off by their own rounding and by little else, where single
+// was computed in fp32 (the chunk's triangular system, its solutions, states) takes 3 planes, 24 bits, where states come of it, which are results
+// in 32 bits, and 2 planes, 2^-17 of a value, where it ends in results of 16 bits.  Sums are the matrix cores' fp32.  So results are off by their own rounding and by little else, where single
 // bf16 operands had put 2^-9 of every intermediate into them; and fp32 takes 6 products of 16 cycles where the fp32 matrix instruction takes
 // eight of 32.
 //
@@ -37,8 +37,12 @@ struct DeltaArgs {
     const int* lengths;                    // [O], or null (T)
     // between the kernels, by chain and chunk
     bf16_t *wp, *kt, *s0, *u, *ka, *ds1;
-    float *ub, *du, *c0, *dec;
-    long long T, NC;                       // steps; chunks of a chain
+    float *ub, *du, *c0;
+    struct DeltaGates* gates;
+    bf16_t* maps;                          // by chain and segment: the map's matrix, and what it adds
+    float* shifts;
+    long long T, NC, seg;                  // steps; chunks of a chain, of a segment
+    int segments;
     int O, W, Hk, Hv, dk, dv, dvp;         // dvp: dv up to whole 32s
     int chains;                            // O * W * Hv, one state each
     long long first;                       // the launch's first workgroup (launch_parts)
@@ -48,6 +52,9 @@ struct DeltaArgs {
 };
 
 enum : int { kVecQ = 1, kVecK = 2, kVecV = 4, kVecGy = 8, kVecY = 16, kVecGqk = 32, kVecGv = 64 };
+
+// Planes of what states are made of: they are results in 32 bits.
+constexpr int kChainPlanes = 3;
 
 template <typename T>
 struct DeltaPlanes;
@@ -278,9 +285,9 @@ __device__ __forceinline__ void stage_planes(bf16_t* to, const bf16_t* from, int
     }
 }
 
-// The gates of a chunk.  c_i, the sum of the log decays up to step i, is summed in 64 bits and kept as two floats, so that differences of
+// The gates of a chunk.  c_i, the sum of the log decays (base 2) up to step i, is summed in 64 bits and kept as two floats, so that differences of
 // far sums lose nothing; log decays below -10000 count as that: e^-10000 is 0 in 32 bits, and differences behind it stay exact where a
-// mask's lowest value, summed, had swallowed them.
+// mask's lowest value, summed, had swallowed them.  The forward's first launch makes them, the others read them.
 struct DeltaGates {
     float hi[kDeltaChunk], lo[kDeltaChunk], beta[kDeltaChunk], D[kDeltaChunk], E[kDeltaChunk];   // D = e^c, E = e^(c_end - c)
     float slope[kDeltaChunk], bslope[kDeltaChunk];   // of the log decay by g, of beta by b
@@ -312,8 +319,8 @@ __device__ __forceinline__ void write_strength(float b, int logits, float& beta,
     }
 }
 
-// By the first wavefront; the caller's barrier follows.
-__device__ __forceinline__ void chunk_gates(DeltaGates& s, const DeltaArgs& p, const DeltaChain& c, long long first, int type) {
+// Into LDS and memory, by the first wavefront; the caller's barrier follows.
+__device__ __forceinline__ void make_gates(DeltaGates& s, DeltaGates* to, const DeltaArgs& p, const DeltaChain& c, long long first, int type) {
     if (threadIdx.x >= 64) return;
     const int lane = threadIdx.x;
     const long long i = first + lane;
@@ -323,21 +330,25 @@ __device__ __forceinline__ void chunk_gates(DeltaGates& s, const DeltaArgs& p, c
         log_decay(gate_value(p.g, c.at(p.gs, c.hv) + t * p.gs.t, p.gates_f32, type), p.logits, la, slope);
         write_strength(gate_value(p.b, c.at(p.bs, c.hv) + t * p.bs.t, p.gates_f32, type), p.logits, beta, bslope);
     }
-    double sum = la;
+    double sum = la * 1.4426950408889634;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
         const double other = __shfl_up(sum, d);
         if (lane >= d) sum += other;
     }
     const double end = __shfl(sum, 63);
-    s.hi[lane] = (float)sum;
-    s.lo[lane] = (float)(sum - (double)s.hi[lane]);
-    s.beta[lane] = beta, s.slope[lane] = slope, s.bslope[lane] = bslope;
-    s.D[lane] = expf((float)sum), s.E[lane] = expf((float)(end - sum));
+    const float hi = (float)sum, lo = (float)(sum - (double)hi), D = __builtin_amdgcn_exp2f(hi), E = __builtin_amdgcn_exp2f((float)(end - sum));
+    s.hi[lane] = to->hi[lane] = hi, s.lo[lane] = to->lo[lane] = lo, s.beta[lane] = to->beta[lane] = beta;
+    s.D[lane] = to->D[lane] = D, s.E[lane] = to->E[lane] = E;
+    s.slope[lane] = to->slope[lane] = slope, s.bslope[lane] = to->bslope[lane] = bslope;
+}
+__device__ __forceinline__ void load_gates(DeltaGates& s, const DeltaGates* from) {
+    if (threadIdx.x < sizeof(DeltaGates) / 16)
+        reinterpret_cast<f32x4*>(&s)[threadIdx.x] = reinterpret_cast<const f32x4*>(from)[threadIdx.x];
 }
 
 __device__ __forceinline__ float decay_between(const DeltaGates& s, int i, int j) {   // e^(c_i - c_j), i >= j
-    return expf((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
+    return __builtin_amdgcn_exp2f((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
 }
 
 // (I + A)^-1 of a chunk, A strictly lower, as blocks of 16 x 16 for a substitution by blocks: -A_ba below the diagonal, the inverses of the
@@ -418,17 +429,27 @@ __device__ __forceinline__ void solve_back(const bf16_t* blocks, f32x4 (&x)[4], 
     }
 }
 
+// A uniform address and a lane's own bytes behind it: one addition less a load than with 64-bit lane addresses.
+template <typename V>
+__device__ __forceinline__ V load_at(const void* base, unsigned bytes) {
+    return *reinterpret_cast<const V*>((const char*)base + bytes);
+}
+template <typename V>
+__device__ __forceinline__ void store_at(void* base, unsigned bytes, V v) {
+    *reinterpret_cast<V*>((char*)base + bytes) = v;
+}
+
 // Fragments in memory: [fragment][plane][lane][8].
 template <int NP>
 __device__ __forceinline__ void store_frag(bf16_t* base, int fragment, const Frag<NP>& f, int lane) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) *reinterpret_cast<bf16x8*>(base + ((long long)(fragment * NP + p) * 64 + lane) * 8) = f.p[p];
+    for (int p = 0; p < NP; ++p) store_at(base + (fragment * NP + p) * 512, lane * 16, f.p[p]);
 }
 template <int NP>
 __device__ __forceinline__ Frag<NP> load_frag(const bf16_t* base, int fragment, int lane) {
     Frag<NP> f;
 #pragma unroll
-    for (int p = 0; p < NP; ++p) f.p[p] = *reinterpret_cast<const bf16x8*>(base + ((long long)(fragment * NP + p) * 64 + lane) * 8);
+    for (int p = 0; p < NP; ++p) f.p[p] = load_at<bf16x8>(base + (fragment * NP + p) * 512, lane * 16);
     return f;
 }
 // one of the two tiles of a fragment
@@ -436,7 +457,7 @@ template <int NP>
 __device__ __forceinline__ void store_half(bf16_t* base, int fragment, int half, const Half<NP>& h, int lane) {
 #pragma unroll
     for (int p = 0; p < NP; ++p)
-        *reinterpret_cast<bf16x4*>(base + ((long long)(fragment * NP + p) * 64 + lane) * 8 + 4 * half) = h.p[p];
+        store_at(base + (fragment * NP + p) * 512 + 4 * half, lane * 16, h.p[p]);
 }
 
 // Four neighbouring values of a row of d to memory.
@@ -460,12 +481,13 @@ __device__ __forceinline__ float group_sum(float v) {
     return v + __shfl_xor(v, 32);
 }
 
-// Sizes of what lies between the kernels, in elements of a chunk.
+// Sizes of what lies between the kernels, in elements of a chunk; of a segment's map.
 struct DeltaSizes {
-    long long rows, frag_made, frag_raw, state, u, cols;
-    __host__ __device__ DeltaSizes(int DK, int dvp, int raw, int made)
-        : rows(kDeltaChunk * (long long)DK), frag_made(rows * made), frag_raw(rows * raw), state((long long)DK * dvp * made),
-          u((long long)kDeltaChunk * dvp * made), cols((long long)kDeltaChunk * dvp) {}
+    long long rows, frag_chain, frag_raw, state, u, cols, c0, map, shift;
+    __host__ __device__ DeltaSizes(int DK, int dvp, int raw, int made, int chain)
+        : rows(kDeltaChunk * (long long)DK), frag_chain(rows * chain), frag_raw(rows * raw), state((long long)DK * dvp * made),
+          u((long long)kDeltaChunk * dvp * made), cols((long long)kDeltaChunk * dvp), c0((long long)DK * dvp), map((long long)DK * DK * chain),
+          shift((long long)DK * dvp) {}
 };
 
 }  // namespace pdw

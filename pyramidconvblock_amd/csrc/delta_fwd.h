@@ -14,7 +14,7 @@
 // from memory; results of the first are operands of the second without an exchange.  It leaves the states before the chunks and U.
 // delta_out_k, a workgroup a chunk again: Y.
 #pragma once
-#include "delta_common.h"
+#include "delta_chain.h"
 
 namespace pdw {
 
@@ -56,12 +56,12 @@ constexpr int delta_rows_bytes() {
 template <typename T, int DK>
 constexpr int delta_prepare_lds() {
     typedef DeltaPlanes<T> P;
-    return delta_rows_bytes<P::kRaw, DK>() + Blocks<P::kMade>::kValues * 2 + 4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
+    return delta_rows_bytes<P::kRaw, DK>() + Blocks<kChainPlanes>::kValues * 2 + 4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
 }
 
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
-    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
+    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = kChainPlanes;
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
     const long long first = (id - chain * p.NC) * kDeltaChunk;
     const DeltaChain c(p, chain);
 
-    chunk_gates(s, p, c, first, type);
+    make_gates(s, p.gates + id, p, c, first, type);
     stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
     __syncthreads();
     float* tile = tiles + wave * 16 * 20;
@@ -85,11 +85,7 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
     Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, wave), split<MADE>(invert_block<true>(tile, lane)), lane);
     __syncthreads();
 
-    if (threadIdx.x < 64) {
-        float* dec = p.dec + id * 2 * kDeltaChunk;
-        dec[lane] = s.D[lane], dec[64 + lane] = s.E[lane];
-    }
-    const DeltaSizes z(DK, p.dvp, RAW, MADE);
+    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
     const bf16x4 unit = unit_half(lane);
     const int colv = p.dvp / 16;
     for (int ct = wave; ct < DK / 16 + colv; ct += 4) {
@@ -112,7 +108,7 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
                 Half<MADE> h = split<MADE>(-x[b]);
 #pragma unroll
                 for (int n = 0; n < MADE; ++n) h.p[n] = turned(h.p[n], unit);
-                store_half(p.wp + id * z.frag_made, b * (DK / 32) + ct / 2, ct & 1, h, lane);
+                store_half(p.wp + id * z.frag_chain, b * (DK / 32) + ct / 2, ct & 1, h, lane);
             }
         } else {
             const int cv = ct - DK / 16, at = 16 * cv + col;
@@ -128,102 +124,9 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
             solve_fore<MADE>(blocks, x, lane);
             float* ub = p.ub + id * z.cols + cv * 1024;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) *reinterpret_cast<f32x4*>(ub + (b * 64 + lane) * 4) = x[b];
+            for (int b = 0; b < 4; ++b) store_at(ub + b * 256, lane * 16, x[b]);
         }
     }
-}
-
-// A state's 16 columns: X[d] has rows 16 d + 4 g + r, lane = column.  From and to the user's [dk][dv].
-template <int DK>
-__device__ __forceinline__ void load_state(f32x4 (&x)[DK / 16], const float* s, int dk, int dv, int at, int lane) {
-#pragma unroll
-    for (int d = 0; d < DK / 16; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * d + 4 * (lane >> 4) + r;
-            x[d][r] = s && row < dk && at < dv ? s[row * (long long)dv + at] : 0.f;
-        }
-}
-template <int DK>
-__device__ __forceinline__ void store_state(float* s, const f32x4 (&x)[DK / 16], int dk, int dv, int at, int lane) {
-    if (!s) return;
-#pragma unroll
-    for (int d = 0; d < DK / 16; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * d + 4 * (lane >> 4) + r;
-            if (row < dk && at < dv) s[row * (long long)dv + at] = x[d][r];
-        }
-}
-// Planes of a tile (lane = column, values = rows) to [plane][row][ld]: turned, so that a lane has four neighbours of a row.
-template <int NP>
-__device__ __forceinline__ void store_turned(bf16_t* to, long long plane, int ld, int row, int at, const Half<NP>& h, bf16x4 unit, int lane) {
-#pragma unroll
-    for (int n = 0; n < NP; ++n)
-        *reinterpret_cast<bf16x4*>(to + n * plane + (long long)(row + (lane & 15)) * ld + at + 4 * (lane >> 4)) = turned(h.p[n], unit);
-}
-
-// Workgroup -> chain and columns: the parts of a chain, which read the same operands, on one die (workgroups go to the dies in turn).
-__device__ __forceinline__ bool chain_part(const DeltaArgs& p, int parts, int& chain, int& part) {
-    const long long id = p.first + blockIdx.x, turn = id >> 3;
-    part = (int)(turn % parts);
-    const long long n = (turn / parts) * 8 + (id & 7);
-    chain = (int)n;
-    return n < p.chains;
-}
-
-template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_chain_k(DeltaArgs p) {
-    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
-    const int lane = threadIdx.x & 63, waves = blockDim.x >> 6, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g4 = 4 * (lane >> 4), colv = p.dvp / 16;
-    int chain, part;
-    if (!chain_part(p, (colv + waves - 1) / waves, chain, part)) return;
-    const int cv = part * waves + wave;
-    if (cv >= colv) return;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE);
-    const bf16x4 unit = unit_half(lane);
-    const int at = 16 * cv + (lane & 15);
-    const long long state = (long long)chain * p.dk * p.dv;
-    f32x4 x[DK / 16];
-    load_state<DK>(x, p.h0 ? p.h0 + state : nullptr, p.dk, p.dv, at, lane);
-    for (long long m = 0; m < p.NC; ++m) {
-        const long long id = chain * p.NC + m;
-        const bf16_t *wp = p.wp + id * z.frag_made, *kt = p.kt + id * z.frag_raw;
-        const float *ub = p.ub + id * z.cols + cv * 1024, *dec = p.dec + id * 2 * kDeltaChunk;
-        bf16_t *s0 = p.s0 + id * z.state, *u = p.u + id * z.u;
-        Frag<MADE> xs[DK / 32];
-#pragma unroll
-        for (int d = 0; d < DK / 32; ++d) {
-            const Half<MADE> a = split<MADE>(x[2 * d]), b = split<MADE>(x[2 * d + 1]);
-            store_turned(s0, (long long)DK * p.dvp, p.dvp, 32 * d, 16 * cv, a, unit, lane);
-            store_turned(s0, (long long)DK * p.dvp, p.dvp, 32 * d + 16, 16 * cv, b, unit, lane);
-            xs[d] = join(a, b);
-        }
-        f32x4 y[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            y[b] = *reinterpret_cast<const f32x4*>(ub + (b * 64 + lane) * 4);
-#pragma unroll
-            for (int d = 0; d < DK / 32; ++d) y[b] = mma(load_frag<MADE>(wp, b * (DK / 32) + d, lane), xs[d], y[b]);
-        }
-        Half<MADE> e[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            store_turned(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * b, 16 * cv, split<MADE>(y[b]), unit, lane);
-            const f32x4 E = *reinterpret_cast<const f32x4*>(dec + 64 + 16 * b + g4);
-            e[b] = split<MADE>(y[b] * E);
-        }
-        const Frag<MADE> e0 = join(e[0], e[1]), e1 = join(e[2], e[3]);
-        const float end = dec[63];
-#pragma unroll
-        for (int d = 0; d < DK / 16; ++d) {
-            f32x4 n = x[d] * end;
-            n = mma(load_frag<RAW>(kt, 2 * d, lane), e0, n);
-            x[d] = mma(load_frag<RAW>(kt, 2 * d + 1, lane), e1, n);
-        }
-    }
-    store_state<DK>(p.last ? p.last + state : nullptr, x, p.dk, p.dv, at, lane);
 }
 
 constexpr int kDeltaCols = 64;   // columns of v that a workgroup of delta_out_k and delta_grads_k has in LDS
@@ -254,7 +157,7 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const long long first = (id - chain * p.NC) * kDeltaChunk;
     const DeltaChain c(p, chain);
 
-    chunk_gates(s, p, c, first, type);
+    load_gates(s, p.gates + id);
     stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
     stage_rows<T, RAW, DK>(q, (const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
     __syncthreads();
@@ -281,7 +184,7 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const long long step = first + i;
     const bool there = step < c.len;
     T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE);
+    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
     for (int at = 0; at < p.dv; at += kDeltaCols) {
         __syncthreads();
         stage_planes<MADE, DK, kDeltaCols>(s0, p.s0 + id * z.state, p.dvp, at);

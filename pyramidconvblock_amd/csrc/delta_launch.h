@@ -16,42 +16,52 @@ inline void delta_launch(K kernel, int lds, std::once_flag& once, long long grid
     });
 }
 
-inline long long delta_chain_grid(const DeltaArgs& p, int& waves) {
-    const int cols = p.dvp / 16;
-    waves = cols < 4 ? cols : 4;
-    return ((long long)p.chains + 7) / 8 * 8 * ((cols + waves - 1) / waves);
+template <typename T, int DK, bool BACK, int CP, bool MAPS>
+void delta_chains(const DeltaArgs& p, hipStream_t s) {
+    static std::once_flag once;
+    const int cols = p.dvp / 16 + (MAPS ? DK / 16 : 0), waves = cols < 4 && delta_least_waves<DK>() < 4 ? cols : 4;
+    const long long grid = ((long long)p.chains + 7) / 8 * 8 * ((cols + waves - 1) / waves) * (MAPS ? p.segments - 1 : p.segments);
+    delta_launch(delta_chain_k<T, DK, BACK, CP, MAPS>, delta_chain_lds<T, DK, BACK, CP>(), once, grid, 128 * waves, p, s);
 }
 
 template <typename T, int DK>
 void delta_forward(const DeltaArgs& p, hipStream_t s) {
     static std::once_flag once[2];
     const long long chunks = p.chains * p.NC;
-    int waves;
-    const long long chains = delta_chain_grid(p, waves);
-    if (chunks) delta_launch(delta_prepare_k<T, DK>, delta_prepare_lds<T, DK>(), once[0], chunks, 256, p, s);
-    std::once_flag none;
-    delta_launch(delta_chain_k<T, DK>, 0, none, chains, 64 * waves, p, s);
-    if (chunks) delta_launch(delta_out_k<T, DK>, delta_out_lds<T, DK>(), once[1], chunks, 256, p, s);
+    delta_launch(delta_prepare_k<T, DK>, delta_prepare_lds<T, DK>(), once[0], chunks, 256, p, s);
+    if (p.segments > 1) delta_chains<T, DK, false, kChainPlanes, true>(p, s);
+    delta_chains<T, DK, false, kChainPlanes, false>(p, s);
+    delta_launch(delta_out_k<T, DK>, delta_out_lds<T, DK>(), once[1], chunks, 256, p, s);
 }
 
-template <typename T, int DK>
+template <typename T, int DK, int CP>
 void delta_backward(const DeltaArgs& p, hipStream_t s) {
-    static std::once_flag once[2];
+    static std::once_flag once[3];
     const long long chunks = p.chains * p.NC;
-    int waves;
-    const long long chains = delta_chain_grid(p, waves);
-    if (chunks) delta_launch(delta_back_prepare_k<T, DK>, delta_back_prepare_lds<T, DK>(), once[0], chunks, 256, p, s);
-    std::once_flag none;
-    delta_launch(delta_back_chain_k<T, DK>, 0, none, chains, 64 * waves, p, s);
-    if (chunks) delta_launch(delta_grads_k<T, DK>, delta_grads_lds<T, DK>(), once[1], chunks / p.Hv * p.Hk, 256, p, s);
+    delta_launch(delta_back_prepare_k<T, DK, CP>, delta_back_prepare_lds<T, DK, CP>(), once[0], chunks, 256, p, s);
+    if (p.segments > 1) delta_chains<T, DK, true, CP, true>(p, s);
+    delta_chains<T, DK, true, CP, false>(p, s);
+    if (p.Hv > p.Hk) delta_launch(delta_grads_k<T, DK, true>, delta_grads_lds<T, DK>(), once[1], chunks / p.Hv * p.Hk, 256, p, s);
+    else delta_launch(delta_grads_k<T, DK, false>, delta_grads_lds<T, DK>(), once[2], chunks, 256, p, s);
+}
+
+// The gradient of an initial state is a result in 32 bits; the others of 16-bit tensors are rounded to those.
+template <typename T, int DK>
+void delta_pass(const DeltaArgs& p, bool backward, hipStream_t s) {
+    if (!backward) return delta_forward<T, DK>(p, s);
+    if constexpr (DeltaPlanes<T>::kMade < kChainPlanes)
+        if (!p.gh0) return delta_backward<T, DK, DeltaPlanes<T>::kMade>(p, s);
+    delta_backward<T, DK, kChainPlanes>(p, s);
 }
 
 template <typename T>
 void delta_dispatch(const DeltaArgs& p, bool backward, hipStream_t s) {
-    static_assert(delta_grads_lds<T, 128>() <= 160 * 1024 && delta_back_prepare_lds<T, 128>() <= 160 * 1024 && delta_out_lds<T, 128>() <= 160 * 1024, "LDS");
-    if (p.dk <= 32) backward ? delta_backward<T, 32>(p, s) : delta_forward<T, 32>(p, s);
-    else if (p.dk <= 64) backward ? delta_backward<T, 64>(p, s) : delta_forward<T, 64>(p, s);
-    else backward ? delta_backward<T, 128>(p, s) : delta_forward<T, 128>(p, s);
+    static_assert(delta_grads_lds<T, 128>() <= 160 * 1024 && delta_back_prepare_lds<T, 128, kChainPlanes>() <= 160 * 1024 &&
+                      delta_out_lds<T, 128>() <= 160 * 1024,
+                  "LDS");
+    if (p.dk <= 32) delta_pass<T, 32>(p, backward, s);
+    else if (p.dk <= 64) delta_pass<T, 64>(p, backward, s);
+    else delta_pass<T, 128>(p, backward, s);
 }
 
 }  // namespace pdw
