@@ -12,13 +12,13 @@ static int padded_dk(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
 static int padded_dv(int dv) { return (dv + 31) / 32 * 32; }
 static long long delta_chunks(long long T) { return (T + kDeltaChunk - 1) / kDeltaChunk; }
 
-// Chunks of a segment.  A chain's way through n chunks in s segments takes about 2 n / s steps (once for the maps, once with the states) and s - 1 folds,
-// n steps with one; more segments than fill the chip's 512 places for workgroups gain nothing.
+// Chunks of a segment.  A chain's way through n chunks in s segments takes about 2 n / s steps (once for the maps, once with the states), s - 1 products of
+// half a step's time and two launches more, n steps with one; more segments than fill the chip's 512 places for workgroups gain nothing.
 static long long segment_chunks(long long chains, long long NC, int DK, int dvp) {
     const long long parts = (dvp / 16 + 3) / 4, columns = chains * parts;
     long long best = NC, cost = NC;
     for (long long s = 2; s <= NC && s <= 64 && columns * (s - 1) < 512; ++s) {
-        const long long seg = (NC + s - 1) / s, c = 2 * seg + s + 4;
+        const long long seg = (NC + s - 1) / s, c = 2 * seg + s / 2 + 6;
         if (c < cost) cost = c, best = seg;
     }
     return best < 1 ? 1 : best;
@@ -65,6 +65,7 @@ static void delta_buffers(DeltaArgs& p, const DeltaPlan& d, bool backward, F f) 
     } else {
         take(p.ka, n * d.z.frag_raw * 2);
         take(p.ds1, n * d.z.state * 2);
+        take(p.blocks, n * d.z.blocks * 2);
         take(p.du, n * d.z.cols * 4);
         take(p.c0, n * d.z.c0 * 4);
     }

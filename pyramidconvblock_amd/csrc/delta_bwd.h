@@ -16,6 +16,12 @@
 #pragma once
 #include "delta_fwd.h"
 
+#ifndef FRESH
+#define FRESH int lane = threadIdx.x & 63; asm volatile("" : "+v"(lane)); const int col = lane & 15, g = lane >> 4, g4 = 4 * g, me = 16 * wave + col; const long long place = first + me; const bool there = place < ck.len; const long long step = ck.step(p, place); (void)g; (void)g4; (void)there; (void)step; (void)col
+#endif
+#ifndef SB
+#define SB __builtin_amdgcn_sched_barrier(0)
+#endif
 namespace pdw {
 
 template <typename T, int NP>
@@ -50,7 +56,6 @@ constexpr int delta_back_prepare_lds() {
 template <typename T, int DK, int MADE>
 __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw;
-    constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *wl = k;
@@ -59,15 +64,19 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
     DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = 4 * (lane >> 4);
-    const long long id = p.first + blockIdx.x;
-    const int chain = (int)(id / p.NC);
-    const long long first = (id - chain * p.NC) * kDeltaChunk;
+    int chain;
+    long long m;
+    if (!chunk_of(p, p.Hv, chain, m)) return;
+    const long long id = chain * p.NC + m, first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
     const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
 
-    load_gates(s, p.gates + id);
-    stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
-    stage_rows<T, RAW, DK>(q, (const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+    Run<sizeof(DeltaGates)> gates;
+    Staged<T, RAW, DK> ks, qs;
+    ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+    qs.load((const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+    gates.load(p.gates + id);
+    ks.put(k), qs.put(q), gates.put(&s);
     __syncthreads();
     float* tile = tiles + wave * 16 * 20;
     make_blocks<RAW, MADE, DK, true>(blocks, tile, k, s, wave, lane);
@@ -78,18 +87,26 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
         if (t < wave) continue;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < DK; n += 32) acc = mma(L::natural(q, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
+        for (int n = 0; n < DK; n += 32) acc = mma<MADE>(L::natural(q, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
+        const TileDecay decay(s, 16 * wave + col, 16 * t + g4, false);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = 16 * t + g4 + r, j = 16 * wave + col;
-            acc[r] = j <= i ? p.scale * decay_between(s, i, j) * acc[r] : 0.f;
-        }
+        for (int r = 0; r < 4; ++r) acc[r] = t != wave || col <= g4 + r ? p.scale * decay.G[r] * acc[r] : 0.f;
         Blocks<MADE>::put(pb, Blocks<MADE>::at(t, wave), split<MADE>(acc), lane);
     }
     // K as the chain's first operand
 #pragma unroll
     for (int n = 0; n < DK / 32; ++n) store_frag(p.ka + id * z.frag_raw, wave * (DK / 32) + n, L::tiles(k, 16 * wave, 32 * n, lane), lane);
     __syncthreads();
+    // the blocks for the transposed system, of the planes that delta_grads_k takes
+    const bf16x4 unit = unit_half(lane);
+    constexpr int NG = DeltaPlanes<T>::kMade;
+    for (int n = wave; n < 10; n += 4) {
+        const Half<MADE> h = Blocks<MADE>::get(blocks, n, lane);
+        Half<NG> t;
+#pragma unroll
+        for (int m = 0; m < NG; ++m) t.p[m] = turned(h.p[m], unit);
+        Blocks<NG>::put(p.blocks + id * 10 * NG * 256, n, t, lane);
+    }
     // -W^T: lane = channel of k, values = steps
     constexpr int NT = DK / 16 < 4 ? 1 : DK / 64;
     Frag<MADE> wt[NT][2];
@@ -167,43 +184,31 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
     }
 }
 
-// 8 neighbouring values of a row of d, 0 where there are none.
+// 4 neighbouring values of a row of d, 0 where there are none.
 template <typename T>
-__device__ __forceinline__ void load_eight(T (&v)[8], const T* row, bool there, int at, int d, bool vec) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(0.f);
-    if (!there || at >= d) return;
+__device__ __forceinline__ f32x4 load_four(const T* row, bool there, int at, int d, bool vec) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (!there || at >= d) return v;
     if (vec) {
-        constexpr int VEC = 16 / sizeof(T);
+        const ChanVec<T, 4> r = *reinterpret_cast<const ChanVec<T, 4>*>(row + at);
 #pragma unroll
-        for (int m = 0; m < 8 / VEC; ++m) {
-            const ChanVec<T, VEC> r = *reinterpret_cast<const ChanVec<T, VEC>*>(row + at + m * VEC);
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) v[m * VEC + j] = r.v[j];
-        }
+        for (int j = 0; j < 4; ++j) v[j] = to_f32(r.v[j]);
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (at + j < d) v[j] = row[at + j];
+        for (int j = 0; j < 4; ++j)
+            if (at + j < d) v[j] = to_f32(row[at + j]);
     }
+    return v;
 }
+// The two tiles of a fragment, summed over planes.
 template <int NP>
-__device__ __forceinline__ void sum_eight(const Frag<NP>& f, float (&v)[8]) {
+__device__ __forceinline__ void sum_tiles(const Frag<NP>& f, f32x4& lo, f32x4& hi) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        v[j] = (float)f.p[NP - 1][j];
+    for (int j = 0; j < 4; ++j) {
+        lo[j] = (float)f.p[NP - 1][j], hi[j] = (float)f.p[NP - 1][4 + j];
 #pragma unroll
-        for (int p = NP - 2; p >= 0; --p) v[j] += (float)f.p[p][j];
+        for (int p = NP - 2; p >= 0; --p) lo[j] += (float)f.p[p][j], hi[j] += (float)f.p[p][4 + j];
     }
-}
-// 8 values of a lane's row of planes in memory [plane][..][ld]
-template <int NP>
-__device__ __forceinline__ Frag<NP> load_planes(const bf16_t* from, long long plane, int ld, int row, int at, int lane) {
-    Frag<NP> f;
-#pragma unroll
-    for (int n = 0; n < NP; ++n)
-        f.p[n] = load_at<bf16x8>(from + n * plane + (long long)row * ld + at, ((lane & 15) * ld + 8 * (lane >> 4)) * 2);
-    return f;
 }
 
 // Columns of v that a workgroup has in LDS at a time: as many as leave room for two workgroups on a compute unit, or for one.
@@ -223,29 +228,30 @@ constexpr int delta_grads_lds() {
 // t <= wave (lane = i, its own step, values = j), and those of its column, t >= wave (lane = j, its own step, values = i).  SHARED: value heads share
 // key heads.
 template <typename T, int DK, bool SHARED>
-__global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void delta_grads_k(DeltaArgs p) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delta_grads_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
-    constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     constexpr int ND = DK / 16, COLS = delta_grads_cols<T, DK>();
     typedef Rows<RAW, kDeltaChunk, DK> L;
     typedef Rows<MADE, kDeltaChunk, COLS> LZ;
     typedef Rows<RAW, kDeltaChunk, COLS> LG;
-    static_assert(LZ::kValues * 2 >= 4 * 16 * 20 * 4, "the diagonal's blocks lie in Z's place");
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *zl = k + L::kValues, *gl = zl + LZ::kValues, *blocks = gl + LG::kValues;
     DeltaGates& s = *(DeltaGates*)(blocks + Blocks<MADE>::kValues);
     float* dcs = (float*)(&s + 1);   // [64]; x [64]; a part of <S0, dS1> from each wavefront
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long long block = p.first + blockIdx.x;
-    const int kchain = (int)(block / p.NC), group = SHARED ? p.Hv / p.Hk : 1;
-    const long long m = block - kchain * p.NC, first = m * kDeltaChunk;
+    int kchain;
+    long long m;
+    if (!chunk_of(p, p.Hk, kchain, m)) return;
+    const int group = SHARED ? p.Hv / p.Hk : 1;
+    const long long first = m * kDeltaChunk;
     const int chain0 = SHARED ? kchain / p.Hk * p.Hv + kchain % p.Hk * group : kchain;
     const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
     const DeltaChain ck(p, chain0);
-    stage_rows<T, RAW, DK>(k, (const T*)p.k + ck.at(p.ks, ck.hk), p.ks.t, p, ck, first, 0, p.dk, p.vec & kVecK);
-    stage_rows<T, RAW, DK>(q, (const T*)p.q + ck.at(p.qs, ck.hk), p.qs.t, p, ck, first, 0, p.dk, p.vec & kVecQ);
+    Staged<T, RAW, DK> ks, qs;
+    ks.load((const T*)p.k + ck.at(p.ks, ck.hk), p.ks.t, p, ck, first, 0, p.dk, p.vec & kVecK);
+    qs.load((const T*)p.q + ck.at(p.qs, ck.hk), p.qs.t, p, ck, first, 0, p.dk, p.vec & kVecQ);
     f32x4 gq[ND], gk[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) gq[d] = gk[d] = zero;
@@ -254,7 +260,6 @@ __global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void de
         const int chain = chain0 + e;
         const DeltaChain c(p, chain);
         const long long id = chain * p.NC + m;
-        if (SHARED) __syncthreads();
         // (a lane that the compiler takes for another one with every head: else it keeps all addresses of all heads' passes, in scratch memory)
         int lane = threadIdx.x & 63;
         if (SHARED) asm volatile("" : "+v"(lane)::"memory");
@@ -264,11 +269,9 @@ __global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void de
         const long long place = first + me;
         const bool there = place < ck.len;
         const long long step = ck.step(p, place);
-        load_gates(s, p.gates + id);
-        __syncthreads();
-        float* tile = (float*)zl + wave * 16 * 20;
-        make_blocks<RAW, MADE, DK, false>(blocks, tile, k, s, wave, lane);
-        Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, wave), split<MADE>(invert_block<false>(tile, lane)), lane);
+        Run<sizeof(DeltaGates)> gates;
+        Run<Blocks<MADE>::kValues * 2> system;
+        gates.load(p.gates + id), system.load(p.blocks + id * z.blocks);
 
         f32x4 aq[ND], az[ND], au[ND];   // dY S0^T, Z S0^T, U dS1^T: lane = step, values = channels of k
         f32x4 dp[5], da[5];             // dP and -dA
@@ -278,40 +281,50 @@ __global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void de
         for (int j = 0; j < 5; ++j) dp[j] = da[j] = zero;
         float zv = 0.f, ss = 0.f;       // Z_i.V_i; <S0, dS1>
         const bf16_t *s0 = p.s0 + id * z.state, *ds1 = p.ds1 + id * z.state, *u = p.u + id * z.u;
-        const T* v = (const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t;
-        T* gv = (T*)p.gv + c.at(p.gvs, c.hv) + step * p.gvs.t;
-        const float beta = s.beta[me];
+        float beta;
         for (int at = 0; at < p.dvp; at += COLS) {
-            __syncthreads();
             const int cv = at / 16 + wave;
-            stage_rows<T, RAW, COLS>(gl, (const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
-            if (16 * wave < COLS && cv < p.dvp / 16) {
+            const bool mine = 16 * wave < COLS && cv < p.dvp / 16;
+            Staged<T, RAW, COLS> gs;
+            gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
+            f32x4 x[4];
+            if (mine) {
                 const float* du = p.du + id * z.cols + cv * 1024;
-                f32x4 x[4];
 #pragma unroll
                 for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(du + b * 256, lane * 16);
+            }
+            if (e || at) __syncthreads();
+            if (at == 0) {
+                if (e == 0) ks.put(k), qs.put(q);
+                gates.put(&s), system.put(blocks);
+            }
+            gs.put(gl);
+            __syncthreads();
+            beta = s.beta[me];
+            if (mine) {
                 solve_back<MADE>(blocks, x, lane);
 #pragma unroll
-                for (int b = 0; b < 4; ++b) store_turned(zl, LZ::kPlane, LZ::kStride, 16 * b, 16 * wave, split<MADE>(x[b]), unit, lane);
+                for (int b = 0; b < 4; ++b) LZ::put_turned(zl, 16 * b, 16 * wave, split<MADE>(x[b]), unit, lane);
             }
             __syncthreads();
 #pragma unroll 1
             for (int n = 0; n < COLS && at + n < p.dvp; n += 32) {
-                const int here = at + n + 8 * g;
-                const Frag<RAW> om = LG::natural(gl, 16 * wave, n, lane);
-                const Frag<MADE> zm = LZ::natural(zl, 16 * wave, n, lane);
-                const Frag<MADE> um = load_planes<MADE>(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * wave, at + n, lane);
+                FRESH;
+                const int here = at + n + g4, cw = (at + n) / 16;
+                const Frag<RAW> om = LG::tiles(gl, 16 * wave, n, lane);
+                const Frag<MADE> zm = LZ::tiles(zl, 16 * wave, n, lane);
+                const Frag<MADE> um = load_turned<MADE>(u, cw * 2 + wave / 2, 2, wave & 1, unit, lane);
                 {
-                    T vv[8];
-                    load_eight(vv, v, there, here, p.dv, p.vec & kVecV);
-                    float out[8];
-                    sum_eight(zm, out);
+                    const T* v = (const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t;
+                    T* gv = (T*)p.gv + c.at(p.gvs, c.hv) + step * p.gvs.t;
+                    f32x4 lo, hi;
+                    sum_tiles(zm, lo, hi);
+                    const f32x4 vl = load_four(v, there, here, p.dv, p.vec & kVecV), vh = load_four(v, there, here + 16, p.dv, p.vec & kVecV);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) zv = __builtin_fmaf(out[j], to_f32(vv[j]), zv), out[j] = there ? beta * out[j] : 0.f;
+                    for (int j = 0; j < 4; ++j) zv = __builtin_fmaf(lo[j], vl[j], __builtin_fmaf(hi[j], vh[j], zv));
                     if (p.gv && place < p.T) {
-                        const f32x4 lo = {out[0], out[1], out[2], out[3]}, hi = {out[4], out[5], out[6], out[7]};
-                        store_four(gv, here, p.dv, lo, p.vec & kVecGv);
-                        store_four(gv, here + 4, p.dv, hi, p.vec & kVecGv);
+                        store_four(gv, here, p.dv, there ? lo * beta : zero, p.vec & kVecGv);
+                        store_four(gv, here + 16, p.dv, there ? hi * beta : zero, p.vec & kVecGv);
                     }
                 }
 #pragma unroll
@@ -319,31 +332,35 @@ __global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void de
                     const bool row = j <= wave;
                     const int t = row ? j : j - 1;
                     if (row) {
-                        const Frag<MADE> uf = load_planes<MADE>(u, (long long)kDeltaChunk * p.dvp, p.dvp, 16 * t, at + n, lane);
+                        const Frag<MADE> uf = load_turned<MADE>(u, cw * 2 + t / 2, 2, t & 1, unit, lane);
                         dp[j] = mma(uf, om, dp[j]);
                         da[j] = mma(uf, zm, da[j]);
                     } else {
-                        dp[j] = mma(LG::natural(gl, 16 * t, n, lane), um, dp[j]);
-                        da[j] = mma(LZ::natural(zl, 16 * t, n, lane), um, da[j]);
+                        dp[j] = mma(LG::tiles(gl, 16 * t, n, lane), um, dp[j]);
+                        da[j] = mma(LZ::tiles(zl, 16 * t, n, lane), um, da[j]);
                     }
+                    SB;
                 }
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    const Frag<MADE> sf = load_planes<MADE>(s0, (long long)DK * p.dvp, p.dvp, 16 * d, at + n, lane);
-                    const Frag<MADE> df = load_planes<MADE>(ds1, (long long)DK * p.dvp, p.dvp, 16 * d, at + n, lane);
+                    const Frag<MADE> sf = load_turned<MADE>(s0, cw * (DK / 32) + d / 2, DK / 32, d & 1, unit, lane);
+                    const Frag<MADE> df = load_turned<MADE>(ds1, cw * (DK / 32) + d / 2, DK / 32, d & 1, unit, lane);
                     aq[d] = mma(sf, om, aq[d]);
                     az[d] = mma(sf, zm, az[d]);
                     au[d] = mma(df, um, au[d]);
                     if ((d & 3) == wave) {
-                        float a[8], b[8];
-                        sum_eight(sf, a), sum_eight(df, b);
+                        f32x4 a0, a1, b0, b1;
+                        sum_tiles(sf, a0, a1), sum_tiles(df, b0, b1);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(a[j], b[j], ss);
+                        for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(a0[j], b0[j], __builtin_fmaf(a1[j], b1[j], ss));
                     }
+                    SB;
                 }
             }
         }
 
+        {
+        FRESH;
         const float D = s.D[me], E = s.E[me], sD = p.scale * D, Db = -D * beta;
         float qd = 0.f, kz = 0.f, ku = 0.f;
 #pragma unroll
@@ -362,34 +379,37 @@ __global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void de
         for (int j = 0; j < 5; ++j) {
             const bool row = j <= wave;
             const int t = row ? j : j - 1;
-            const bf16_t* qi = q + (row ? 0 : 16 * t * L::kStride);   // rows i of Q: those of this block, or the tile's
+            FRESH;
+            // lane = i, values = j: K of the tile by Q of this block; the other way: Q by K
+            const bf16_t *far = row ? k : q, *near = row ? q : k;
             f32x4 qk = zero, kk = zero;
 #pragma unroll
             for (int n = 0; n < DK; n += 32) {
-                const Frag<RAW> kt = L::natural(k, 16 * t, n, lane), kw = L::natural(k, 16 * wave, n, lane);
-                kk = mma(kt, kw, kk);
-                if (row) qk = mma(kt, L::natural(q, 16 * wave, n, lane), qk);
-                else qk = mma(L::natural(qi, 0, n, lane), kw, qk);
+                qk = mma(L::natural(far, 16 * t, n, lane), L::natural(near, 16 * wave, n, lane), qk);
+                kk = mma(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), kk);
             }
+            const TileDecay decay(s, me, 16 * t + g4, row);
             f32x4 x, y;
+            float n = 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int other = 16 * t + g4 + r, i = row ? me : other, c = row ? other : me;
-                const float G = c <= i ? decay_between(s, i, c) : 0.f, A = c < i ? -G * da[j][r] : 0.f;
-                x[r] = p.scale * G * dp[j][r];
-                y[r] = s.beta[i] * A;
-                const float n = c < i ? x[r] * qk[r] + y[r] * kk[r] : 0.f;   // (the diagonal is in both sums: it cancels)
-                if (row) rown += n, db += A * kk[r];
-                else coln += n;
+                const bool diagonal = t == wave, below = !diagonal || (row ? g4 + r < col : col < g4 + r), at_all = below || (diagonal && g4 + r == col);
+                const float A = below ? -decay.G[r] * da[j][r] : 0.f;
+                x[r] = at_all ? p.scale * decay.G[r] * dp[j][r] : 0.f;
+                y[r] = decay.beta[r] * A;
+                n += (below ? x[r] * qk[r] : 0.f) + y[r] * kk[r];   // (the diagonal of N is in both sums: it cancels)
+                db += row ? A * kk[r] : 0.f;
             }
+            rown += row ? n : 0.f, coln += row ? 0.f : n;
             const Half<MADE> xs = split<MADE>(x), ys = split<MADE>(y);
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                const Half<RAW> kt = L::down(k, 16 * t, 16 * d, lane);
-                if (row) gq[d] = mma(kt, xs, gq[d]);
-                else gk[d] = mma(L::down(q, 16 * t, 16 * d, lane), xs, gk[d]);
+                const Half<RAW> kt = L::down(k, 16 * t, 16 * d, lane), ft = L::down(far, 16 * t, 16 * d, lane);
+                if (row) gq[d] = mma(ft, xs, gq[d]);
+                else gk[d] = mma(ft, xs, gk[d]);
                 gk[d] = mma(kt, ys, gk[d]);
             }
+            SB;
         }
         rown = group_sum(rown), coln = group_sum(coln), db = group_sum(db), zv = group_sum(zv);
         qd = group_sum(qd), kz = group_sum(kz), ku = group_sum(ku) * E;
@@ -424,6 +444,7 @@ __global__ __launch_bounds__(256, DK == 32 ? 3 : sizeof(T) == 2 ? 2 : 1) void de
                 if (p.gates_f32) ((float*)p.gg)[to] = out;
                 else ((T*)p.gg)[to] = from_f32<T>(out);
             }
+        }
         }
     }
     const int lane = threadIdx.x & 63, g4 = 4 * (lane >> 4);

@@ -36,7 +36,7 @@ struct DeltaArgs {
     float *last, *gh0;                     // [chain][dk][dv], or null
     const int* lengths;                    // [O], or null (T)
     // between the kernels, by chain and chunk
-    bf16_t *wp, *kt, *s0, *u, *ka, *ds1;
+    bf16_t *wp, *kt, *s0, *u, *ka, *ds1, *blocks;
     float *ub, *du, *c0;
     struct DeltaGates* gates;
     bf16_t* maps;                          // by chain and segment: the map's matrix, and what it adds
@@ -85,10 +85,11 @@ struct Half {   // inner axis of 16: value j of lane group g is 4 g + j
     bf16x4 p[NP];
 };
 
-// c + a b: the products of planes i and j with i + j below the larger number of planes, the small ones first.
-template <int NA, int NB>
+// c + a b: the products of planes i and j with i + j below N, by default the larger number of planes, the small ones first.  (N = 3 for products of
+// tensors that states come of: of fp16's two planes each the last product is 2^-18.)
+template <int N_ = 0, int NA, int NB>
 __device__ __forceinline__ f32x4 mma(const Frag<NA>& a, const Frag<NB>& b, f32x4 c) {
-    constexpr int N = NA > NB ? NA : NB;
+    constexpr int N = N_ ? N_ : NA > NB ? NA : NB;
 #pragma unroll
     for (int s = N - 1; s >= 0; --s)
 #pragma unroll
@@ -108,6 +109,28 @@ __device__ __forceinline__ f32x4 mma(const Half<NA>& a, const Half<NB>& b, f32x4
         for (int i = 0; i <= s; ++i)
             if (i < NA && s - i < NB) c = mma16(a.p[i], b.p[s - i], c);
     return c;
+}
+
+// The same for several first operands, their products in turn: one waits for the last only when all have had theirs.
+template <int R, int NA, int NB>
+__device__ __forceinline__ void mma_rows(const Frag<NA> (&a)[R], const Frag<NB>& b, f32x4 (&c)[R]) {
+    constexpr int N = NA > NB ? NA : NB;
+#pragma unroll
+    for (int s = N - 1; s >= 0; --s)
+#pragma unroll
+        for (int i = 0; i <= s; ++i)
+            if (i < NA && s - i < NB) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) c[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[r].p[i], b.p[s - i], c[r], 0, 0, 0);
+            }
+}
+// The first planes.
+template <int NP, int N>
+__device__ __forceinline__ Frag<NP> planes(const Frag<N>& f) {
+    Frag<NP> r;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) r.p[p] = f.p[p];
+    return r;
 }
 
 template <int NP>
@@ -141,6 +164,16 @@ __device__ __forceinline__ f32x4 sum_of(const Half<NP>& h) {
         for (int p = NP - 2; p >= 0; --p) v[i] += (float)h.p[p][i];
     }
     return v;
+}
+
+// A uniform address and a lane's own bytes behind it: one addition less a load than with 64-bit lane addresses.
+template <typename V>
+__device__ __forceinline__ V load_at(const void* base, unsigned bytes) {
+    return *reinterpret_cast<const V*>((const char*)base + bytes);
+}
+template <typename V>
+__device__ __forceinline__ void store_at(void* base, unsigned bytes, V v) {
+    *reinterpret_cast<V*>((char*)base + bytes) = v;
 }
 
 // The planes of 8 values of a tensor.
@@ -206,6 +239,12 @@ struct Rows {
     static __device__ __forceinline__ Frag<NP> tiles(const bf16_t* base, int row, int at, int lane) {
         return join(half(base, row, at, lane), half(base, row, at + 16, lane));
     }
+    // a tile (lane = column, values = rows) to its rows, turned
+    static __device__ __forceinline__ void put_turned(bf16_t* base, int row, int at, const Half<NP>& h, bf16x4 unit, int lane) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p)
+            *reinterpret_cast<bf16x4*>(base + p * kPlane + (row + (lane & 15)) * kStride + at + 4 * (lane >> 4)) = turned(h.p[p], unit);
+    }
     // lane = column `at` + l % 16, values = rows row + 4 g ..: every group of 16 lanes reads four rows of 16 values, transposed on the way
     static __device__ __forceinline__ Half<NP> down(const bf16_t* base, int row, int at, int lane) {
         typedef __attribute__((address_space(3))) s16x4 lds_t;
@@ -240,50 +279,88 @@ struct DeltaChain {
     __device__ __forceinline__ long long at(const DeltaStrides& s, int head) const { return o * s.o + w * s.w + head * s.h; }
 };
 
-// A chunk of a tensor's rows as planes in LDS: 0 behind the chain's end, behind the row's end d, and up to R values.
-template <typename T, int NP, int R>
-__device__ __forceinline__ void stage_rows(bf16_t* to, const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first,
-                                           int col, int d, bool vec) {
-    typedef Rows<NP, kDeltaChunk, R> L;
-    for (int e = threadIdx.x; e < kDeltaChunk * (R / 8); e += blockDim.x) {
-        const int row = e / (R / 8), at = e % (R / 8) * 8;
-        const long long i = first + row;
-        T v[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = from_f32<T>(0.f);
-        if (i < c.len && col + at < d) {
-            const T* q = base + c.step(p, i) * st + col + at;
-            if (vec) {
-                constexpr int VEC = 16 / sizeof(T);
-#pragma unroll
-                for (int m = 0; m < 8 / VEC; ++m) {
-                    const ChanVec<T, VEC> r = *reinterpret_cast<const ChanVec<T, VEC>*>(q + m * VEC);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[m * VEC + j] = r.v[j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (col + at + j < d) v[j] = q[j];
-            }
-        }
-        const Frag<NP> f = planes_of<T, NP>(v);
-#pragma unroll
-        for (int n = 0; n < NP; ++n) *reinterpret_cast<bf16x8*>(to + n * L::kPlane + row * L::kStride + at) = f.p[n];
-    }
+// Workgroup -> chunk m of a chain: the heads (H of them) of a chunk follow one another on one die (workgroups go to the eight dies in turn), since rows of
+// neighbouring heads share lines of memory, which a die's cache holds.  false: there is none.
+__device__ __forceinline__ bool chunk_of(const DeltaArgs& p, int H, int& chain, long long& m) {
+    const long long id = p.first + blockIdx.x, turn = id >> 3;
+    const int head = (int)(turn % H);
+    const long long place = turn / H * 8 + (id & 7), row = place / p.NC;   // (batch element, chunk)
+    m = place - row * p.NC;
+    chain = (int)row * H + head;
+    return row < (long long)p.O * p.W;
 }
 
-// Planes [plane][row][ld] in memory (states, U) to LDS: columns [col, col + R), those of them that there are.
-template <int NP, int ROWS, int R>
-__device__ __forceinline__ void stage_planes(bf16_t* to, const bf16_t* from, int ld, int col) {
-    typedef Rows<NP, ROWS, R> L;
-    for (int e = threadIdx.x; e < NP * ROWS * (R / 8); e += blockDim.x) {
-        const int at = e % (R / 8) * 8, row = e / (R / 8) % ROWS, n = e / (R / 8) / ROWS;
-        if (col + at < ld)
-            *reinterpret_cast<bf16x8*>(to + n * L::kPlane + row * L::kStride + at) =
-                *reinterpret_cast<const bf16x8*>(from + (long long)(n * ROWS + row) * ld + col + at);
+// A chunk of a tensor's rows, columns [col, col + R), on its way to LDS: `load` makes the loads, all without a condition where rows lie in pieces of
+// 8 (what is not there is read from row 0 and dropped), so that they are under way together with others; `put` leaves planes, 0 behind
+// the chain's end and behind the row's end d.  By 256 threads.
+template <typename T, int NP, int R>
+struct Staged {
+    static constexpr int N = kDeltaChunk * (R / 8) / 256;
+    T v[N][8];
+    bool on[N];
+    __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first, int col, int d, bool vec) {
+        int at[N];
+        const T* q[N];
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = threadIdx.x + n * 256;
+            const long long i = first + e / (R / 8);
+            at[n] = col + e % (R / 8) * 8;
+            on[n] = i < c.len && at[n] < d;
+            q[n] = base + (on[n] ? c.step(p, i) * st + at[n] : 0);
+        }
+        if (vec) {
+            constexpr int VEC = 16 / sizeof(T);
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int m = 0; m < 8 / VEC; ++m) {
+                    const ChanVec<T, VEC> r = *reinterpret_cast<const ChanVec<T, VEC>*>(q[n] + m * VEC);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) v[n][m * VEC + j] = r.v[j];
+                }
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[n][j] = on[n] && at[n] + j < d ? q[n][j] : from_f32<T>(0.f);
+        }
     }
-}
+    __device__ __forceinline__ void put(bf16_t* to) {
+        typedef Rows<NP, kDeltaChunk, R> L;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = threadIdx.x + n * 256;
+            Frag<NP> f = planes_of<T, NP>(v[n]);
+#pragma unroll
+            for (int m = 0; m < NP; ++m) {
+                if (!on[n]) f.p[m] = bf16x8{};
+                *reinterpret_cast<bf16x8*>(to + m * L::kPlane + e / (R / 8) * L::kStride + e % (R / 8) * 8) = f.p[m];
+            }
+        }
+    }
+};
+
+// A plain run of 16-byte pieces from memory to LDS, by 256 threads.
+template <int BYTES>
+struct Run {
+    static constexpr int N = (BYTES / 16 + 255) / 256;
+    f32x4 v[N];
+    __device__ __forceinline__ void load(const void* from) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = threadIdx.x + n * 256;
+            v[n] = load_at<f32x4>(from, (e < BYTES / 16 ? e : 0) * 16);
+        }
+    }
+    __device__ __forceinline__ void put(void* to) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = threadIdx.x + n * 256;
+            if (e < BYTES / 16) *reinterpret_cast<f32x4*>((char*)to + e * 16) = v[n];
+        }
+    }
+};
 
 // The gates of a chunk.  c_i, the sum of the log decays (base 2) up to step i, is summed in 64 bits and kept as two floats, so that differences of
 // far sums lose nothing; log decays below -10000 count as that: e^-10000 is 0 in 32 bits, and differences behind it stay exact where a
@@ -342,14 +419,21 @@ __device__ __forceinline__ void make_gates(DeltaGates& s, DeltaGates* to, const 
     s.D[lane] = to->D[lane] = D, s.E[lane] = to->E[lane] = E;
     s.slope[lane] = to->slope[lane] = slope, s.bslope[lane] = to->bslope[lane] = bslope;
 }
-__device__ __forceinline__ void load_gates(DeltaGates& s, const DeltaGates* from) {
-    if (threadIdx.x < sizeof(DeltaGates) / 16)
-        reinterpret_cast<f32x4*>(&s)[threadIdx.x] = reinterpret_cast<const f32x4*>(from)[threadIdx.x];
-}
-
-__device__ __forceinline__ float decay_between(const DeltaGates& s, int i, int j) {   // e^(c_i - c_j), i >= j
-    return __builtin_amdgcn_exp2f((s.hi[i] - s.hi[j]) + (s.lo[i] - s.lo[j]));
-}
+// e^(c_i - c_j) of a tile: this lane's step and four others of it, which is i and which j: rows: this lane's is i.  Above the diagonal (i < j) it may
+// be infinite: the caller selects.
+struct TileDecay {
+    f32x4 G, beta;   // beta of the rows i
+    __device__ __forceinline__ TileDecay(const DeltaGates& s, int mine, int others, bool rows) {
+        const f32x4 hi = *reinterpret_cast<const f32x4*>(s.hi + others), lo = *reinterpret_cast<const f32x4*>(s.lo + others);
+        beta = *reinterpret_cast<const f32x4*>(s.beta + others);
+        const float h = s.hi[mine], l = s.lo[mine], b = s.beta[mine], sign = rows ? 1.f : -1.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            G[r] = __builtin_amdgcn_exp2f(sign * ((h - hi[r]) + (l - lo[r])));
+            beta[r] = rows ? b : beta[r];
+        }
+    }
+};
 
 // (I + A)^-1 of a chunk, A strictly lower, as blocks of 16 x 16 for a substitution by blocks: -A_ba below the diagonal, the inverses of the
 // diagonal's blocks on it.  Block (b, a) is number b (b + 1) / 2 + a.  FORE: lane = row, values = columns, an operand for products with
@@ -383,12 +467,16 @@ __device__ __forceinline__ f32x4 invert_block(const float* tile, int lane) {
         float a[16];
 #pragma unroll
         for (int m = 0; m < 16; m += 4) {
+            if (FORE ? m + 3 <= j : m >= j) continue;
             const f32x4 r = *reinterpret_cast<const f32x4*>(tile + j * 20 + m);
             a[m] = r[0], a[m + 1] = r[1], a[m + 2] = r[2], a[m + 3] = r[3];
         }
+        // (the latest of t last: it is what there is to wait for)
 #pragma unroll
-        for (int m = 0; m < 16; ++m)
+        for (int k = 0; k < 16; ++k) {
+            const int m = FORE ? 15 - k : k;
             if (FORE ? m > j : m < j) s = __builtin_fmaf(-t[m], a[m], s);
+        }
         t[j] = s;
     }
     f32x4 v;
@@ -429,16 +517,6 @@ __device__ __forceinline__ void solve_back(const bf16_t* blocks, f32x4 (&x)[4], 
     }
 }
 
-// A uniform address and a lane's own bytes behind it: one addition less a load than with 64-bit lane addresses.
-template <typename V>
-__device__ __forceinline__ V load_at(const void* base, unsigned bytes) {
-    return *reinterpret_cast<const V*>((const char*)base + bytes);
-}
-template <typename V>
-__device__ __forceinline__ void store_at(void* base, unsigned bytes, V v) {
-    *reinterpret_cast<V*>((char*)base + bytes) = v;
-}
-
 // Fragments in memory: [fragment][plane][lane][8].
 template <int NP>
 __device__ __forceinline__ void store_frag(bf16_t* base, int fragment, const Frag<NP>& f, int lane) {
@@ -451,6 +529,20 @@ __device__ __forceinline__ Frag<NP> load_frag(const bf16_t* base, int fragment, 
 #pragma unroll
     for (int p = 0; p < NP; ++p) f.p[p] = load_at<bf16x8>(base + (fragment * NP + p) * 512, lane * 16);
     return f;
+}
+// A tile of what lies as fragments with lane = column of v and values = rows (states, U), with lane = row and values = columns: rows of tile `t` of 16,
+// two tiles of columns, whose fragments are `stride` apart.
+template <int NP>
+__device__ __forceinline__ Frag<NP> load_turned(const bf16_t* base, int fragment, int stride, int half, bf16x4 unit, int lane) {
+    Half<NP> a, b;
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        a.p[p] = load_at<bf16x4>(base + (fragment * NP + p) * 512 + 4 * half, lane * 16);
+        b.p[p] = load_at<bf16x4>(base + ((fragment + stride) * NP + p) * 512 + 4 * half, lane * 16);
+    }
+#pragma unroll
+    for (int p = 0; p < NP; ++p) a.p[p] = turned(a.p[p], unit), b.p[p] = turned(b.p[p], unit);
+    return join(a, b);
 }
 // one of the two tiles of a fragment
 template <int NP>
@@ -483,11 +575,11 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // Sizes of what lies between the kernels, in elements of a chunk; of a segment's map.
 struct DeltaSizes {
-    long long rows, frag_chain, frag_raw, state, u, cols, c0, map, shift;
+    long long rows, frag_chain, frag_raw, state, u, cols, c0, map, shift, blocks;
     __host__ __device__ DeltaSizes(int DK, int dvp, int raw, int made, int chain)
         : rows(kDeltaChunk * (long long)DK), frag_chain(rows * chain), frag_raw(rows * raw), state((long long)DK * dvp * made),
           u((long long)kDeltaChunk * dvp * made), cols((long long)kDeltaChunk * dvp), c0((long long)DK * dvp), map((long long)DK * DK * chain),
-          shift((long long)DK * dvp) {}
+          shift((long long)DK * dvp), blocks(10 * made * 256) {}
 };
 
 }  // namespace pdw

@@ -29,13 +29,13 @@ __device__ __forceinline__ void make_blocks(bf16_t* blocks, float* tile, const b
         if (FORE ? t > wave : t < wave) continue;
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < DK; n += 32) acc = mma(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
+        for (int n = 0; n < DK; n += 32) acc = mma<MADE>(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
         // FORE: lane = row i of the wavefront's block row, values = columns j of block t; else lane = column j, values = rows i
+        const TileDecay decay(s, 16 * wave + col, 16 * t + g4, FORE);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int mine = 16 * wave + col, other = 16 * t + g4 + r;
-            const int i = FORE ? mine : other, j = FORE ? other : mine;
-            acc[r] = j < i ? s.beta[i] * decay_between(s, i, j) * acc[r] : 0.f;
+            const bool below = t != wave || (FORE ? g4 + r < col : col < g4 + r);
+            acc[r] = below ? decay.beta[r] * decay.G[r] * acc[r] : 0.f;
         }
         if (t == wave) {
             // [column][row] (FORE), [row][column]: the lane's index is the inner one
@@ -53,10 +53,16 @@ template <int RAW, int DK>
 constexpr int delta_rows_bytes() {
     return Rows<RAW, kDeltaChunk, DK>::kValues * 2;
 }
+// Columns of v that a workgroup has in LDS at a time.
+template <typename T, int DK>
+constexpr int delta_prepare_cols() {
+    return DK == 32 ? 32 : 64;
+}
 template <typename T, int DK>
 constexpr int delta_prepare_lds() {
     typedef DeltaPlanes<T> P;
-    return delta_rows_bytes<P::kRaw, DK>() + Blocks<kChainPlanes>::kValues * 2 + 4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
+    return delta_rows_bytes<P::kRaw, DK>() + delta_rows_bytes<P::kRaw, delta_prepare_cols<T, DK>()>() + Blocks<kChainPlanes>::kValues * 2 +
+           4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
 }
 
 template <typename T, int DK>
@@ -65,19 +71,25 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
-    bf16_t* k = (bf16_t*)lds;
-    bf16_t* blocks = k + L::kValues;
+    constexpr int COLS = delta_prepare_cols<T, DK>();
+    typedef Rows<RAW, kDeltaChunk, COLS> LV;
+    bf16_t *k = (bf16_t*)lds, *vl = k + L::kValues, *blocks = vl + LV::kValues;
     float* tiles = (float*)(blocks + Blocks<MADE>::kValues);
     DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g4 = 4 * (lane >> 4);
-    const long long id = p.first + blockIdx.x;
-    const int chain = (int)(id / p.NC);
-    const long long first = (id - chain * p.NC) * kDeltaChunk;
+    const int g4 = 4 * (lane >> 4);
+    int chain;
+    long long m;
+    if (!chunk_of(p, p.Hv, chain, m)) return;
+    const long long id = chain * p.NC + m, first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
 
+    Staged<T, RAW, DK> ks;
+    Staged<T, RAW, COLS> vs;
+    ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+    vs.load((const T*)p.v + c.at(p.vs, c.hv), p.vs.t, p, c, first, 0, p.dv, p.vec & kVecV);
     make_gates(s, p.gates + id, p, c, first, type);
-    stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+    ks.put(k), vs.put(vl);
     __syncthreads();
     float* tile = tiles + wave * 16 * 20;
     make_blocks<RAW, MADE, DK, true>(blocks, tile, k, s, wave, lane);
@@ -87,96 +99,98 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
 
     const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
     const bf16x4 unit = unit_half(lane);
-    const int colv = p.dvp / 16;
-    for (int ct = wave; ct < DK / 16 + colv; ct += 4) {
-        f32x4 x[4];
-        if (ct < DK / 16) {
-            Half<RAW> kr[4];
+    f32x4 beta[4], decay[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                kr[b] = L::down(k, 16 * b, 16 * ct, lane);
-                x[b] = sum_of(kr[b]);
+    for (int b = 0; b < 4; ++b) {
+        beta[b] = *reinterpret_cast<const f32x4*>(s.beta + 16 * b + g4);
+        decay[b] = beta[b] * *reinterpret_cast<const f32x4*>(s.D + 16 * b + g4);
+    }
+    // columns of W, and with them the first ones of Ub; then the others of Ub
+    for (int at = 0; at < p.dvp; at += COLS) {
+        if (at) {
+            vs.load((const T*)p.v + c.at(p.vs, c.hv), p.vs.t, p, c, first, at, p.dv, p.vec & kVecV);
+            __syncthreads();
+            vs.put(vl);
+            __syncthreads();
+        }
+        const int end = (p.dvp - at < COLS ? p.dvp - at : COLS) / 16;
+        for (int ct = (at ? DK / 16 : 0) + wave; ct < DK / 16 + end; ct += 4) {
+            f32x4 x[4];
+            if (ct < DK / 16) {
+                Half<RAW> kr[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[b][r] *= s.beta[16 * b + g4 + r] * s.D[16 * b + g4 + r];
-            }
-            store_frag(p.kt + id * z.frag_raw, 2 * ct, join(kr[0], kr[1]), lane);
-            store_frag(p.kt + id * z.frag_raw, 2 * ct + 1, join(kr[2], kr[3]), lane);
-            solve_fore<MADE>(blocks, x, lane);
-            // -W, lane = step: the first operand of the chain's first product
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                Half<MADE> h = split<MADE>(-x[b]);
-#pragma unroll
-                for (int n = 0; n < MADE; ++n) h.p[n] = turned(h.p[n], unit);
-                store_half(p.wp + id * z.frag_chain, b * (DK / 32) + ct / 2, ct & 1, h, lane);
-            }
-        } else {
-            const int cv = ct - DK / 16, at = 16 * cv + col;
-            const T* v = (const T*)p.v + c.at(p.vs, c.hv) + at;
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = 16 * b + g4 + r;
-                    const long long i = first + row;
-                    x[b][r] = i < c.len && at < p.dv ? s.beta[row] * to_f32(v[c.step(p, i) * p.vs.t]) : 0.f;
+                for (int b = 0; b < 4; ++b) {
+                    kr[b] = L::down(k, 16 * b, 16 * ct, lane);
+                    x[b] = sum_of(kr[b]) * decay[b];
                 }
-            solve_fore<MADE>(blocks, x, lane);
-            float* ub = p.ub + id * z.cols + cv * 1024;
+                store_frag(p.kt + id * z.frag_raw, 2 * ct, join(kr[0], kr[1]), lane);
+                store_frag(p.kt + id * z.frag_raw, 2 * ct + 1, join(kr[2], kr[3]), lane);
+                solve_fore<MADE>(blocks, x, lane);
+                // -W, lane = step: the first operand of the chain's first product
 #pragma unroll
-            for (int b = 0; b < 4; ++b) store_at(ub + b * 256, lane * 16, x[b]);
+                for (int b = 0; b < 4; ++b) {
+                    Half<MADE> h = split<MADE>(-x[b]);
+#pragma unroll
+                    for (int n = 0; n < MADE; ++n) h.p[n] = turned(h.p[n], unit);
+                    store_half(p.wp + id * z.frag_chain, b * (DK / 32) + ct / 2, ct & 1, h, lane);
+                }
+            } else {
+                const int cv = ct - DK / 16;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) x[b] = sum_of(LV::down(vl, 16 * b, 16 * cv, lane)) * beta[b];
+                solve_fore<MADE>(blocks, x, lane);
+                float* ub = p.ub + id * z.cols + (at / 16 + cv) * 1024;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) store_at(ub + b * 256, lane * 16, x[b]);
+            }
         }
     }
 }
 
-constexpr int kDeltaCols = 64;   // columns of v that a workgroup of delta_out_k and delta_grads_k has in LDS
-
 template <typename T, int DK>
 constexpr int delta_out_lds() {
-    typedef DeltaPlanes<T> P;
-    const int in = 2 * delta_rows_bytes<P::kRaw, DK>();
-    const int made = (Rows<P::kMade, DK, kDeltaCols>::kValues + Rows<P::kMade, kDeltaChunk, kDeltaCols>::kValues) * 2;
-    return (in > made ? in : made) + (int)sizeof(DeltaGates);
+    return 2 * delta_rows_bytes<DeltaPlanes<T>::kRaw, DK>() + (int)sizeof(DeltaGates);
 }
 
 template <typename T, int DK>
 __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
-    constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     typedef Rows<RAW, kDeltaChunk, DK> L;
-    typedef Rows<MADE, DK, kDeltaCols> LS;
-    typedef Rows<MADE, kDeltaChunk, kDeltaCols> LU;
     extern __shared__ __align__(16) unsigned char lds[];
     DeltaGates& s = *(DeltaGates*)lds;
     bf16_t *k = (bf16_t*)(lds + sizeof(DeltaGates)), *q = k + L::kValues;
-    bf16_t *s0 = k, *u = s0 + LS::kValues;   // (behind the products with K and Q)
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = 4 * (lane >> 4);
-    const long long id = p.first + blockIdx.x;
-    const int chain = (int)(id / p.NC);
-    const long long first = (id - chain * p.NC) * kDeltaChunk;
+    int chain;
+    long long m;
+    if (!chunk_of(p, p.Hv, chain, m)) return;
+    const long long id = chain * p.NC + m, first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
 
-    load_gates(s, p.gates + id);
-    stage_rows<T, RAW, DK>(k, (const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
-    stage_rows<T, RAW, DK>(q, (const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+    Run<sizeof(DeltaGates)> gates;
+    Staged<T, RAW, DK> ks, qs;
+    ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+    qs.load((const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+    gates.load(p.gates + id);
+    ks.put(k), qs.put(q), gates.put(&s);
     __syncthreads();
     // the wavefront's 16 steps i: scale G_ij q_i.k_j, lane = i, values = j; and its rows of Q
     const int i = 16 * wave + col;
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     Half<MADE> pr[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-        if (t > wave) continue;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        f32x4 acc = zero;
+        if (t <= wave) {
 #pragma unroll
-        for (int n = 0; n < DK; n += 32) acc = mma(L::natural(k, 16 * t, n, lane), L::natural(q, 16 * wave, n, lane), acc);
+            for (int n = 0; n < DK; n += 32) acc = mma(L::natural(k, 16 * t, n, lane), L::natural(q, 16 * wave, n, lane), acc);
+            const TileDecay decay(s, i, 16 * t + g4, true);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int j = 16 * t + g4 + r;
-            acc[r] = j <= i ? p.scale * decay_between(s, i, j) * acc[r] : 0.f;
+            for (int r = 0; r < 4; ++r) acc[r] = t != wave || g4 + r <= col ? p.scale * decay.G[r] * acc[r] : 0.f;
         }
         pr[t] = split<MADE>(acc);
     }
+    const Frag<MADE> pf[2] = {join(pr[0], pr[1]), join(pr[2], pr[3])};
     Frag<RAW> qf[DK / 32];
 #pragma unroll
     for (int n = 0; n < DK / 32; ++n) qf[n] = L::tiles(q, 16 * wave, 32 * n, lane);
@@ -185,25 +199,16 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const bool there = step < c.len;
     T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
     const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
-    for (int at = 0; at < p.dv; at += kDeltaCols) {
-        __syncthreads();
-        stage_planes<MADE, DK, kDeltaCols>(s0, p.s0 + id * z.state, p.dvp, at);
-        stage_planes<MADE, kDeltaChunk, kDeltaCols>(u, p.u + id * z.u, p.dvp, at);
-        __syncthreads();
+    const bf16_t *s0 = p.s0 + id * z.state, *u = p.u + id * z.u;
+    // (states and U lie with lane = column of v, values = rows: first operands of the transposed products as they are)
+    for (int cv = 0; cv < p.dvp / 16; ++cv) {
+        f32x4 acc = zero;
 #pragma unroll
-        for (int cv = 0; cv < kDeltaCols; cv += 16) {
-            if (at + cv >= p.dvp) break;
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int n = 0; n < DK / 32; ++n)
-                acc = mma(join(LS::down(s0, 32 * n, cv, lane), LS::down(s0, 32 * n + 16, cv, lane)), qf[n], acc);
-            acc *= D;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (t <= wave) acc = mma(LU::down(u, 16 * t, cv, lane), pr[t], acc);
-            if (!there) acc = f32x4{0.f, 0.f, 0.f, 0.f};
-            if (step < p.T) store_four(row, at + cv + g4, p.dv, acc, p.vec & kVecY);
-        }
+        for (int n = 0; n < DK / 32; ++n) acc = mma(load_frag<MADE>(s0, cv * (DK / 32) + n, lane), qf[n], acc);
+        acc *= D;
+        acc = mma(load_frag<MADE>(u, cv * 2, lane), pf[0], acc);
+        if (wave >= 2) acc = mma(load_frag<MADE>(u, cv * 2 + 1, lane), pf[1], acc);
+        if (step < p.T) store_four(row, 16 * cv + g4, p.dv, there ? acc : zero, p.vec & kVecY);
     }
 }
 

@@ -16,6 +16,8 @@ inline void delta_launch(K kernel, int lds, std::once_flag& once, long long grid
     });
 }
 
+inline long long delta_chunk_grid(const DeltaArgs& p, int H) { return ((long long)p.O * p.W * p.NC + 7) / 8 * 8 * H; }
+
 template <typename T, int DK, bool BACK, int CP, bool MAPS>
 void delta_chains(const DeltaArgs& p, hipStream_t s) {
     static std::once_flag once;
@@ -24,24 +26,32 @@ void delta_chains(const DeltaArgs& p, hipStream_t s) {
     delta_launch(delta_chain_k<T, DK, BACK, CP, MAPS>, delta_chain_lds<T, DK, BACK, CP>(), once, grid, 128 * waves, p, s);
 }
 
+template <typename T, int DK, bool BACK, int CP>
+void delta_all_chains(const DeltaArgs& p, hipStream_t s) {
+    if (p.segments > 1) {
+        std::once_flag none;
+        delta_chains<T, DK, BACK, CP, true>(p, s);
+        delta_launch(delta_join_k<T, DK, BACK, CP>, 0, none, (long long)p.chains * (p.dvp / 16), DK * 4, p, s);
+    }
+    delta_chains<T, DK, BACK, CP, false>(p, s);
+}
+
 template <typename T, int DK>
 void delta_forward(const DeltaArgs& p, hipStream_t s) {
     static std::once_flag once[2];
-    const long long chunks = p.chains * p.NC;
+    const long long chunks = delta_chunk_grid(p, p.Hv);
     delta_launch(delta_prepare_k<T, DK>, delta_prepare_lds<T, DK>(), once[0], chunks, 256, p, s);
-    if (p.segments > 1) delta_chains<T, DK, false, kChainPlanes, true>(p, s);
-    delta_chains<T, DK, false, kChainPlanes, false>(p, s);
+    delta_all_chains<T, DK, false, kChainPlanes>(p, s);
     delta_launch(delta_out_k<T, DK>, delta_out_lds<T, DK>(), once[1], chunks, 256, p, s);
 }
 
 template <typename T, int DK, int CP>
 void delta_backward(const DeltaArgs& p, hipStream_t s) {
     static std::once_flag once[3];
-    const long long chunks = p.chains * p.NC;
+    const long long chunks = delta_chunk_grid(p, p.Hv);
     delta_launch(delta_back_prepare_k<T, DK, CP>, delta_back_prepare_lds<T, DK, CP>(), once[0], chunks, 256, p, s);
-    if (p.segments > 1) delta_chains<T, DK, true, CP, true>(p, s);
-    delta_chains<T, DK, true, CP, false>(p, s);
-    if (p.Hv > p.Hk) delta_launch(delta_grads_k<T, DK, true>, delta_grads_lds<T, DK>(), once[1], chunks / p.Hv * p.Hk, 256, p, s);
+    delta_all_chains<T, DK, true, CP>(p, s);
+    if (p.Hv > p.Hk) delta_launch(delta_grads_k<T, DK, true>, delta_grads_lds<T, DK>(), once[1], delta_chunk_grid(p, p.Hk), 256, p, s);
     else delta_launch(delta_grads_k<T, DK, false>, delta_grads_lds<T, DK>(), once[2], chunks, 256, p, s);
 }
 
