@@ -30,8 +30,7 @@ struct DeltaPlan {
     long long NC, seg;
     int segments, dvp;
     DeltaPlan(long long chains, long long T, int dk, int dv, bool backward, bool state_gradient, int dtype)
-        : z(padded_dk(dk), padded_dv(dv), dtype == kF32 ? 3 : dtype == kF16 ? 2 : 1, dtype == kF32 ? 3 : 2,
-            dtype == kF32 || !backward || state_gradient ? kChainPlanes : 2),
+        : z(padded_dk(dk), padded_dv(dv), dtype == kF32 ? 3 : 2, dtype == kF32 || !backward || state_gradient ? kChainPlanes : 2),
           NC(delta_chunks(T)), seg(segment_chunks(chains, NC, padded_dk(dk), padded_dv(dv))),
           segments(NC ? (int)((NC + seg - 1) / seg) : 1), dvp(padded_dv(dv)) {}
 };
@@ -42,33 +41,44 @@ bool delta_few_steps(long long T) { return T <= kDeltaFewSteps; }
 
 static size_t whole(size_t n) { return (n + 255) / 256 * 256; }
 
-static size_t states_bytes(long long chains, const DeltaPlan& d) {
-    const size_t n = (size_t)(chains * d.NC);
-    return whole(n * d.z.state * 2) + whole(n * d.z.u * 2) + n * sizeof(DeltaGates);
+// What a forward keeps for its backward, and a forward without one has in its workspace (but for A's blocks), one after another: f(bytes) -> the
+// address of each.
+template <typename F>
+static void delta_kept(DeltaArgs& p, const DeltaPlan& d, bool blocks, F f) {
+    const size_t n = (size_t)(p.chains * d.NC);
+    auto take = [&](auto*& ptr, size_t bytes) { ptr = (std::remove_reference_t<decltype(ptr)>)f(whole(bytes)); };
+    take(p.s0, n * d.z.state * 2);
+    take(p.u, n * d.z.u * 2);
+    take(p.gates, n * sizeof(DeltaGates));
+    take(p.w, n * d.z.w * 4);
+    if (blocks) take(p.blocks, n * d.z.blocks * 2);
 }
-
-size_t delta_states_bytes(long long chains, long long T, int dk, int dv, int dtype) {
-    return states_bytes(chains, DeltaPlan(chains, T, dk, dv, false, false, dtype));
-}
-
-// The buffers of one call one after another: f(bytes) -> the address of each.
+// What else a call has between its launches.
 template <typename F>
 static void delta_buffers(DeltaArgs& p, const DeltaPlan& d, bool backward, F f) {
     const size_t n = (size_t)(p.chains * d.NC), maps = (size_t)p.chains * (d.segments - 1);
     auto take = [&](auto*& ptr, size_t bytes) { ptr = (std::remove_reference_t<decltype(ptr)>)f(whole(bytes)); };
-    take(p.wp, n * d.z.frag_chain * 2);
     take(p.maps, maps * d.z.map * 2);
     take(p.shifts, maps * d.z.shift * 4);
     if (!backward) {
-        take(p.kt, n * d.z.frag_raw * 2);
         take(p.ub, n * d.z.cols * 4);
     } else {
-        take(p.ka, n * d.z.frag_raw * 2);
         take(p.ds1, n * d.z.state * 2);
-        take(p.blocks, n * d.z.blocks * 2);
         take(p.du, n * d.z.cols * 4);
         take(p.c0, n * d.z.c0 * 4);
     }
+}
+
+static size_t states_bytes(long long chains, const DeltaPlan& d, bool blocks) {
+    DeltaArgs p{};
+    p.chains = (int)chains;
+    size_t total = 0;
+    delta_kept(p, d, blocks, [&](size_t bytes) { return total += bytes, (char*)nullptr; });
+    return total;
+}
+
+size_t delta_states_bytes(long long chains, long long T, int dk, int dv, int dtype) {
+    return states_bytes(chains, DeltaPlan(chains, T, dk, dv, false, false, dtype), true);
 }
 
 static size_t workspace_bytes_of(long long chains, const DeltaPlan& d, bool backward, bool states) {
@@ -76,7 +86,7 @@ static size_t workspace_bytes_of(long long chains, const DeltaPlan& d, bool back
     p.chains = (int)chains;
     size_t total = 0;
     delta_buffers(p, d, backward, [&](size_t bytes) { return total += bytes, (char*)nullptr; });
-    return total + (backward || states ? 0 : states_bytes(chains, d));
+    return total + (backward || states ? 0 : states_bytes(chains, d, false));
 }
 
 // (the most that a backward takes: with the gradient of a state)
@@ -114,10 +124,9 @@ int delta_run(const DeltaArgs& in, void* states, bool backward, void* workspace,
     }
     char* at = (char*)workspace;
     delta_buffers(p, d, backward, [&](size_t bytes) { return at += bytes, at - bytes; });
-    if (!states) states = at;
-    p.s0 = (bf16_t*)states;
-    p.u = (bf16_t*)((char*)states + whole((size_t)(p.chains * p.NC) * d.z.state * 2));
-    p.gates = (DeltaGates*)((char*)p.u + whole((size_t)(p.chains * p.NC) * d.z.u * 2));
+    const bool blocks = states != nullptr;
+    if (states) at = (char*)states;
+    delta_kept(p, d, blocks, [&](size_t bytes) { return at += bytes, at - bytes; });
     const int es = dtype == kF32 ? 4 : 2;
     p.vec = (pieces(p.q, p.qs, p.dk, es) ? kVecQ : 0) | (pieces(p.k, p.ks, p.dk, es) ? kVecK : 0) | (pieces(p.v, p.vs, p.dv, es) ? kVecV : 0) |
             (pieces(p.gy, p.ys, p.dv, es) ? kVecGy : 0) | (pieces(p.y, p.ys, p.dv, es) ? kVecY : 0) |

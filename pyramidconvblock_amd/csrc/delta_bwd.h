@@ -9,9 +9,9 @@
 //   dc_i = sum_j N_ij - sum_j N_ji + scale D_i q_i.(dY S0^T)_i - D_i beta_i k_i.(Z S0^T)_i - x_i,   N = dP o P + dA o A,  x_i = E_i k_i.(U dS1^T)_i
 //   dc_end += sum_i x_i + e^c_end <S0, dS1>,          d(log a)_t = sum of dc_i over i >= t within the chunk
 //
-// Three launches again.  delta_back_prepare_k, a workgroup a chunk: W, dU without dS1's part, and C = scale Q^T D dY - W^T dU of that.
-// delta_back_chain_k, from the last chunk to the first: dS0 = e^c_end dS1 + C - W^T (E K dS1), the forward's chain with the operands' parts
-// exchanged; it leaves the dS1 of every chunk and completes dU.  delta_grads_k, a workgroup a chunk and key head: all gradients; value heads that
+// Three launches and more again; W and A's blocks are kept from the forward.  delta_back_prepare_k, a workgroup a chunk: dU without dS1's part, and
+// C = scale Q^T D dY - W^T dU of that.  delta_chain.h, from the last chunk to the first: dS0 = e^c_end dS1 + C - W^T (E K dS1), the forward's chain with
+// the operands' parts exchanged; it leaves the dS1 of every chunk.  delta_grads_k, a workgroup a chunk and key head: all gradients; value heads that
 // share a key head one after another, their dQ and dK summed in registers, in one order.
 #pragma once
 #include "delta_fwd.h"
@@ -37,128 +37,77 @@ __device__ __forceinline__ Half<NP> half_of(const T (&v)[4]) {
     return h;
 }
 
-template <int MADE, int DK>
-constexpr int delta_wt_values() {
-    return DK / 16 * 2 * MADE * 64 * 8;
-}
-template <typename T, int DK, int MADE>
-constexpr int delta_back_prepare_k_values() {   // K, and later W^T in its place
-    constexpr int RAW = DeltaPlanes<T>::kRaw;
-    return Rows<RAW, kDeltaChunk, DK>::kValues > delta_wt_values<MADE, DK>() ? Rows<RAW, kDeltaChunk, DK>::kValues : delta_wt_values<MADE, DK>();
-}
 template <typename T, int DK, int MADE>
 constexpr int delta_back_prepare_lds() {
-    return delta_rows_bytes<DeltaPlanes<T>::kRaw, DK>() + delta_back_prepare_k_values<T, DK, MADE>() * 2 + 2 * Blocks<MADE>::kValues * 2 +
-           4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
+    return 2 * delta_rows_bytes<DeltaPlanes<T>::kRaw, DK>() + Blocks<MADE>::kValues * 2 + (int)sizeof(DeltaGates);
 }
 
 // MADE: planes of what the chain's operands are made of: kChainPlanes where the gradient of a state is wanted.
 template <typename T, int DK, int MADE>
-__global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
+__global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
-    bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *wl = k;
-    bf16_t *blocks = k + delta_back_prepare_k_values<T, DK, MADE>(), *pb = blocks + Blocks<MADE>::kValues;
-    float* tiles = (float*)(pb + Blocks<MADE>::kValues);
-    DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g4 = 4 * (lane >> 4);
+    bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *pb = k + L::kValues;
+    DeltaGates& s = *(DeltaGates*)(pb + Blocks<MADE>::kValues);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int chain;
     long long m;
     if (!chunk_of(p, p.Hv, chain, m)) return;
     const long long id = chain * p.NC + m, first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
-    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
+    const DeltaSizes z(DK, p.dvp, DeltaPlanes<T>::kMade, MADE);
 
-    Run<sizeof(DeltaGates)> gates;
-    Staged<T, RAW, DK> ks, qs;
-    ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
-    qs.load((const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
-    gates.load(p.gates + id);
-    ks.put(k), qs.put(q), gates.put(&s);
-    __syncthreads();
-    float* tile = tiles + wave * 16 * 20;
-    make_blocks<RAW, MADE, DK, true>(blocks, tile, k, s, wave, lane);
-    Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, wave), split<MADE>(invert_block<true>(tile, lane)), lane);
-    // P's column of blocks: lane = j, values = i
+    {
+        const int lane = threadIdx.x & 63, col = lane & 15, g4 = 4 * (lane >> 4);
+        Run<sizeof(DeltaGates)> gates;
+        Staged<T, RAW, DK> ks, qs;
+        gates.load(p.gates + id);
+        ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
+        qs.load((const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+        gates.put(&s), ks.put(k), qs.put(q);
+        __syncthreads();
+        // P's column of blocks: lane = j, values = i
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        if (t < wave) continue;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 4; ++t) {
+            if (t < wave) continue;
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < DK; n += 32) acc = mma<MADE>(L::natural(q, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
-        const TileDecay decay(s, 16 * wave + col, 16 * t + g4, false);
+            for (int n = 0; n < DK; n += 32) acc = mma<MADE>(L::natural(q, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
+            const TileDecay decay(s, 16 * wave + col, 16 * t + g4, false);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[r] = t != wave || col <= g4 + r ? p.scale * decay.G[r] * acc[r] : 0.f;
-        Blocks<MADE>::put(pb, Blocks<MADE>::at(t, wave), split<MADE>(acc), lane);
-    }
-    // K as the chain's first operand
-#pragma unroll
-    for (int n = 0; n < DK / 32; ++n) store_frag(p.ka + id * z.frag_raw, wave * (DK / 32) + n, L::tiles(k, 16 * wave, 32 * n, lane), lane);
-    __syncthreads();
-    // the blocks for the transposed system, of the planes that delta_grads_k takes
-    const bf16x4 unit = unit_half(lane);
-    constexpr int NG = DeltaPlanes<T>::kMade;
-    for (int n = wave; n < 10; n += 4) {
-        const Half<MADE> h = Blocks<MADE>::get(blocks, n, lane);
-        Half<NG> t;
-#pragma unroll
-        for (int m = 0; m < NG; ++m) t.p[m] = turned(h.p[m], unit);
-        Blocks<NG>::put(p.blocks + id * 10 * NG * 256, n, t, lane);
-    }
-    // -W^T: lane = channel of k, values = steps
-    constexpr int NT = DK / 16 < 4 ? 1 : DK / 64;
-    Frag<MADE> wt[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int ct = wave + 4 * n;
-        if (ct >= DK / 16) continue;
-        f32x4 x[4];
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            x[b] = sum_of(L::down(k, 16 * b, 16 * ct, lane));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) x[b][r] *= s.beta[16 * b + g4 + r] * s.D[16 * b + g4 + r];
+            for (int r = 0; r < 4; ++r) acc[r] = t != wave || col <= g4 + r ? p.scale * decay.G[r] * acc[r] : 0.f;
+            Blocks<MADE>::put(pb, Blocks<MADE>::at(t, wave), split<MADE>(acc), lane);
         }
-        solve_fore<MADE>(blocks, x, lane);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            wt[n][h] = join(split<MADE>(-x[2 * h]), split<MADE>(-x[2 * h + 1]));
-            store_frag(p.wp + id * z.frag_chain, 2 * ct + h, wt[n][h], lane);
-        }
+        __syncthreads();
     }
-    __syncthreads();
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int ct = wave + 4 * n;
-        if (ct >= DK / 16) continue;
-        store_frag(wl, 2 * ct, wt[n][0], lane);
-        store_frag(wl, 2 * ct + 1, wt[n][1], lane);
-    }
-    __syncthreads();
-    const int lane0 = lane;
-    for (int cv = wave; cv < p.dvp / 16; cv += 4) {
-        // (another lane with every turn, for all that the compiler knows: else it reads all of Q^T and W^T ahead of the loop, into registers that
-        // there are not)
-        int lane = lane0;
+    // columns of v: dU without dS1's part, and C; DK = 32: two wavefronts share a tile of columns where there are few, each half of C's rows
+    const int share = p.dvp <= 32 ? 2 : 1;
+    for (int cw = wave; cw < p.dvp / 16 * share; cw += 4) {
+        // (another lane with every turn, for all that the compiler knows: else it reads all of Q^T ahead of the loop, into registers that there are not)
+        int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
-        const int col = lane & 15, g4 = 4 * (lane >> 4), at = 16 * cv + col;
+        const int cv = cw / share, part = cw % share, col = lane & 15, g4 = 4 * (lane >> 4), at = 16 * cv + col;
         const T* gy = (const T*)p.gy + c.at(p.ys, c.hv) + at;
         Half<RAW> dr[4];
         Half<MADE> ds[4];
+        T v[4][4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            T v[4];
-            f32x4 f;
+        for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int row = 16 * b + g4 + r;
-                const long long i = first + row;
-                v[r] = i < c.len && at < p.dv ? gy[c.step(p, i) * p.ys.t] : from_f32<T>(0.f);
-                f[r] = p.scale * s.D[row] * to_f32(v[r]);
+                const long long i = first + 16 * b + g4 + r;
+                const bool on = i < c.len && at < p.dv;
+                v[b][r] = gy[on ? c.step(p, i) * p.ys.t : -(long long)at];   // (what is not there is read from the first row and dropped)
+                if (!on) v[b][r] = from_f32<T>(0.f);
             }
-            dr[b] = half_of<T, RAW>(v), ds[b] = split<MADE>(f);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const f32x4 D = *reinterpret_cast<const f32x4*>(s.D + 16 * b + g4);
+            f32x4 f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) f[r] = p.scale * D[r] * to_f32(v[b][r]);
+            dr[b] = half_of<T, RAW>(v[b]), ds[b] = split<MADE>(f);
         }
         Half<MADE> us[4];
         float* du = p.du + id * z.cols + cv * 1024;
@@ -167,19 +116,22 @@ __global__ __launch_bounds__(256) void delta_back_prepare_k(DeltaArgs p) {
             f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = b; t < 4; ++t) acc = mma(Blocks<MADE>::get(pb, Blocks<MADE>::at(t, b), lane), dr[t], acc);
-            store_at(du + b * 256, lane * 16, acc);
+            if (part == 0) store_at(du + b * 256, lane * 16, acc);
             us[b] = split<MADE>(acc);
         }
         const Frag<MADE> d0 = join(ds[0], ds[1]), d1 = join(ds[2], ds[3]), u0 = join(us[0], us[1]), u1 = join(us[2], us[3]);
         float* c0 = p.c0 + id * z.c0 + cv * (DK * 16);
+        for (int d = part; d < DK / 16; d += share) {
+            const float* w = p.w + id * z.w + d * 1024;   // -W, lane = channel of k, values = steps
+            f32x4 wt[4];
 #pragma unroll
-        for (int d = 0; d < DK / 16; ++d) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            for (int b = 0; b < 4; ++b) wt[b] = load_at<f32x4>(w + b * 256, lane * 16);
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f}, add = acc;
             acc = mma(join(L::down(q, 0, 16 * d, lane), L::down(q, 16, 16 * d, lane)), d0, acc);
             acc = mma(join(L::down(q, 32, 16 * d, lane), L::down(q, 48, 16 * d, lane)), d1, acc);
-            acc = mma(load_frag<MADE>(wl, 2 * d, lane), u0, acc);
-            acc = mma(load_frag<MADE>(wl, 2 * d + 1, lane), u1, acc);
-            store_at(c0 + d * 256, lane * 16, acc);
+            add = mma(join(split<MADE>(wt[0]), split<MADE>(wt[1])), u0, add);
+            add = mma(join(split<MADE>(wt[2]), split<MADE>(wt[3])), u1, add);
+            store_at(c0 + d * 256, lane * 16, acc + add);
         }
     }
 }
@@ -245,7 +197,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delt
     const int group = SHARED ? p.Hv / p.Hk : 1;
     const long long first = m * kDeltaChunk;
     const int chain0 = SHARED ? kchain / p.Hk * p.Hv + kchain % p.Hk * group : kchain;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
+    const DeltaSizes z(DK, p.dvp, MADE, MADE);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
     const DeltaChain ck(p, chain0);
@@ -288,10 +240,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delt
             Staged<T, RAW, COLS> gs;
             gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
             f32x4 x[4];
+            Frag<MADE> xs[DK / 32];
             if (mine) {
                 const float* du = p.du + id * z.cols + cv * 1024;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(du + b * 256, lane * 16);
+#pragma unroll
+                for (int d = 0; d < DK / 32; ++d) xs[d] = load_frag<MADE>(ds1, cv * (DK / 32) + d, lane);
             }
             if (e || at) __syncthreads();
             if (at == 0) {
@@ -302,6 +257,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delt
             __syncthreads();
             beta = s.beta[me];
             if (mine) {
+                // dU = that without dS1's part, and E K dS1
+                f32x4 y[4] = {zero, zero, zero, zero};
+#pragma unroll
+                for (int d = 0; d < DK / 32; ++d) {
+                    Frag<RAW> a[4];
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) a[b] = L::tiles(k, 16 * b, 32 * d, lane);
+                    mma_rows(a, xs[d], y);
+                }
+#pragma unroll
+                for (int b = 0; b < 4; ++b) x[b] += y[b] * *reinterpret_cast<const f32x4*>(s.E + 16 * b + g4);
                 solve_back<MADE>(blocks, x, lane);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) LZ::put_turned(zl, 16 * b, 16 * wave, split<MADE>(x[b]), unit, lane);

@@ -1,12 +1,11 @@
 // The gated delta rule's chains, forward and backward: the only part with an order in time.  A state's columns X pass through the chunks,
 //
-//   forward    U = Ub - W X,          leaves X (the state before the chunk) and U,       X' = e^c_end X + K^T E U
-//   backward   Y = E K X, dU += Y,    leaves X (the gradient of the state behind it),    X' = e^c_end X + C - W^T Y       (from the last chunk)
+//   forward    U = Ub - W X,    leaves X (the state before the chunk) and U,      X' = e^c_end X + K^T E U
+//   backward   Y = E K X,       leaves X (the gradient of the state behind it),   X' = e^c_end X + C - W^T Y       (from the last chunk)
 //
-// two products a chunk: A X, and B of the first one's result.  A wavefront carries 16 columns in registers; results of one product are
-// operands of the next as they are.  A and B come as fragments from memory and are the same for all columns of a chain, so other wavefronts of
-// the workgroup fetch them, several chunks ahead in registers, and put them into LDS: A's place is filled while B is in use and the other way round, two
-// barriers a chunk.  What bounds it: latencies, of the products and of the exchange between the wavefronts, one chunk after another.
+// two products a chunk, with W (from memory in fp32: fewer bytes than its planes) and K (from the tensor).  A wavefront carries 16 columns in registers;
+// results of one product are operands of the next as they are.  W and K are the same for all columns of a chain, so other wavefronts of the workgroup
+// fetch them, several chunks ahead in registers, and put them into LDS: one's place is filled while the other is in use, two barriers a chunk.  What bounds it: latencies, of the products and of the exchange between the wavefronts, one chunk after another.
 //
 // Where there are too few chains to fill the chip, the chunks are cut into segments.  Through a segment X goes to M X + N, and the same kernel
 // (MAPS) finds both: N from X = 0, and M as what becomes of the unit matrix' columns without what the chunks add.  delta_join_k takes the states
@@ -38,15 +37,10 @@ __device__ __forceinline__ void store_state(float* s, const f32x4 (&x)[DK / 16],
             if (row < dk && at < dv) s[row * (long long)dv + at] = x[d][r];
         }
 }
-template <typename T, bool BACK, int CP>
-struct ChainPlanes {
-    static constexpr int kRaw = DeltaPlanes<T>::kRaw;
-    static constexpr int kA = BACK ? kRaw : CP, kB = BACK ? CP : kRaw;   // planes of A and of B
-};
-template <typename T, int DK, bool BACK, int CP>
+// W's planes as its tiles come (lane = channel of k, values = steps), [plane][tile of channels][tile of steps][lane][4], and K's rows.
+template <typename T, int DK, int CP>
 constexpr int delta_chain_lds() {
-    typedef ChainPlanes<T, BACK, CP> P;
-    return kDeltaChunk * DK * (P::kA + P::kB) * 2;
+    return (kDeltaChunk * DK * CP + Rows<DeltaPlanes<T>::kRaw, kDeltaChunk, DK>::kValues) * 2;
 }
 
 // What a workgroup's index stands for: segments of a chain's column parts; the parts of a chain, which read the same operands, on one die (workgroups go to
@@ -73,74 +67,96 @@ constexpr int delta_ahead() {
     return DK == 32 ? 4 : DK == 64 ? 3 : 2;
 }
 
+// What is fetched of a chunk by NT threads of NT / 64 wavefronts: W's tiles (in fp32, split on the way) and K's rows.
+template <typename T, int DK, int CP, int NT>
+struct ChainFetch {
+    static constexpr int RAW = DeltaPlanes<T>::kRaw, N = DK / 16 * 4 * 64 / NT;
+    f32x4 w[N];
+    Staged<T, RAW, DK, NT> k;
+    __device__ __forceinline__ void load_w(const DeltaArgs& p, const DeltaSizes& z, long long id, int thread) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = load_at<f32x4>(p.w + id * z.w, (i * NT + thread) * 16);
+    }
+    __device__ __forceinline__ void put_w(bf16_t* to, int thread) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const Half<CP> h = split<CP>(w[i]);
+#pragma unroll
+            for (int q = 0; q < CP; ++q) *reinterpret_cast<bf16x4*>(to + q * (kDeltaChunk * DK) + (i * NT + thread) * 4) = h.p[q];
+        }
+    }
+    __device__ __forceinline__ void load_k(const DeltaArgs& p, const DeltaChain& c, long long chunk, int thread) {
+        k.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, chunk * kDeltaChunk, 0, p.dk, p.vec & kVecK, thread);
+    }
+};
+
+template <typename T, int DK, bool BACK, int CP, int NT, int AHEAD>
+__device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes& z, int chain, long long chunk, long long by, long long n, bf16_t* lw, bf16_t* lk,
+                                            int thread) {
+    const DeltaChain c(p, chain);
+    const long long id = chain * p.NC + chunk;
+    ChainFetch<T, DK, CP, NT> f[AHEAD];
+    // A is what the first product takes, B the second's: W and K, or (BACK) K and W
+    auto fetch_a = [&](int j, long long m) {
+        if (m >= n) return;
+        if constexpr (BACK) f[j].load_k(p, c, chunk + m * by, thread);
+        else f[j].load_w(p, z, id + m * by, thread);
+    };
+    auto fetch_b = [&](int j, long long m) {
+        if (m >= n) return;
+        if constexpr (BACK) f[j].load_w(p, z, id + m * by, thread);
+        else f[j].load_k(p, c, chunk + m * by, thread);
+    };
+    auto put_a = [&](int j) {
+        if constexpr (BACK) f[j].k.put(lk, thread);
+        else f[j].put_w(lw, thread);
+    };
+    auto put_b = [&](int j) {
+        if constexpr (BACK) f[j].put_w(lw, thread);
+        else f[j].k.put(lk, thread);
+    };
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) fetch_a(j, j), fetch_b(j, j);
+    put_a(0);
+    fetch_a(0, AHEAD);
+    __syncthreads();
+    for (long long m0 = 0; m0 < n; m0 += AHEAD) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const long long m = m0 + j;
+            if (m >= n) break;
+            put_b(j);
+            fetch_b(j, m + AHEAD);
+            __syncthreads();
+            const int k = j == AHEAD - 1 ? 0 : j + 1;
+            if (m + 1 < n) put_a(k);
+            fetch_a(k, m + 1 + AHEAD);
+            __syncthreads();
+        }
+    }
+}
+
 // Half of the workgroup's wavefronts carry columns, half fetch.
-template <typename T, int DK, bool BACK, int CP, bool MAPS>
-__global__ __launch_bounds__(512) void delta_chain_k(DeltaArgs p) {
-    typedef ChainPlanes<T, BACK, CP> P;
-    constexpr int RAW = P::kRaw, MADE = DeltaPlanes<T>::kMade, ND = DK / 16, NA = 4 * (DK / 32) * P::kA, NB = ND * 2 * P::kB;   // fragments' planes
-    constexpr int kLeast = delta_least_waves<DK>(), AHEAD = delta_ahead<DK, BACK>(), ROWS = ND < 4 ? ND : 4;
+template <typename T, int DK, bool BACK, int CP, bool MAPS, int WAVES>
+__global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
+    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade, ND = DK / 16, NK = DK / 32;
+    constexpr int AHEAD = delta_ahead<DK, BACK>(), ROWS = ND < 4 ? ND : 4, PLANE = kDeltaChunk * DK;
+    typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
-    bf16_t *la = (bf16_t*)lds, *lb = la + NA * 512;
-    const int lane = threadIdx.x & 63, waves = blockDim.x >> 7, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    bf16_t *lw = (bf16_t*)lds, *lk = lw + CP * PLANE;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int g4 = 4 * (lane >> 4), colv = p.dvp / 16, cols = MAPS ? colv + ND : colv;
     int chain, part, segment;
-    if (!chain_part(p, (cols + waves - 1) / waves, MAPS ? p.segments - 1 : p.segments, chain, part, segment)) return;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE, CP);
+    if (!chain_part(p, (cols + WAVES - 1) / WAVES, MAPS ? p.segments - 1 : p.segments, chain, part, segment)) return;
+    const DeltaSizes z(DK, p.dvp, MADE, CP);
     // chunks in the chain's order: n of them from `from`, each `by` behind the last
     const long long place = segment * p.seg, n = p.NC - place < p.seg ? p.NC - place : p.seg;
-    const long long by = BACK ? -1 : 1, from = chain * p.NC + (BACK ? p.NC - 1 - place : place);
+    const long long by = BACK ? -1 : 1, chunk = BACK ? p.NC - 1 - place : place, from = chain * p.NC + chunk;
 
-    if (wave >= waves) {
-        const int w = wave - waves;
-        const bf16_t* ga = BACK ? p.ka : p.wp;
-        const bf16_t* gb = BACK ? p.wp : p.kt;
-        const long long sa = kDeltaChunk * DK * P::kA, sb = kDeltaChunk * DK * P::kB;
-        constexpr int RA = (NA + kLeast - 1) / kLeast, RB = (NB + kLeast - 1) / kLeast;
-        bf16x8 a[AHEAD][RA], b[AHEAD][RB];
-        auto fetch = [&](bf16x8* r, const bf16_t* base, int count, int most) {
-#pragma unroll
-            for (int i = 0; i < most; ++i) {
-                const int f = i * waves + w;
-                if (f < count) r[i] = load_at<bf16x8>(base + f * 512, lane * 16);
-            }
-        };
-        auto put = [&](const bf16x8* r, bf16_t* base, int count, int most) {
-#pragma unroll
-            for (int i = 0; i < most; ++i) {
-                const int f = i * waves + w;
-                if (f < count) store_at(base + f * 512, lane * 16, r[i]);
-            }
-        };
-        auto fetch_a = [&](int j, long long m) {
-            if (m < n) fetch(a[j], ga + (from + m * by) * sa, NA, RA);
-        };
-        auto fetch_b = [&](int j, long long m) {
-            if (m < n) fetch(b[j], gb + (from + m * by) * sb, NB, RB);
-        };
-#pragma unroll
-        for (int j = 0; j < AHEAD; ++j) fetch_a(j, j), fetch_b(j, j);
-        put(a[0], la, NA, RA);
-        fetch_a(0, AHEAD);
-        __syncthreads();
-        for (long long m0 = 0; m0 < n; m0 += AHEAD) {
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                const long long m = m0 + j;
-                if (m >= n) break;
-                put(b[j], lb, NB, RB);
-                fetch_b(j, m + AHEAD);
-                __syncthreads();
-                constexpr int last = AHEAD - 1;
-                const int k = j == last ? 0 : j + 1;
-                if (m + 1 < n) put(a[k], la, NA, RA);
-                fetch_a(k, m + 1 + AHEAD);
-                __syncthreads();
-            }
-        }
-        return;
-    }
+    if (wave >= WAVES)
+        return chain_fetch<T, DK, BACK, CP, 64 * WAVES, AHEAD>(p, z, chain, chunk, by, n, lw, lk, threadIdx.x - 64 * WAVES);
 
-    const int cv = part * waves + wave;
+    const int cv = part * WAVES + wave;
     const bool on = cv < cols, unit_cols = MAPS && cv >= colv;   // (a wavefront without columns of its own goes along)
     const bf16x4 unit = unit_half(lane);
     const int at = 16 * cv + (lane & 15);
@@ -164,16 +180,15 @@ __global__ __launch_bounds__(512) void delta_chain_k(DeltaArgs p) {
 
     // what a chunk brings to these columns
     struct Chunk {
-        f32x4 y0[4], E[4];
+        f32x4 y0[BACK ? 1 : 4], E[4];
         float end;
     };
     auto fetch = [&](Chunk& c, long long id) {
-        const float *y0 = (BACK ? p.du : p.ub) + id * z.cols + cv * 1024;
         const DeltaGates* s = p.gates + id;
         const bool own = on && !unit_cols;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            c.y0[b] = own && !(BACK && MAPS) ? load_at<f32x4>(y0 + b * 256, lane * 16) : f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (!BACK) c.y0[b] = own ? load_at<f32x4>(p.ub + id * z.cols + cv * 1024 + b * 256, lane * 16) : f32x4{0.f, 0.f, 0.f, 0.f};
             c.E[b] = load_at<f32x4>(s->E + 16 * b, g4 * 4);
         }
         c.end = s->D[kDeltaChunk - 1];
@@ -197,22 +212,31 @@ __global__ __launch_bounds__(512) void delta_chain_k(DeltaArgs p) {
         }
         Frag<CP> xs[DK / 32];
 #pragma unroll
-        for (int d = 0; d < DK / 32; ++d) xs[d] = join(split<CP>(x[2 * d]), split<CP>(x[2 * d + 1]));
+        for (int d = 0; d < NK; ++d) xs[d] = join(split<CP>(x[2 * d]), split<CP>(x[2 * d + 1]));
         f32x4 y[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) y[b] = BACK ? f32x4{0.f, 0.f, 0.f, 0.f} : c.y0[b];
 #pragma unroll
-        for (int d = 0; d < DK / 32; ++d) {
-            Frag<P::kA> a[4];
+        for (int d = 0; d < NK; ++d) {
+            // (lane = step, values = channels of k)
+            if constexpr (BACK) {
+                Frag<RAW> a[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b) a[b] = load_frag<P::kA>(la, b * (DK / 32) + d, lane);
-            mma_rows(a, xs[d], y);
+                for (int b = 0; b < 4; ++b) a[b] = L::tiles(lk, 16 * b, 32 * d, lane);
+                mma_rows(a, xs[d], y);
+            } else {
+                Frag<CP> a[4];
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    a[b] = join(read_turned<CP>(lw + (2 * d * 4 + b) * 256, PLANE, lane), read_turned<CP>(lw + ((2 * d + 1) * 4 + b) * 256, PLANE, lane));
+                mma_rows(a, xs[d], y);
+            }
         }
         if constexpr (!MAPS) {
             if (on) {
                 bf16_t* to = (BACK ? p.ds1 : p.s0) + id * z.state;
 #pragma unroll
-                for (int d = 0; d < DK / 32; ++d) store_frag(to, cv * (DK / 32) + d, planes<MADE>(xs[d]), lane);
+                for (int d = 0; d < NK; ++d) store_frag(to, cv * NK + d, planes<MADE>(xs[d]), lane);
             }
         }
         __syncthreads();
@@ -229,25 +253,34 @@ __global__ __launch_bounds__(512) void delta_chain_k(DeltaArgs p) {
         for (int d0 = 0; d0 < ND; d0 += ROWS) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                Frag<P::kB> a[ROWS];
+                // (lane = channel of k, values = steps)
+                Frag<BACK ? CP : RAW> a[ROWS];
                 f32x4 t[ROWS];
 #pragma unroll
-                for (int d = 0; d < ROWS; ++d) a[d] = load_frag<P::kB>(lb, 2 * (d0 + d) + h, lane), t[d] = x[d0 + d];
+                for (int i = 0; i < ROWS; ++i) {
+                    const int d = d0 + i;
+                    if constexpr (BACK) {
+#pragma unroll
+                        for (int q = 0; q < CP; ++q) {
+                            const bf16x4 lo = *reinterpret_cast<const bf16x4*>(lw + q * PLANE + ((d * 4 + 2 * h) * 64 + lane) * 4);
+                            const bf16x4 hi = *reinterpret_cast<const bf16x4*>(lw + q * PLANE + ((d * 4 + 2 * h + 1) * 64 + lane) * 4);
+                            a[i].p[q] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        }
+                    } else {
+                        a[i] = join(L::down(lk, 32 * h, 16 * d, lane), L::down(lk, 32 * h + 16, 16 * d, lane));
+                    }
+                    t[i] = x[d];
+                }
                 mma_rows(a, h ? e1 : e0, t);
 #pragma unroll
-                for (int d = 0; d < ROWS; ++d) x[d0 + d] = t[d];
+                for (int i = 0; i < ROWS; ++i) x[d0 + i] = t[i];
             }
         }
-        if constexpr (!MAPS) {
+        if constexpr (!MAPS && !BACK) {
             if (on) {
-                if constexpr (BACK) {
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) store_at(p.du + id * z.cols + cv * 1024 + b * 256, lane * 16, c.y0[b] + y[b] * c.E[b]);
-                } else {
-                    bf16_t* to = p.u + id * z.u;
-                    store_frag(to, cv * 2, join(split<MADE>(y[0]), split<MADE>(y[1])), lane);
-                    store_frag(to, cv * 2 + 1, join(split<MADE>(y[2]), split<MADE>(y[3])), lane);
-                }
+                bf16_t* to = p.u + id * z.u;
+                store_frag(to, cv * 2, join(split<MADE>(y[0]), split<MADE>(y[1])), lane);
+                store_frag(to, cv * 2 + 1, join(split<MADE>(y[2]), split<MADE>(y[3])), lane);
             }
         }
         if (m + AHEAD < n) fetch(chunks[j], id + AHEAD * by);
@@ -285,7 +318,7 @@ __global__ __launch_bounds__(DK * 4) void delta_join_k(DeltaArgs p) {
     const int lane = threadIdx.x & 63, d = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), colv = p.dvp / 16;
     const long long id = p.first + blockIdx.x;
     const int chain = (int)(id / colv), cv = (int)(id - (long long)chain * colv);
-    const DeltaSizes z(DK, p.dvp, 1, 1, CP);
+    const DeltaSizes z(DK, p.dvp, 1, CP);
     const float* h = BACK ? p.glast : p.h0;
     const int at = 16 * cv + (lane & 15);
     f32x4 x;

@@ -36,8 +36,8 @@ struct DeltaArgs {
     float *last, *gh0;                     // [chain][dk][dv], or null
     const int* lengths;                    // [O], or null (T)
     // between the kernels, by chain and chunk
-    bf16_t *wp, *kt, *s0, *u, *ka, *ds1, *blocks;
-    float *ub, *du, *c0;
+    bf16_t *s0, *u, *ds1, *blocks;
+    float *w, *ub, *du, *c0;
     struct DeltaGates* gates;
     bf16_t* maps;                          // by chain and segment: the map's matrix, and what it adds
     float* shifts;
@@ -216,6 +216,19 @@ __device__ __forceinline__ bf16x4 turned(bf16x4 t, bf16x4 unit) {
     return o;
 }
 
+// A tile as it was made (lane = column, values = rows; 8 bytes a lane and plane, planes `plane` values apart) from LDS, with lane = row, values = columns:
+// lane l of each 16 hands in column 4 g + l / 4, rows 4 (l % 4) .., and gets row l % 16, columns 4 g ...
+template <int NP>
+__device__ __forceinline__ Half<NP> read_turned(const bf16_t* base, int plane, int lane) {
+    typedef __attribute__((address_space(3))) s16x4 lds_t;
+    const int i = lane & 15, from = (i & 3) * 16 + 4 * (lane >> 4) + (i >> 2);
+    Half<NP> f;
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+        f.p[p] = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(__attribute__((address_space(3))) void*)(base + p * plane + from * 4)));
+    return f;
+}
+
 // LDS rows of R values of planes: value i of row r of plane p at [p][r][i].
 template <int NP, int ROWS, int R>
 struct Rows {
@@ -292,18 +305,19 @@ __device__ __forceinline__ bool chunk_of(const DeltaArgs& p, int H, int& chain, 
 
 // A chunk of a tensor's rows, columns [col, col + R), on its way to LDS: `load` makes the loads, all without a condition where rows lie in pieces of
 // 8 (what is not there is read from row 0 and dropped), so that they are under way together with others; `put` leaves planes, 0 behind
-// the chain's end and behind the row's end d.  By 256 threads.
-template <typename T, int NP, int R>
+// the chain's end and behind the row's end d.  By NT threads, this one `thread` of them.
+template <typename T, int NP, int R, int NT = 256>
 struct Staged {
-    static constexpr int N = kDeltaChunk * (R / 8) / 256;
+    static constexpr int N = kDeltaChunk * (R / 8) / NT;
     T v[N][8];
     bool on[N];
-    __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first, int col, int d, bool vec) {
+    __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first, int col, int d, bool vec,
+                                         int thread = threadIdx.x) {
         int at[N];
         const T* q[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int e = threadIdx.x + n * 256;
+            const int e = thread + n * NT;
             const long long i = first + e / (R / 8);
             at[n] = col + e % (R / 8) * 8;
             on[n] = i < c.len && at[n] < d;
@@ -326,11 +340,11 @@ struct Staged {
                 for (int j = 0; j < 8; ++j) v[n][j] = on[n] && at[n] + j < d ? q[n][j] : from_f32<T>(0.f);
         }
     }
-    __device__ __forceinline__ void put(bf16_t* to) {
+    __device__ __forceinline__ void put(bf16_t* to, int thread = threadIdx.x) const {
         typedef Rows<NP, kDeltaChunk, R> L;
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int e = threadIdx.x + n * 256;
+            const int e = thread + n * NT;
             Frag<NP> f = planes_of<T, NP>(v[n]);
 #pragma unroll
             for (int m = 0; m < NP; ++m) {
@@ -396,29 +410,37 @@ __device__ __forceinline__ void write_strength(float b, int logits, float& beta,
     }
 }
 
-// Into LDS and memory, by the first wavefront; the caller's barrier follows.
-__device__ __forceinline__ void make_gates(DeltaGates& s, DeltaGates* to, const DeltaArgs& p, const DeltaChain& c, long long first, int type) {
-    if (threadIdx.x >= 64) return;
-    const int lane = threadIdx.x;
-    const long long i = first + lane;
-    float la = 0.f, slope = 0.f, beta = 0.f, bslope = 0.f;
-    if (i < c.len) {
-        const long long t = c.step(p, i);
-        log_decay(gate_value(p.g, c.at(p.gs, c.hv) + t * p.gs.t, p.gates_f32, type), p.logits, la, slope);
-        write_strength(gate_value(p.b, c.at(p.bs, c.hv) + t * p.bs.t, p.gates_f32, type), p.logits, beta, bslope);
+// Made by the first wavefront, in two steps (loads ahead of others; the rest), into LDS and memory; the caller's barrier follows.
+struct GateMaker {
+    float g, b;
+    bool on;
+    __device__ __forceinline__ void load(const DeltaArgs& p, const DeltaChain& c, long long first, int type) {
+        const long long i = first + (threadIdx.x & 63);
+        on = i < c.len;
+        const long long t = on ? c.step(p, i) : 0;
+        g = gate_value(p.g, c.at(p.gs, c.hv) + t * p.gs.t, p.gates_f32, type);
+        b = gate_value(p.b, c.at(p.bs, c.hv) + t * p.bs.t, p.gates_f32, type);
     }
-    double sum = la * 1.4426950408889634;
+    __device__ __forceinline__ void make(DeltaGates& s, DeltaGates* to, const DeltaArgs& p) {
+        const int lane = threadIdx.x & 63;
+        float la, slope, beta, bslope;
+        log_decay(g, p.logits, la, slope);
+        write_strength(b, p.logits, beta, bslope);
+        if (!on) la = slope = beta = bslope = 0.f;
+        double sum = la * 1.4426950408889634;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double other = __shfl_up(sum, d);
-        if (lane >= d) sum += other;
+        for (int d = 1; d < 64; d *= 2) {
+            const double other = __shfl_up(sum, d);
+            if (lane >= d) sum += other;
+        }
+        const double end = __shfl(sum, 63);
+        const float hi = (float)sum, lo = (float)(sum - (double)hi), D = __builtin_amdgcn_exp2f(hi), E = __builtin_amdgcn_exp2f((float)(end - sum));
+        s.hi[lane] = to->hi[lane] = hi, s.lo[lane] = to->lo[lane] = lo, s.beta[lane] = to->beta[lane] = beta;
+        s.D[lane] = to->D[lane] = D, s.E[lane] = to->E[lane] = E;
+        s.slope[lane] = to->slope[lane] = slope, s.bslope[lane] = to->bslope[lane] = bslope;
     }
-    const double end = __shfl(sum, 63);
-    const float hi = (float)sum, lo = (float)(sum - (double)hi), D = __builtin_amdgcn_exp2f(hi), E = __builtin_amdgcn_exp2f((float)(end - sum));
-    s.hi[lane] = to->hi[lane] = hi, s.lo[lane] = to->lo[lane] = lo, s.beta[lane] = to->beta[lane] = beta;
-    s.D[lane] = to->D[lane] = D, s.E[lane] = to->E[lane] = E;
-    s.slope[lane] = to->slope[lane] = slope, s.bslope[lane] = to->bslope[lane] = bslope;
-}
+};
+
 // e^(c_i - c_j) of a tile: this lane's step and four others of it, which is i and which j: rows: this lane's is i.  Above the diagonal (i < j) it may
 // be infinite: the caller selects.
 struct TileDecay {
@@ -436,8 +458,8 @@ struct TileDecay {
 };
 
 // (I + A)^-1 of a chunk, A strictly lower, as blocks of 16 x 16 for a substitution by blocks: -A_ba below the diagonal, the inverses of the
-// diagonal's blocks on it.  Block (b, a) is number b (b + 1) / 2 + a.  FORE: lane = row, values = columns, an operand for products with
-// solutions by their rows; else lane = column, values = rows: the same for the transposed system.
+// diagonal's blocks on it.  Block (b, a) is number b (b + 1) / 2 + a.  Lane = row, values = columns, an operand for products with
+// solutions by their rows; turned, lane = column, values = rows: the same for the transposed system.
 template <int NP>
 struct Blocks {
     static constexpr int kValues = 10 * NP * 64 * 4;
@@ -454,28 +476,19 @@ struct Blocks {
     }
 };
 
-// The inverse of a block I + A, its A in `tile` [16][20] of LDS: FORE [column][row], else [row][column].  Lane l % 16 has a row (FORE) or a
-// column of it; -> values 4 g .. 4 g + 3 of that.  Row i of T = (I + A)^-1 from T (I + A) = I: t_j = [i = j] - sum over m > j of t_m A_mj.
-template <bool FORE>
-__device__ __forceinline__ f32x4 invert_block(const float* tile, int lane) {
+// The inverse T of a block I + A, strictly lower A with lane = row, values = columns, as it is: row i of T from T (I + A) = I,
+// t_j = [i = j] - sum over m > j of t_m A_mj, from the last column.  A lane has a row; A's elements come to all lanes as scalars.
+__device__ __forceinline__ f32x4 invert_block(f32x4 A, int lane) {
     const int me = lane & 15;
     float t[16];
 #pragma unroll
-    for (int n = 0; n < 16; ++n) {
-        const int j = FORE ? 15 - n : n;
+    for (int j = 15; j >= 0; --j) {
         float s = j == me ? 1.f : 0.f;
-        float a[16];
-#pragma unroll
-        for (int m = 0; m < 16; m += 4) {
-            if (FORE ? m + 3 <= j : m >= j) continue;
-            const f32x4 r = *reinterpret_cast<const f32x4*>(tile + j * 20 + m);
-            a[m] = r[0], a[m + 1] = r[1], a[m + 2] = r[2], a[m + 3] = r[3];
-        }
         // (the latest of t last: it is what there is to wait for)
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-            const int m = FORE ? 15 - k : k;
-            if (FORE ? m > j : m < j) s = __builtin_fmaf(-t[m], a[m], s);
+        for (int m = 15; m > j; --m) {
+            const float row = A[j & 3];   // (a bit cast of an element would take the first one)
+            s = __builtin_fmaf(-t[m], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, row), (j >> 2) * 16 + m)), s);
         }
         t[j] = s;
     }
@@ -488,32 +501,28 @@ __device__ __forceinline__ f32x4 invert_block(const float* tile, int lane) {
     return v;
 }
 
-// Solutions X of (I + A) X = R by blocks of rows, in place: lane = column, values = rows.
+// Solutions X of (I + A) X = R by blocks of rows, in place: lane = column, values = rows.  A solved block goes at once into the rows behind it.
 template <int NP>
 __device__ __forceinline__ void solve_fore(const bf16_t* blocks, f32x4 (&x)[4], int lane) {
-    Half<NP> s[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        f32x4 r = x[b];
-#pragma unroll
-        for (int a = 0; a < b; ++a) r = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s[a], r);
+    for (int a = 0; a < 4; ++a) {
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        x[b] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, b), lane), split<NP>(r), zero);
-        s[b] = split<NP>(x[b]);
+        x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(a, a), lane), split<NP>(x[a]), zero);
+        const Half<NP> s = split<NP>(x[a]);
+#pragma unroll
+        for (int b = a + 1; b < 4; ++b) x[b] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s, x[b]);
     }
 }
 // of (I + A)^T X = R, from the last block.
 template <int NP>
 __device__ __forceinline__ void solve_back(const bf16_t* blocks, f32x4 (&x)[4], int lane) {
-    Half<NP> s[4];
 #pragma unroll
-    for (int a = 3; a >= 0; --a) {
-        f32x4 r = x[a];
-#pragma unroll
-        for (int b = 3; b > a; --b) r = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s[b], r);
+    for (int b = 3; b >= 0; --b) {
         const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(a, a), lane), split<NP>(r), zero);
-        s[a] = split<NP>(x[a]);
+        x[b] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, b), lane), split<NP>(x[b]), zero);
+        const Half<NP> s = split<NP>(x[b]);
+#pragma unroll
+        for (int a = b - 1; a >= 0; --a) x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s, x[a]);
     }
 }
 
@@ -575,11 +584,11 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // Sizes of what lies between the kernels, in elements of a chunk; of a segment's map.
 struct DeltaSizes {
-    long long rows, frag_chain, frag_raw, state, u, cols, c0, map, shift, blocks;
-    __host__ __device__ DeltaSizes(int DK, int dvp, int raw, int made, int chain)
-        : rows(kDeltaChunk * (long long)DK), frag_chain(rows * chain), frag_raw(rows * raw), state((long long)DK * dvp * made),
-          u((long long)kDeltaChunk * dvp * made), cols((long long)kDeltaChunk * dvp), c0((long long)DK * dvp), map((long long)DK * DK * chain),
-          shift((long long)DK * dvp), blocks(10 * made * 256) {}
+    long long w, state, u, cols, c0, map, shift, blocks;
+    __host__ __device__ DeltaSizes(int DK, int dvp, int made, int chain)
+        : w(kDeltaChunk * (long long)DK), state((long long)DK * dvp * made), u((long long)kDeltaChunk * dvp * made),
+          cols((long long)kDeltaChunk * dvp), c0((long long)DK * dvp), map((long long)DK * DK * chain), shift((long long)DK * dvp),
+          blocks(10 * made * 256) {}
 };
 
 }  // namespace pdw

@@ -8,46 +8,13 @@
 //   (I + A) U = beta (V - D K S0),   A_ij = beta_i G_ij k_i.k_j for j < i          U = Ub - W S0,  (I + A) [W Ub] = [beta D K   beta V]
 //   S1 = e^c_end S0 + K^T E U                                                      Y = scale (D Q S0 + (G o Q K^T) U),  j <= i
 //
-// Three launches.  delta_prepare_k, a workgroup a chunk: A, then W and Ub by substitution (16 x 16 blocks: the diagonal's are inverted row by row
-// in fp32, the rest is products; powers of A, the other way to its inverse, cancel where keys repeat).  delta_chain_k, the only part with an
-// order: a wavefront carries 16 columns of a chain's state in registers through its chunks, two products a chunk, whose operands come ready made
-// from memory; results of the first are operands of the second without an exchange.  It leaves the states before the chunks and U.
-// delta_out_k, a workgroup a chunk again: Y.
+// Three launches and more.  delta_prepare_k, a workgroup a chunk: A, then W and Ub by substitution (16 x 16 blocks: the diagonal's are inverted row by
+// row in fp32, the rest is products; powers of A, the other way to its inverse, cancel where keys repeat).  delta_chain.h, the only part with an
+// order: states through the chunks.  It leaves the states before the chunks and U.  delta_out_k, a workgroup a chunk again: Y.
 #pragma once
 #include "delta_chain.h"
 
 namespace pdw {
-
-// A's blocks of the wavefront's row of blocks (FORE) or column of blocks, into LDS; the caller's barrier follows, then invert_blocks.
-// tile: this wavefront's [16][20].
-template <int RAW, int MADE, int DK, bool FORE>
-__device__ __forceinline__ void make_blocks(bf16_t* blocks, float* tile, const bf16_t* k, const DeltaGates& s, int wave, int lane) {
-    typedef Rows<RAW, kDeltaChunk, DK> L;
-    const int col = lane & 15, g4 = 4 * (lane >> 4);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        if (FORE ? t > wave : t < wave) continue;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int n = 0; n < DK; n += 32) acc = mma<MADE>(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
-        // FORE: lane = row i of the wavefront's block row, values = columns j of block t; else lane = column j, values = rows i
-        const TileDecay decay(s, 16 * wave + col, 16 * t + g4, FORE);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const bool below = t != wave || (FORE ? g4 + r < col : col < g4 + r);
-            acc[r] = below ? decay.beta[r] * decay.G[r] * acc[r] : 0.f;
-        }
-        if (t == wave) {
-            // [column][row] (FORE), [row][column]: the lane's index is the inner one
-#pragma unroll
-            for (int r = 0; r < 4; ++r) tile[(g4 + r) * 20 + col] = acc[r];
-        } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[r] = -acc[r];
-            Blocks<MADE>::put(blocks, FORE ? Blocks<MADE>::at(wave, t) : Blocks<MADE>::at(t, wave), split<MADE>(acc), lane);
-        }
-    }
-}
 
 template <int RAW, int DK>
 constexpr int delta_rows_bytes() {
@@ -62,43 +29,68 @@ template <typename T, int DK>
 constexpr int delta_prepare_lds() {
     typedef DeltaPlanes<T> P;
     return delta_rows_bytes<P::kRaw, DK>() + delta_rows_bytes<P::kRaw, delta_prepare_cols<T, DK>()>() + Blocks<kChainPlanes>::kValues * 2 +
-           4 * 16 * 20 * 4 + (int)sizeof(DeltaGates);
+           (int)sizeof(DeltaGates);
 }
 
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
+__global__ __launch_bounds__(256, 4) void delta_prepare_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = kChainPlanes;
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
-    typedef Rows<RAW, kDeltaChunk, DK> L;
-    extern __shared__ __align__(16) unsigned char lds[];
     constexpr int COLS = delta_prepare_cols<T, DK>();
+    typedef Rows<RAW, kDeltaChunk, DK> L;
     typedef Rows<RAW, kDeltaChunk, COLS> LV;
+    extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *k = (bf16_t*)lds, *vl = k + L::kValues, *blocks = vl + LV::kValues;
-    float* tiles = (float*)(blocks + Blocks<MADE>::kValues);
-    DeltaGates& s = *(DeltaGates*)(tiles + 4 * 16 * 20);
+    DeltaGates& s = *(DeltaGates*)(blocks + Blocks<MADE>::kValues);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int g4 = 4 * (lane >> 4);
+    const int col = lane & 15, g4 = 4 * (lane >> 4);
     int chain;
     long long m;
     if (!chunk_of(p, p.Hv, chain, m)) return;
     const long long id = chain * p.NC + m, first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
 
+    GateMaker gates;
     Staged<T, RAW, DK> ks;
     Staged<T, RAW, COLS> vs;
+    if (wave == 0) gates.load(p, c, first, type);
     ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
     vs.load((const T*)p.v + c.at(p.vs, c.hv), p.vs.t, p, c, first, 0, p.dv, p.vec & kVecV);
-    make_gates(s, p.gates + id, p, c, first, type);
+    if (wave == 0) gates.make(s, p.gates + id, p);
     ks.put(k), vs.put(vl);
     __syncthreads();
-    float* tile = tiles + wave * 16 * 20;
-    make_blocks<RAW, MADE, DK, true>(blocks, tile, k, s, wave, lane);
-    // (the tile is this wavefront's own: its LDS operations are in order)
-    Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, wave), split<MADE>(invert_block<true>(tile, lane)), lane);
+    // A's blocks of the wavefront's row of blocks: lane = row i of it, values = columns j of block t
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (t > wave) continue;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < DK; n += 32) acc = mma<MADE>(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), acc);
+        const TileDecay decay(s, 16 * wave + col, 16 * t + g4, true);
+        acc = decay.beta * decay.G * acc;
+        if (t == wave) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[r] = g4 + r < col ? acc[r] : 0.f;
+            acc = invert_block(acc, lane);
+        } else {
+            acc = -acc;
+        }
+        Blocks<MADE>::put(blocks, Blocks<MADE>::at(wave, t), split<MADE>(acc), lane);
+    }
     __syncthreads();
 
-    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
-    const bf16x4 unit = unit_half(lane);
+    const DeltaSizes z(DK, p.dvp, DeltaPlanes<T>::kMade, MADE);
+    if (p.blocks) {   // for the backward's transposed system, of the planes that it takes
+        constexpr int NG = DeltaPlanes<T>::kMade;
+        const bf16x4 unit = unit_half(lane);
+        for (int n = wave; n < 10; n += 4) {
+            const Half<MADE> h = Blocks<MADE>::get(blocks, n, lane);
+            Half<NG> t;
+#pragma unroll
+            for (int i = 0; i < NG; ++i) t.p[i] = turned(h.p[i], unit);
+            Blocks<NG>::put(p.blocks + id * z.blocks, n, t, lane);
+        }
+    }
     f32x4 beta[4], decay[4];
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
@@ -115,34 +107,16 @@ __global__ __launch_bounds__(256) void delta_prepare_k(DeltaArgs p) {
         }
         const int end = (p.dvp - at < COLS ? p.dvp - at : COLS) / 16;
         for (int ct = (at ? DK / 16 : 0) + wave; ct < DK / 16 + end; ct += 4) {
+            const bool w = ct < DK / 16;
+            const int cv = ct - DK / 16;
             f32x4 x[4];
-            if (ct < DK / 16) {
-                Half<RAW> kr[4];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    kr[b] = L::down(k, 16 * b, 16 * ct, lane);
-                    x[b] = sum_of(kr[b]) * decay[b];
-                }
-                store_frag(p.kt + id * z.frag_raw, 2 * ct, join(kr[0], kr[1]), lane);
-                store_frag(p.kt + id * z.frag_raw, 2 * ct + 1, join(kr[2], kr[3]), lane);
-                solve_fore<MADE>(blocks, x, lane);
-                // -W, lane = step: the first operand of the chain's first product
+            for (int b = 0; b < 4; ++b)
+                x[b] = w ? sum_of(L::down(k, 16 * b, 16 * ct, lane)) * decay[b] : sum_of(LV::down(vl, 16 * b, 16 * cv, lane)) * beta[b];
+            solve_fore<MADE>(blocks, x, lane);
+            float* to = w ? p.w + id * z.w + ct * 1024 : p.ub + id * z.cols + (at / 16 + cv) * 1024;   // (-W: as the products take it)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    Half<MADE> h = split<MADE>(-x[b]);
-#pragma unroll
-                    for (int n = 0; n < MADE; ++n) h.p[n] = turned(h.p[n], unit);
-                    store_half(p.wp + id * z.frag_chain, b * (DK / 32) + ct / 2, ct & 1, h, lane);
-                }
-            } else {
-                const int cv = ct - DK / 16;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) x[b] = sum_of(LV::down(vl, 16 * b, 16 * cv, lane)) * beta[b];
-                solve_fore<MADE>(blocks, x, lane);
-                float* ub = p.ub + id * z.cols + (at / 16 + cv) * 1024;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) store_at(ub + b * 256, lane * 16, x[b]);
-            }
+            for (int b = 0; b < 4; ++b) store_at(to + b * 256, lane * 16, w ? -x[b] : x[b]);
         }
     }
 }
@@ -198,7 +172,7 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const long long step = first + i;
     const bool there = step < c.len;
     T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
-    const DeltaSizes z(DK, p.dvp, RAW, MADE, MADE);
+    const DeltaSizes z(DK, p.dvp, MADE, MADE);
     const bf16_t *s0 = p.s0 + id * z.state, *u = p.u + id * z.u;
     // (states and U lie with lane = column of v, values = rows: first operands of the transposed products as they are)
     for (int cv = 0; cv < p.dvp / 16; ++cv) {

@@ -18,12 +18,18 @@ inline void delta_launch(K kernel, int lds, std::once_flag& once, long long grid
 
 inline long long delta_chunk_grid(const DeltaArgs& p, int H) { return ((long long)p.O * p.W * p.NC + 7) / 8 * 8 * H; }
 
+template <typename T, int DK, bool BACK, int CP, bool MAPS, int WAVES>
+void delta_chains_of(const DeltaArgs& p, int cols, hipStream_t s) {
+    static std::once_flag once;
+    const long long grid = ((long long)p.chains + 7) / 8 * 8 * ((cols + WAVES - 1) / WAVES) * (MAPS ? p.segments - 1 : p.segments);
+    delta_launch(delta_chain_k<T, DK, BACK, CP, MAPS, WAVES>, delta_chain_lds<T, DK, CP>(), once, grid, 128 * WAVES, p, s);
+}
 template <typename T, int DK, bool BACK, int CP, bool MAPS>
 void delta_chains(const DeltaArgs& p, hipStream_t s) {
-    static std::once_flag once;
-    const int cols = p.dvp / 16 + (MAPS ? DK / 16 : 0), waves = cols < 4 && delta_least_waves<DK>() < 4 ? cols : 4;
-    const long long grid = ((long long)p.chains + 7) / 8 * 8 * ((cols + waves - 1) / waves) * (MAPS ? p.segments - 1 : p.segments);
-    delta_launch(delta_chain_k<T, DK, BACK, CP, MAPS>, delta_chain_lds<T, DK, BACK, CP>(), once, grid, 128 * waves, p, s);
+    const int cols = p.dvp / 16 + (MAPS ? DK / 16 : 0);
+    if constexpr (delta_least_waves<DK>() < 4)
+        if (cols < 4) return delta_chains_of<T, DK, BACK, CP, MAPS, 2>(p, cols, s);
+    delta_chains_of<T, DK, BACK, CP, MAPS, 4>(p, cols, s);
 }
 
 template <typename T, int DK, bool BACK, int CP>
