@@ -16,12 +16,6 @@
 #pragma once
 #include "delta_fwd.h"
 
-#ifndef FRESH
-#define FRESH int lane = threadIdx.x & 63; asm volatile("" : "+v"(lane)); const int col = lane & 15, g = lane >> 4, g4 = 4 * g, me = 16 * wave + col; const long long place = first + me; const bool there = place < ck.len; const long long step = ck.step(p, place); (void)g; (void)g4; (void)there; (void)step; (void)col
-#endif
-#ifndef SB
-#define SB __builtin_amdgcn_sched_barrier(0)
-#endif
 namespace pdw {
 
 template <typename T, int NP>
@@ -163,34 +157,50 @@ __device__ __forceinline__ void sum_tiles(const Frag<NP>& f, f32x4& lo, f32x4& h
     }
 }
 
-// Columns of v that a workgroup has in LDS at a time: as many as leave room for two workgroups on a compute unit, or for one.
+// Rows of Q and K; in their wake Z's and dY's columns, A's blocks and the states' and U's columns, and in the place of those later the tiles of
+// scale G o dP and beta G o dA; gates; sums.
+constexpr int kGradsCols = 32, kGradsThreads = 512;
 template <typename T, int DK>
-constexpr int delta_grads_cols() {
-    return DK == 32 || (sizeof(T) == 4 && DK == 128) ? 32 : 64;
-}
+struct GradsLds {
+    static constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
+    // (with fp32's three planes and 128 channels the states find no room, and each wavefront turns its own)
+    static constexpr bool kStage = !(sizeof(T) == 4 && DK == 128);
+    static constexpr int kRows = 2 * Rows<RAW, kDeltaChunk, DK>::kValues;
+    static constexpr int kZ = Rows<MADE, kDeltaChunk, kGradsCols>::kValues, kG = Rows<RAW, kDeltaChunk, kGradsCols>::kValues;
+    static constexpr int kBlocks = Blocks<MADE>::kValues, kState = 2 * (DK / 32) * MADE * 512, kU = 2 * 2 * MADE * 512;
+    static constexpr int kFirst = kZ + kG + kBlocks + (kStage ? 2 * kState + kU : 0), kRounds = kStage ? 1 : 2;
+    static constexpr int kSecond = 2 * (kRounds == 1 ? 2 : 1) * Blocks<MADE>::kValues;
+    static constexpr int kSums = 3 * 4 * 64 + 4 * 2 * 64 + 8;
+    static constexpr int kBytes = (kRows + (kFirst > kSecond ? kFirst : kSecond)) * 2 + (int)sizeof(DeltaGates) + kSums * 4;
+};
 template <typename T, int DK>
 constexpr int delta_grads_lds() {
-    typedef DeltaPlanes<T> P;
-    constexpr int COLS = delta_grads_cols<T, DK>();
-    return 2 * delta_rows_bytes<P::kRaw, DK>() + (Rows<P::kMade, kDeltaChunk, COLS>::kValues + Rows<P::kRaw, kDeltaChunk, COLS>::kValues) * 2 +
-           Blocks<P::kMade>::kValues * 2 + (int)sizeof(DeltaGates) + (2 * kDeltaChunk + 4) * 4;
+    return GradsLds<T, DK>::kBytes;
 }
 
-// A wavefront has a block of 16 steps: its rows of dQ, dK, dV.  What of dP and dA concerns them are five tiles ("slots"): those of its row, blocks
-// t <= wave (lane = i, its own step, values = j), and those of its column, t >= wave (lane = j, its own step, values = i).  SHARED: value heads share
-// key heads.
+// A sum over 16 neighbouring lanes, in all of them.
+__device__ __forceinline__ float sixteen_sum(float v) {
+    v = dpp_add<0xB1>(v), v = dpp_add<0x4E>(v), v = dpp_add<0x141>(v);
+    return dpp_add<0x140>(v);
+}
+
+// Eight wavefronts: each has a block of 16 steps (`row`) and half of the channels of k (`half`): those parts of dQ and dK.  The ten tiles of dP and dA go
+// round the wavefronts (lane = step i, values = steps j); what becomes of them goes to all through LDS, both ways round.  SHARED: value
+// heads share key heads.
 template <typename T, int DK, bool SHARED>
-__global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delta_grads_k(DeltaArgs p) {
-    constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
-    constexpr int ND = DK / 16, COLS = delta_grads_cols<T, DK>();
+__global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4) void delta_grads_k(DeltaArgs p) {
+    typedef GradsLds<T, DK> S;
+    constexpr int RAW = S::RAW, MADE = S::MADE, NT = kGradsThreads, COLS = kGradsCols, ND = DK / 32, NK = DK / 32;   // ND: tiles of this half
     typedef Rows<RAW, kDeltaChunk, DK> L;
     typedef Rows<MADE, kDeltaChunk, COLS> LZ;
     typedef Rows<RAW, kDeltaChunk, COLS> LG;
     extern __shared__ __align__(16) unsigned char lds[];
-    bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *zl = k + L::kValues, *gl = zl + LZ::kValues, *blocks = gl + LG::kValues;
-    DeltaGates& s = *(DeltaGates*)(blocks + Blocks<MADE>::kValues);
-    float* dcs = (float*)(&s + 1);   // [64]; x [64]; a part of <S0, dS1> from each wavefront
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *zl = k + L::kValues, *gl = zl + S::kZ, *blocks = gl + S::kG;
+    bf16_t *sl = blocks + S::kBlocks, *dl = sl + S::kState, *ul = dl + S::kState;
+    bf16_t* tiles = zl;
+    DeltaGates& s = *(DeltaGates*)(zl + (S::kFirst > S::kSecond ? S::kFirst : S::kSecond));
+    float *rows_n = (float*)(&s + 1), *cols_n = rows_n + 256, *rows_b = cols_n + 256, *dots = rows_b + 256, *inner = dots + 512;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave & 3, half = wave >> 2;
     int kchain;
     long long m;
     if (!chunk_of(p, p.Hk, kchain, m)) return;
@@ -201,7 +211,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delt
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
     const DeltaChain ck(p, chain0);
-    Staged<T, RAW, DK> ks, qs;
+    Staged<T, RAW, DK, NT> ks, qs;
     ks.load((const T*)p.k + ck.at(p.ks, ck.hk), p.ks.t, p, ck, first, 0, p.dk, p.vec & kVecK);
     qs.load((const T*)p.q + ck.at(p.qs, ck.hk), p.qs.t, p, ck, first, 0, p.dk, p.vec & kVecQ);
     f32x4 gq[ND], gk[ND];
@@ -212,216 +222,266 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DK == 128 ? 1 : 2) void delt
         const int chain = chain0 + e;
         const DeltaChain c(p, chain);
         const long long id = chain * p.NC + m;
-        // (a lane that the compiler takes for another one with every head: else it keeps all addresses of all heads' passes, in scratch memory)
+        // (a lane that the compiler takes for another one with every head, and in every part below: else it keeps all addresses of all parts, in
+        // scratch memory)
         int lane = threadIdx.x & 63;
         if (SHARED) asm volatile("" : "+v"(lane)::"memory");
-        const int col = lane & 15, g = lane >> 4, g4 = 4 * g;
-        const bf16x4 unit = unit_half(lane);
-        const int me = 16 * wave + col;   // this lane's step
-        const long long place = first + me;
-        const bool there = place < ck.len;
-        const long long step = ck.step(p, place);
-        Run<sizeof(DeltaGates)> gates;
-        Run<Blocks<MADE>::kValues * 2> system;
-        gates.load(p.gates + id), system.load(p.blocks + id * z.blocks);
-
-        f32x4 aq[ND], az[ND], au[ND];   // dY S0^T, Z S0^T, U dS1^T: lane = step, values = channels of k
-        f32x4 dp[5], da[5];             // dP and -dA
+        const bf16_t *s0 = p.s0 + id * z.state, *ds1 = p.ds1 + id * z.state, *u = p.u + id * z.u;
+        {
+            Run<sizeof(DeltaGates), NT> gates;
+            Run<Blocks<MADE>::kValues * 2, NT> system;
+            gates.load(p.gates + id), system.load(p.blocks + id * z.blocks);
+            if (e) __syncthreads();
+            if (e == 0) ks.put(k), qs.put(q);
+            gates.put(&s), system.put(blocks);
+        }
+        f32x4 aq[ND], az[ND], au[ND];   // dY S0^T, Z S0^T, U dS1^T: lane = step of `row`, values = channels of k
+        f32x4 dp[2], da[2];             // dP and -dA of tiles `wave` and wave + 8
 #pragma unroll
         for (int d = 0; d < ND; ++d) aq[d] = az[d] = au[d] = zero;
 #pragma unroll
-        for (int j = 0; j < 5; ++j) dp[j] = da[j] = zero;
+        for (int n = 0; n < 2; ++n) dp[n] = da[n] = zero;
         float zv = 0.f, ss = 0.f;       // Z_i.V_i; <S0, dS1>
-        const bf16_t *s0 = p.s0 + id * z.state, *ds1 = p.ds1 + id * z.state, *u = p.u + id * z.u;
-        float beta;
         for (int at = 0; at < p.dvp; at += COLS) {
-            const int cv = at / 16 + wave;
-            const bool mine = 16 * wave < COLS && cv < p.dvp / 16;
-            Staged<T, RAW, COLS> gs;
-            gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
+            const int cw = at / 16;
+            {
+                Staged<T, RAW, COLS, NT> gs;
+                gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
+                if constexpr (S::kStage) {
+                    Run<S::kState * 2, NT> rs, rd;
+                    Run<S::kU * 2, NT> ru;
+                    rs.load(s0 + cw * NK * MADE * 512), rd.load(ds1 + cw * NK * MADE * 512), ru.load(u + cw * 2 * MADE * 512);
+                    if (at) __syncthreads();
+                    rs.put(sl), rd.put(dl), ru.put(ul);
+                } else if (at) {
+                    __syncthreads();
+                }
+                gs.put(gl);
+            }
             f32x4 x[4];
-            Frag<MADE> xs[DK / 32];
-            if (mine) {
-                const float* du = p.du + id * z.cols + cv * 1024;
+            if (wave < 2) {
 #pragma unroll
-                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(du + b * 256, lane * 16);
-#pragma unroll
-                for (int d = 0; d < DK / 32; ++d) xs[d] = load_frag<MADE>(ds1, cv * (DK / 32) + d, lane);
+                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(p.du + id * z.cols + (cw + wave) * 1024 + b * 256, lane * 16);
             }
-            if (e || at) __syncthreads();
-            if (at == 0) {
-                if (e == 0) ks.put(k), qs.put(q);
-                gates.put(&s), system.put(blocks);
-            }
-            gs.put(gl);
             __syncthreads();
-            beta = s.beta[me];
-            if (mine) {
-                // dU = that without dS1's part, and E K dS1
+            asm volatile("" : "+v"(lane));
+            const bf16x4 unit = unit_half(lane);
+            // rows of a tile of steps or channels from what lies as the products left it
+            auto turned_rows = [&](const bf16_t* staged, const bf16_t* from, int n, int t) {
+                if constexpr (S::kStage) {
+                    const bf16_t* a = staged + (t / 2) * MADE * 512 + 4 * (t & 1);
+                    return join(read_turned<MADE, 8>(a, 512, lane), read_turned<MADE, 8>(a + n * MADE * 512, 512, lane));
+                } else {
+                    return load_turned<MADE>(from, cw * n + t / 2, n, t & 1, unit, lane);
+                }
+            };
+            if (wave < 2) {
+                // dU = that without dS1's part, and E K dS1; then Z
                 f32x4 y[4] = {zero, zero, zero, zero};
 #pragma unroll
-                for (int d = 0; d < DK / 32; ++d) {
+                for (int d = 0; d < NK; ++d) {
+                    const Frag<MADE> xs = S::kStage ? load_frag<MADE>(dl, wave * NK + d, lane) : load_frag<MADE>(ds1, (cw + wave) * NK + d, lane);
                     Frag<RAW> a[4];
 #pragma unroll
                     for (int b = 0; b < 4; ++b) a[b] = L::tiles(k, 16 * b, 32 * d, lane);
-                    mma_rows(a, xs[d], y);
+                    mma_rows(a, xs, y);
                 }
 #pragma unroll
-                for (int b = 0; b < 4; ++b) x[b] += y[b] * *reinterpret_cast<const f32x4*>(s.E + 16 * b + g4);
+                for (int b = 0; b < 4; ++b) x[b] += y[b] * *reinterpret_cast<const f32x4*>(s.E + 16 * b + 4 * (lane >> 4));
                 solve_back<MADE>(blocks, x, lane);
 #pragma unroll
                 for (int b = 0; b < 4; ++b) LZ::put_turned(zl, 16 * b, 16 * wave, split<MADE>(x[b]), unit, lane);
             }
-            __syncthreads();
-#pragma unroll 1
-            for (int n = 0; n < COLS && at + n < p.dvp; n += 32) {
-                FRESH;
-                const int here = at + n + g4, cw = (at + n) / 16;
-                const Frag<RAW> om = LG::tiles(gl, 16 * wave, n, lane);
-                const Frag<MADE> zm = LZ::tiles(zl, 16 * wave, n, lane);
-                const Frag<MADE> um = load_turned<MADE>(u, cw * 2 + wave / 2, 2, wave & 1, unit, lane);
-                {
-                    const T* v = (const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t;
-                    T* gv = (T*)p.gv + c.at(p.gvs, c.hv) + step * p.gvs.t;
-                    f32x4 lo, hi;
-                    sum_tiles(zm, lo, hi);
-                    const f32x4 vl = load_four(v, there, here, p.dv, p.vec & kVecV), vh = load_four(v, there, here + 16, p.dv, p.vec & kVecV);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) zv = __builtin_fmaf(lo[j], vl[j], __builtin_fmaf(hi[j], vh[j], zv));
-                    if (p.gv && place < p.T) {
-                        store_four(gv, here, p.dv, there ? lo * beta : zero, p.vec & kVecGv);
-                        store_four(gv, here + 16, p.dv, there ? hi * beta : zero, p.vec & kVecGv);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < 5; ++j) {
-                    const bool row = j <= wave;
-                    const int t = row ? j : j - 1;
-                    if (row) {
-                        const Frag<MADE> uf = load_turned<MADE>(u, cw * 2 + t / 2, 2, t & 1, unit, lane);
-                        dp[j] = mma(uf, om, dp[j]);
-                        da[j] = mma(uf, zm, da[j]);
-                    } else {
-                        dp[j] = mma(LG::tiles(gl, 16 * t, n, lane), um, dp[j]);
-                        da[j] = mma(LZ::tiles(zl, 16 * t, n, lane), um, da[j]);
-                    }
-                    SB;
-                }
+            // what Z has no part in
+            const Frag<MADE> um = turned_rows(ul, u, 2, row);
+            {
+                const Frag<RAW> om = LG::tiles(gl, 16 * row, 0, lane);
 #pragma unroll
                 for (int d = 0; d < ND; ++d) {
-                    const Frag<MADE> sf = load_turned<MADE>(s0, cw * (DK / 32) + d / 2, DK / 32, d & 1, unit, lane);
-                    const Frag<MADE> df = load_turned<MADE>(ds1, cw * (DK / 32) + d / 2, DK / 32, d & 1, unit, lane);
+                    const Frag<MADE> sf = turned_rows(sl, s0, NK, half * ND + d), df = turned_rows(dl, ds1, NK, half * ND + d);
                     aq[d] = mma(sf, om, aq[d]);
-                    az[d] = mma(sf, zm, az[d]);
                     au[d] = mma(df, um, au[d]);
-                    if ((d & 3) == wave) {
+                    if ((d & 3) == row) {
                         f32x4 a0, a1, b0, b1;
                         sum_tiles(sf, a0, a1), sum_tiles(df, b0, b1);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(a0[j], b0[j], __builtin_fmaf(a1[j], b1[j], ss));
                     }
-                    SB;
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int t = wave + 8 * n, b = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, a = t - b * (b + 1) / 2;
+                    if (t < 10) dp[n] = mma(turned_rows(ul, u, 2, a), LG::tiles(gl, 16 * b, 0, lane), dp[n]);
+                }
+            }
+            __syncthreads();
+            asm volatile("" : "+v"(lane));
+            {
+                const int col = lane & 15, g4 = 4 * (lane >> 4);
+                const Frag<MADE> zm = LZ::tiles(zl, 16 * row, 0, lane);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) az[d] = mma(turned_rows(sl, s0, NK, half * ND + d), zm, az[d]);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int t = wave + 8 * n, b = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, a = t - b * (b + 1) / 2;
+                    if (t < 10) da[n] = mma(turned_rows(ul, u, 2, a), LZ::tiles(zl, 16 * b, 0, lane), da[n]);
+                }
+                const long long place = first + 16 * row + col, step = c.step(p, place);
+                const bool there = place < c.len;
+                f32x4 lo, hi;
+                sum_tiles(zm, lo, hi);
+                if (half) lo = hi;
+                const int here = at + 16 * half + g4;
+                const f32x4 v = load_four((const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t, there, here, p.dv, p.vec & kVecV);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) zv = __builtin_fmaf(lo[j], v[j], zv);
+                if (p.gv && place < p.T)
+                    store_four((T*)p.gv + c.at(p.gvs, c.hv) + step * p.gvs.t, here, p.dv, there ? lo * s.beta[16 * row + col] : zero, p.vec & kVecGv);
+            }
+        }
+        __syncthreads();
+        asm volatile("" : "+v"(lane));
+        const int col = lane & 15, g = lane >> 4, g4 = 4 * g, me = 16 * row + col;
+        const bf16x4 unit = unit_half(lane);
+        {
+            const float D = s.D[me], E = s.E[me], sD = p.scale * D, Db = -D * s.beta[me];
+            float qd = 0.f, kz = 0.f, ku = 0.f;
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                const int dc = 16 * (half * ND + d);
+                const f32x4 qv = sum_of(L::half(q, 16 * row, dc, lane)), kv = sum_of(L::half(k, 16 * row, dc, lane));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    qd = __builtin_fmaf(qv[r], aq[d][r], qd);
+                    kz = __builtin_fmaf(kv[r], az[d][r], kz);
+                    ku = __builtin_fmaf(kv[r], au[d][r], ku);
+                }
+                gq[d] += aq[d] * sD, gk[d] += az[d] * Db + au[d] * E;
+            }
+            qd = group_sum(qd), kz = group_sum(kz), ku = group_sum(ku), zv = group_sum(zv);
+            const float dot = g == 0 ? qd : g == 1 ? kz : g == 2 ? ku : zv;
+            dots[(g * 2 + half) * 64 + me] = dot;
+            ss = group_sum(sixteen_sum(ss));
+            if (lane == 0) inner[wave] = ss;
+        }
+        f32x4 xs[2], ys[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const int t = wave + 8 * n, b = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, a = t - b * (b + 1) / 2;
+            if (t >= 10) continue;
+            f32x4 qk = zero, kk = zero;
+#pragma unroll
+            for (int i = 0; i < DK; i += 32) {
+                const Frag<RAW> kt = L::natural(k, 16 * a, i, lane);
+                qk = mma(kt, L::natural(q, 16 * b, i, lane), qk);
+                kk = mma(kt, L::natural(k, 16 * b, i, lane), kk);
+            }
+            const TileDecay decay(s, 16 * b + col, 16 * a + g4, true);
+            float rn = 0.f, rb = 0.f;
+            f32x4 cn;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool below = a != b || g4 + r < col, at_all = below || (a == b && g4 + r == col);
+                const float A = below ? -decay.G[r] * da[n][r] : 0.f;
+                xs[n][r] = at_all ? p.scale * decay.G[r] * dp[n][r] : 0.f;
+                ys[n][r] = decay.beta[r] * A;
+                cn[r] = (below ? xs[n][r] * qk[r] : 0.f) + ys[n][r] * kk[r];   // (the diagonal of N is in both sums: it cancels)
+                rn += cn[r], rb += A * kk[r];
+            }
+            rn = group_sum(rn), rb = group_sum(rb);
+            if (g == 0) rows_n[a * 64 + 16 * b + col] = rn, rows_b[a * 64 + 16 * b + col] = rb;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) cn[r] = sixteen_sum(cn[r]);
+            if (col == 0) *reinterpret_cast<f32x4*>(cols_n + b * 64 + 16 * a + g4) = cn;
+        }
+        // to all: tiles of x and of y, as they are (lane = i) and turned (lane = j)
+#pragma unroll
+        for (int round = 0; round < S::kRounds; ++round) {
+            if (round) __syncthreads();
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int t = wave + 8 * n;
+                if (t >= 10) continue;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    if (S::kRounds == 2 && w != round) continue;
+                    bf16_t* to = tiles + (S::kRounds == 1 ? w * 2 : 0) * Blocks<MADE>::kValues;
+                    Half<MADE> h = split<MADE>(w ? ys[n] : xs[n]);
+                    Blocks<MADE>::put(to, t, h, lane);
+#pragma unroll
+                    for (int i = 0; i < MADE; ++i) h.p[i] = turned(h.p[i], unit);
+                    Blocks<MADE>::put(to + Blocks<MADE>::kValues, t, h, lane);
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                if (S::kRounds == 2 && w != round) continue;
+                const bf16_t *t1 = tiles + (S::kRounds == 1 ? w * 2 : 0) * Blocks<MADE>::kValues, *t2 = t1 + Blocks<MADE>::kValues;
+#pragma unroll
+                for (int j = 0; j < 5; ++j) {
+                    const bool mine = j <= row;   // a tile of this row of blocks, else one of this column
+                    const int t = mine ? j : j - 1;
+                    const Half<MADE> h = mine ? Blocks<MADE>::get(t1, Blocks<MADE>::at(row, t), lane) : Blocks<MADE>::get(t2, Blocks<MADE>::at(t, row), lane);
+                    const bf16_t* by = w || mine ? k : q;
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        const Half<RAW> r = L::down(by, 16 * t, 16 * (half * ND + d), lane);
+                        if (w == 0 && mine) gq[d] = mma(r, h, gq[d]);
+                        else gk[d] = mma(r, h, gk[d]);
+                    }
                 }
             }
         }
-
-        {
-        FRESH;
-        const float D = s.D[me], E = s.E[me], sD = p.scale * D, Db = -D * beta;
-        float qd = 0.f, kz = 0.f, ku = 0.f;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) {
-            const f32x4 qv = sum_of(L::half(q, 16 * wave, 16 * d, lane)), kv = sum_of(L::half(k, 16 * wave, 16 * d, lane));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                qd = __builtin_fmaf(qv[r], aq[d][r], qd);
-                kz = __builtin_fmaf(kv[r], az[d][r], kz);
-                ku = __builtin_fmaf(kv[r], au[d][r], ku);
-            }
-            gq[d] += aq[d] * sD, gk[d] += az[d] * Db + au[d] * E;
-        }
-        float rown = 0.f, coln = 0.f, db = 0.f;
-#pragma unroll
-        for (int j = 0; j < 5; ++j) {
-            const bool row = j <= wave;
-            const int t = row ? j : j - 1;
-            FRESH;
-            // lane = i, values = j: K of the tile by Q of this block; the other way: Q by K
-            const bf16_t *far = row ? k : q, *near = row ? q : k;
-            f32x4 qk = zero, kk = zero;
-#pragma unroll
-            for (int n = 0; n < DK; n += 32) {
-                qk = mma(L::natural(far, 16 * t, n, lane), L::natural(near, 16 * wave, n, lane), qk);
-                kk = mma(L::natural(k, 16 * t, n, lane), L::natural(k, 16 * wave, n, lane), kk);
-            }
-            const TileDecay decay(s, me, 16 * t + g4, row);
-            f32x4 x, y;
-            float n = 0.f;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool diagonal = t == wave, below = !diagonal || (row ? g4 + r < col : col < g4 + r), at_all = below || (diagonal && g4 + r == col);
-                const float A = below ? -decay.G[r] * da[j][r] : 0.f;
-                x[r] = at_all ? p.scale * decay.G[r] * dp[j][r] : 0.f;
-                y[r] = decay.beta[r] * A;
-                n += (below ? x[r] * qk[r] : 0.f) + y[r] * kk[r];   // (the diagonal of N is in both sums: it cancels)
-                db += row ? A * kk[r] : 0.f;
-            }
-            rown += row ? n : 0.f, coln += row ? 0.f : n;
-            const Half<MADE> xs = split<MADE>(x), ys = split<MADE>(y);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                const Half<RAW> kt = L::down(k, 16 * t, 16 * d, lane), ft = L::down(far, 16 * t, 16 * d, lane);
-                if (row) gq[d] = mma(ft, xs, gq[d]);
-                else gk[d] = mma(ft, xs, gk[d]);
-                gk[d] = mma(kt, ys, gk[d]);
-            }
-            SB;
-        }
-        rown = group_sum(rown), coln = group_sum(coln), db = group_sum(db), zv = group_sum(zv);
-        qd = group_sum(qd), kz = group_sum(kz), ku = group_sum(ku) * E;
-        if (g == 0) dcs[me] = rown - coln + sD * qd + Db * kz, dcs[kDeltaChunk + me] = ku;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) ss += __shfl_xor(ss, o);
-        if (lane == 0) dcs[2 * kDeltaChunk + wave] = ss;
-        const float gbeta = (zv - D * kz + db) * s.bslope[me];
-        if (p.gb && g == 0 && place < p.T) {
-            const long long to = c.at(p.ggs, c.hv) + step * p.ggs.t;
-            const float out = there ? gbeta : 0.f;
-            if (p.gates_f32) ((float*)p.gb)[to] = out;
-            else ((T*)p.gb)[to] = from_f32<T>(out);
-        }
-        __syncthreads();
         if (wave == 0) {
+            // the gates' gradients: a lane has a step
+            float n = 0.f, b = 0.f, dot[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                const int mine = lane >> 4;
+                if (t <= mine) n += rows_n[t * 64 + lane], b += rows_b[t * 64 + lane];
+                if (t >= mine) n -= cols_n[t * 64 + lane];
+                dot[t] = dots[t * 128 + lane] + dots[t * 128 + 64 + lane];
+            }
+            const float D = s.D[lane], x = s.E[lane] * dot[2];
             // sum of dc over i >= lane; x is subtracted from its own dc and added to the end's, so what is left is the x before this step
-            const float own = dcs[kDeltaChunk + lane];
-            double sum = dcs[lane], xs = own;
+            double sum = n + p.scale * D * dot[0] - D * s.beta[lane] * dot[1], before = x;
 #pragma unroll
             for (int o = 1; o < 64; o *= 2) {
-                const double behind = __shfl_down(sum, o), before = __shfl_up(xs, o);
+                const double behind = __shfl_down(sum, o), ahead = __shfl_up(before, o);
                 if (lane + o < 64) sum += behind;
-                if (lane >= o) xs += before;
+                if (lane >= o) before += ahead;
             }
-            sum += xs - own;
-            sum += (double)s.D[kDeltaChunk - 1] * ((dcs[128] + dcs[129]) + (dcs[130] + dcs[131]));
+            sum += before - x;
+            float in = 0.f;
+#pragma unroll
+            for (int w = 0; w < 8; ++w) in += inner[w];
+            sum += (double)s.D[kDeltaChunk - 1] * in;
             const long long i = first + lane;
-            if (p.gg && i < p.T) {
+            if (i < p.T) {
+                const bool there = i < c.len;
                 const long long to = c.at(p.ggs, c.hv) + c.step(p, i) * p.ggs.t;
-                const float out = i < c.len ? (float)sum * s.slope[lane] : 0.f;
-                if (p.gates_f32) ((float*)p.gg)[to] = out;
-                else ((T*)p.gg)[to] = from_f32<T>(out);
+                const float gg = there ? (float)sum * s.slope[lane] : 0.f, gb = there ? (dot[3] - D * dot[1] + b) * s.bslope[lane] : 0.f;
+                if (p.gates_f32) {
+                    if (p.gg) ((float*)p.gg)[to] = gg;
+                    if (p.gb) ((float*)p.gb)[to] = gb;
+                } else {
+                    if (p.gg) ((T*)p.gg)[to] = from_f32<T>(gg);
+                    if (p.gb) ((T*)p.gb)[to] = from_f32<T>(gb);
+                }
             }
-        }
         }
     }
     const int lane = threadIdx.x & 63, g4 = 4 * (lane >> 4);
-    const long long place = first + 16 * wave + (lane & 15), step = ck.step(p, place);
+    const long long place = first + 16 * row + (lane & 15), step = ck.step(p, place);
     const bool there = place < ck.len;
     if (place < p.T) {
         T *rq = (T*)p.gq + ck.at(p.gqs, ck.hk) + step * p.gqs.t, *rk = (T*)p.gk + ck.at(p.gqs, ck.hk) + step * p.gqs.t;
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            if (p.gq) store_four(rq, 16 * d + g4, p.dk, there ? gq[d] : zero, p.vec & kVecGqk);
-            if (p.gk) store_four(rk, 16 * d + g4, p.dk, there ? gk[d] : zero, p.vec & kVecGqk);
+            const int at = 16 * (half * ND + d) + g4;
+            if (p.gq) store_four(rq, at, p.dk, there ? gq[d] : zero, p.vec & kVecGqk);
+            if (p.gk) store_four(rk, at, p.dk, there ? gk[d] : zero, p.vec & kVecGqk);
         }
     }
 }

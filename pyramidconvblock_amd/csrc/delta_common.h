@@ -217,15 +217,15 @@ __device__ __forceinline__ bf16x4 turned(bf16x4 t, bf16x4 unit) {
 }
 
 // A tile as it was made (lane = column, values = rows; 8 bytes a lane and plane, planes `plane` values apart) from LDS, with lane = row, values = columns:
-// lane l of each 16 hands in column 4 g + l / 4, rows 4 (l % 4) .., and gets row l % 16, columns 4 g ...
-template <int NP>
+// lane l of each 16 hands in column 4 g + l / 4, rows 4 (l % 4) .., and gets row l % 16, columns 4 g ...  (WIDTH: values between lanes' pieces.)
+template <int NP, int WIDTH = 4>
 __device__ __forceinline__ Half<NP> read_turned(const bf16_t* base, int plane, int lane) {
     typedef __attribute__((address_space(3))) s16x4 lds_t;
     const int i = lane & 15, from = (i & 3) * 16 + 4 * (lane >> 4) + (i >> 2);
     Half<NP> f;
 #pragma unroll
     for (int p = 0; p < NP; ++p)
-        f.p[p] = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(__attribute__((address_space(3))) void*)(base + p * plane + from * 4)));
+        f.p[p] = __builtin_bit_cast(bf16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t*)(__attribute__((address_space(3))) void*)(base + p * plane + from * WIDTH)));
     return f;
 }
 
@@ -308,7 +308,7 @@ __device__ __forceinline__ bool chunk_of(const DeltaArgs& p, int H, int& chain, 
 // the chain's end and behind the row's end d.  By NT threads, this one `thread` of them.
 template <typename T, int NP, int R, int NT = 256>
 struct Staged {
-    static constexpr int N = kDeltaChunk * (R / 8) / NT;
+    static constexpr int ALL = kDeltaChunk * (R / 8), N = (ALL + NT - 1) / NT;
     T v[N][8];
     bool on[N];
     __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first, int col, int d, bool vec,
@@ -320,7 +320,7 @@ struct Staged {
             const int e = thread + n * NT;
             const long long i = first + e / (R / 8);
             at[n] = col + e % (R / 8) * 8;
-            on[n] = i < c.len && at[n] < d;
+            on[n] = i < c.len && at[n] < d && e < ALL;
             q[n] = base + (on[n] ? c.step(p, i) * st + at[n] : 0);
         }
         if (vec) {
@@ -345,6 +345,7 @@ struct Staged {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int e = thread + n * NT;
+            if (ALL % NT && e >= ALL) continue;
             Frag<NP> f = planes_of<T, NP>(v[n]);
 #pragma unroll
             for (int m = 0; m < NP; ++m) {
@@ -355,22 +356,22 @@ struct Staged {
     }
 };
 
-// A plain run of 16-byte pieces from memory to LDS, by 256 threads.
-template <int BYTES>
+// A plain run of 16-byte pieces from memory to LDS, by NT threads.
+template <int BYTES, int NT = 256>
 struct Run {
-    static constexpr int N = (BYTES / 16 + 255) / 256;
+    static constexpr int N = (BYTES / 16 + NT - 1) / NT;
     f32x4 v[N];
     __device__ __forceinline__ void load(const void* from) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int e = threadIdx.x + n * 256;
+            const int e = threadIdx.x + n * NT;
             v[n] = load_at<f32x4>(from, (e < BYTES / 16 ? e : 0) * 16);
         }
     }
     __device__ __forceinline__ void put(void* to) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int e = threadIdx.x + n * 256;
+            const int e = threadIdx.x + n * NT;
             if (e < BYTES / 16) *reinterpret_cast<f32x4*>((char*)to + e * 16) = v[n];
         }
     }

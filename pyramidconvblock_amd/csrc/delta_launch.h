@@ -57,8 +57,8 @@ void delta_backward(const DeltaArgs& p, hipStream_t s) {
     const long long chunks = delta_chunk_grid(p, p.Hv);
     delta_launch(delta_back_prepare_k<T, DK, CP>, delta_back_prepare_lds<T, DK, CP>(), once[0], chunks, 256, p, s);
     delta_all_chains<T, DK, true, CP>(p, s);
-    if (p.Hv > p.Hk) delta_launch(delta_grads_k<T, DK, true>, delta_grads_lds<T, DK>(), once[1], delta_chunk_grid(p, p.Hk), 256, p, s);
-    else delta_launch(delta_grads_k<T, DK, false>, delta_grads_lds<T, DK>(), once[2], chunks, 256, p, s);
+    if (p.Hv > p.Hk) delta_launch(delta_grads_k<T, DK, true>, delta_grads_lds<T, DK>(), once[1], delta_chunk_grid(p, p.Hk), kGradsThreads, p, s);
+    else delta_launch(delta_grads_k<T, DK, false>, delta_grads_lds<T, DK>(), once[2], chunks, kGradsThreads, p, s);
 }
 
 // The gradient of an initial state is a result in 32 bits; the others of 16-bit tensors are rounded to those.
