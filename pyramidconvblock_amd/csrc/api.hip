@@ -955,7 +955,7 @@ int pdw_rotary_bwd(const pdw_rotary* c, const void* const gy[2], void* const gx[
 static int delta_args(const char* fn, const pdw_delta* c, DeltaArgs& p) {
     if (!c) return set_error("%s: null pointer", fn), 1;
     if (!valid_dtype(c->dtype)) return set_error("%s: unknown dtype %d", fn, c->dtype), 1;
-    if (c->O < 0 || c->W < 0 || c->T < 0 || c->T > 0x7fffffffLL || c->Hk < 0 || c->Hv < 0)
+    if (c->O < 0 || c->W < 0 || c->T < 0 || c->T > 0x7fffffffLL - kDeltaChunk || c->Hk < 0 || c->Hv < 0)
         return set_error("%s: bad extents O=%d T=%lld W=%d heads=%d,%d", fn, c->O, c->T, c->W, c->Hk, c->Hv), 1;
     if (c->dk < 1 || c->dk > PDW_DELTA_MAX_CHANNELS || c->dv < 1 || c->dv > PDW_DELTA_MAX_CHANNELS)
         return set_error("%s: %d and %d channels of a head, 1 to %d are possible", fn, c->dk, c->dv, PDW_DELTA_MAX_CHANNELS), 1;
@@ -968,7 +968,7 @@ static int delta_args(const char* fn, const pdw_delta* c, DeltaArgs& p) {
     p.qs = strides(c->qs), p.ks = strides(c->ks), p.vs = strides(c->vs), p.gs = strides(c->gs), p.bs = strides(c->bs);
     auto dense = [&](long long H, long long d) { return DeltaStrides{c->T * c->W * H * d, c->W * H * d, H * d, d}; };
     p.ys = dense(c->Hv, c->dv), p.gqs = dense(c->Hk, c->dk), p.gvs = p.ys, p.ggs = dense(c->Hv, 1);
-    p.h0 = c->h0, p.lengths = c->lengths, p.T = c->T, p.O = c->O, p.W = c->W, p.Hk = c->Hk, p.Hv = c->Hv, p.dk = c->dk, p.dv = c->dv;
+    p.h0 = c->h0, p.lengths = c->lengths, p.T = (int)c->T, p.O = c->O, p.W = c->W, p.Hk = c->Hk, p.Hv = c->Hv, p.dk = c->dk, p.dv = c->dv;
     p.chains = (int)(rows * c->Hv), p.reverse = c->reverse != 0, p.logits = c->logits != 0, p.gates_f32 = c->gates_f32 != 0, p.scale = c->scale;
     return 0;
 }

@@ -113,7 +113,9 @@ int delta_run(const DeltaArgs& in, void* states, bool backward, void* workspace,
     DeltaArgs p = in;
     if (!backward && !states && delta_few_steps(p.T)) return delta_steps_run(p, dtype, s);
     const DeltaPlan d(p.chains, p.T, p.dk, p.dv, backward, p.gh0 != nullptr, dtype);
-    p.NC = d.NC, p.dvp = d.dvp, p.seg = d.seg, p.segments = d.segments;
+    // (workgroups are counted in 32 bits; the buffers of so many chunks would not fit the card)
+    if (p.chains * d.NC > 1 << 28) return set_error("delta: more than 2^28 chunks"), 1;
+    p.NC = (int)d.NC, p.dvp = d.dvp, p.seg = (int)d.seg, p.segments = d.segments;
     const size_t need = workspace_bytes_of(p.chains, d, backward, states != nullptr);
     if (need && (!workspace || workspace_bytes < need))
         return set_error("delta: workspace too small (%zu of %zu bytes)", workspace_bytes, need), 1;

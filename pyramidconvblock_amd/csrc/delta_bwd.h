@@ -46,9 +46,10 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
     DeltaGates& s = *(DeltaGates*)(pb + Blocks<MADE>::kValues);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int chain;
-    long long m;
+    int m;
     if (!chunk_of(p, p.Hv, chain, m)) return;
-    const long long id = chain * p.NC + m, first = m * kDeltaChunk;
+    const long long id = (long long)chain * p.NC + m;
+    const int first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
     const DeltaSizes z(DK, p.dvp, DeltaPlanes<T>::kMade, MADE);
 
@@ -90,7 +91,7 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
         for (int b = 0; b < 4; ++b)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const long long i = first + 16 * b + g4 + r;
+                const int i = first + 16 * b + g4 + r;
                 const bool on = i < c.len && at < p.dv;
                 v[b][r] = gy[on ? c.step(p, i) * p.ys.t : -(long long)at];   // (what is not there is read from the first row and dropped)
                 if (!on) v[b][r] = from_f32<T>(0.f);
@@ -178,6 +179,12 @@ constexpr int delta_grads_lds() {
     return GradsLds<T, DK>::kBytes;
 }
 
+// Wavefronts of a SIMD that registers are to be left for: two workgroups of a CU where their LDS lets them be.
+template <typename T, int DK, bool SHARED>
+constexpr int delta_grads_waves() {
+    return !SHARED && delta_grads_lds<T, DK>() <= 80 * 1024 ? 4 : 2;
+}
+
 // A sum over 16 neighbouring lanes, in all of them.
 __device__ __forceinline__ float sixteen_sum(float v) {
     v = dpp_add<0xB1>(v), v = dpp_add<0x4E>(v), v = dpp_add<0x141>(v);
@@ -188,7 +195,7 @@ __device__ __forceinline__ float sixteen_sum(float v) {
 // round the wavefronts (lane = step i, values = steps j); what becomes of them goes to all through LDS, both ways round.  SHARED: value
 // heads share key heads.
 template <typename T, int DK, bool SHARED>
-__global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4) void delta_grads_k(DeltaArgs p) {
+__global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())) void delta_grads_k(DeltaArgs p) {
     typedef GradsLds<T, DK> S;
     constexpr int RAW = S::RAW, MADE = S::MADE, NT = kGradsThreads, COLS = kGradsCols, ND = DK / 32, NK = DK / 32;   // ND: tiles of this half
     typedef Rows<RAW, kDeltaChunk, DK> L;
@@ -202,10 +209,10 @@ __global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4)
     float *rows_n = (float*)(&s + 1), *cols_n = rows_n + 256, *rows_b = cols_n + 256, *dots = rows_b + 256, *inner = dots + 512;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), row = wave & 3, half = wave >> 2;
     int kchain;
-    long long m;
+    int m;
     if (!chunk_of(p, p.Hk, kchain, m)) return;
     const int group = SHARED ? p.Hv / p.Hk : 1;
-    const long long first = m * kDeltaChunk;
+    const int first = m * kDeltaChunk;
     const int chain0 = SHARED ? kchain / p.Hk * p.Hv + kchain % p.Hk * group : kchain;
     const DeltaSizes z(DK, p.dvp, MADE, MADE);
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -221,7 +228,7 @@ __global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4)
     for (int e = 0; e < group; ++e) {
         const int chain = chain0 + e;
         const DeltaChain c(p, chain);
-        const long long id = chain * p.NC + m;
+        const long long id = (long long)chain * p.NC + m;
         // (a lane that the compiler takes for another one with every head, and in every part below: else it keeps all addresses of all parts, in
         // scratch memory)
         int lane = threadIdx.x & 63;
@@ -326,7 +333,7 @@ __global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4)
                     const int t = wave + 8 * n, b = t < 1 ? 0 : t < 3 ? 1 : t < 6 ? 2 : 3, a = t - b * (b + 1) / 2;
                     if (t < 10) da[n] = mma(turned_rows(ul, u, 2, a), LZ::tiles(zl, 16 * b, 0, lane), da[n]);
                 }
-                const long long place = first + 16 * row + col, step = c.step(p, place);
+                const int place = first + 16 * row + col, step = c.step(p, place);
                 const bool there = place < c.len;
                 f32x4 lo, hi;
                 sum_tiles(zm, lo, hi);
@@ -457,7 +464,7 @@ __global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4)
 #pragma unroll
             for (int w = 0; w < 8; ++w) in += inner[w];
             sum += (double)s.D[kDeltaChunk - 1] * in;
-            const long long i = first + lane;
+            const int i = first + lane;
             if (i < p.T) {
                 const bool there = i < c.len;
                 const long long to = c.at(p.ggs, c.hv) + c.step(p, i) * p.ggs.t;
@@ -473,7 +480,7 @@ __global__ __launch_bounds__(kGradsThreads, DK == 128 || sizeof(T) == 4 ? 2 : 4)
         }
     }
     const int lane = threadIdx.x & 63, g4 = 4 * (lane >> 4);
-    const long long place = first + 16 * row + (lane & 15), step = ck.step(p, place);
+    const int place = first + 16 * row + (lane & 15), step = ck.step(p, place);
     const bool there = place < ck.len;
     if (place < p.T) {
         T *rq = (T*)p.gq + ck.at(p.gqs, ck.hk) + step * p.gqs.t, *rk = (T*)p.gk + ck.at(p.gqs, ck.hk) + step * p.gqs.t;

@@ -46,13 +46,11 @@ constexpr int delta_chain_lds() {
 // What a workgroup's index stands for: segments of a chain's column parts; the parts of a chain, which read the same operands, on one die (workgroups go to
 // the eight dies in turn).
 __device__ __forceinline__ bool chain_part(const DeltaArgs& p, int parts, int segments, int& chain, int& part, int& segment) {
-    const long long id = p.first + blockIdx.x;
-    long long turn = id >> 3;
-    part = (int)(turn % parts), turn /= parts;
-    segment = (int)(turn % segments);
-    const long long n = turn / segments * 8 + (id & 7);
-    chain = (int)n;
-    return n < p.chains;
+    const unsigned id = (unsigned)p.first + blockIdx.x, turn = id >> 3, turns = turn / (unsigned)parts, round = turns / (unsigned)segments;
+    part = (int)(turn - turns * parts);
+    segment = (int)(turns - round * segments);
+    chain = (int)(round * 8 + (id & 7));
+    return chain < p.chains;
 }
 
 // Wavefronts that carry columns, at least (and as many fetch): with 64 channels fewer had no registers for what they fetch.
@@ -85,24 +83,24 @@ struct ChainFetch {
             for (int q = 0; q < CP; ++q) *reinterpret_cast<bf16x4*>(to + q * (kDeltaChunk * DK) + (i * NT + thread) * 4) = h.p[q];
         }
     }
-    __device__ __forceinline__ void load_k(const DeltaArgs& p, const DeltaChain& c, long long chunk, int thread) {
+    __device__ __forceinline__ void load_k(const DeltaArgs& p, const DeltaChain& c, int chunk, int thread) {
         k.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, chunk * kDeltaChunk, 0, p.dk, p.vec & kVecK, thread);
     }
 };
 
 template <typename T, int DK, bool BACK, int CP, int NT, int AHEAD>
-__device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes& z, int chain, long long chunk, long long by, long long n, bf16_t* lw, bf16_t* lk,
+__device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes& z, int chain, int chunk, int by, int n, bf16_t* lw, bf16_t* lk,
                                             int thread) {
     const DeltaChain c(p, chain);
-    const long long id = chain * p.NC + chunk;
+    const long long id = (long long)chain * p.NC + chunk;
     ChainFetch<T, DK, CP, NT> f[AHEAD];
     // A is what the first product takes, B the second's: W and K, or (BACK) K and W
-    auto fetch_a = [&](int j, long long m) {
+    auto fetch_a = [&](int j, int m) {
         if (m >= n) return;
         if constexpr (BACK) f[j].load_k(p, c, chunk + m * by, thread);
         else f[j].load_w(p, z, id + m * by, thread);
     };
-    auto fetch_b = [&](int j, long long m) {
+    auto fetch_b = [&](int j, int m) {
         if (m >= n) return;
         if constexpr (BACK) f[j].load_w(p, z, id + m * by, thread);
         else f[j].load_k(p, c, chunk + m * by, thread);
@@ -120,10 +118,10 @@ __device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes
     put_a(0);
     fetch_a(0, AHEAD);
     __syncthreads();
-    for (long long m0 = 0; m0 < n; m0 += AHEAD) {
+    for (int m0 = 0; m0 < n; m0 += AHEAD) {
 #pragma unroll
         for (int j = 0; j < AHEAD; ++j) {
-            const long long m = m0 + j;
+            const int m = m0 + j;
             if (m >= n) break;
             put_b(j);
             fetch_b(j, m + AHEAD);
@@ -150,8 +148,9 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
     if (!chain_part(p, (cols + WAVES - 1) / WAVES, MAPS ? p.segments - 1 : p.segments, chain, part, segment)) return;
     const DeltaSizes z(DK, p.dvp, MADE, CP);
     // chunks in the chain's order: n of them from `from`, each `by` behind the last
-    const long long place = segment * p.seg, n = p.NC - place < p.seg ? p.NC - place : p.seg;
-    const long long by = BACK ? -1 : 1, chunk = BACK ? p.NC - 1 - place : place, from = chain * p.NC + chunk;
+    const int place = segment * p.seg, n = p.NC - place < p.seg ? p.NC - place : p.seg;
+    const int by = BACK ? -1 : 1, chunk = BACK ? p.NC - 1 - place : place;
+    const long long from = (long long)chain * p.NC + chunk;
 
     if (wave >= WAVES)
         return chain_fetch<T, DK, BACK, CP, 64 * WAVES, AHEAD>(p, z, chain, chunk, by, n, lw, lk, threadIdx.x - 64 * WAVES);
@@ -198,10 +197,11 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
     for (int j = 0; j < AHEAD; ++j)
         if (j < n) fetch(chunks[j], from + j * by);
     __syncthreads();
-    for (long long m0 = 0; m0 < n; m0 += AHEAD)
+    for (int m0 = 0; m0 < n; m0 += AHEAD)
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
-        const long long m = m0 + j, id = from + m * by;
+        const int m = m0 + j;
+        const long long id = from + m * by;
         if (m >= n) break;
         const Chunk& c = chunks[j];
         f32x4 c0[BACK ? ND : 1];
@@ -316,8 +316,8 @@ __global__ __launch_bounds__(DK * 4) void delta_join_k(DeltaArgs p) {
     constexpr int NK = DK / 32;
     __shared__ __align__(16) bf16_t lx[2][NK * CP * 512];
     const int lane = threadIdx.x & 63, d = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), colv = p.dvp / 16;
-    const long long id = p.first + blockIdx.x;
-    const int chain = (int)(id / colv), cv = (int)(id - (long long)chain * colv);
+    const unsigned id = (unsigned)p.first + blockIdx.x;
+    const int chain = (int)(id / (unsigned)colv), cv = (int)(id - (unsigned)chain * colv);
     const DeltaSizes z(DK, p.dvp, 1, CP);
     const float* h = BACK ? p.glast : p.h0;
     const int at = 16 * cv + (lane & 15);

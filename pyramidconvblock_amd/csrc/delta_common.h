@@ -41,7 +41,7 @@ struct DeltaArgs {
     struct DeltaGates* gates;
     bf16_t* maps;                          // by chain and segment: the map's matrix, and what it adds
     float* shifts;
-    long long T, NC, seg;                  // steps; chunks of a chain, of a segment
+    int T, NC, seg;                        // steps; chunks of a chain, of a segment
     int segments;
     int O, W, Hk, Hv, dk, dv, dvp;         // dvp: dv up to whole 32s
     int chains;                            // O * W * Hv, one state each
@@ -275,7 +275,7 @@ struct Rows {
 // Where a chain stands in its tensors.
 struct DeltaChain {
     int o, w, hv, hk;
-    long long len;   // valid steps
+    int len;   // valid steps
     __device__ __forceinline__ DeltaChain(const DeltaArgs& p, int chain) {
         hv = chain % p.Hv;
         const int ow = chain / p.Hv;
@@ -284,23 +284,23 @@ struct DeltaChain {
         len = p.T;
         if (p.lengths) {
             const int n = p.lengths[o];
-            len = n < 0 ? 0 : n < p.T ? n : p.T;
+            len = n < 0 ? 0 : n < len ? n : len;
         }
     }
     // The step at place i of the chain: from the end of what is valid with `reverse`, and places behind it for themselves.
-    __device__ __forceinline__ long long step(const DeltaArgs& p, long long i) const { return p.reverse && i < len ? len - 1 - i : i; }
+    __device__ __forceinline__ int step(const DeltaArgs& p, int i) const { return p.reverse && i < len ? len - 1 - i : i; }
     __device__ __forceinline__ long long at(const DeltaStrides& s, int head) const { return o * s.o + w * s.w + head * s.h; }
 };
 
 // Workgroup -> chunk m of a chain: the heads (H of them) of a chunk follow one another on one die (workgroups go to the eight dies in turn), since rows of
 // neighbouring heads share lines of memory, which a die's cache holds.  false: there is none.
-__device__ __forceinline__ bool chunk_of(const DeltaArgs& p, int H, int& chain, long long& m) {
-    const long long id = p.first + blockIdx.x, turn = id >> 3;
-    const int head = (int)(turn % H);
-    const long long place = turn / H * 8 + (id & 7), row = place / p.NC;   // (batch element, chunk)
-    m = place - row * p.NC;
-    chain = (int)row * H + head;
-    return row < (long long)p.O * p.W;
+// (indexes in 32 bits, delta_run sees to it: divisions in 64 were a fifth of a wavefront's instructions in these kernels)
+__device__ __forceinline__ bool chunk_of(const DeltaArgs& p, int H, int& chain, int& m) {
+    const unsigned id = (unsigned)p.first + blockIdx.x, turn = id >> 3, turns = turn / (unsigned)H;
+    const unsigned place = turns * 8 + (id & 7), row = place / (unsigned)p.NC;   // (batch element, chunk)
+    m = (int)(place - row * (unsigned)p.NC);
+    chain = (int)(row * H + (turn - turns * H));
+    return row < (unsigned)(p.O * p.W);
 }
 
 // A chunk of a tensor's rows, columns [col, col + R), on its way to LDS: `load` makes the loads, all without a condition where rows lie in pieces of
@@ -311,17 +311,17 @@ struct Staged {
     static constexpr int ALL = kDeltaChunk * (R / 8), N = (ALL + NT - 1) / NT;
     T v[N][8];
     bool on[N];
-    __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, long long first, int col, int d, bool vec,
+    __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, int first, int col, int d, bool vec,
                                          int thread = threadIdx.x) {
         int at[N];
         const T* q[N];
 #pragma unroll
         for (int n = 0; n < N; ++n) {
             const int e = thread + n * NT;
-            const long long i = first + e / (R / 8);
+            const int i = first + e / (R / 8);
             at[n] = col + e % (R / 8) * 8;
             on[n] = i < c.len && at[n] < d && e < ALL;
-            q[n] = base + (on[n] ? c.step(p, i) * st + at[n] : 0);
+            q[n] = base + (on[n] ? (long long)c.step(p, i) * st + at[n] : 0);
         }
         if (vec) {
             constexpr int VEC = 16 / sizeof(T);
@@ -415,8 +415,8 @@ __device__ __forceinline__ void write_strength(float b, int logits, float& beta,
 struct GateMaker {
     float g, b;
     bool on;
-    __device__ __forceinline__ void load(const DeltaArgs& p, const DeltaChain& c, long long first, int type) {
-        const long long i = first + (threadIdx.x & 63);
+    __device__ __forceinline__ void load(const DeltaArgs& p, const DeltaChain& c, int first, int type) {
+        const int i = first + (threadIdx.x & 63);
         on = i < c.len;
         const long long t = on ? c.step(p, i) : 0;
         g = gate_value(p.g, c.at(p.gs, c.hv) + t * p.gs.t, p.gates_f32, type);

@@ -32,8 +32,15 @@ constexpr int delta_prepare_lds() {
            (int)sizeof(DeltaGates);
 }
 
+// Wavefronts of a SIMD that registers are to be left for: as many as LDS has room for, up to four.
 template <typename T, int DK>
-__global__ __launch_bounds__(256, 4) void delta_prepare_k(DeltaArgs p) {
+constexpr int delta_prepare_waves() {
+    const int n = 160 * 1024 / delta_prepare_lds<T, DK>();
+    return n > 4 ? 4 : n;
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_prepare_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = kChainPlanes;
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     constexpr int COLS = delta_prepare_cols<T, DK>();
@@ -45,9 +52,10 @@ __global__ __launch_bounds__(256, 4) void delta_prepare_k(DeltaArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = 4 * (lane >> 4);
     int chain;
-    long long m;
+    int m;
     if (!chunk_of(p, p.Hv, chain, m)) return;
-    const long long id = chain * p.NC + m, first = m * kDeltaChunk;
+    const long long id = (long long)chain * p.NC + m;
+    const int first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
 
     GateMaker gates;
@@ -136,9 +144,10 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g4 = 4 * (lane >> 4);
     int chain;
-    long long m;
+    int m;
     if (!chunk_of(p, p.Hv, chain, m)) return;
-    const long long id = chain * p.NC + m, first = m * kDeltaChunk;
+    const long long id = (long long)chain * p.NC + m;
+    const int first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
 
     Run<sizeof(DeltaGates)> gates;
@@ -169,7 +178,7 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
 #pragma unroll
     for (int n = 0; n < DK / 32; ++n) qf[n] = L::tiles(q, 16 * wave, 32 * n, lane);
     const float D = p.scale * s.D[i];
-    const long long step = first + i;
+    const int step = first + i;
     const bool there = step < c.len;
     T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
     const DeltaSizes z(DK, p.dvp, MADE, MADE);
