@@ -399,6 +399,7 @@ __device__ __forceinline__ void log_decay(float g, int logits, float& la, float&
         slope = (g < 0.f ? 1.f : e) / (1.f + e);   // sigmoid(-g)
         if (g != g) la = slope = g;
     }
+    if (la < -104.f) slope = 0.f;   // e^la is 0 in 32 bits, and so is the gradient, which the backward sums of terms that cancel
     if (la < -1e4f) la = -1e4f;
 }
 __device__ __forceinline__ void write_strength(float b, int logits, float& beta, float& slope) {

@@ -8,7 +8,8 @@
 // Bound by memory: a row's channels stay in registers between one load and one store.  A unit is 2 VEC channels, VEC whole pairs (or channels
 // behind the pairs); a row has up to LPR lanes with a unit each, so its sum is a few exchanges in the vector unit.  A workgroup has TT tokens:
 // it makes their cosines and sines once, into LDS, for all heads of q and k.  An angle counts in turns and in 64 bits up to the nearest
-// quarter: what is left is below 1/8 of a turn and exact to 2^-28, at positions up to 2^31 as at 0; cosine and sine of that are their series.
+// quarter: what is left is below 1/8 of a turn and off by some 2^-53 of the angle itself (2^-24 of a turn at position 2^31, nothing that counts at 2^20);
+// cosine and sine of that are their series.
 #pragma once
 #include "common.h"
 #include "row_norm.h"

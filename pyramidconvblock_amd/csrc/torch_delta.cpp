@@ -69,8 +69,9 @@ struct RotaryNode : public torch::autograd::Node {
             // (without a norm the input itself is not read)
             call.x[s] = xs[s].defined() ? ptr(xs[s]) : ptr(gy[s]);
         }
-        params.make(options, c.tokens == 0);
-        if (c.tokens == 0) return out;
+        const bool none = c.tokens == 0 || (call.heads[0] == 0 && call.heads[1] == 0);
+        params.make(options, none);
+        if (none) return out;
         pos = packed(pos), freq = packed(freq);
         call.positions = ptr(pos), call.frequencies = (const float*)ptr(freq);
         Tensor work;
