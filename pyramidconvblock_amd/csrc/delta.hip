@@ -35,7 +35,8 @@ struct DeltaPlan {
           segments(NC ? (int)((NC + seg - 1) / seg) : 1), dvp(padded_dv(dv)) {}
 };
 
-// Steps up to which a call without gradients goes step by step.
+// Steps up to which a call without gradients goes step by step: a step takes 1.6 us (1 to 64 streams of 8 heads of 64 channels in bf16: 10.5 us for 8, 16.5
+// for 16, 22.5 for 24), a chunk's launches 20.4 whatever its steps; with 128 channels 37, 61 and 84 against 70, for 256 streams 50, 85 and 120 against 96.
 constexpr long long kDeltaFewSteps = 16;
 bool delta_few_steps(long long T) { return T <= kDeltaFewSteps; }
 
