@@ -234,10 +234,26 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
         int lane = threadIdx.x & 63;
         if (SHARED) asm volatile("" : "+v"(lane)::"memory");
         const bf16_t *s0 = p.s0 + id * z.state, *ds1 = p.ds1 + id * z.state, *u = p.u + id * z.u;
+        // what a round of columns takes: dY, states, U, and dU without dS1's part
+        Staged<T, RAW, COLS, NT> gs;
+        Run<S::kState * 2, NT> rs, rd;
+        Run<S::kU * 2, NT> ru;
+        f32x4 x[4];
+        auto fetch = [&](int at) {
+            const int cw = at / 16;
+            gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
+            if constexpr (S::kStage)
+                rs.load(s0 + cw * NK * MADE * 512), rd.load(ds1 + cw * NK * MADE * 512), ru.load(u + cw * 2 * MADE * 512);
+            if (wave < 2) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(p.du + id * z.cols + (cw + wave) * 1024 + b * 256, lane * 16);
+            }
+        };
         {
             Run<sizeof(DeltaGates), NT> gates;
             Run<Blocks<MADE>::kValues * 2, NT> system;
             gates.load(p.gates + id), system.load(p.blocks + id * z.blocks);
+            fetch(0);
             if (e) __syncthreads();
             if (e == 0) ks.put(k), qs.put(q);
             gates.put(&s), system.put(blocks);
@@ -251,25 +267,12 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
         float zv = 0.f, ss = 0.f;       // Z_i.V_i; <S0, dS1>
         for (int at = 0; at < p.dvp; at += COLS) {
             const int cw = at / 16;
-            {
-                Staged<T, RAW, COLS, NT> gs;
-                gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
-                if constexpr (S::kStage) {
-                    Run<S::kState * 2, NT> rs, rd;
-                    Run<S::kU * 2, NT> ru;
-                    rs.load(s0 + cw * NK * MADE * 512), rd.load(ds1 + cw * NK * MADE * 512), ru.load(u + cw * 2 * MADE * 512);
-                    if (at) __syncthreads();
-                    rs.put(sl), rd.put(dl), ru.put(ul);
-                } else if (at) {
-                    __syncthreads();
-                }
-                gs.put(gl);
+            if (at) {
+                fetch(at);
+                __syncthreads();
             }
-            f32x4 x[4];
-            if (wave < 2) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(p.du + id * z.cols + (cw + wave) * 1024 + b * 256, lane * 16);
-            }
+            if constexpr (S::kStage) rs.put(sl), rd.put(dl), ru.put(ul);
+            gs.put(gl);
             __syncthreads();
             asm volatile("" : "+v"(lane));
             const bf16x4 unit = unit_half(lane);
@@ -452,14 +455,9 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
             }
             const float D = s.D[lane], x = s.E[lane] * dot[2];
             // sum of dc over i >= lane; x is subtracted from its own dc and added to the end's, so what is left is the x before this step
-            double sum = n + p.scale * D * dot[0] - D * s.beta[lane] * dot[1], before = x;
-#pragma unroll
-            for (int o = 1; o < 64; o *= 2) {
-                const double behind = __shfl_down(sum, o), ahead = __shfl_up(before, o);
-                if (lane + o < 64) sum += behind;
-                if (lane >= o) before += ahead;
-            }
-            sum += before - x;
+            const double dc = n + p.scale * D * dot[0] - D * s.beta[lane] * dot[1];
+            double sum = __shfl(sums_up_to(__shfl(dc, 63 - lane)), 63 - lane);   // (lanes the other way round, and back)
+            sum += sums_up_to(x) - x;
             float in = 0.f;
 #pragma unroll
             for (int w = 0; w < 8; ++w) in += inner[w];

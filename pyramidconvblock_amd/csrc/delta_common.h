@@ -412,6 +412,24 @@ __device__ __forceinline__ void write_strength(float b, int logits, float& beta,
     }
 }
 
+// Sums over a wavefront's lanes up to each, in 64 bits: moves within rows of 16 lanes and from row to row, no exchange through LDS.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double lanes_before(double v) {
+    const unsigned long long bits = __builtin_bit_cast(unsigned long long, v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)bits, CTRL, ROWS, 0xf, false);
+    const unsigned hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(bits >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);   // (0 where there is no such lane)
+}
+__device__ __forceinline__ double sums_up_to(double v) {
+    v += lanes_before<0x111, 0xf>(v);   // 1, 2, 4 and 8 lanes before
+    v += lanes_before<0x112, 0xf>(v);
+    v += lanes_before<0x114, 0xf>(v);
+    v += lanes_before<0x118, 0xf>(v);
+    v += lanes_before<0x142, 0xa>(v);   // the last lane of row 0 to row 1, of row 2 to row 3
+    v += lanes_before<0x143, 0xc>(v);   // of row 1 to rows 2 and 3
+    return v;
+}
+
 // Made by the first wavefront, in two steps (loads ahead of others; the rest), into LDS and memory; the caller's barrier follows.
 struct GateMaker {
     float g, b;
@@ -429,13 +447,7 @@ struct GateMaker {
         log_decay(g, p.logits, la, slope);
         write_strength(b, p.logits, beta, bslope);
         if (!on) la = slope = beta = bslope = 0.f;
-        double sum = la * 1.4426950408889634;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const double other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
-        }
-        const double end = __shfl(sum, 63);
+        const double sum = sums_up_to(la * 1.4426950408889634), end = __shfl(sum, 63);
         const float hi = (float)sum, lo = (float)(sum - (double)hi), D = __builtin_amdgcn_exp2f(hi), E = __builtin_amdgcn_exp2f((float)(end - sum));
         s.hi[lane] = to->hi[lane] = hi, s.lo[lane] = to->lo[lane] = lo, s.beta[lane] = to->beta[lane] = beta;
         s.D[lane] = to->D[lane] = D, s.E[lane] = to->E[lane] = E;
