@@ -155,6 +155,21 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
     qs.load((const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
     gates.load(p.gates + id);
+    // states and U of 16 columns, under way a turn ahead (they lie with lane = column of v, values = rows: first operands of the transposed products
+    // as they are)
+    const DeltaSizes z(DK, p.dvp, MADE, MADE);
+    struct Columns {
+        Frag<MADE> s[DK / 32], u[2];
+    };
+    auto fetch = [&](int cv) {
+        Columns f;
+#pragma unroll
+        for (int n = 0; n < DK / 32; ++n) f.s[n] = load_frag<MADE>(p.s0 + id * z.state, cv * (DK / 32) + n, lane);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) f.u[n] = load_frag<MADE>(p.u + id * z.u, cv * 2 + n, lane);
+        return f;
+    };
+    Columns next = fetch(0);
     ks.put(k), qs.put(q), gates.put(&s);
     __syncthreads();
     // the wavefront's 16 steps i: scale G_ij q_i.k_j, lane = i, values = j; and its rows of Q
@@ -181,16 +196,15 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const int step = first + i;
     const bool there = step < c.len;
     T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
-    const DeltaSizes z(DK, p.dvp, MADE, MADE);
-    const bf16_t *s0 = p.s0 + id * z.state, *u = p.u + id * z.u;
-    // (states and U lie with lane = column of v, values = rows: first operands of the transposed products as they are)
     for (int cv = 0; cv < p.dvp / 16; ++cv) {
+        const Columns f = next;
+        if (cv + 1 < p.dvp / 16) next = fetch(cv + 1);
         f32x4 acc = zero;
 #pragma unroll
-        for (int n = 0; n < DK / 32; ++n) acc = mma(load_frag<MADE>(s0, cv * (DK / 32) + n, lane), qf[n], acc);
+        for (int n = 0; n < DK / 32; ++n) acc = mma(f.s[n], qf[n], acc);
         acc *= D;
-        acc = mma(load_frag<MADE>(u, cv * 2, lane), pf[0], acc);
-        if (wave >= 2) acc = mma(load_frag<MADE>(u, cv * 2 + 1, lane), pf[1], acc);
+        acc = mma(f.u[0], pf[0], acc);
+        if (wave >= 2) acc = mma(f.u[1], pf[1], acc);
         if (step < p.T) store_four(row, 16 * cv + g4, p.dv, there ? acc : zero, p.vec & kVecY);
     }
 }
