@@ -9,10 +9,16 @@
 //   dc_i = sum_j N_ij - sum_j N_ji + scale D_i q_i.(dY S0^T)_i - D_i beta_i k_i.(Z S0^T)_i - x_i,   N = dP o P + dA o A,  x_i = E_i k_i.(U dS1^T)_i
 //   dc_end += sum_i x_i + e^c_end <S0, dS1>,          d(log a)_t = sum of dc_i over i >= t within the chunk
 //
-// Three launches and more again; W and A's blocks are kept from the forward.  delta_back_prepare_k, a workgroup a chunk: dU without dS1's part, and
+// W and A's blocks are kept from the forward.  delta_back_prepare_k, a workgroup a chunk: dU without dS1's part, and
 // C = scale Q^T D dY - W^T dU of that.  delta_chain.h, from the last chunk to the first: dS0 = e^c_end dS1 + C - W^T (E K dS1), the forward's chain with
 // the operands' parts exchanged; it leaves the dS1 of every chunk.  delta_grads_k, a workgroup a chunk and key head: all gradients; value heads that
 // share a key head one after another, their dQ and dK summed in registers, in one order.
+//
+// Measured, us a launch (back_prepare, the chains' three, grads), the sizes of delta_fwd.h:
+//   bf16, 32 x 3136 x 4 heads of 32 49, 32 + 5 + 26, 177;  bf16, 2 x 4096 x 4 and 8 of 128 57, 53 + 19 + 42, 155;  fp16, 2 x 16384 x 6 of 64 97, 100 + 22 + 55, 249
+// delta_back_prepare_k is bound by memory at 32 channels (34 KB a chunk, 4.3 TB/s).  delta_grads_k, half the backward's time, waits: its eight wavefronts meet
+// at six barriers a round of columns and have 59 % of their time behind them, the vector unit is busy for 53 %; two workgroups a compute unit are what LDS
+// and 128 registers hold.
 #pragma once
 #include "delta_fwd.h"
 

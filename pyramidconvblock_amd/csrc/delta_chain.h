@@ -5,7 +5,9 @@
 //
 // two products a chunk, with W (from memory in fp32: fewer bytes than its planes) and K (from the tensor).  A wavefront carries 16 columns in registers;
 // results of one product are operands of the next as they are.  W and K are the same for all columns of a chain, so other wavefronts of the workgroup
-// fetch them, several chunks ahead in registers, and put them into LDS: one's place is filled while the other is in use, two barriers a chunk.  What bounds it: latencies, of the products and of the exchange between the wavefronts, one chunk after another.
+// fetch them, several chunks ahead in registers, and put them into LDS: one's place is filled while the other is in use, two barriers
+// a chunk.  What bounds it: with many chains memory (512 segments of 13 chunks at 32 channels in bf16: 200 MB in 41 us), with few the latencies of the products
+// and of the exchange between the wavefronts, one chunk after another.
 //
 // Where there are too few chains to fill the chip, the chunks are cut into segments.  Through a segment X goes to M X + N, and the same kernel
 // (MAPS) finds both: N from X = 0, and M as what becomes of the unit matrix' columns without what the chunks add.  delta_join_k takes the states
@@ -60,7 +62,7 @@ constexpr int delta_least_waves() {
 }
 
 // Chunks that are under way: a chunk is done in less time than its operands take from memory; as many as there are registers for.
-template <int DK, bool BACK>
+template <int DK>
 constexpr int delta_ahead() {
     return DK == 32 ? 4 : DK == 64 ? 3 : 2;
 }
@@ -138,7 +140,7 @@ __device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes
 template <typename T, int DK, bool BACK, int CP, bool MAPS, int WAVES>
 __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade, ND = DK / 16, NK = DK / 32;
-    constexpr int AHEAD = delta_ahead<DK, BACK>(), ROWS = ND < 4 ? ND : 4, PLANE = kDeltaChunk * DK;
+    constexpr int AHEAD = delta_ahead<DK>(), ROWS = ND < 4 ? ND : 4, PLANE = kDeltaChunk * DK;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *lw = (bf16_t*)lds, *lk = lw + CP * PLANE;
