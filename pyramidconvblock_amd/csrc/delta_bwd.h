@@ -42,10 +42,18 @@ constexpr int delta_back_prepare_lds() {
     return 2 * delta_rows_bytes<DeltaPlanes<T>::kRaw, DK>() + Blocks<MADE>::kValues * 2 + (int)sizeof(DeltaGates);
 }
 
+template <typename T, int DK, int MADE>
+constexpr int delta_back_prepare_waves() {
+    return delta_waves_of(delta_back_prepare_lds<T, DK, MADE>());
+}
+
 // MADE: planes of what the chain's operands are made of: kChainPlanes where the gradient of a state is wanted.
 template <typename T, int DK, int MADE>
-__global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
+__global__ __launch_bounds__(256, (delta_back_prepare_waves<T, DK, MADE>())) void delta_back_prepare_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw;
+    // with 32 channels seven workgroups a compute unit wait for one another's loads better than four with their own under way (49 us for 59 at 32 x 3136 steps,
+    // 4 heads; with 128 channels 57 us for 49)
+    constexpr bool AHEAD = DK > 32;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *pb = k + L::kValues;
@@ -58,6 +66,23 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
     const int first = m * kDeltaChunk;
     const DeltaChain c(p, chain);
     const DeltaSizes z(DK, p.dvp, DeltaPlanes<T>::kMade, MADE);
+    // columns of v: dU without dS1's part, and C; DK = 32: two wavefronts share a tile of columns where there are few, each half of C's rows
+    const int share = p.dvp <= 32 ? 2 : 1, turns = p.dvp / 16 * share;
+    // dY's columns (what is not there is read from the first row and dropped)
+    T v[4][4];
+    auto fetch = [&](int cw, int lane) {
+        const int at = cw / share * 16 + (lane & 15);
+        const T* gy = (const T*)p.gy + c.at(p.ys, c.hv) + at;
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = first + 16 * b + 4 * (lane >> 4) + r;
+                const bool on = i < c.len && at < p.dv;
+                v[b][r] = gy[on ? c.step(p, i) * p.ys.t : -(long long)at];
+                if (!on) v[b][r] = from_f32<T>(0.f);
+            }
+    };
 
     {
         const int lane = threadIdx.x & 63, col = lane & 15, g4 = 4 * (lane >> 4);
@@ -66,6 +91,7 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
         gates.load(p.gates + id);
         ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
         qs.load((const T*)p.q + c.at(p.qs, c.hk), p.qs.t, p, c, first, 0, p.dk, p.vec & kVecQ);
+        if (AHEAD && wave < turns) fetch(wave, lane);
         gates.put(&s), ks.put(k), qs.put(q);
         __syncthreads();
         // P's column of blocks: lane = j, values = i
@@ -82,26 +108,20 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
         }
         __syncthreads();
     }
-    // columns of v: dU without dS1's part, and C; DK = 32: two wavefronts share a tile of columns where there are few, each half of C's rows
-    const int share = p.dvp <= 32 ? 2 : 1;
-    for (int cw = wave; cw < p.dvp / 16 * share; cw += 4) {
+    for (int cw = wave; cw < turns; cw += 4) {
         // (another lane with every turn, for all that the compiler knows: else it reads all of Q^T ahead of the loop, into registers that there are not)
         int lane = threadIdx.x & 63;
         asm volatile("" : "+v"(lane));
-        const int cv = cw / share, part = cw % share, col = lane & 15, g4 = 4 * (lane >> 4), at = 16 * cv + col;
-        const T* gy = (const T*)p.gy + c.at(p.ys, c.hv) + at;
+        const int cv = cw / share, part = cw % share, g4 = 4 * (lane >> 4);
         Half<RAW> dr[4];
         Half<MADE> ds[4];
-        T v[4][4];
+        f32x4 wt[4];   // -W, lane = channel of k, values = steps
+        auto fetch_w = [&](int d) {
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = first + 16 * b + g4 + r;
-                const bool on = i < c.len && at < p.dv;
-                v[b][r] = gy[on ? c.step(p, i) * p.ys.t : -(long long)at];   // (what is not there is read from the first row and dropped)
-                if (!on) v[b][r] = from_f32<T>(0.f);
-            }
+            for (int b = 0; b < 4; ++b) wt[b] = load_at<f32x4>(p.w + id * z.w + d * 1024 + b * 256, lane * 16);
+        };
+        if (AHEAD) fetch_w(part);
+        else fetch(cw, lane);
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const f32x4 D = *reinterpret_cast<const f32x4*>(s.D + 16 * b + g4);
@@ -110,6 +130,7 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
             for (int r = 0; r < 4; ++r) f[r] = p.scale * D[r] * to_f32(v[b][r]);
             dr[b] = half_of<T, RAW>(v[b]), ds[b] = split<MADE>(f);
         }
+        if (AHEAD && cw + 4 < turns) fetch(cw + 4, lane);
         Half<MADE> us[4];
         float* du = p.du + id * z.cols + cv * 1024;
 #pragma unroll
@@ -123,15 +144,14 @@ __global__ __launch_bounds__(256, 4) void delta_back_prepare_k(DeltaArgs p) {
         const Frag<MADE> d0 = join(ds[0], ds[1]), d1 = join(ds[2], ds[3]), u0 = join(us[0], us[1]), u1 = join(us[2], us[3]);
         float* c0 = p.c0 + id * z.c0 + cv * (DK * 16);
         for (int d = part; d < DK / 16; d += share) {
-            const float* w = p.w + id * z.w + d * 1024;   // -W, lane = channel of k, values = steps
-            f32x4 wt[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) wt[b] = load_at<f32x4>(w + b * 256, lane * 16);
+            if (!AHEAD) fetch_w(d);
+            const Frag<MADE> w0 = join(split<MADE>(wt[0]), split<MADE>(wt[1])), w1 = join(split<MADE>(wt[2]), split<MADE>(wt[3]));
+            if (AHEAD && d + share < DK / 16) fetch_w(d + share);
             f32x4 acc = {0.f, 0.f, 0.f, 0.f}, add = acc;
             acc = mma(join(L::down(q, 0, 16 * d, lane), L::down(q, 16, 16 * d, lane)), d0, acc);
             acc = mma(join(L::down(q, 32, 16 * d, lane), L::down(q, 48, 16 * d, lane)), d1, acc);
-            add = mma(join(split<MADE>(wt[0]), split<MADE>(wt[1])), u0, add);
-            add = mma(join(split<MADE>(wt[2]), split<MADE>(wt[3])), u1, add);
+            add = mma(w0, u0, add);
+            add = mma(w1, u1, add);
             store_at(c0 + d * 256, lane * 16, acc + add);
         }
     }

@@ -41,11 +41,14 @@ constexpr int delta_prepare_lds() {
            (int)sizeof(DeltaGates);
 }
 
-// Wavefronts of a SIMD that registers are to be left for: as many as LDS has room for, up to four.
+// Wavefronts of a SIMD that registers are to be left for, of workgroups of 256: as many as LDS has room for, up to four.
+constexpr int delta_waves_of(int lds) {
+    const int n = 160 * 1024 / lds;
+    return n > 4 ? 4 : n;
+}
 template <typename T, int DK>
 constexpr int delta_prepare_waves() {
-    const int n = 160 * 1024 / delta_prepare_lds<T, DK>();
-    return n > 4 ? 4 : n;
+    return delta_waves_of(delta_prepare_lds<T, DK>());
 }
 
 template <typename T, int DK>
