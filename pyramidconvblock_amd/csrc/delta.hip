@@ -12,13 +12,28 @@ static int padded_dk(int dk) { return dk <= 32 ? 32 : dk <= 64 ? 64 : 128; }
 static int padded_dv(int dv) { return (dv + 31) / 32 * 32; }
 static long long delta_chunks(long long T) { return (T + kDeltaChunk - 1) / kDeltaChunk; }
 
-// Chunks of a segment.  A chain's way through n chunks in s segments takes about 2 n / s steps (once for the maps, once with the states), s - 1 products of
-// half a step's time and two launches more, n steps with one; more segments than fill the chip's 512 places for workgroups gain nothing.
+// Chunks of a segment, by what the chains' launches then take, counted in steps (a chunk in a workgroup that has its place: 1.6, 2.7 and 3.5 us for 32, 64
+// and 128 channels).  A launch takes its segments' steps as often as it has more workgroups than the chip has places for, the one that leaves
+// states at least what memory takes for them (200 chunks a step); the maps' launch and the joining one take 3 more, and 0.3 a segment.  Measured both
+// ways, us of the forward's chains: 128 chains of 49 chunks of 32 channels 80 without segments, 91 with 4; 12 chains of 256 chunks of 64 133 with 20 segments
+// (the choice), 138 with 11, 149 with 16, 155 with 29; 16 of 64 chunks of 128 120 with 8, 125 with 4, 144 with 13; 4 of 49 of 32 25 with 17, 51 with 4.
 static long long segment_chunks(long long chains, long long NC, int DK, int dvp) {
-    const long long parts = (dvp / 16 + 3) / 4, columns = chains * parts;
-    long long best = NC, cost = NC;
-    for (long long s = 2; s <= NC && s <= 64 && columns * (s - 1) < 512; ++s) {
-        const long long seg = (NC + s - 1) / s, c = 2 * seg + s / 2 + 6;
+    // (workgroups of four wavefronts that carry columns, of 16 each, and four that fetch: one a compute unit; of two and two: two)
+    auto rounds = [&](long long segments, int cols) {
+        const bool few = DK == 32 && cols < 4;
+        const long long n = chains * segments * (few ? (cols + 1) / 2 : (cols + 3) / 4), places = few ? 512 : 256;
+        return (double)((n + places - 1) / places);
+    };
+    auto memory = [&](double steps) {
+        const double least = (double)chains * NC / 200;
+        return steps < least ? least : steps;
+    };
+    const int cols = dvp / 16, more = cols + DK / 16;
+    long long best = NC;
+    double cost = memory(NC * rounds(1, cols));
+    for (long long s = 2; s <= NC && s <= 64; ++s) {
+        const long long seg = (NC + s - 1) / s, n = (NC + seg - 1) / seg;
+        const double c = seg * rounds(n - 1, more) + memory(seg * rounds(n, cols)) + 0.3 * n + 3;
         if (c < cost) cost = c, best = seg;
     }
     return best < 1 ? 1 : best;

@@ -21,7 +21,7 @@ inline long long delta_chunk_grid(const DeltaArgs& p, int H) { return ((long lon
 template <typename T, int DK, bool BACK, int CP, bool MAPS, int WAVES>
 void delta_chains_of(const DeltaArgs& p, int cols, hipStream_t s) {
     static std::once_flag once;
-    const long long grid = ((long long)p.chains + 7) / 8 * 8 * ((cols + WAVES - 1) / WAVES) * (MAPS ? p.segments - 1 : p.segments);
+    const long long grid = ((long long)p.chains * (MAPS ? p.segments - 1 : p.segments) + 7) / 8 * 8 * ((cols + WAVES - 1) / WAVES);
     delta_launch(delta_chain_k<T, DK, BACK, CP, MAPS, WAVES>, delta_chain_lds<T, DK, CP>(), once, grid, 128 * WAVES, p, s);
 }
 template <typename T, int DK, bool BACK, int CP, bool MAPS>
