@@ -5,9 +5,10 @@
 //
 // two products a chunk, with W (from memory in fp32: fewer bytes than its planes) and K (from the tensor).  A wavefront carries 16 columns in registers;
 // results of one product are operands of the next as they are.  W and K are the same for all columns of a chain, so other wavefronts of the workgroup
-// fetch them, several chunks ahead in registers, and put them into LDS: one's place is filled while the other is in use, two barriers
-// a chunk.  What bounds it: with many chains memory (512 segments of 13 chunks at 32 channels in bf16: 200 MB in 41 us), with few the latencies of the products
-// and of the exchange between the wavefronts, one chunk after another.
+// fetch them, several chunks ahead in registers, and put them into LDS: one's place is filled while the other is in use, a barrier
+// a chunk, or two where LDS has no room for both.  What bounds it: with many chains memory (240 segments of 13 chunks at 64 channels
+// in fp16: 221 MB in 45 us), with few the latencies of splits, products and the exchange between the wavefronts, one chunk after another (1.6 us a chunk at 32
+// channels, 2.7 at 64, 3.5 at 128).
 //
 // Where there are too few chains to fill the chip, the chunks are cut into segments.  Through a segment X goes to M X + N, and the same kernel
 // (MAPS) finds both: N from X = 0, and M as what becomes of the unit matrix' columns without what the chunks add.  delta_join_k takes the states
@@ -41,12 +42,23 @@ __device__ __forceinline__ void store_state(float* s, const f32x4 (&x)[DK / 16],
 }
 // W's planes as its tiles come (lane = channel of k, values = steps), [plane][tile of channels][tile of steps][lane][4], and K's rows.
 template <typename T, int DK, int CP>
+constexpr int delta_chain_values() {
+    return kDeltaChunk * DK * CP + Rows<DeltaPlanes<T>::kRaw, kDeltaChunk, DK>::kValues;
+}
+// Twice where there is room: a chunk's operands are put while the last one's are in use, with one barrier a chunk (77 us for 80 with two at 128 chains of 49
+// chunks of 32 channels in bf16, 110 for 116 at 12 of 256 of 64 in fp16); fp16's and fp32's 128 channels have none.
+template <typename T, int DK, int CP>
+constexpr bool delta_chain_twice() {
+    return delta_chain_values<T, DK, CP>() * 4 <= 160 * 1024;
+}
+template <typename T, int DK, int CP>
 constexpr int delta_chain_lds() {
-    return (kDeltaChunk * DK * CP + Rows<DeltaPlanes<T>::kRaw, kDeltaChunk, DK>::kValues) * 2;
+    return delta_chain_values<T, DK, CP>() * (delta_chain_twice<T, DK, CP>() ? 4 : 2);
 }
 
 // What a workgroup's index stands for: the column parts of a chain's segments; the parts of a segment, which read the same operands, on one die (workgroups
-// go to the eight dies in turn), and segments on one after another (a chain to a die leaves half of the dies idle with twelve chains: 96 us for 80).
+// go to the eight dies in turn), and segments on one after another (with a chain to a die, twelve chains leave half of the dies
+// half idle: 99 us for 71, 20 segments each at 64 channels).
 __device__ __forceinline__ bool chain_part(const DeltaArgs& p, int parts, int segments, int& chain, int& part, int& segment) {
     const unsigned id = (unsigned)p.first + blockIdx.x, turn = id >> 3, turns = turn / (unsigned)parts, n = turns * 8 + (id & 7);
     part = (int)(turn - turns * parts);
@@ -107,6 +119,28 @@ __device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes
         if constexpr (BACK) f[j].load_w(p, z, id + m * by, thread);
         else f[j].load_k(p, c, chunk + m * by, thread);
     };
+    if constexpr (delta_chain_twice<T, DK, CP>()) {
+        auto put = [&](int j, int m) {
+            const int other = (m & 1) * delta_chain_values<T, DK, CP>();
+            f[j].put_w(lw + other, thread), f[j].k.put(lk + other, thread);
+        };
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) fetch_a(j, j), fetch_b(j, j);
+        put(0, 0);
+        fetch_a(0, AHEAD), fetch_b(0, AHEAD);
+        __syncthreads();
+        for (int m0 = 0; m0 < n; m0 += AHEAD) {
+#pragma unroll
+            for (int j = 0; j < AHEAD; ++j) {
+                const int m = m0 + j, k = j == AHEAD - 1 ? 0 : j + 1;
+                if (m >= n) break;
+                if (m + 1 < n) put(k, m + 1);
+                fetch_a(k, m + 1 + AHEAD), fetch_b(k, m + 1 + AHEAD);
+                __syncthreads();
+            }
+        }
+        return;
+    }
     auto put_a = [&](int j) {
         if constexpr (BACK) f[j].k.put(lk, thread);
         else f[j].put_w(lw, thread);
@@ -142,6 +176,7 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade, ND = DK / 16, NK = DK / 32;
     constexpr int AHEAD = delta_ahead<DK>(), ROWS = ND < 4 ? ND : 4, PLANE = kDeltaChunk * DK;
     typedef Rows<RAW, kDeltaChunk, DK> L;
+    constexpr bool TWICE = delta_chain_twice<T, DK, CP>();
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *lw = (bf16_t*)lds, *lk = lw + CP * PLANE;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -241,7 +276,7 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
                 for (int d = 0; d < NK; ++d) store_frag(to, cv * NK + d, planes<MADE>(xs[d]), lane);
             }
         }
-        __syncthreads();
+        if constexpr (!TWICE) __syncthreads();
         Half<CP> e[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) e[b] = split<CP>(y[b] * c.E[b]);
@@ -286,6 +321,10 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
             }
         }
         if (m + AHEAD < n) fetch(chunks[j], id + AHEAD * by);
+        if constexpr (TWICE) {
+            const int other = m & 1 ? -delta_chain_values<T, DK, CP>() : delta_chain_values<T, DK, CP>();
+            lw += other, lk += other;
+        }
         __syncthreads();
     }
     if constexpr (MAPS) {
