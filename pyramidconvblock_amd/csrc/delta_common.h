@@ -308,8 +308,9 @@ __device__ __forceinline__ bool chunk_of(const DeltaArgs& p, int H, int& chain, 
 // the chain's end and behind the row's end d.  By NT threads, this one `thread` of them.
 template <typename T, int NP, int R, int NT = 256>
 struct Staged {
-    static constexpr int ALL = kDeltaChunk * (R / 8), N = (ALL + NT - 1) / NT;
-    T v[N][8];
+    static constexpr int ALL = kDeltaChunk * (R / 8), N = (ALL + NT - 1) / NT, QUADS = sizeof(T) / 2;
+    // (as they come: values taken apart here would be waited for here)
+    f32x4 v[N][QUADS];
     bool on[N];
     __device__ __forceinline__ void load(const T* base, long long st, const DeltaArgs& p, const DeltaChain& c, int first, int col, int d, bool vec,
                                          int thread = threadIdx.x) {
@@ -324,20 +325,18 @@ struct Staged {
             q[n] = base + (on[n] ? (long long)c.step(p, i) * st + at[n] : 0);
         }
         if (vec) {
-            constexpr int VEC = 16 / sizeof(T);
 #pragma unroll
             for (int n = 0; n < N; ++n)
 #pragma unroll
-                for (int m = 0; m < 8 / VEC; ++m) {
-                    const ChanVec<T, VEC> r = *reinterpret_cast<const ChanVec<T, VEC>*>(q[n] + m * VEC);
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) v[n][m * VEC + j] = r.v[j];
-                }
+                for (int m = 0; m < QUADS; ++m) v[n][m] = reinterpret_cast<const f32x4*>(q[n])[m];
         } else {
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+            for (int n = 0; n < N; ++n) {
+                T one[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[n][j] = on[n] && at[n] + j < d ? q[n][j] : from_f32<T>(0.f);
+                for (int j = 0; j < 8; ++j) one[j] = on[n] && at[n] + j < d ? q[n][j] : from_f32<T>(0.f);
+                __builtin_memcpy(v[n], one, sizeof one);
+            }
         }
     }
     __device__ __forceinline__ void put(bf16_t* to, int thread = threadIdx.x) const {
@@ -346,7 +345,9 @@ struct Staged {
         for (int n = 0; n < N; ++n) {
             const int e = thread + n * NT;
             if (ALL % NT && e >= ALL) continue;
-            Frag<NP> f = planes_of<T, NP>(v[n]);
+            T one[8];
+            __builtin_memcpy(one, v[n], sizeof one);
+            Frag<NP> f = planes_of<T, NP>(one);
 #pragma unroll
             for (int m = 0; m < NP; ++m) {
                 if (!on[n]) f.p[m] = bf16x8{};
