@@ -78,9 +78,7 @@ __global__ __launch_bounds__(256, (delta_back_prepare_waves<T, DK, MADE>())) voi
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int i = first + 16 * b + 4 * (lane >> 4) + r;
-                const bool on = i < c.len && at < p.dv;
-                v[b][r] = gy[on ? c.step(p, i) * p.ys.t : -(long long)at];
-                if (!on) v[b][r] = from_f32<T>(0.f);
+                v[b][r] = gy[i < c.len && at < p.dv ? c.step(p, i) * p.ys.t : -(long long)at];
             }
     };
 
@@ -125,6 +123,9 @@ __global__ __launch_bounds__(256, (delta_back_prepare_waves<T, DK, MADE>())) voi
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const f32x4 D = *reinterpret_cast<const f32x4*>(s.D + 16 * b + g4);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (first + 16 * b + g4 + r >= c.len || 16 * cv + (lane & 15) >= p.dv) v[b][r] = from_f32<T>(0.f);
             f32x4 f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) f[r] = p.scale * D[r] * to_f32(v[b][r]);

@@ -108,14 +108,15 @@ __device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes
     const DeltaChain c(p, chain);
     const long long id = (long long)chain * p.NC + chunk;
     ChainFetch<T, DK, CP, NT> f[AHEAD];
-    // A is what the first product takes, B the second's: W and K, or (BACK) K and W
+    // A is what the first product takes, B the second's: W and K, or (BACK) K and W.  (Behind the last chunk the last once more: loads on a condition would all
+    // be waited for where the first of them is, since their number is not known there.)
     auto fetch_a = [&](int j, int m) {
-        if (m >= n) return;
+        m = m < n ? m : n - 1;
         if constexpr (BACK) f[j].load_k(p, c, chunk + m * by, thread);
         else f[j].load_w(p, z, id + m * by, thread);
     };
     auto fetch_b = [&](int j, int m) {
-        if (m >= n) return;
+        m = m < n ? m : n - 1;
         if constexpr (BACK) f[j].load_w(p, z, id + m * by, thread);
         else f[j].load_k(p, c, chunk + m * by, thread);
     };
@@ -134,7 +135,7 @@ __device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes
             for (int j = 0; j < AHEAD; ++j) {
                 const int m = m0 + j, k = j == AHEAD - 1 ? 0 : j + 1;
                 if (m >= n) break;
-                if (m + 1 < n) put(k, m + 1);
+                put(k, m + 1);
                 fetch_a(k, m + 1 + AHEAD), fetch_b(k, m + 1 + AHEAD);
                 __syncthreads();
             }
@@ -163,7 +164,7 @@ __device__ __forceinline__ void chain_fetch(const DeltaArgs& p, const DeltaSizes
             fetch_b(j, m + AHEAD);
             __syncthreads();
             const int k = j == AHEAD - 1 ? 0 : j + 1;
-            if (m + 1 < n) put_a(k);
+            put_a(k);
             fetch_a(k, m + 1 + AHEAD);
             __syncthreads();
         }
@@ -193,7 +194,15 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
         return chain_fetch<T, DK, BACK, CP, 64 * WAVES, AHEAD>(p, z, chain, chunk, by, n, lw, lk, threadIdx.x - 64 * WAVES);
 
     const int cv = part * WAVES + wave;
-    const bool on = cv < cols, unit_cols = MAPS && cv >= colv;   // (a wavefront without columns of its own goes along)
+    if (cv >= cols) {   // without columns: along to the barriers
+        __syncthreads();
+        for (int m = 0; m < n; ++m) {
+            if constexpr (!TWICE) __syncthreads();
+            __syncthreads();
+        }
+        return;
+    }
+    const bool unit_cols = MAPS && cv >= colv;
     const bf16x4 unit = unit_half(lane);
     const int at = 16 * cv + (lane & 15);
     const long long state = (long long)chain * p.dk * p.dv;
@@ -206,33 +215,42 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
     } else {
         const float* h = BACK ? p.glast : p.h0;
         if (segment == 0) {
-            load_state<DK>(x, h ? h + state : nullptr, p.dk, p.dv, on ? at : p.dv, lane);
+            load_state<DK>(x, h ? h + state : nullptr, p.dk, p.dv, at, lane);
         } else {
             const float* from_maps = p.shifts + (chain * (long long)(p.segments - 1) + segment - 1) * z.shift + cv * (DK * 16);
 #pragma unroll
-            for (int d = 0; d < ND; ++d) x[d] = on ? load_at<f32x4>(from_maps + d * 256, lane * 16) : f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < ND; ++d) x[d] = load_at<f32x4>(from_maps + d * 256, lane * 16);
         }
     }
 
-    // what a chunk brings to these columns
+    // what a chunk brings to these columns (to the unit matrix' nothing: it is loaded for another and dropped, as behind the last chunk)
+    const int source = unit_cols ? 0 : cv;
     struct Chunk {
         f32x4 y0[BACK ? 1 : 4], E[4];
         float end;
     };
-    auto fetch = [&](Chunk& c, long long id) {
+    auto fetch = [&](Chunk& c, int m) {
+        const long long id = from + (m < n ? m : n - 1) * by;
         const DeltaGates* s = p.gates + id;
-        const bool own = on && !unit_cols;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            if constexpr (!BACK) c.y0[b] = own ? load_at<f32x4>(p.ub + id * z.cols + cv * 1024 + b * 256, lane * 16) : f32x4{0.f, 0.f, 0.f, 0.f};
+            if constexpr (!BACK) c.y0[b] = load_at<f32x4>(p.ub + id * z.cols + source * 1024 + b * 256, lane * 16);
             c.E[b] = load_at<f32x4>(s->E + 16 * b, g4 * 4);
         }
         c.end = s->D[kDeltaChunk - 1];
     };
-    Chunk chunks[AHEAD];
+    f32x4 c0[BACK ? ND : 1];   // of the next chunk
+    auto fetch_c0 = [&](int m) {
+        const long long id = from + (m < n ? m : n - 1) * by;
+        if constexpr (BACK) {
 #pragma unroll
-    for (int j = 0; j < AHEAD; ++j)
-        if (j < n) fetch(chunks[j], from + j * by);
+            for (int d = 0; d < ND; ++d) c0[d] = load_at<f32x4>(p.c0 + id * z.c0 + source * (DK * 16) + d * 256, lane * 16);
+        }
+    };
+    Chunk chunks[AHEAD];
+    fetch_c0(0);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) fetch(chunks[j], j);
     __syncthreads();
     for (int m0 = 0; m0 < n; m0 += AHEAD)
 #pragma unroll
@@ -241,18 +259,12 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
         const long long id = from + m * by;
         if (m >= n) break;
         const Chunk& c = chunks[j];
-        f32x4 c0[BACK ? ND : 1];
-        if constexpr (BACK) {
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-                c0[d] = on && !unit_cols ? load_at<f32x4>(p.c0 + id * z.c0 + cv * (DK * 16) + d * 256, lane * 16) : f32x4{0.f, 0.f, 0.f, 0.f};
-        }
         Frag<CP> xs[DK / 32];
 #pragma unroll
         for (int d = 0; d < NK; ++d) xs[d] = join(split<CP>(x[2 * d]), split<CP>(x[2 * d + 1]));
         f32x4 y[4];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) y[b] = BACK ? f32x4{0.f, 0.f, 0.f, 0.f} : c.y0[b];
+        for (int b = 0; b < 4; ++b) y[b] = BACK || unit_cols ? f32x4{0.f, 0.f, 0.f, 0.f} : c.y0[b];
 #pragma unroll
         for (int d = 0; d < NK; ++d) {
             // (lane = step, values = channels of k)
@@ -270,11 +282,9 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
             }
         }
         if constexpr (!MAPS) {
-            if (on) {
-                bf16_t* to = (BACK ? p.ds1 : p.s0) + id * z.state;
+            bf16_t* to = (BACK ? p.ds1 : p.s0) + id * z.state;
 #pragma unroll
-                for (int d = 0; d < NK; ++d) store_frag(to, cv * NK + d, planes<MADE>(xs[d]), lane);
-            }
+            for (int d = 0; d < NK; ++d) store_frag(to, cv * NK + d, planes<MADE>(xs[d]), lane);
         }
         if constexpr (!TWICE) __syncthreads();
         Half<CP> e[4];
@@ -284,8 +294,9 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
             x[d] = x[d] * c.end;
-            if constexpr (BACK) x[d] += c0[d];
+            if constexpr (BACK) x[d] += unit_cols ? f32x4{0.f, 0.f, 0.f, 0.f} : c0[d];
         }
+        fetch_c0(m + 1);
 #pragma unroll
         for (int d0 = 0; d0 < ND; d0 += ROWS) {
 #pragma unroll
@@ -314,13 +325,11 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
             }
         }
         if constexpr (!MAPS && !BACK) {
-            if (on) {
-                bf16_t* to = p.u + id * z.u;
-                store_frag(to, cv * 2, join(split<MADE>(y[0]), split<MADE>(y[1])), lane);
-                store_frag(to, cv * 2 + 1, join(split<MADE>(y[2]), split<MADE>(y[3])), lane);
-            }
+            bf16_t* to = p.u + id * z.u;
+            store_frag(to, cv * 2, join(split<MADE>(y[0]), split<MADE>(y[1])), lane);
+            store_frag(to, cv * 2 + 1, join(split<MADE>(y[2]), split<MADE>(y[3])), lane);
         }
-        if (m + AHEAD < n) fetch(chunks[j], id + AHEAD * by);
+        fetch(chunks[j], m + AHEAD);
         if constexpr (TWICE) {
             const int other = m & 1 ? -delta_chain_values<T, DK, CP>() : delta_chain_values<T, DK, CP>();
             lw += other, lk += other;
@@ -329,7 +338,6 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
     }
     if constexpr (MAPS) {
         const long long id = chain * (long long)(p.segments - 1) + segment;
-        if (!on) return;
         if (!unit_cols) {
 #pragma unroll
             for (int d = 0; d < ND; ++d) store_at(p.shifts + id * z.shift + cv * (DK * 16) + d * 256, lane * 16, x[d]);
@@ -344,7 +352,7 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
                 store_half(p.maps + id * z.map, d * (DK / 32) + ct / 2, ct & 1, h, lane);
             }
         }
-    } else if (segment == p.segments - 1 && on) {
+    } else if (segment == p.segments - 1) {
         float* to = BACK ? p.gh0 : p.last;
         store_state<DK>(to ? to + state : nullptr, x, p.dk, p.dv, at, lane);
     }
