@@ -158,22 +158,33 @@ __global__ __launch_bounds__(256, (delta_back_prepare_waves<T, DK, MADE>())) voi
     }
 }
 
-// 4 neighbouring values of a row of d, 0 where there are none.
+// 4 neighbouring values of a row of d, 0 where there are none: as they come, and what they are.
 template <typename T>
-__device__ __forceinline__ f32x4 load_four(const T* row, bool there, int at, int d, bool vec) {
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (!there || at >= d) return v;
-    if (vec) {
-        const ChanVec<T, 4> r = *reinterpret_cast<const ChanVec<T, 4>*>(row + at);
+struct Four {
+    typedef unsigned words_t __attribute__((ext_vector_type(sizeof(T))));
+    words_t words;
+    bool on;
+    __device__ __forceinline__ void load(const T* base, long long row, bool there, int at, int d, bool vec) {
+        on = there && at < d;
+        const T* from = base + (on ? row + at : 0);
+        if (vec) {
+            words = *reinterpret_cast<const words_t*>(from);
+        } else {
+            T one[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = to_f32(r.v[j]);
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (at + j < d) v[j] = to_f32(row[at + j]);
+            for (int j = 0; j < 4; ++j) one[j] = on && at + j < d ? from[j] : from_f32<T>(0.f);
+            __builtin_memcpy(&words, one, sizeof one);
+        }
     }
-    return v;
-}
+    __device__ __forceinline__ f32x4 values() const {
+        T one[4];
+        __builtin_memcpy(one, &words, sizeof one);
+        f32x4 v;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = on ? to_f32(one[j]) : 0.f;
+        return v;
+    }
+};
 // The two tiles of a fragment, summed over planes.
 template <int NP>
 __device__ __forceinline__ void sum_tiles(const Frag<NP>& f, f32x4& lo, f32x4& hi) {
@@ -261,13 +272,15 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
         int lane = threadIdx.x & 63;
         if (SHARED) asm volatile("" : "+v"(lane)::"memory");
         const bf16_t *s0 = p.s0 + id * z.state, *ds1 = p.ds1 + id * z.state, *u = p.u + id * z.u;
-        // what a round of columns takes: dY, states, U, and dU without dS1's part
+        // what a round of columns takes: dY, states, U, dU without dS1's part, and V
         Staged<T, RAW, COLS, NT> gs;
         Run<S::kState * 2, NT> rs, rd;
         Run<S::kU * 2, NT> ru;
         f32x4 x[4];
+        Four<T> vs;
         auto fetch = [&](int at) {
-            const int cw = at / 16;
+            const int cw = at / 16, place = first + 16 * row + (lane & 15);
+            vs.load((const T*)p.v + c.at(p.vs, c.hv), c.step(p, place) * p.vs.t, place < c.len, at + 16 * half + 4 * (lane >> 4), p.dv, p.vec & kVecV);
             gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
             if constexpr (S::kStage)
                 rs.load(s0 + cw * NK * MADE * 512), rd.load(ds1 + cw * NK * MADE * 512), ru.load(u + cw * 2 * MADE * 512);
@@ -369,7 +382,7 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
                 sum_tiles(zm, lo, hi);
                 if (half) lo = hi;
                 const int here = at + 16 * half + g4;
-                const f32x4 v = load_four((const T*)p.v + c.at(p.vs, c.hv) + step * p.vs.t, there, here, p.dv, p.vec & kVecV);
+                const f32x4 v = vs.values();
 #pragma unroll
                 for (int j = 0; j < 4; ++j) zv = __builtin_fmaf(lo[j], v[j], zv);
                 if (p.gv && place < p.T)

@@ -431,19 +431,31 @@ __device__ __forceinline__ double sums_up_to(double v) {
     return v;
 }
 
+// The same in two steps, a load and what its bits mean.
+__device__ __forceinline__ unsigned gate_bits(const void* base, long long at, bool wide) {
+    return wide ? ((const unsigned*)base)[at] : ((const unsigned short*)base)[at];
+}
+__device__ __forceinline__ float gate_of(unsigned bits, bool wide, int type) {
+    if (wide) return __builtin_bit_cast(float, bits);
+    return type == kF16 ? to_f32(__builtin_bit_cast(f16_t, (unsigned short)bits)) : to_f32(__builtin_bit_cast(bf16_t, (unsigned short)bits));
+}
+
 // Made by the first wavefront, in two steps (loads ahead of others; the rest), into LDS and memory; the caller's barrier follows.
 struct GateMaker {
-    float g, b;
+    unsigned gbits, bbits;
     bool on;
     __device__ __forceinline__ void load(const DeltaArgs& p, const DeltaChain& c, int first, int type) {
         const int i = first + (threadIdx.x & 63);
         on = i < c.len;
         const long long t = on ? c.step(p, i) : 0;
-        g = gate_value(p.g, c.at(p.gs, c.hv) + t * p.gs.t, p.gates_f32, type);
-        b = gate_value(p.b, c.at(p.bs, c.hv) + t * p.bs.t, p.gates_f32, type);
+        const bool wide = p.gates_f32 || type == kF32;
+        gbits = gate_bits(p.g, c.at(p.gs, c.hv) + t * p.gs.t, wide);
+        bbits = gate_bits(p.b, c.at(p.bs, c.hv) + t * p.bs.t, wide);
     }
-    __device__ __forceinline__ void make(DeltaGates& s, DeltaGates* to, const DeltaArgs& p) {
+    __device__ __forceinline__ void make(DeltaGates& s, DeltaGates* to, const DeltaArgs& p, int type) {
         const int lane = threadIdx.x & 63;
+        const bool wide = p.gates_f32 || type == kF32;
+        const float g = gate_of(gbits, wide, type), b = gate_of(bbits, wide, type);
         float la, slope, beta, bslope;
         log_decay(g, p.logits, la, slope);
         write_strength(b, p.logits, beta, bslope);

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
     if (wave == 0) gates.load(p, c, first, type);
     ks.load((const T*)p.k + c.at(p.ks, c.hk), p.ks.t, p, c, first, 0, p.dk, p.vec & kVecK);
     vs.load((const T*)p.v + c.at(p.vs, c.hv), p.vs.t, p, c, first, 0, p.dv, p.vec & kVecV);
-    if (wave == 0) gates.make(s, p.gates + id, p);
+    if (wave == 0) gates.make(s, p.gates + id, p, type);
     ks.put(k), vs.put(vl);
     __syncthreads();
     // A's blocks of the wavefront's row of blocks: lane = row i of it, values = columns j of block t
