@@ -11,8 +11,8 @@
 // quarter: what is left is below 1/8 of a turn and off by some 2^-53 of the angle itself (2^-24 of a turn at position 2^31, nothing that counts at 2^20);
 // cosine and sine of that are their series.
 //
-// Measured: 50176 tokens of 8 and 4 heads of 64 in bf16 (rms, three axes) 37 us forward, 154 MB moved, 4.2 TB/s; backward 73 + 7 us, 231 MB.  16384 tokens of 9
-// and 9 heads of 128 in fp16, 32 pairs turned, no norm: 36 us forward, 40 to 48 backward, 151 MB each.  3136 tokens of 4 and 4 heads of 32: 7 us,
+// Measured: 50176 tokens of 8 and 4 heads of 64 in bf16 (rms, three axes) 37 us forward, 154 MB moved, 4.2 TB/s; backward 68 + 7 us, 231 MB.  16384 tokens of 9
+// and 9 heads of 128 in fp16, 32 pairs turned, no norm: 36 us forward, 41 backward, 151 MB each.  3136 tokens of 4 and 4 heads of 32: 7 us,
 // angles and latencies.
 #pragma once
 #include "common.h"
@@ -140,24 +140,30 @@ __global__ __launch_bounds__(256) void rotary_k(RotaryArgs p) {
                 const int tok = r / H, h = r - tok * H;
                 const long long dense = ((t0 + tok) * H + h) * p.d;
                 const T* x = (const T*)p.x[s] + (t0 + tok) * p.xt[s] + h * p.xh[s];
-                float v[UPL][2 * VEC], q[UPL][2 * VEC];   // x (then its norm); backward: the gradient
-                float sum = 0.f;
-                if (!BWD || p.kind != kRotaryNone) {
+                // (all as they come: what is taken apart ahead of the next load is waited for there)
+                typedef typename Access<T, VEC>::word word;
+                typedef typename Access<T, VEC>::type any;
+                word rx[UPL][2], rg[UPL][2];
+                const bool normed = !BWD || p.kind != kRotaryNone;
 #pragma unroll
-                    for (int n = 0; n < UPL; ++n) {
-                        const Piece<T, VEC> a = load_any<T, VEC>(x + at[n]), c = load_any<T, VEC>(x + to[n]);
-#pragma unroll
-                        for (int i = 0; i < VEC; ++i) v[n][i] = on[n] ? to_f32(a.v[i]) : 0.f, v[n][VEC + i] = on[n] && !odd[n] ? to_f32(c.v[i]) : 0.f;
-                    }
-                }
+                for (int n = 0; n < UPL; ++n)
+                    if (normed) rx[n][0] = *reinterpret_cast<const any*>(x + at[n]), rx[n][1] = *reinterpret_cast<const any*>(x + to[n]);
                 if constexpr (BWD) {
                     const T* gy = (const T*)p.gy[s] + dense;
 #pragma unroll
-                    for (int n = 0; n < UPL; ++n) {
-                        const Piece<T, VEC> a = load_any<T, VEC>(gy + at[n]), c = load_any<T, VEC>(gy + to[n]);
+                    for (int n = 0; n < UPL; ++n) rg[n][0] = *reinterpret_cast<const any*>(gy + at[n]), rg[n][1] = *reinterpret_cast<const any*>(gy + to[n]);
+                }
+                float v[UPL][2 * VEC], q[UPL][2 * VEC];   // x (then its norm); backward: the gradient
+                float sum = 0.f;
+                auto floats = [&](const word(&from)[2], int n, float(&o)[2 * VEC]) {
+                    const Piece<T, VEC> a = __builtin_bit_cast(Piece<T, VEC>, from[0]), c = __builtin_bit_cast(Piece<T, VEC>, from[1]);
 #pragma unroll
-                        for (int i = 0; i < VEC; ++i) q[n][i] = on[n] ? to_f32(a.v[i]) : 0.f, q[n][VEC + i] = on[n] && !odd[n] ? to_f32(c.v[i]) : 0.f;
-                    }
+                    for (int i = 0; i < VEC; ++i) o[i] = on[n] ? to_f32(a.v[i]) : 0.f, o[VEC + i] = on[n] && !odd[n] ? to_f32(c.v[i]) : 0.f;
+                };
+#pragma unroll
+                for (int n = 0; n < UPL; ++n) {
+                    if (normed) floats(rx[n], n, v[n]);
+                    if constexpr (BWD) floats(rg[n], n, q[n]);
                 }
                 float rs = 1.f;
                 const float part = p.kind == kRotaryRms ? 1.f / p.d : 1.f;

@@ -12,7 +12,7 @@ void rotary_launch_f32(const RotaryArgs& p, unsigned grid, bool backward, hipStr
 void rotary_launch_f16(const RotaryArgs& p, unsigned grid, bool backward, hipStream_t s);
 void rotary_launch_bf16(const RotaryArgs& p, unsigned grid, bool backward, hipStream_t s);
 
-// Workgroups that leave sums for the weights: four on every compute unit (with two, 50176 tokens of 8 and 4 heads of 64 channels in bf16 took 87 us instead of 73;
+// Workgroups that leave sums for the weights: four on every compute unit (with two, 50176 tokens of 8 and 4 heads of 64 channels in bf16 took 87 us instead of 73 then;
 // with more their sums cost what they save).
 constexpr long long kRotarySums = 1024;
 
@@ -37,7 +37,7 @@ __global__ __launch_bounds__(1024) void rotary_sums_k(const float* __restrict__ 
     if (to) to[c < d ? c : c - d] = from_f32<T>(red[0][cl]);
 }
 
-// Tokens of a workgroup: four rounds of rows (with two the gradients above took 88 us, with eight 78), fewer where the call is small (512 workgroups at least;
+// Tokens of a workgroup: four rounds of rows (with two those gradients took 88 us, with eight 78), fewer where the call is small (512 workgroups at least;
 // with 1024, of a few tokens each, one call of 1024 tokens took 8.9 us instead of 7.0), and angles that fit 16 KB.
 static int rotary_tokens(const RotaryArgs& p, int lanes) {
     const int heads = p.heads[0] > p.heads[1] ? p.heads[0] : p.heads[1];
