@@ -235,6 +235,9 @@ __device__ __forceinline__ float sixteen_sum(float v) {
 template <typename T, int DK, bool SHARED>
 __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())) void delta_grads_k(DeltaArgs p) {
     typedef GradsLds<T, DK> S;
+    // the next round's operands under way meanwhile: with shared heads 154 us for 140 (2 x 4096 steps, 4 and 8 heads of 128, bf16), with 128 channels a backward
+    // of 523 us for 515 (4 x 4096, 8 heads, bf16); with 64 in fp16 133 for 138, so not there
+    constexpr bool AHEAD = SHARED || DK == 128;
     constexpr int RAW = S::RAW, MADE = S::MADE, NT = kGradsThreads, COLS = kGradsCols, ND = DK / 32, NK = DK / 32;   // ND: tiles of this half
     typedef Rows<RAW, kDeltaChunk, DK> L;
     typedef Rows<MADE, kDeltaChunk, COLS> LZ;
@@ -278,22 +281,27 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
         Run<S::kU * 2, NT> ru;
         f32x4 x[4];
         Four<T> vs;
-        auto fetch = [&](int at) {
-            const int cw = at / 16, place = first + 16 * row + (lane & 15);
+        auto fetch_v = [&](int at) {
+            const int place = first + 16 * row + (lane & 15);
             vs.load((const T*)p.v + c.at(p.vs, c.hv), c.step(p, place) * p.vs.t, place < c.len, at + 16 * half + 4 * (lane >> 4), p.dv, p.vec & kVecV);
+        };
+        auto fetch_x = [&](int at) {
+            if (wave < 2) {
+#pragma unroll
+                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(p.du + id * z.cols + (at / 16 + wave) * 1024 + b * 256, lane * 16);
+            }
+        };
+        auto fetch = [&](int at) {
+            const int cw = at / 16;
             gs.load((const T*)p.gy + c.at(p.ys, c.hv), p.ys.t, p, c, first, at, p.dv, p.vec & kVecGy);
             if constexpr (S::kStage)
                 rs.load(s0 + cw * NK * MADE * 512), rd.load(ds1 + cw * NK * MADE * 512), ru.load(u + cw * 2 * MADE * 512);
-            if (wave < 2) {
-#pragma unroll
-                for (int b = 0; b < 4; ++b) x[b] = load_at<f32x4>(p.du + id * z.cols + (cw + wave) * 1024 + b * 256, lane * 16);
-            }
         };
         {
             Run<sizeof(DeltaGates), NT> gates;
             Run<Blocks<MADE>::kValues * 2, NT> system;
             gates.load(p.gates + id), system.load(p.blocks + id * z.blocks);
-            fetch(0);
+            fetch_v(0), fetch(0), fetch_x(0);
             if (e) __syncthreads();
             if (e == 0) ks.put(k), qs.put(q);
             gates.put(&s), system.put(blocks);
@@ -307,13 +315,15 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
         float zv = 0.f, ss = 0.f;       // Z_i.V_i; <S0, dS1>
         for (int at = 0; at < p.dvp; at += COLS) {
             const int cw = at / 16;
+            const bool more = at + COLS < p.dvp;
             if (at) {
-                fetch(at);
+                if (!AHEAD) fetch_v(at), fetch(at), fetch_x(at);
                 __syncthreads();
             }
             if constexpr (S::kStage) rs.put(sl), rd.put(dl), ru.put(ul);
             gs.put(gl);
             __syncthreads();
+            if (AHEAD && more) fetch(at + COLS);
             asm volatile("" : "+v"(lane));
             const bf16x4 unit = unit_half(lane);
             // rows of a tile of steps or channels from what lies as the products left it
@@ -342,6 +352,7 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
 #pragma unroll
                 for (int b = 0; b < 4; ++b) LZ::put_turned(zl, 16 * b, 16 * wave, split<MADE>(x[b]), unit, lane);
             }
+            if (AHEAD && more) fetch_x(at + COLS);
             // what Z has no part in
             const Frag<MADE> um = turned_rows(ul, u, 2, row);
             {
@@ -383,6 +394,7 @@ __global__ __launch_bounds__(kGradsThreads, (delta_grads_waves<T, DK, SHARED>())
                 if (half) lo = hi;
                 const int here = at + 16 * half + g4;
                 const f32x4 v = vs.values();
+                if (AHEAD && more) fetch_v(at + COLS);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) zv = __builtin_fmaf(lo[j], v[j], zv);
                 if (p.gv && place < p.T)
