@@ -120,11 +120,11 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
     // columns of W, and with them the first ones of Ub; then the others of Ub
     for (int at = 0; at < p.dvp; at += COLS) {
         if (at) {
-            vs.load((const T*)p.v + c.at(p.vs, c.hv), p.vs.t, p, c, first, at, p.dv, p.vec & kVecV);
             __syncthreads();
             vs.put(vl);
             __syncthreads();
         }
+        if (at + COLS < p.dvp) vs.load((const T*)p.v + c.at(p.vs, c.hv), p.vs.t, p, c, first, at + COLS, p.dv, p.vec & kVecV);
         const int end = (p.dvp - at < COLS ? p.dvp - at : COLS) / 16;
         for (int ct = (at ? DK / 16 : 0) + wave; ct < DK / 16 + end; ct += 4) {
             const bool w = ct < DK / 16;
