@@ -15,7 +15,7 @@
 // share a key head one after another, their dQ and dK summed in registers, in one order.
 //
 // Measured, us a launch (back_prepare, the chains' three, grads), the sizes of delta_fwd.h:
-//   bf16, 32 x 3136 x 4 heads of 32 48, 53, 154;  bf16, 2 x 4096 x 4 and 8 of 128 50, 49 + 13 + 39, 142;  fp16, 2 x 16384 x 6 of 64 77, 65 + 16 + 38, 228
+//   bf16, 32 x 3136 x 4 heads of 32 48, 53, 154;  bf16, 2 x 4096 x 4 and 8 of 128 50, 49 + 13 + 39, 142;  fp16, 2 x 16384 x 6 of 64 77, 65 + 13 + 38, 228
 // delta_back_prepare_k is bound by memory at 32 channels (34 KB a chunk, 4.3 TB/s).  delta_grads_k, half the backward's time, waits: its eight wavefronts meet
 // at six barriers a round of columns and wait for 47 % of their time, the vector unit is busy for 60 %; two workgroups a compute unit are what LDS
 // and 128 registers hold.

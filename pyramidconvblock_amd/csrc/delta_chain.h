@@ -359,10 +359,12 @@ __global__ __launch_bounds__(128 * WAVES) void delta_chain_k(DeltaArgs p) {
 }
 
 // The state before every segment but the first, in the place of its predecessor's shift N: X = M X + N from segment to segment.  A workgroup has 16 columns
-// of a chain, a wavefront 16 rows of them: its rows of M are under way while the last segment's product is made, X goes round through LDS.
+// of a chain, a wavefront 16 rows of them: its rows of the next segments' M are under way, X goes round through LDS (20 segments at 64 channels 16 us
+// with one segment's under way, 13.5 with four).
 template <typename T, int DK, bool BACK, int CP>
 __global__ __launch_bounds__(DK * 4) void delta_join_k(DeltaArgs p) {
-    constexpr int NK = DK / 32;
+    // (maps of 128 x 128 are bound by their bytes: three segments ahead, the last one's map once or twice more, took 18 us for 16)
+    constexpr int NK = DK / 32, AHEAD = DK == 128 ? 1 : 4;
     __shared__ __align__(16) bf16_t lx[2][NK * CP * 512];
     const int lane = threadIdx.x & 63, d = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), colv = p.dvp / 16;
     const unsigned id = (unsigned)p.first + blockIdx.x;
@@ -378,27 +380,37 @@ __global__ __launch_bounds__(DK * 4) void delta_join_k(DeltaArgs p) {
     }
     const bf16_t* maps = p.maps + chain * (long long)(p.segments - 1) * z.map;
     float* shifts = p.shifts + chain * (long long)(p.segments - 1) * z.shift + cv * (DK * 16) + d * 256;
-    Frag<CP> m[NK];
-    f32x4 n;
-    auto fetch = [&](int s) {
-#pragma unroll
-        for (int k = 0; k < NK; ++k) m[k] = load_frag<CP>(maps + s * z.map, d * NK + k, lane);
-        n = load_at<f32x4>(shifts + s * z.shift, lane * 16);
+    // (behind the last segment's the last once more: loads on a condition would be waited for all together)
+    struct Map {
+        Frag<CP> m[NK];
+        f32x4 n;
     };
-    fetch(0);
-    for (int s = 0; s + 1 < p.segments; ++s) {
+    const int last = p.segments - 2;
+    auto fetch = [&](Map& f, int s) {
+        s = s < last ? s : last;
+#pragma unroll
+        for (int k = 0; k < NK; ++k) f.m[k] = load_frag<CP>(maps + s * z.map, d * NK + k, lane);
+        f.n = load_at<f32x4>(shifts + s * z.shift, lane * 16);
+    };
+    Map ahead[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) fetch(ahead[j], j);
+    for (int s0 = 0; s0 <= last; s0 += AHEAD)
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+        const int s = s0 + j;
+        if (s > last) break;
         bf16_t* l = lx[s & 1];
         store_half(l, d / 2, d & 1, split<CP>(x), lane);
         __syncthreads();
         f32x4 t[NK];
 #pragma unroll
-        for (int k = 0; k < NK; ++k) t[k] = mma(m[k], load_frag<CP>(l, k, lane), k ? f32x4{0.f, 0.f, 0.f, 0.f} : n);
+        for (int k = 0; k < NK; ++k) t[k] = mma(ahead[j].m[k], load_frag<CP>(l, k, lane), k ? f32x4{0.f, 0.f, 0.f, 0.f} : ahead[j].n);
         x = t[0];
 #pragma unroll
         for (int k = 1; k < NK; ++k) x += t[k];
-        float* to = shifts + s * z.shift;
-        if (s + 2 < p.segments) fetch(s + 1);
-        store_at(to, lane * 16, x);
+        if (AHEAD > 1 || s < last) fetch(ahead[j], s + AHEAD);
+        store_at(shifts + s * z.shift, lane * 16, x);
     }
 }
 
