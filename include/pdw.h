@@ -576,7 +576,9 @@ int pdw_rotary_bwd(const pdw_rotary *call, const void *const gy[2], void *const 
  * valid steps, limited to 0..T; what lies behind is not read, y and the gradients are 0 there.  reverse: from the last valid step to the first.
  * gates_f32: g and b are fp32 whatever dtype is.
  * `states` (pdw_delta_states_bytes; NULL where no backward follows): what the backward needs.  States and sums are fp32; y is rounded once.  Products
- * are made of bf16 planes: infinities in k, q, v or a state come out as NaN. */
+ * are made of bf16 planes: infinities in k, q, v or a state come out as NaN (in calls that go step by step as a loop has them).  A value that is not
+ * finite reaches what the rule hands it to, y of its own step and the later ones and the last state (in v: of its channel), and no other step, channel or
+ * head; among the gradients it can reach all steps of its chunk of 64, and what the rule hands those to. */
 #define PDW_DELTA_MAX_CHANNELS 128
 typedef struct {
     const void *q, *k, *v, *g, *b;

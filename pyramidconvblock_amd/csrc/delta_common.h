@@ -74,6 +74,7 @@ struct DeltaPlanes<float> {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <int NP>
@@ -145,6 +146,19 @@ __device__ __forceinline__ Half<NP> split(f32x4 v) {
             for (int i = 0; i < 4; ++i) v[i] -= (float)h.p[p][i];
         }
     }
+    return h;
+}
+// of a b, unrounded
+template <int NP>
+__device__ __forceinline__ Half<NP> split_product(f32x4 a, f32x4 b) {
+    Half<NP> h;
+    const f32x4 v = a * b;
+    f32x4 rest;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h.p[0][i] = (__bf16)v[i], rest[i] = __builtin_fmaf(a[i], b[i], -(float)h.p[0][i]);
+    const Half<NP - 1> more = split<NP - 1>(rest);
+#pragma unroll
+    for (int p = 1; p < NP; ++p) h.p[p] = more.p[p - 1];
     return h;
 }
 template <int NP>
@@ -528,17 +542,75 @@ __device__ __forceinline__ f32x4 invert_block(f32x4 A, int lane) {
     return v;
 }
 
-// Solutions X of (I + A) X = R by blocks of rows, in place: lane = column, values = rows.  A solved block goes at once into the rows behind it.
+// What is not finite.  A chunk's products run over blocks of steps, with zeros where a step has no part in another, and 0 times NaN is NaN: a bad row
+// would reach the steps before it.  Where a result says that there may be one (rare: one comparison), the product is made again without the rows
+// from a column's first bad one on, and from that step on the column is NaN, as its state is from there on.  (The limit: rounded to bf16 it is infinite.)
+__device__ __forceinline__ bool is_bad(float v) { return !(__builtin_fabsf(v) < 0x1.ffp127f); }
+__device__ __forceinline__ int first_of_groups(int n) {   // the least over the four lane groups
+    int m = __shfl_xor(n, 16);
+    n = m < n ? m : n;
+    m = __shfl_xor(n, 32);
+    return m < n ? m : n;
+}
+
+// A block's inverse with such rows (a lane has a row): those before them have no part in them.
+__device__ __forceinline__ f32x4 invert_rows(f32x4 A, int lane) {
+    const unsigned long long b = __ballot(is_bad(A[0]) || is_bad(A[1]) || is_bad(A[2]) || is_bad(A[3]));
+    const unsigned rows = (unsigned)(b | b >> 16 | b >> 32 | b >> 48) & 0xffffu;
+    const bool behind = rows && (lane & 15) >= __builtin_ctz(rows | 0x10000u);
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f}, nan = zero + __builtin_nanf("");
+    const f32x4 t = invert_block(behind ? zero : A, lane);
+    return behind ? nan : t;
+}
+
+// Solutions X of (I + A) X = R f by blocks of rows: lane = column, values = rows, each with a factor of its own.  A solved block goes at once into the rows
+// behind it.
 template <int NP>
-__device__ __forceinline__ void solve_fore(const bf16_t* blocks, f32x4 (&x)[4], int lane) {
+__device__ __forceinline__ void solve_fore(const bf16_t* blocks, const f32x4 (&R)[4], const f32x4 (&f)[4], f32x4 (&x)[4], int lane) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 1; b < 4; ++b) x[b] = R[b] * f[b];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-        const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-        x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(a, a), lane), split<NP>(x[a]), zero);
+        x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(a, a), lane), a ? split<NP>(x[a]) : split_product<NP>(R[0], f[0]), zero);
         const Half<NP> s = split<NP>(x[a]);
 #pragma unroll
         for (int b = a + 1; b < 4; ++b) x[b] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s, x[b]);
     }
+}
+// The same where rows are bad, of R f or of the system.  (After solve_fore a column's row 48 is NaN where a bad row has reached others.)
+template <int NP>
+__device__ __forceinline__ void solve_fore_until(const bf16_t* blocks, f32x4 (&R)[4], f32x4 (&f)[4], f32x4 (&x)[4], int lane) {
+    const int g4 = 4 * (lane >> 4);
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    int first = kDeltaChunk;
+    auto look = [&](int a) {
+        int n = kDeltaChunk;
+#pragma unroll
+        for (int r = 3; r >= 0; --r) n = is_bad(x[a][r]) ? 16 * a + g4 + r : n;
+        n = first_of_groups(n);
+        first = n < first ? n : first;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool before = 16 * a + g4 + r < first;
+            x[a][r] = before ? x[a][r] : 0.f, R[a][r] = before ? R[a][r] : 0.f, f[a][r] = before ? f[a][r] : 0.f;
+        }
+    };
+#pragma unroll
+    for (int b = 0; b < 4; ++b) x[b] = R[b] * f[b];
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+        look(a);
+        x[a] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(a, a), lane), a ? split<NP>(x[a]) : split_product<NP>(R[0], f[0]), zero);
+        look(a);
+        const Half<NP> s = split<NP>(x[a]);
+#pragma unroll
+        for (int b = a + 1; b < 4; ++b) x[b] = mma(Blocks<NP>::get(blocks, Blocks<NP>::at(b, a), lane), s, x[b]);
+    }
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[a][r] = 16 * a + g4 + r < first ? x[a][r] : __builtin_nanf("");
 }
 // of (I + A)^T X = R, from the last block.
 template <int NP>

@@ -91,7 +91,7 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
         if (t == wave) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[r] = g4 + r < col ? acc[r] : 0.f;
-            acc = invert_block(acc, lane);
+            acc = invert_rows(acc, lane);
         } else {
             acc = -acc;
         }
@@ -117,6 +117,7 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
         beta[b] = *reinterpret_cast<const f32x4*>(s.beta + 16 * b + g4);
         decay[b] = beta[b] * *reinterpret_cast<const f32x4*>(s.D + 16 * b + g4);
     }
+    unsigned bad = 0;   // tiles of columns with solutions that are none (delta_common.h): of W, then of Ub
     // columns of W, and with them the first ones of Ub; then the others of Ub
     for (int at = 0; at < p.dvp; at += COLS) {
         if (at) {
@@ -129,16 +130,71 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
         for (int ct = (at ? DK / 16 : 0) + wave; ct < DK / 16 + end; ct += 4) {
             const bool w = ct < DK / 16;
             const int cv = ct - DK / 16;
-            f32x4 x[4];
+            f32x4 R[4], x[4], f[4];
 #pragma unroll
-            for (int b = 0; b < 4; ++b)
-                x[b] = w ? sum_of(L::down(k, 16 * b, 16 * ct, lane)) * decay[b] : sum_of(LV::down(vl, 16 * b, 16 * cv, lane)) * beta[b];
-            solve_fore<MADE>(blocks, x, lane);
+            for (int b = 0; b < 4; ++b) {
+                R[b] = w ? sum_of(L::down(k, 16 * b, 16 * ct, lane)) : sum_of(LV::down(vl, 16 * b, 16 * cv, lane));
+                f[b] = w ? decay[b] : beta[b];
+            }
+            solve_fore<MADE>(blocks, R, f, x, lane);
+            bad |= __any(x[3][0] != x[3][0]) ? 1u << (w ? ct : DK / 16 + at / 16 + cv) : 0;
             float* to = w ? p.w + id * z.w + ct * 1024 : p.ub + id * z.cols + (at / 16 + cv) * 1024;   // (-W: as the products take it)
 #pragma unroll
             for (int b = 0; b < 4; ++b) store_at(to + b * 256, lane * 16, w ? -x[b] : x[b]);
         }
     }
+    for (; bad; bad &= bad - 1) {
+        // (another lane for all that the compiler knows: else it makes this part's addresses ahead of the loop that is always run)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int ct = __builtin_ctz(bad), cv = ct - DK / 16, g4 = 4 * (lane >> 4);
+        const bool w = ct < DK / 16;
+        const int at = 16 * (w ? ct : cv) + (lane & 15);
+        const T* from = w ? (const T*)p.k + c.at(p.ks, c.hk) + at : (const T*)p.v + c.at(p.vs, c.hv) + at;
+        const long long stride = w ? p.ks.t : p.vs.t;
+        f32x4 R[4], x[4], f[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = first + 16 * b + g4 + r;
+                R[b][r] = i < c.len && at < (w ? p.dk : p.dv) ? to_f32(from[c.step(p, i) * stride]) : 0.f;
+                f[b][r] = s.beta[i - first] * (w ? s.D[i - first] : 1.f);
+            }
+        solve_fore_until<MADE>(blocks, R, f, x, lane);
+        float* to = w ? p.w + id * z.w + ct * 1024 : p.ub + id * z.cols + cv * 1024;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) store_at(to + b * 256, lane * 16, w ? -x[b] : x[b]);
+    }
+}
+
+// acc + P U where rows of U are bad: lane = step of P and of the result, its values columns; U's lanes are columns.
+template <int NP>
+__device__ __forceinline__ f32x4 product_until(const bf16_t* us, int fragment, const Frag<NP> (&p)[2], f32x4 acc, int step, int lane) {
+    auto row = [&](int n, int j) { return 32 * n + 16 * (j / 4) + 4 * (lane >> 4) + j % 4; };
+    int first = kDeltaChunk;
+#pragma unroll
+    for (int n = 1; n >= 0; --n) {
+        const u32x4 u = load_at<u32x4>(us + (fragment + n) * NP * 512, lane * 16);
+#pragma unroll
+        for (int j = 7; j >= 0; --j) first = (u[j / 2] >> (j & 1) * 16 & 0x7f80) == 0x7f80 ? row(n, j) : first;
+    }
+    first = first_of_groups(first);
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        Frag<NP> u = load_frag<NP>(us, fragment + n, lane);
+        u32x4 there;
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) there[j / 2] = (row(n, j) < first ? 0xffffu : 0) | (row(n, j + 1) < first ? 0xffff0000u : 0);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) u.p[i] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, u.p[i]) & there);
+        acc = mma(u, p[n], acc);
+        asm volatile("" : "+v"(lane));   // (one after the other: few registers)
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (step >= __shfl(first, 4 * (lane >> 4) + r)) acc[r] = __builtin_nanf("");
+    return acc;
 }
 
 template <typename T, int DK>
@@ -146,8 +202,14 @@ constexpr int delta_out_lds() {
     return 2 * delta_rows_bytes<DeltaPlanes<T>::kRaw, DK>() + (int)sizeof(DeltaGates);
 }
 
+// Wavefronts of a SIMD that registers are left for: as many as its loop over columns needs by itself.
 template <typename T, int DK>
-__global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
+constexpr int delta_out_waves() {
+    return sizeof(T) == 2 ? (DK == 32 ? 5 : DK == 64 ? 4 : 3) : (DK == 128 ? 2 : 3);
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(256, (delta_out_waves<T, DK>())) void delta_out_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = DeltaPlanes<T>::kMade;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
@@ -208,6 +270,7 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
     const int step = first + i;
     const bool there = step < c.len;
     T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
+    unsigned bad = 0;   // tiles of columns with results that are none (delta_common.h)
     for (int cv = 0; cv < p.dvp / 16; ++cv) {
         const Columns f = next;
         if (cv + 1 < p.dvp / 16) next = fetch(cv + 1);
@@ -217,7 +280,21 @@ __global__ __launch_bounds__(256) void delta_out_k(DeltaArgs p) {
         acc *= D;
         acc = mma(f.u[0], pf[0], acc);
         if (wave >= 2) acc = mma(f.u[1], pf[1], acc);
+        bad |= __any(__builtin_isunordered(acc[0], acc[1]) || __builtin_isunordered(acc[2], acc[3])) ? 1u << cv : 0;
         if (step < p.T) store_four(row, 16 * cv + g4, p.dv, there ? acc : zero, p.vec & kVecY);
+    }
+    for (; bad; bad &= bad - 1) {
+        // (another lane for all that the compiler knows: else it makes this part's addresses ahead of the loop that is always run)
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));
+        const int i = 16 * wave + (lane & 15), g4 = 4 * (lane >> 4), step = first + i;
+        const int cv = __builtin_ctz(bad);
+        T* row = (T*)p.y + c.at(p.ys, c.hv) + c.step(p, step) * p.ys.t;
+        f32x4 acc = zero;
+#pragma unroll
+        for (int n = 0; n < DK / 32; ++n) acc = mma(load_frag<MADE>(p.s0 + id * z.state, cv * (DK / 32) + n, lane), qf[n], acc);
+        acc = product_until(p.u + id * z.u, cv * 2, pf, acc * (p.scale * s.D[i]), i, lane);
+        if (step < p.T) store_four(row, 16 * cv + g4, p.dv, step < c.len ? acc : zero, p.vec & kVecY);
     }
 }
 

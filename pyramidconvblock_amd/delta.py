@@ -6,7 +6,8 @@ dk x dv,
 the recurrence of ``scan.py`` with a matrix for a state: what a key had stood for is replaced by beta of the way, everything fades by a.  float32, float16
 and bfloat16, 1 to 128 channels a head; states are 32-bit throughout, results are the same from call to call.  It runs in chunks: results differ
 from a loop's by roundings; keys longer than 1 can make the rule itself grow (a step takes S along k by 1 - beta |k|^2), so rows of unit length are
-its usual input (``head_rotary`` with ``kind="l2"``).  Infinities come out as NaN.  For gradients of gradients and captures see ``norm.py``.
+its usual input (``head_rotary`` with ``kind="l2"``).  Infinities come out as NaN.  What is not finite reaches y from its own step on (in v: in its
+channel) and no step before it; among the gradients it can reach the whole chunk of 64 steps.  For gradients of gradients and captures see ``norm.py``.
 """
 from __future__ import annotations
 
