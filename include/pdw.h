@@ -546,7 +546,7 @@ int pdw_scan_step(const void *x, const void *g, const float *state, float *new_s
  * Tensor 0 has heads[0] heads, tensor 1 (may be NULL) heads[1]; element (token, head, i) of it is x[token * xt + head * xh + i].
  * Positions: NULL, tokens are a grid whose last axes have the extents grid[0..axes); or rows of `axes` numbers of position_type, one for each
  * of the last `positions_rows` tokens' places, repeated (token modulo rows).  Frequencies (device, fp32, radians, P of them): NULL, then
- * base^(-j / section) for pair j of each section.  Weights have the tensors' type; NULL: 1. */
+ * base^(-j / section) for pair j of each section.  Weights have the tensors' type; NULL: 1.  PDW_HEAD_NONE has none, and no gradients of any. */
 enum { PDW_HEAD_NONE = 0, PDW_HEAD_RMS = 1, PDW_HEAD_L2 = 2 };
 enum { PDW_POSITIONS_GRID = 0, PDW_POSITIONS_I32 = 1, PDW_POSITIONS_I64 = 2, PDW_POSITIONS_F32 = 3 };
 #define PDW_HEAD_MAX_CHANNELS 256

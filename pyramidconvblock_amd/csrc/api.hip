@@ -909,6 +909,7 @@ static int rotary_args(const char* fn, const pdw_rotary* c, RotaryArgs& p) {
     }
     for (int a = c->axes; a < 3; ++a) p.ends[a] = P;
     if (2 * P > c->d) return set_error("%s: %d pairs of %d channels", fn, P, c->d), 1;
+    if (c->kind == kRotaryNone && (c->weight[0] || c->weight[1])) return set_error("%s: weight without a norm", fn), 1;
     if (c->tokens > 0 && ((c->heads[0] && !c->x[0]) || (c->heads[1] && !c->x[1]))) return set_error("%s: null pointer", fn), 1;
     p.grid[0] = p.grid[1] = p.grid[2] = 1;
     if (c->position_type == kPositionGrid) {
@@ -946,6 +947,7 @@ int pdw_rotary_bwd(const pdw_rotary* c, const void* const gy[2], void* const gx[
                    size_t workspace_bytes, void* stream) {
     RotaryArgs p{};
     if (int e = rotary_args("pdw_rotary_bwd", c, p)) return e;
+    if (c->kind == kRotaryNone && gweight && (gweight[0] || gweight[1])) return set_error("pdw_rotary_bwd: gradient of a weight without a norm"), 1;
     if (p.N == 0 || (!p.heads[0] && !p.heads[1])) return 0;
     if (!gy || !gx || !gweight || (p.heads[0] && !gy[0]) || (p.heads[1] && !gy[1])) return set_error("pdw_rotary_bwd: null pointer"), 1;
     for (int s = 0; s < 2; ++s) p.gy[s] = gy[s], p.y[s] = gx[s];

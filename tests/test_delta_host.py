@@ -202,6 +202,21 @@ def test_library_refuses_rotary_calls_before_any_launch():
         assert L.pdw_rotary_fwd(ctypes.addressof(c), ctypes.addressof(two), None) == 0, nothing
 
 
+def test_library_refuses_weights_without_a_norm():
+    L = lib()
+    one, none = (ctypes.c_void_p * 2)(1, None), (ctypes.c_void_p * 2)()
+    for weight in ((1, None), (None, 1)):
+        for tokens in (10, 0):
+            c = rotary_call(kind=0, weight=weight, tokens=tokens)
+            assert L.pdw_rotary_fwd(ctypes.addressof(c), ctypes.addressof(one), None) == 1 and b"without a norm" in L.pdw_last_error()
+            assert L.pdw_rotary_bwd(ctypes.addressof(c), *[ctypes.addressof(one)] * 2, ctypes.addressof(none), None, 0, None) == 1
+            assert b"without a norm" in L.pdw_last_error()
+    for gweight in (one, (ctypes.c_void_p * 2)(None, 1)):
+        c = rotary_call(kind=0)
+        assert L.pdw_rotary_bwd(ctypes.addressof(c), *[ctypes.addressof(one)] * 2, ctypes.addressof(gweight), 1, 1 << 30, None) == 1
+        assert b"without a norm" in L.pdw_last_error()
+
+
 def delta_call(**other):
     from pyramidconvblock_amd import _lib
 
