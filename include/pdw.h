@@ -562,7 +562,7 @@ typedef struct {
 } pdw_rotary;
 /* y[0], y[1] dense [token][head][d]. */
 int pdw_rotary_fwd(const pdw_rotary *call, void *const y[2], void *stream);
-/* gx[2] (dense) and gweight[2] from gy[2] (dense); each result may be NULL.  Workspace: needed where a gweight is wanted. */
+/* gx[2] (dense) and gweight[2] from gy[2] (dense); each result may be NULL.  Workspace: needed where a gweight is wanted (of no rows: zeros, without). */
 size_t pdw_rotary_bwd_workspace_bytes(int d);
 int pdw_rotary_bwd(const pdw_rotary *call, const void *const gy[2], void *const gx[2], void *const gweight[2], void *workspace,
                    size_t workspace_bytes, void *stream);

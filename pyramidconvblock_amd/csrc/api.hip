@@ -948,7 +948,8 @@ int pdw_rotary_bwd(const pdw_rotary* c, const void* const gy[2], void* const gx[
     RotaryArgs p{};
     if (int e = rotary_args("pdw_rotary_bwd", c, p)) return e;
     if (c->kind == kRotaryNone && gweight && (gweight[0] || gweight[1])) return set_error("pdw_rotary_bwd: gradient of a weight without a norm"), 1;
-    if (p.N == 0 || (!p.heads[0] && !p.heads[1])) return 0;
+    if (p.N == 0 || (!p.heads[0] && !p.heads[1]))
+        return gweight ? rotary_no_rows(gweight[0], gweight[1], p.d, c->dtype, (hipStream_t)stream) : 0;
     if (!gy || !gx || !gweight || (p.heads[0] && !gy[0]) || (p.heads[1] && !gy[1])) return set_error("pdw_rotary_bwd: null pointer"), 1;
     for (int s = 0; s < 2; ++s) p.gy[s] = gy[s], p.y[s] = gx[s];
     return rotary_run(p, true, gweight[0], gweight[1], workspace, workspace_bytes, c->dtype, (hipStream_t)stream);

@@ -217,6 +217,7 @@ int scan_step_launch(const void* x, const void* g, const float* state, float* ne
 
 // rotary.hip: norms of heads with rotated positions (arguments: rotary.h)
 size_t rotary_workspace(int d);
+int rotary_no_rows(void* gw, void* gkw, int d, int dtype, hipStream_t s);
 int rotary_run(const struct RotaryArgs& p, bool backward, void* gw, void* gkw, void* workspace, size_t workspace_bytes, int dtype, hipStream_t s);
 
 // delta.hip: the gated delta rule (arguments: delta_common.h); delta_step.hip: its form for single tokens

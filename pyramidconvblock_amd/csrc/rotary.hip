@@ -48,6 +48,17 @@ static int rotary_tokens(const RotaryArgs& p, int lanes) {
     return t < 1 ? 1 : (int)t;
 }
 
+static int rotary_sums(const float* parts, void* gw, void* gkw, int workgroups, int d, int dtype, hipStream_t s) {
+    const unsigned n = (2 * d + 15) / 16;
+    if (dtype == kF32) rotary_sums_k<float><<<n, 1024, 0, s>>>(parts, (float*)gw, (float*)gkw, workgroups, d);
+    else if (dtype == kF16) rotary_sums_k<f16_t><<<n, 1024, 0, s>>>(parts, (f16_t*)gw, (f16_t*)gkw, workgroups, d);
+    else rotary_sums_k<bf16_t><<<n, 1024, 0, s>>>(parts, (bf16_t*)gw, (bf16_t*)gkw, workgroups, d);
+    return check_launch("rotary_sums_k");
+}
+
+// The weights' gradients of a call without rows: sums of nothing.
+int rotary_no_rows(void* gw, void* gkw, int d, int dtype, hipStream_t s) { return gw || gkw ? rotary_sums(nullptr, gw, gkw, 0, d, dtype, s) : 0; }
+
 size_t rotary_workspace(int d) { return (size_t)kRotarySums * 2 * d * sizeof(float); }
 
 int rotary_run(const RotaryArgs& in, bool backward, void* gw, void* gkw, void* workspace, size_t workspace_bytes, int dtype, hipStream_t s) {
@@ -65,12 +76,7 @@ int rotary_run(const RotaryArgs& in, bool backward, void* gw, void* gkw, void* w
     else if (dtype == kF16) rotary_launch_f16(p, (unsigned)grid, backward, s);
     else rotary_launch_bf16(p, (unsigned)grid, backward, s);
     if (int e = check_launch("rotary_k")) return e;
-    if (!sums) return 0;
-    const unsigned n = (2 * p.d + 15) / 16;
-    if (dtype == kF32) rotary_sums_k<float><<<n, 1024, 0, s>>>(p.parts, (float*)gw, (float*)gkw, (int)grid, p.d);
-    else if (dtype == kF16) rotary_sums_k<f16_t><<<n, 1024, 0, s>>>(p.parts, (f16_t*)gw, (f16_t*)gkw, (int)grid, p.d);
-    else rotary_sums_k<bf16_t><<<n, 1024, 0, s>>>(p.parts, (bf16_t*)gw, (bf16_t*)gkw, (int)grid, p.d);
-    return check_launch("rotary_sums_k");
+    return sums ? rotary_sums(p.parts, gw, gkw, (int)grid, p.d, dtype, s) : 0;
 }
 
 }  // namespace pdw

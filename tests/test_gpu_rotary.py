@@ -347,3 +347,33 @@ def test_streams():
         for r in results[i]:
             for k in r:
                 assert torch.equal(r[k], alone[i][k]), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("nothing", [dict(tokens=0), dict(heads=(0, 0)), dict(heads=(0, 2))], ids=str)
+def test_library_writes_the_gradients_of_weights_without_rows(nothing, dtype):
+    """From C: zeros into each gradient that is asked for, and no other memory."""
+    import ctypes
+
+    from pyramidconvblock_amd import _lib
+
+    L, d = _lib.lib(), 24
+    c = _lib.Rotary()
+    x, w = torch.ones(5, 2, d, device="cuda", dtype=dtype), torch.ones(2, d, device="cuda", dtype=dtype)
+    c.tokens, c.d, c.axes, c.kind, c.dtype, c.eps, c.base = nothing.get("tokens", 5), d, 1, 1, _lib.dtype_code(dtype), 1e-6, 1e4
+    c.x[:], c.heads[:], c.sections[:], c.grid[:] = (x.data_ptr(),) * 2, nothing.get("heads", (2, 2)), (4, 0, 0), (5, 0, 0)
+    c.xt[:], c.xh[:], c.weight[:] = (2 * d, 2 * d), (d, d), (w[0].data_ptr(), w[1].data_ptr())
+    gw = torch.full((4, d), float("nan"), device="cuda", dtype=dtype)
+    work = torch.empty(L.pdw_rotary_bwd_workspace_bytes(d), device="cuda", dtype=torch.uint8)
+    two = lambda a, b: (ctypes.c_void_p * 2)(a, b)
+    gys, gxs = two(x.data_ptr(), x.data_ptr()), two(None, None)
+    for rows in ((0, 2), (0, None), (None, 2)):
+        gw.fill_(float("nan"))
+        to = two(*(None if r is None else gw[r].data_ptr() for r in rows))
+        assert L.pdw_rotary_bwd(ctypes.addressof(c), *(ctypes.addressof(a) for a in (gys, gxs, to)), work.data_ptr(), work.numel(),
+                                torch.cuda.current_stream().cuda_stream) == 0, L.pdw_last_error()
+        for r in range(4):
+            if r not in rows:
+                assert gw[r].isnan().all(), (rows, r)
+            elif r == 0 or c.tokens == 0 or c.heads[1] == 0:
+                assert not gw[r].any() and not gw[r].isnan().any(), (rows, r)
