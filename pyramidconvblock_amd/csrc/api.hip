@@ -962,7 +962,7 @@ static int delta_args(const char* fn, const pdw_delta* c, DeltaArgs& p) {
         return set_error("%s: bad extents O=%d T=%lld W=%d heads=%d,%d", fn, c->O, c->T, c->W, c->Hk, c->Hv), 1;
     if (c->dk < 1 || c->dk > PDW_DELTA_MAX_CHANNELS || c->dv < 1 || c->dv > PDW_DELTA_MAX_CHANNELS)
         return set_error("%s: %d and %d channels of a head, 1 to %d are possible", fn, c->dk, c->dv, PDW_DELTA_MAX_CHANNELS), 1;
-    if (c->Hv && (c->Hk < 1 || c->Hv % c->Hk)) return set_error("%s: %d value heads for %d key heads", fn, c->Hv, c->Hk), 1;
+    if (c->Hv ? c->Hk < 1 || c->Hv % c->Hk : c->Hk) return set_error("%s: %d value heads for %d key heads", fn, c->Hv, c->Hk), 1;
     const long long rows = (long long)c->O * c->W;
     if (rows > 0x7fffffffLL || rows * c->Hv > 0x7fffffffLL) return set_error("%s: more than 2^31 - 1 chains", fn), 1;
     if (rows * c->Hv && c->T && (!c->q || !c->k || !c->v || !c->g || !c->b)) return set_error("%s: null pointer", fn), 1;

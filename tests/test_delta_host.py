@@ -228,6 +228,14 @@ def delta_call(**other):
     return c
 
 
+def test_library_refuses_key_heads_without_value_heads():
+    """(The gradients of q and k would have elements that no launch writes.)"""
+    L, c = lib(), delta_call(Hv=0, Hk=2)
+    assert L.pdw_delta_fwd(ctypes.addressof(c), 1, None, None, None, 0, None) == 1 and b"value heads" in L.pdw_last_error()
+    assert L.pdw_delta_bwd(ctypes.addressof(c), 1, None, 1, 1, 1, 1, 1, 1, None, None, 0, None) == 1
+    assert L.pdw_delta_step(ctypes.addressof(c), 1, 1, None) == 1
+
+
 def test_library_refuses_delta_calls_before_any_launch():
     L = lib()
     fwd = lambda c, y=1, states=None, ws=None, n=0: L.pdw_delta_fwd(ctypes.addressof(c), y, None, states, ws, n, None)
