@@ -56,6 +56,10 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
     constexpr int RAW = DeltaPlanes<T>::kRaw, MADE = kChainPlanes;
     constexpr int type = sizeof(T) == 4 ? kF32 : __is_same(T, f16_t) ? kF16 : kBF16;
     constexpr int COLS = delta_prepare_cols<T, DK>();
+    // Where LDS lets four workgroups be, their 128 registers do not hold the system's blocks from tile to tile, which the compiler tries: it is told
+    // of another lane with every tile (66 us for 72 at 32 x 3136 steps of 4 heads of 32 in bf16, 54 for 70, with spills, at 8 x 4096 of 6 of 64); the registers of
+    // three hold them (37 us, 39 without, with 128 channels in bf16).
+    constexpr bool KEEP = delta_prepare_waves<T, DK>() < 4;
     typedef Rows<RAW, kDeltaChunk, DK> L;
     typedef Rows<RAW, kDeltaChunk, COLS> LV;
     extern __shared__ __align__(16) unsigned char lds[];
@@ -111,12 +115,13 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
             Blocks<NG>::put(p.blocks + id * z.blocks, n, t, lane);
         }
     }
+    auto factor = [&](int b, bool w, int lane) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(s.beta + 16 * b + 4 * (lane >> 4));
+        return w ? v * *reinterpret_cast<const f32x4*>(s.D + 16 * b + 4 * (lane >> 4)) : v;
+    };
     f32x4 beta[4], decay[4];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        beta[b] = *reinterpret_cast<const f32x4*>(s.beta + 16 * b + g4);
-        decay[b] = beta[b] * *reinterpret_cast<const f32x4*>(s.D + 16 * b + g4);
-    }
+    for (int b = 0; b < 4; ++b) beta[b] = factor(b, false, lane), decay[b] = factor(b, true, lane);
     unsigned bad = 0;   // tiles of columns with solutions that are none (delta_common.h): of W, then of Ub
     // columns of W, and with them the first ones of Ub; then the others of Ub
     for (int at = 0; at < p.dvp; at += COLS) {
@@ -130,11 +135,13 @@ __global__ __launch_bounds__(256, (delta_prepare_waves<T, DK>())) void delta_pre
         for (int ct = (at ? DK / 16 : 0) + wave; ct < DK / 16 + end; ct += 4) {
             const bool w = ct < DK / 16;
             const int cv = ct - DK / 16;
+            int lane = threadIdx.x & 63;
+            if (!KEEP) asm volatile("" : "+v"(lane));
             f32x4 R[4], x[4], f[4];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
                 R[b] = w ? sum_of(L::down(k, 16 * b, 16 * ct, lane)) : sum_of(LV::down(vl, 16 * b, 16 * cv, lane));
-                f[b] = w ? decay[b] : beta[b];
+                f[b] = KEEP ? w ? decay[b] : beta[b] : factor(b, w, lane);
             }
             solve_fore<MADE>(blocks, R, f, x, lane);
             bad |= __any(x[3][0] != x[3][0]) ? 1u << (w ? ct : DK / 16 + at / 16 + cv) : 0;
