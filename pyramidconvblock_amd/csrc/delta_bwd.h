@@ -52,8 +52,9 @@ template <typename T, int DK, int MADE>
 __global__ __launch_bounds__(256, (delta_back_prepare_waves<T, DK, MADE>())) void delta_back_prepare_k(DeltaArgs p) {
     constexpr int RAW = DeltaPlanes<T>::kRaw;
     // with 32 channels seven workgroups a compute unit wait for one another's loads better than four with their own under way (49 us for 59 at 32 x 3136 steps,
-    // 4 heads; with 128 channels 57 us for 49)
-    constexpr bool AHEAD = DK > 32;
+    // 4 heads; with 128 channels 57 us for 49); nor do three planes leave room for them in the 128 registers of four workgroups (64 channels in bf16: 57 us for 66, with
+    // spills, at 8 x 4096 steps of 6 heads)
+    constexpr bool AHEAD = DK > 32 && !(MADE == kChainPlanes && delta_back_prepare_waves<T, DK, MADE>() == 4);
     typedef Rows<RAW, kDeltaChunk, DK> L;
     extern __shared__ __align__(16) unsigned char lds[];
     bf16_t *q = (bf16_t*)lds, *k = q + L::kValues, *pb = k + L::kValues;
