@@ -2,11 +2,13 @@
 //
 // Products run on the bf16 matrix cores whatever the tensors' type: a value is a sum of bf16 planes (the value rounded, what that left
 // rounded, and so on), and a product of two such sums leaves out the products of planes that are below the result's precision.  What comes from
-// the tensors takes as many planes as hold it exactly, except the last bits of fp32 and of fp16 (1 for bf16, 2 for fp16, 3 for fp32); what
-// was computed in fp32 (the chunk's triangular system, its solutions, states) takes 3 planes, 24 bits, where states come of it, which are results
-// in 32 bits, and 2 planes, 2^-17 of a value, where it ends in results of 16 bits.  Sums are the matrix cores' fp32.  So results are off by
-// their own rounding and by little else, where single bf16 operands had put 2^-9 of every intermediate into them; and fp32 takes 6
-// products of 16 cycles where the fp32 matrix instruction takes eight of 32.
+// the tensors takes as many planes as hold it exactly (1 for bf16, 2 for fp16, 3 for fp32); what was computed in fp32 (the chunk's triangular system,
+// its solutions, states) takes 3 planes, 24 bits, where states come of it, which are results in 32 bits, and 2 planes, 2^-17 of a value, where
+// it ends in results of 16 bits, and in the gradients of fp32 gates beside 16-bit tensors: those gradients hold some 17 bits of what they are sums of (off by 3e-6 to 8e-6 of
+// their norm), more than the 8 or 11 that came in with dY, and a third plane would cost a launch that waits for LDS its second workgroup a compute unit.  Sums are the matrix
+// cores' fp32.  So results are off by their own rounding and by little else (bf16, 32 x 3136 steps: 0.35 % are not the nearest value, and off by up to 1.11 half
+// steps), where single bf16 operands had put 2^-9 of every intermediate into them; and fp32 takes 6 products of 16 cycles where the fp32 matrix
+// instruction takes eight of 32.
 //
 // Fragments of the 16x16x32 instruction: lane l has row (column) l % 16 and 8 values along the inner axis.  A result has column l % 16 and
 // rows 4 (l / 16) + r, so results turn into operands of a next product whose inner axis is their rows without an exchange of lanes: an inner

@@ -61,7 +61,7 @@ void delta_backward(const DeltaArgs& p, hipStream_t s) {
     else delta_launch(delta_grads_k<T, DK, false>, delta_grads_lds<T, DK>(), once[2], chunks, kGradsThreads, p, s);
 }
 
-// The gradient of an initial state is a result in 32 bits; the others of 16-bit tensors are rounded to those.
+// The gradient of an initial state is a result in 32 bits; the others of 16-bit tensors are rounded to those, or (of fp32 gates) hold 17 bits (delta_common.h).
 template <typename T, int DK>
 void delta_pass(const DeltaArgs& p, bool backward, hipStream_t s) {
     if (!backward) return delta_forward<T, DK>(p, s);

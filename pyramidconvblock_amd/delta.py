@@ -50,8 +50,8 @@ def gated_delta(q, k, v, g, b, state=None, lengths=None, dim=-3, reverse=False, 
 
     q, k [..., T, ..., hk, dk], v [..., T, ..., hv, dv], g, b [..., T, ..., hv]: the rule runs along ``dim`` of q (any but the heads' and the
     channels'), from its end with ``reverse``.  hv is a multiple of hk: neighbouring value heads share a key head.  g and b are logits, or with
-    ``logits=False`` the log decay (at most 0) and the write strength themselves; of q's type or float32.  scale: None is dk^-1/2.  state: before the first
-    step, like the last one (None: 0).  lengths (int32, q.shape[:dim]): valid steps of each sequence, limited to 0..T; what lies behind them is not
+    ``logits=False`` the log decay (at most 0) and the write strength themselves; of q's type or float32 (beside 16-bit tensors their gradients hold
+    some 17 bits of the terms that they are sums of).  scale: None is dk^-1/2.  state: before the first step, like the last one (None: 0).  lengths (int32, q.shape[:dim]): valid steps of each sequence, limited to 0..T; what lies behind them is not
     read, y and the gradients are 0 there, and the last state is the one after the last valid step.  A g of -inf or its type's lowest value forgets all
     that was before its step.  Slices of a wider tensor's channels are read where they lie."""
     args = (q, k, v, g, b, state, lengths, dim, reverse, _scale(q, scale), logits)
