@@ -573,7 +573,8 @@ int pdw_rotary_bwd(const pdw_rotary *call, const void *const gy[2], void *const 
  * g and b a number for each of Hv; value heads share key heads in groups of Hv / Hk.  dk, dv: 1 to PDW_DELTA_MAX_CHANNELS.
  * Element (o, t, w, head, i) is x[o * s[0] + t * s[1] + w * s[2] + head * s[3] + i].  y and the gradients are dense.
  * h0, last [O][W][Hv][dk][dv], fp32, either may be NULL; they must not overlap, nor may a backward's glast and gh0.  lengths[O] (device, may be NULL):
- * valid steps, limited to 0..T; what lies behind is not read, y and the gradients are 0 there.  reverse: from the last valid step to the first.
+ * valid steps, limited to 0..T; what lies behind has no part in any result (of an empty sequence the first step is loaded
+ * and dropped), y and the gradients are 0 there.  reverse: from the last valid step to the first.
  * gates_f32: g and b are fp32 whatever dtype is, and so are their gradients, which hold some 17 bits of the terms that they are sums of in 16-bit calls.
  * `states` (pdw_delta_states_bytes; NULL where no backward follows): what the backward needs.  States and sums are fp32; y is rounded once.  Products
  * are made of bf16 planes: infinities in k, q, v or a state come out as NaN (in calls that go step by step as a loop has them).  A value that is not

@@ -15,10 +15,11 @@
 // share a key head one after another, their dQ and dK summed in registers, in one order.
 //
 // Measured, us a launch (back_prepare, the chains' three, grads), the sizes of delta_fwd.h:
-//   bf16, 32 x 3136 x 4 heads of 32 48, 53, 154;  bf16, 2 x 4096 x 4 and 8 of 128 50, 49 + 13 + 39, 142;  fp16, 2 x 16384 x 6 of 64 77, 65 + 13 + 38, 228
-// delta_back_prepare_k is bound by memory at 32 channels (34 KB a chunk, 4.3 TB/s).  delta_grads_k, half the backward's time, waits: its eight wavefronts meet
-// at six barriers a round of columns and wait for 47 % of their time, the vector unit is busy for 60 %; two workgroups a compute unit are what LDS
-// and 128 registers hold.
+//   bf16, 32 x 3136 x 4 heads of 32 48, 54, 152;  bf16, 8 x 4096 x 6 of 64 48, 42 + 8 + 36, 152;  bf16, 2 x 4096 x 4 and 8 of 128 49, 49 + 13 + 40, 138;
+//   fp16, 2 x 16384 x 6 of 64 with a state's gradient 78, 69 + 14 + 39, 237
+// delta_back_prepare_k is bound by memory and vector instructions at 32 channels (34 KB a chunk, 4.5 TB/s; they are issued in 83 % of the time).  delta_grads_k, half the
+// backward's time, waits: its eight wavefronts meet at six barriers a round of columns and wait for 47 % of their time, vector instructions are issued in 55 %
+// (in fp16 with 64 channels, one workgroup a compute unit, 51 and 33 %); two workgroups a compute unit are what LDS and 128 registers hold.
 #pragma once
 #include "delta_fwd.h"
 

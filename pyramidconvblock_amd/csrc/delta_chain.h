@@ -7,7 +7,7 @@
 // results of one product are operands of the next as they are.  W and K are the same for all columns of a chain, so other wavefronts of the workgroup
 // fetch them, several chunks ahead in registers, and put them into LDS: one's place is filled while the other is in use, a barrier
 // a chunk, or two where LDS has no room for both.  What bounds it: with many chains memory (240 segments of 13 chunks at 64 channels
-// in fp16: 221 MB in 45 us), with few the latencies of splits, products and the exchange between the wavefronts, one chunk after another (1.6 us a chunk at 32
+// in fp16: 232 MB in 43 us), with few the latencies of splits, products and the exchange between the wavefronts, one chunk after another (1.6 us a chunk at 32
 // channels, 2.7 at 64, 3.5 at 128).
 //
 // Where there are too few chains to fill the chip, the chunks are cut into segments.  Through a segment X goes to M X + N, and the same kernel

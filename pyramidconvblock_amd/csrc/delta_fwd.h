@@ -14,12 +14,13 @@
 // workgroup a chunk again: Y.  64 steps a chunk: what lies between the launches (states, W) falls with longer ones, the triangle's work rises.
 //
 // Measured, us a launch (prepare, the chains' three, out):
-//   bf16, 32 sequences of 3136 steps, 4 heads of 32      69, 67 (without segments), 36
-//   bf16, 2 of 4096, 4 key and 8 value heads of 128      36, 60 + 16 + 42, 32
-//   fp16, 2 of 16384, 6 heads of 64                      75, 61 + 13 + 42, 44
-//   bf16, 1 of 3136, 4 heads of 32, no gradients         10, 8 + 7 + 8, 5
-// delta_prepare_k is bound by vector instructions (1040 a wavefront at 32 channels, 81 % of the cycles that its 16 wavefronts a compute unit have):
-// splitting solutions into planes between products, the inverses, decays.  delta_out_k is bound by memory: 26 KB a chunk at 32 channels in bf16, 4.3 TB/s.
+//   bf16, 32 sequences of 3136 steps, 4 heads of 32      66, 70 (without segments), 36
+//   bf16, 8 of 4096, 6 heads of 64                       54, 56 + 10 + 51, 42
+//   bf16, 2 of 4096, 4 key and 8 value heads of 128      37, 61 + 17 + 41, 32
+//   fp16, 2 of 16384, 6 heads of 64                      78, 64 + 14 + 43, 44
+//   bf16, 1 of 3136, 4 heads of 32, no gradients         11, 7 + 7 + 8, 5
+// delta_prepare_k is bound by vector instructions with 32 channels (1049 a wavefront in bf16, issued in 82 % of the SIMDs' time): splitting solutions into planes
+// between products, the inverses, decays.  delta_out_k is bound by memory: 26 KB a chunk at 32 channels in bf16, 4.6 TB/s.
 #pragma once
 #include "delta_chain.h"
 

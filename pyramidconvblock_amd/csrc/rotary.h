@@ -11,9 +11,9 @@
 // quarter: what is left is below 1/8 of a turn and off by some 2^-53 of the angle itself (2^-24 of a turn at position 2^31, nothing that counts at 2^20);
 // cosine and sine of that are their series.
 //
-// Measured: 50176 tokens of 8 and 4 heads of 64 in bf16 (rms, three axes) 37 us forward, 154 MB moved, 4.2 TB/s; backward 66 + 6 us, 231 MB.  16384 tokens of 9
-// and 9 heads of 128 in fp16, 32 pairs turned, no norm: 36 us forward, 41 backward, 151 MB each.  3136 tokens of 4 and 4 heads of 32: 7 us,
-// angles and latencies.
+// Measured: 50176 tokens of 8 and 4 heads of 64 in bf16 (rms, three axes) 37 us forward, 154 MB moved, 4.1 TB/s, vector instructions issued in 73 % of the time;
+// backward 68 + 7 us, 232 MB, 3.4 TB/s, 60 %.  16384 tokens of 9 and 9 heads of 128 in fp16, 32 pairs turned, no norm: 37 us forward, 42 backward, 151 MB
+// each.  3136 tokens of 4 and 4 heads of 32: 7 us, angles and latencies.
 #pragma once
 #include "common.h"
 #include "row_norm.h"

@@ -51,8 +51,8 @@ def gated_delta(q, k, v, g, b, state=None, lengths=None, dim=-3, reverse=False, 
     q, k [..., T, ..., hk, dk], v [..., T, ..., hv, dv], g, b [..., T, ..., hv]: the rule runs along ``dim`` of q (any but the heads' and the
     channels'), from its end with ``reverse``.  hv is a multiple of hk: neighbouring value heads share a key head.  g and b are logits, or with
     ``logits=False`` the log decay (at most 0) and the write strength themselves; of q's type or float32 (beside 16-bit tensors their gradients hold
-    some 17 bits of the terms that they are sums of).  scale: None is dk^-1/2.  state: before the first step, like the last one (None: 0).  lengths (int32, q.shape[:dim]): valid steps of each sequence, limited to 0..T; what lies behind them is not
-    read, y and the gradients are 0 there, and the last state is the one after the last valid step.  A g of -inf or its type's lowest value forgets all
+    some 17 bits of the terms that they are sums of).  scale: None is dk^-1/2.  state: before the first step, like the last one (None: 0).  lengths (int32, q.shape[:dim]): valid steps of each sequence, limited to 0..T; what lies behind them has
+    no part in any result, y and the gradients are 0 there, and the last state is the one after the last valid step.  A g of -inf or its type's lowest value forgets all
     that was before its step.  Slices of a wider tensor's channels are read where they lie."""
     args = (q, k, v, g, b, state, lengths, dim, reverse, _scale(q, scale), logits)
     y = _lib.ext().delta(*args)
@@ -62,8 +62,8 @@ def gated_delta(q, k, v, g, b, state=None, lengths=None, dim=-3, reverse=False, 
 
 
 def gated_delta_step(q, k, v, g, b, state=None, new_state=None, scale=None, logits=True):
-    """One step for every stream: q, k [..., hk, dk], v [..., hv, dv], g, b [..., hv], state float32 [..., hv, dk, dv] -> (y, the new state), which is
-    written into ``new_state``, or into ``state`` itself where that is None.  Without gradients."""
+    """One step for every stream: q, k [..., hk, dk], v [..., hv, dv], g, b [..., hv], state float32 [..., hv, dk, dv] (a tensor, always) -> (y, the
+    new state), which is written into ``new_state``, or into ``state`` itself where that is None.  Without gradients."""
     y = _lib.ext().delta_step(q, k, v, g, b, state, new_state, _scale(q, scale), logits)
     return y, state if new_state is None else new_state
 
